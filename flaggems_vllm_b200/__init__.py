@@ -10,11 +10,13 @@ from .align import (  # noqa: F401
     moe_align_block_size_no_tle,
     moe_align_block_size_triton,
 )
+from .balance import moe_balance_loss  # noqa: F401
 from .fused_moe import (  # noqa: F401
     fused_experts_impl,
     inplace_fused_experts,
     outplace_fused_experts,
 )
+from .norm import fused_add_rms_norm, rms_norm, rms_norm_quant  # noqa: F401
 from .quant import SUPPORTED_FP8_DTYPE, moe_sum, per_token_group_quant_fp8  # noqa: F401
 from .router_gemm import (  # noqa: F401
     fp32_router_gemm,
@@ -36,5 +38,5 @@ __all__ = [
     "fused_experts_impl", "inplace_fused_experts", "outplace_fused_experts", "ops_experts_impl", "moe_sum",
     "per_token_group_quant_fp8", "SUPPORTED_FP8_DTYPE", "read_status", "MoeKernelError", "topk_softmax",
     "topk_sigmoid", "router_gemm", "fp32_router_gemm", "supports_fp32_router_gemm", "router_gemm_grouped_topk",
-    "silu_and_mul", "silu_and_mul_out",
+    "silu_and_mul", "silu_and_mul_out", "rms_norm", "fused_add_rms_norm", "rms_norm_quant", "moe_balance_loss",
 ]

@@ -89,6 +89,18 @@ SYMBOLS = {
                           c_void_p]),
     "moe_silu_and_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
     "moe_silu_and_mul_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
+    "moe_rms_norm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int64, c_int64, c_float, c_void_p,
+                             c_int64, c_void_p, c_int64, c_void_p]),
+    "moe_rms_norm_quant": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int64, c_int64, c_float, c_int,
+                                   c_int, c_float, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "moe_rms_norm_grad_workspace": (c_int, [c_int64, c_int64, c_void_p]),
+    "moe_rms_norm_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int64, c_int64, c_float,
+                                  c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "moe_balance_loss_workspace": (c_int, [c_int64, c_int, c_int, c_int, c_void_p]),
+    "moe_balance_loss": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "moe_balance_loss_grad": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p]),
     "moe_sum_ld": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int64, c_void_p, c_int, c_int, c_void_p,
                            c_void_p, c_void_p]),
 }
@@ -131,6 +143,7 @@ def host():
         except ImportError as e:
             raise RuntimeError(f"{os.path.join(HERE, '_host_ext.so')} has not been built or does not load ({e}); "
                                "run `python -m flaggems_vllm_b200.build`.") from None
+        _host_ext.set_error(MoeKernelError)
         _host = _host_ext
     return _host
 

@@ -19,7 +19,8 @@ LIB = os.path.join(HERE, "libmoe_sm100.so")
 HOST_EXT = os.path.join(HERE, "_host_ext.so")
 STAMP = LIB + ".srchash"
 SOURCES = ["common.cu", "grouped_topk.cu", "topk_route.cu", "align.cu", "quant.cu", "gemm_simt.cu", "gemm_tc.cu",
-           "gemm_wt.cu", "gemm_w8t.cu", "plan.cu", "route_rows.cu", "layer.cu", "gemm_w8.cu", "gemm_small.cu", "gemm_api.cu", "router_gemm.cu", "ep_pack.cu"]
+           "gemm_wt.cu", "gemm_w8t.cu", "plan.cu", "route_rows.cu", "layer.cu", "gemm_w8.cu", "gemm_small.cu", "gemm_api.cu", "router_gemm.cu", "ep_pack.cu",
+           "rms_norm.cu", "balance.cu"]
 
 
 def _nvcc() -> str:

@@ -2,19 +2,24 @@
 // each.  A decode-sized layer spends a few microseconds per kernel on the device; checked and launched from Python
 // it cost the host 85 us, most of it interpreter time.
 //
-// Every function here serves the usual types, layouts and options and returns None for anything else (and for
-// every error): the Python operator then goes its own way, which serves the rest and raises the errors.  Nothing
-// is kept between calls.
+// Every function here serves the usual types, layouts and options and returns None for anything else (and, but for the
+// operators with gradients below, for every error): the Python operator then goes its own way, which serves the rest
+// and raises the errors.  Nothing is kept between calls.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
 #include <Python.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <optional>
+#include <stdexcept>
 
 #include "../../include/moe_sm100.h"
 
@@ -304,6 +309,374 @@ PyObject* align(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Operators with gradients: norm of the residual stream, balance loss.  One implementation for every caller: what is not
+// served here (None) the Python operator brings into one of these layouts, or refuses, and calls again.  Errors are raised.
+
+PyObject* g_error = nullptr;  // _lib.MoeKernelError
+struct KernelError : std::runtime_error { using std::runtime_error::runtime_error; };
+void must(int rc) {
+  if (rc != 0) throw KernelError(std::string(moe_last_error()) + " (code " + std::to_string(rc) + ")");
+}
+
+PyObject* set_error(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1) MOE_NONE;
+  Py_INCREF(a[0]);
+  g_error = a[0];  // lives as long as the module
+  MOE_NONE;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Rows of the last dimension and how far apart they are; false where that is no single distance.
+bool rows_of(const at::Tensor& t, int64_t* rows, int64_t* ld) {
+  if (t.dim() < 1) return false;
+  const int64_t H = t.size(-1);
+  *rows = H == 0 ? 0 : t.numel() / H;
+  *ld = H;
+  if (t.is_contiguous()) return true;
+  if (t.dim() != 2 || t.stride(1) != 1 || t.stride(0) < 0) return false;
+  *ld = t.stride(0);
+  return true;
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// Gradients that a second differentiation would go through end in an error there, not in silence.
+variable_list once(variable_list grads, const char* who) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list with;
+  for (at::Tensor& g : grads)
+    if (g.defined()) with.push_back(g.detach().requires_grad_(true));
+  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(who) + " is differentiable once", (int64_t)with.size());
+  with = (*error)(std::move(with));
+  size_t i = 0;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = with[i++];
+  return grads;
+}
+
+cudaStream_t stream_on(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+
+struct NormArgs {
+  int code, weight_code, dev;
+  int64_t rows, cols, x_ld, residual_ld;
+};
+bool norm_args(const at::Tensor& x, const at::Tensor& w, const at::Tensor* residual, NormArgs* p) {
+  if (!x.is_cuda() || x.dim() < 1 || w.dim() != 1) return false;
+  p->dev = x.get_device();
+  p->code = float_code(x);
+  p->weight_code = float_code(w);
+  p->cols = x.size(-1);
+  p->residual_ld = 0;
+  if (p->code < 0 || (p->weight_code != p->code && p->weight_code != MOE_F32) || !cuda_dense(w, p->dev) || w.size(0) != p->cols ||
+      p->cols <= 0 || p->cols > (1 << 24) || !rows_of(x, &p->rows, &p->x_ld) || p->rows > 0x7FFFFFFF)
+    return false;
+  int64_t rows;
+  return !residual || (residual->is_cuda() && residual->get_device() == p->dev && residual->scalar_type() == x.scalar_type() &&
+                       residual->sizes().equals(x.sizes()) && rows_of(*residual, &rows, &p->residual_ld));
+}
+
+// y, and h where there is a residual
+std::pair<at::Tensor, at::Tensor> norm_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor* residual, double eps,
+                                               const NormArgs& p) {
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
+  at::Tensor y = at::empty(x.sizes(), x.options()), h;
+  if (residual) h = at::empty(x.sizes(), x.options());
+  must(moe_rms_norm(x.const_data_ptr(), p.x_ld, residual ? residual->const_data_ptr() : nullptr, p.residual_ld, w.const_data_ptr(), p.code,
+                    p.weight_code, p.rows, p.cols, (float)eps, y.mutable_data_ptr(), p.cols, residual ? h.mutable_data_ptr() : nullptr,
+                    p.cols, stream_on(p.dev)));
+  return {y, h};
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& residual,
+                               double eps) {
+    NormArgs p;
+    const at::Tensor* r = residual ? &*residual : nullptr;
+    if (!norm_args(x, w, r, &p)) throw KernelError("rms_norm: unsupported operands");
+    auto [y, h] = norm_forward(x, w, r, eps, p);
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["residual"] = r != nullptr;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({r ? h : x, w});
+    if (r) return {y, h};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const bool has_residual = ctx->saved_data["residual"].toBool();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    at::Tensor h = saved[0];
+    const at::Tensor& w = saved[1];
+    const at::Tensor dy = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
+    const at::Tensor dh = has_residual && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
+    const bool want_w = ctx->needs_input_grad(1);
+    const bool want_x = ctx->needs_input_grad(0) || (has_residual && ctx->needs_input_grad(2));
+    variable_list out(4);
+    if (!dy.defined()) {  // only the stream was used: its gradient passes through
+      if (want_x && dh.defined()) out[0] = dh;
+      if (has_residual) out[2] = out[0];
+      return once(out, "rms_norm");
+    }
+    NormArgs p;
+    if (!norm_args(h, w, nullptr, &p)) {  // a hook may have handed back another layout
+      h = h.contiguous();
+      if (!norm_args(h, w, nullptr, &p)) throw KernelError("rms_norm: unsupported operands in the backward pass");
+    }
+    {
+      at::AutoDispatchBelowADInplaceOrView below;  // the buffers are no part of a graph
+      c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
+      at::Tensor dx, dw, ws;
+      int64_t bytes = 0;
+      if (want_x) dx = at::empty(h.sizes(), h.options());
+      if (want_w) {
+        dw = at::empty(w.sizes(), w.options());
+        must(moe_rms_norm_grad_workspace(p.rows, p.cols, &bytes));
+        ws = bytes_on(bytes, h);
+      }
+      if (want_x || want_w)
+        must(moe_rms_norm_grad(dy.const_data_ptr(), dh.defined() ? dh.const_data_ptr() : nullptr, h.const_data_ptr(), p.x_ld,
+                               w.const_data_ptr(), p.code, p.weight_code, p.rows, p.cols, (float)eps,
+                               want_x ? dx.mutable_data_ptr() : nullptr, want_w ? dw.mutable_data_ptr() : nullptr,
+                               want_w ? ws.mutable_data_ptr() : nullptr, bytes, stream_on(p.dev)));
+      out[0] = dx;
+      out[1] = dw;
+      if (has_residual) out[2] = dx;  // d h / d x = d h / d residual = 1
+    }
+    return once(out, "rms_norm");
+  }
+};
+
+// rms_norm(x, weight, eps, residual) -> y, or (y, h) with a residual
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double eps;
+  if (n != 4 || !is_tensor(a[0]) || !is_tensor(a[1]) || !as_double(a[2], &eps) || (a[3] != Py_None && !is_tensor(a[3]))) MOE_NONE;
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]);
+  const at::Tensor* residual = a[3] == Py_None ? nullptr : &tensor(a[3]);
+  NormArgs p;
+  if (!(eps >= 0.0 && eps < 3e38) || !norm_args(x, w, residual, &p)) MOE_NONE;
+  at::Tensor y, h;
+  {
+    Unlocked unlocked;
+    if (wants_grad({&x, &w, residual})) {
+      const variable_list out = RmsNorm::apply(x, w, residual ? std::optional<at::Tensor>(*residual) : std::nullopt, eps);
+      y = out[0];
+      if (residual) h = out[1];
+    } else {
+      std::tie(y, h) = norm_forward(x, w, residual, eps, p);
+    }
+  }
+  if (!residual) return THPVariable_Wrap(y);
+  PyObject* r = PyTuple_New(2);
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(y));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(h));
+  return r;
+}
+
+// fused_add_rms_norm(x, residual, weight, eps) -> True when done, in place (the caller has looked at overlaps)
+PyObject* fused_add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double eps;
+  if (n != 4 || !is_tensor(a[0]) || !is_tensor(a[1]) || !is_tensor(a[2]) || !as_double(a[3], &eps)) MOE_NONE;
+  const at::Tensor &x = tensor(a[0]), &residual = tensor(a[1]), &w = tensor(a[2]);
+  NormArgs p;
+  if (!(eps >= 0.0 && eps < 3e38) || !norm_args(x, w, &residual, &p) || wants_grad({&x, &residual, &w})) MOE_NONE;
+  if (p.rows > 1 && (p.x_ld < p.cols || p.residual_ld < p.cols)) MOE_NONE;
+  const char *x0 = (const char*)x.const_data_ptr(), *r0 = (const char*)residual.const_data_ptr();
+  const int64_t size = x.element_size(), x_bytes = ((p.rows - 1) * p.x_ld + p.cols) * size, r_bytes = ((p.rows - 1) * p.residual_ld + p.cols) * size;
+  if (p.rows > 0 && x0 < r0 + r_bytes && r0 < x0 + x_bytes) MOE_NONE;  // the two share memory
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
+    must(moe_rms_norm(x.const_data_ptr(), p.x_ld, residual.const_data_ptr(), p.residual_ld, w.const_data_ptr(), p.code, p.weight_code, p.rows,
+                      p.cols, (float)eps, x.mutable_data_ptr(), p.x_ld, residual.mutable_data_ptr(), p.residual_ld, stream_on(p.dev)));
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+    if (!residual.is_inference()) residual.unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_TRUE;
+}
+
+// rms_norm_quant(x, weight, eps, residual, group, format, quant_eps, scale_flags, return_norm) -> (q, scales, h?, y?)
+PyObject* rms_norm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double eps, quant_eps;
+  long long group, format, flags;
+  if (n != 9 || !is_tensor(a[0]) || !is_tensor(a[1]) || !as_double(a[2], &eps) || (a[3] != Py_None && !is_tensor(a[3])) ||
+      !as_int(a[4], &group) || !as_int(a[5], &format) || !as_double(a[6], &quant_eps) || !as_int(a[7], &flags) || !plain_bool(a[8]))
+    MOE_NONE;
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]);
+  const at::Tensor* residual = a[3] == Py_None ? nullptr : &tensor(a[3]);
+  NormArgs p;
+  if (!(eps >= 0.0 && eps < 3e38) || !(quant_eps >= 0.0 && quant_eps < 3e38) || !norm_args(x, w, residual, &p) ||
+      wants_grad({&x, &w, residual}))
+    MOE_NONE;
+  if (group == 0) group = p.cols;
+  if (group < 0 || p.cols % group != 0 || format < 0 || format > 2 || flags < 0 || flags > 3 || ((flags & 2) && format == 2) ||
+      ((flags & 1) && x.dim() != 2))
+    MOE_NONE;
+  const int64_t groups = p.cols / group;
+  at::Tensor q, s, y, h;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
+    q = at::empty(x.sizes(), x.options().dtype(format == 0 ? at::kFloat8_e4m3fn : format == 1 ? at::kFloat8_e5m2 : at::kChar));
+    if (flags & 1) {
+      s = at::empty({groups, p.rows}, x.options().dtype(at::kFloat));
+    } else {
+      at::DimVector shape(x.sizes().begin(), x.sizes().end());
+      shape.back() = groups;
+      s = at::empty(shape, x.options().dtype(at::kFloat));
+    }
+    if (residual) h = at::empty(x.sizes(), x.options());
+    if (truth(a[8])) y = at::empty(x.sizes(), x.options());
+    must(moe_rms_norm_quant(x.const_data_ptr(), p.x_ld, residual ? residual->const_data_ptr() : nullptr, p.residual_ld, w.const_data_ptr(),
+                            p.code, p.weight_code, p.rows, p.cols, (float)eps, (int)format, (int)group, (float)quant_eps, (int)flags,
+                            q.mutable_data_ptr(), s.mutable_data_ptr<float>(), p.rows, y.defined() ? y.mutable_data_ptr() : nullptr,
+                            residual ? h.mutable_data_ptr() : nullptr, stream_on(p.dev)));
+    if (flags & 1) s = s.t();
+  }
+  PyObject* r = PyTuple_New(2 + (residual != nullptr) + y.defined());
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(q));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(s));
+  if (residual) PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(h));
+  if (y.defined()) PyTuple_SET_ITEM(r, 2 + (residual != nullptr), THPVariable_Wrap(y));
+  return r;
+}
+
+struct BalanceArgs {
+  int code, dev, sequences;
+  int64_t tokens, experts, topk, ld;
+  bool ids64;
+  int32_t* status;
+};
+bool balance_args(const at::Tensor& l, const at::Tensor& ids, const at::Tensor* cu, const at::Tensor* pad, BalanceArgs* p) {
+  if (!l.is_cuda() || l.dim() != 2 || ids.dim() != 2) return false;
+  p->dev = l.get_device();
+  p->code = float_code(l);
+  p->experts = l.size(1);
+  p->topk = ids.size(1);
+  p->ids64 = ids.scalar_type() == at::kLong;
+  p->status = status_of(p->dev);
+  p->sequences = 1;
+  if (p->code < 0 || !p->status || p->experts <= 0 || p->experts > 1024 || p->topk <= 0 || p->topk > 32 || !cuda_dense(ids, p->dev) ||
+      (!p->ids64 && ids.scalar_type() != at::kInt) || !rows_of(l, &p->tokens, &p->ld) || ids.size(0) != p->tokens ||
+      p->tokens * p->topk > 0x7FFFFFFF)
+    return false;
+  if (cu) {
+    if (!cuda_dense(*cu, p->dev) || cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->numel() < 2 || cu->numel() > 65536) return false;
+    p->sequences = (int)cu->numel() - 1;
+  }
+  return !pad || (cuda_dense(*pad, p->dev) && pad->scalar_type() == at::kBool && pad->dim() == 1 && pad->numel() == p->tokens);
+}
+
+const int32_t* cu_pointer(const at::Tensor* cu) { return cu ? cu->const_data_ptr<int32_t>() : nullptr; }
+const uint8_t* pad_pointer(const at::Tensor* pad) { return pad ? (const uint8_t*)pad->const_data_ptr() : nullptr; }
+
+// loss, counts, and what the gradient needs
+std::array<at::Tensor, 3> balance_forward(const at::Tensor& l, const at::Tensor& ids, const at::Tensor* cu, const at::Tensor* pad,
+                                          bool sigmoid, const BalanceArgs& p) {
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
+  int64_t bytes[2];
+  must(moe_balance_loss_workspace(p.tokens, (int)p.experts, (int)p.topk, p.sequences, bytes));
+  const auto ints = l.options().dtype(at::kInt);
+  at::Tensor loss = at::empty({}, l.options().dtype(at::kFloat));
+  at::Tensor counts = cu ? at::empty({p.sequences, p.experts}, ints) : at::empty({p.experts}, ints);
+  at::Tensor saved = bytes_on(bytes[1], l), ws = bytes_on(bytes[0], l);
+  must(moe_balance_loss(l.const_data_ptr(), p.ld, p.code, p.tokens, (int)p.experts, ids.const_data_ptr(), p.ids64, (int)p.topk, sigmoid,
+                        cu_pointer(cu), p.sequences, pad_pointer(pad), loss.mutable_data_ptr<float>(), counts.mutable_data_ptr<int32_t>(),
+                        saved.mutable_data_ptr(), ws.mutable_data_ptr(), bytes[0], p.status, stream_on(p.dev)));
+  return {loss, counts, saved};
+}
+
+struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& l, const at::Tensor& ids, const std::optional<at::Tensor>& cu,
+                               const std::optional<at::Tensor>& pad, bool sigmoid) {
+    BalanceArgs p;
+    const at::Tensor *c = cu ? &*cu : nullptr, *m = pad ? &*pad : nullptr;
+    if (!balance_args(l, ids, c, m, &p)) throw KernelError("moe_balance_loss: unsupported operands");
+    auto out = balance_forward(l, ids, c, m, sigmoid, p);
+    ctx->save_for_backward({l, out[2], c ? *c : at::Tensor(), m ? *m : at::Tensor()});
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["topk"] = p.topk;
+    ctx->saved_data["sequences"] = (int64_t)p.sequences;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out[1]});
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    at::Tensor l = saved[0];
+    const at::Tensor *cu = saved[2].defined() ? &saved[2] : nullptr, *pad = saved[3].defined() ? &saved[3] : nullptr;
+    int64_t tokens, ld;
+    if (!rows_of(l, &tokens, &ld)) {
+      l = l.contiguous();
+      rows_of(l, &tokens, &ld);
+    }
+    const at::Tensor dloss = grads[0].to(at::kFloat).contiguous();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const int dev = l.get_device();
+      c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+      out[0] = at::empty(l.sizes(), l.options());
+      must(moe_balance_loss_grad(l.const_data_ptr(), ld, float_code(l), tokens, (int)l.size(1), (int)ctx->saved_data["topk"].toInt(),
+                                 ctx->saved_data["sigmoid"].toBool(), cu_pointer(cu), (int)ctx->saved_data["sequences"].toInt(),
+                                 pad_pointer(pad), saved[1].const_data_ptr(), dloss.const_data_ptr<float>(), out[0].mutable_data_ptr(),
+                                 stream_on(dev)));
+    }
+    return once(out, "moe_balance_loss");
+  }
+};
+
+// balance_loss(logits, topk_ids, sigmoid, cu_seqlens, is_padding) -> (loss, counts)
+PyObject* balance_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5 || !is_tensor(a[0]) || !is_tensor(a[1]) || !plain_bool(a[2]) || (a[3] != Py_None && !is_tensor(a[3])) ||
+      (a[4] != Py_None && !is_tensor(a[4])))
+    MOE_NONE;
+  const at::Tensor &l = tensor(a[0]), &ids = tensor(a[1]);
+  const at::Tensor *cu = a[3] == Py_None ? nullptr : &tensor(a[3]), *pad = a[4] == Py_None ? nullptr : &tensor(a[4]);
+  BalanceArgs p;
+  if (!balance_args(l, ids, cu, pad, &p)) MOE_NONE;
+  const bool sigmoid = truth(a[2]);
+  at::Tensor loss, counts;
+  {
+    Unlocked unlocked;
+    if (wants_grad({&l})) {
+      const variable_list out = BalanceLoss::apply(l, ids, cu ? std::optional<at::Tensor>(*cu) : std::nullopt,
+                                                   pad ? std::optional<at::Tensor>(*pad) : std::nullopt, sigmoid);
+      loss = out[0];
+      counts = out[1];
+    } else {
+      auto out = balance_forward(l, ids, cu, pad, sigmoid, p);
+      loss = out[0];
+      counts = out[1];
+    }
+  }
+  PyObject* r = PyTuple_New(2);
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(loss));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(counts));
+  return r;
+}
+
+// Exceptions of the operators above become Python's: a failed launch MoeKernelError, torch's own as torch raises them.
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* raising(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    return F(self, a, n);
+  } catch (const KernelError& e) {
+    PyErr_SetString(g_error ? g_error : PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 // No C++ exception crosses into the interpreter (an allocation can throw): it becomes the Python path's problem.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -315,8 +688,10 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define MOE_FN(name) {#name, (PyCFunction)(void (*)(void))guarded<name>, METH_FASTCALL, nullptr}
+#define MOE_OP(name) {#name, (PyCFunction)(void (*)(void))raising<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MOE_FN(set_status), MOE_FN(fused_experts), MOE_FN(grouped_topk), MOE_FN(topk_route),
-                         MOE_FN(router_gemm), MOE_FN(align), {nullptr, nullptr, 0, nullptr}};
+                         MOE_FN(router_gemm), MOE_FN(align), MOE_FN(set_error), MOE_OP(rms_norm), MOE_OP(fused_add_rms_norm),
+                         MOE_OP(rms_norm_quant), MOE_OP(balance_loss), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ext", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

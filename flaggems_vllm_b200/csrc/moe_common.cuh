@@ -108,6 +108,21 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return (g / (1.0f + expf(-g))) * u;
 }
 
+// v / s, correctly rounded, for |v| <= 448 s (1 + ulp) from the rounded reciprocal of s: one correction step by the exact
+// remainder (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990).  Where the quotient is
+// so small that the remainder is not exact it rounds to zero in e4m3 all the same: over every pair of finite bf16 or f16
+// values (amax, |v| <= amax) the e4m3 bytes are those of the division.  The sign is v's, of a zero too.
+__device__ __forceinline__ float div_by_scale(float v, float s, float inv) {
+  const float q = v * inv;
+  return copysignf(fmaf(fmaf(-q, s, v), inv, q), v);
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 __device__ __forceinline__ void set_status(int32_t* status, int bit) {
   if (status != nullptr) atomicOr(status, bit);
 }

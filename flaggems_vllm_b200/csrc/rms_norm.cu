@@ -1,0 +1,642 @@
+// Root-mean-square norm of the residual stream, with the residual's addition in front of it, an 8-bit output behind it, and
+// its gradient.
+//
+//   h = round(x + residual)          the stream as it is stored (h = x without a residual)
+//   r = 1 / sqrt(mean(h^2) + eps),  y_i = w_i h_i r
+//   quantised: s = max(amax |y|, quant_eps) / qmax per group of a row or per row,  q = round(y / s)
+//   dh_i = r (w_i dy_i - h_i r^2 mean(w dy h)) + (gradient that reaches the stream directly),  dw_i = sum over rows dy_i h_i r
+//
+// The norm is that of the rounded h, not of the sum in fp32: what the next layer adds to is what was normed, and the
+// gradient, which has only h, is that of the same function.  y itself is rounded once: the quantiser takes its fp32 value.
+// The gradient computes r again (the row is in registers anyway), so nothing but h is kept between the two passes.
+//
+// Bound: memory.  A row is read once: it stays in the registers of the threads that share it.
+#include "moe_common.cuh"
+
+namespace moe {
+namespace {
+
+// V consecutive elements that one thread moves at once: 16 bytes, or a single element where rows are not made of such pieces.
+template <typename T, int V> struct Piece {
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
+  __device__ __forceinline__ void clear() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ float get(int i) const { return ToF32<T>::get(reinterpret_cast<const T*>(&raw)[i]); }
+  __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+};
+template <typename T> struct Piece<T, 1> {
+  T raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = raw; }
+  __device__ __forceinline__ void clear() { raw = from_f32<T>(0.0f); }
+  __device__ __forceinline__ float get(int) const { return ToF32<T>::get(raw); }
+  __device__ __forceinline__ void set(int, float v) { raw = from_f32<T>(v); }
+};
+
+// The V weights from element `at` on; the weight has the type of the rows or is fp32.
+template <typename T, int V>
+__device__ __forceinline__ void load_weight(const void* w, bool w_f32, int at, float (&v)[V]) {
+  if (w_f32) {
+    const float* p = reinterpret_cast<const float*>(w) + at;
+    if constexpr (V == 1) {
+      v[0] = *p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p + i);
+        v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+      }
+    }
+  } else {
+    Piece<T, V> p;
+    p.load(reinterpret_cast<const T*>(w) + at);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = p.get(i);
+  }
+}
+
+struct Sum { static __device__ __forceinline__ float join(float a, float b) { return a + b; } };
+struct Max { static __device__ __forceinline__ float join(float a, float b) { return max_nan(a, b); } };
+
+// N values joined over the TPR threads of a row; every thread gets the same bits (fixed order).  `sh` holds N floats per
+// warp of the block; a caller that comes again puts a barrier between.
+template <class Op, int N, int TPR>
+__device__ __forceinline__ void join_row(float (&v)[N], float* sh) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = Op::join(v[n], __shfl_xor_sync(0xFFFFFFFFu, v[n], off));
+  if constexpr (TPR > 32) {
+    const int warp = threadIdx.x >> 5, first = warp / (TPR / 32) * (TPR / 32);
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int n = 0; n < N; ++n) sh[warp * N + n] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = sh[first * N + n];
+#pragma unroll
+    for (int i = 1; i < TPR / 32; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] = Op::join(v[n], sh[(first + i) * N + n]);
+  }
+}
+
+enum { kE4M3 = 0, kE5M2 = 1, kInt8 = 2 };
+__device__ __forceinline__ float quant_max(int format) { return format == kE4M3 ? 448.0f : format == kE5M2 ? 57344.0f : 127.0f; }
+
+// The scale of a group from its largest magnitude.  A NaN in the group makes the scale NaN, as it makes the values it stands for.
+__device__ __forceinline__ float group_scale(float amax, float eps, int format, bool ue8m0) {
+  float s = max_nan(amax, eps) * (1.0f / quant_max(format));
+  if (ue8m0 && s < INFINITY) {  // the smallest power of two that is not below it
+    s = fmaxf(s, 1e-10f);
+    const uint32_t b = __float_as_uint(s);
+    s = __uint_as_float((b + 0x7FFFFFu) & 0x7F800000u);
+  }
+  return s;
+}
+
+__device__ __forceinline__ uint8_t to_8bit(float v, int format) {  // fp8 conversions saturate and keep NaN
+  if (format == kE4M3) return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+  if (format == kE5M2) return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E5M2);
+  return (uint8_t)(int8_t)max(-128, min(127, __float2int_rn(v)));  // NaN gives 0; its scale is NaN
+}
+
+// V quotients of one piece as bytes.
+template <int V>
+__device__ __forceinline__ void quantise(const float (&y)[V], float s, int format, uint8_t* dst) {
+  const bool plain = s > 1e-30f && s < 1e30f;  // where the reciprocal and its remainders stay normal numbers
+  const float inv = 1.0f / s;
+  float d[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) d[i] = plain ? div_by_scale(y[i], s, inv) : y[i] / s;
+  uint32_t w[(V + 3) / 4] = {};
+  if (format == kE4M3 && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i + 1 < V; i += 2)
+      w[i / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(d[i], d[i + 1]), __NV_SATFINITE, __NV_E4M3) << (8 * (i & 3));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i / 4] |= (uint32_t)to_8bit(d[i], format) << (8 * (i & 3));
+  }
+  if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+  else *dst = (uint8_t)w[0];
+}
+
+struct Forward {
+  const void *x, *residual, *weight;  // residual: null = none
+  void *y, *h;                        // y: null = not wanted; h: null without a residual
+  int64_t x_ld, residual_ld, y_ld, h_ld, rows;
+  int cols, w_f32;
+  float eps;
+  // 8-bit output
+  uint8_t* q;
+  float* scales;
+  int64_t scale_ld;  // of the transposed layout
+  int group, format, transposed, ue8m0;
+  float quant_eps;
+};
+
+__device__ __forceinline__ float* scale_at(const Forward& p, int64_t row, int group_index) {
+  return p.transposed ? p.scales + (int64_t)group_index * p.scale_ld + row
+                      : p.scales + row * (p.cols / p.group) + group_index;
+}
+
+// One row per TPR threads, kept in registers: CH pieces of V elements per thread.  x and y (residual and h) may be the same
+// memory: a thread has read its pieces before it writes them, and nobody else reads them.
+template <typename T, int V, int TPR, int CH, bool QUANT, int BLOCK = (TPR > 128 ? TPR : 128)>
+__global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sh[2][BLOCK / 32];
+  const int t = threadIdx.x % TPR, pieces = p.cols / V;
+  const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+  if (TPR <= 32 && row >= p.rows) return;  // wider rows fill their block, and the grid has no block too many
+  Piece<T, V> h[CH];
+  {
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_ld;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      h[c].clear();
+      if (t + c * TPR < pieces) h[c].load(x + (t + c * TPR) * V);
+    }
+    if (p.residual != nullptr) {
+      const T* r = reinterpret_cast<const T*>(p.residual) + row * p.residual_ld;
+      Piece<T, V> a[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        a[c].clear();
+        if (t + c * TPR < pieces) a[c].load(r + (t + c * TPR) * V);
+      }
+      T* out = reinterpret_cast<T*>(p.h) + row * p.h_ld;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[c].set(i, h[c].get(i) + a[c].get(i));
+        if (t + c * TPR < pieces) h[c].store(out + (t + c * TPR) * V);
+      }
+    }
+  }
+  float ss[1] = {0.0f};
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) ss[0] = fmaf(h[c].get(i), h[c].get(i), ss[0]);
+  join_row<Sum, 1, TPR>(ss, sh[0]);
+  const float inv = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps);
+  if constexpr (!QUANT) {
+    T* out = reinterpret_cast<T*>(p.y) + row * p.y_ld;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (t + c * TPR < pieces) {
+        float w[V];
+        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[c].set(i, h[c].get(i) * inv * w[i]);
+        h[c].store(out + (t + c * TPR) * V);
+      }
+    }
+  } else {
+    float y[CH][V], amax[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      amax[c] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[c][i] = 0.0f;
+      if (t + c * TPR < pieces) {
+        float w[V];
+        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          y[c][i] = h[c].get(i) * inv * w[i];
+          amax[c] = max_nan(amax[c], fabsf(y[c][i]));
+        }
+        if (p.y != nullptr) {
+          Piece<T, V> o;
+#pragma unroll
+          for (int i = 0; i < V; ++i) o.set(i, y[c][i]);
+          o.store(reinterpret_cast<T*>(p.y) + row * p.y_ld + (t + c * TPR) * V);
+        }
+      }
+    }
+    uint8_t* q = p.q + row * p.cols;
+    if (p.group == p.cols) {
+      float m[1] = {amax[0]};
+#pragma unroll
+      for (int c = 1; c < CH; ++c) m[0] = max_nan(m[0], amax[c]);
+      join_row<Max, 1, TPR>(m, sh[1]);
+      const float s = group_scale(m[0], p.quant_eps, p.format, p.ue8m0);
+      if (t == 0) *scale_at(p, row, 0) = s;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (t + c * TPR < pieces) quantise<V>(y[c], s, p.format, q + (t + c * TPR) * V);
+    } else {
+      const int lanes = p.group / V;  // a power of two up to 32: the pieces of a group lie in one warp
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        float m = amax[c];
+        for (int off = lanes / 2; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+        const int piece = t + c * TPR;
+        if (piece < pieces) {
+          const float s = group_scale(m, p.quant_eps, p.format, p.ue8m0);
+          if (piece % lanes == 0) *scale_at(p, row, piece / lanes) = s;
+          quantise<V>(y[c], s, p.format, q + piece * V);
+        }
+      }
+    }
+  }
+}
+
+// Any row length, alignment and group: a block per row, which is read again instead of kept.
+template <typename T>
+__global__ void __launch_bounds__(256) rms_norm_any_kernel(const Forward p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sh[2][8];
+  const int64_t row = blockIdx.x;
+  const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_ld;
+  const T* src = x;
+  float ss[1] = {0.0f};
+  if (p.residual != nullptr) {
+    const T* r = reinterpret_cast<const T*>(p.residual) + row * p.residual_ld;
+    T* out = reinterpret_cast<T*>(p.h) + row * p.h_ld;
+    for (int i = threadIdx.x; i < p.cols; i += 256) {
+      const T v = from_f32<T>(ToF32<T>::get(x[i]) + ToF32<T>::get(r[i]));
+      out[i] = v;
+      ss[0] = fmaf(ToF32<T>::get(v), ToF32<T>::get(v), ss[0]);
+    }
+    src = out;
+  } else {
+    for (int i = threadIdx.x; i < p.cols; i += 256) ss[0] = fmaf(ToF32<T>::get(x[i]), ToF32<T>::get(x[i]), ss[0]);
+  }
+  join_row<Sum, 1, 256>(ss, sh[0]);  // its barrier also makes h visible to the block
+  const float inv = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps);
+  auto norm = [&](int i) {
+    const float w = p.w_f32 ? reinterpret_cast<const float*>(p.weight)[i] : ToF32<T>::get(reinterpret_cast<const T*>(p.weight)[i]);
+    return ToF32<T>::get(src[i]) * inv * w;
+  };
+  if (p.q != nullptr) {
+    uint8_t* q = p.q + row * p.cols;
+    if (p.group == p.cols) {
+      float m[1] = {0.0f};
+      for (int i = threadIdx.x; i < p.cols; i += 256) m[0] = max_nan(m[0], fabsf(norm(i)));
+      join_row<Max, 1, 256>(m, sh[1]);
+      const float s = group_scale(m[0], p.quant_eps, p.format, p.ue8m0);
+      if (threadIdx.x == 0) *scale_at(p, row, 0) = s;
+      for (int i = threadIdx.x; i < p.cols; i += 256) q[i] = to_8bit(norm(i) / s, p.format);
+    } else {  // a warp per group
+      const int lane = threadIdx.x & 31;
+      for (int g = threadIdx.x >> 5; g < p.cols / p.group; g += 8) {
+        float m[1] = {0.0f};
+        for (int i = lane; i < p.group; i += 32) m[0] = max_nan(m[0], fabsf(norm(g * p.group + i)));
+        join_row<Max, 1, 32>(m, nullptr);
+        const float s = group_scale(m[0], p.quant_eps, p.format, p.ue8m0);
+        if (lane == 0) *scale_at(p, row, g) = s;
+        for (int i = lane; i < p.group; i += 32) q[g * p.group + i] = to_8bit(norm(g * p.group + i) / s, p.format);
+      }
+    }
+  }
+  // y may lie over x, which nothing reads once there is an h, and without an h (no residual) y is memory of its own
+  if (p.y != nullptr) {
+    T* y = reinterpret_cast<T*>(p.y) + row * p.y_ld;
+    for (int i = threadIdx.x; i < p.cols; i += 256) y[i] = from_f32<T>(norm(i));
+  }
+}
+
+struct Backward {
+  const void *dy, *dh, *h, *weight;  // dh: null = none
+  void *dx;                          // null = not wanted
+  float* partial;                    // [blocks, cols] sums of dw; null = not wanted
+  int64_t h_ld, rows;
+  int cols, w_f32;
+  float eps;
+};
+
+// Rows dealt out to the blocks in turn; a thread keeps its columns' part of dw in registers over all of them.
+template <typename T, int V, int TPR, int CH, int BLOCK = (TPR > 128 ? TPR : 128)>
+__global__ void __launch_bounds__(BLOCK) rms_norm_grad_kernel(const Backward p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int RPB = BLOCK / TPR;
+  __shared__ float sh[2][BLOCK / 32 * 2];
+  const int t = threadIdx.x % TPR, pieces = p.cols / V;
+  float dw[CH][V];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[c][i] = 0.0f;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB, turn ^= 1) {
+    Piece<T, V> h[CH], g[CH], d[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      h[c].clear(); g[c].clear();
+      if (t + c * TPR < pieces) {
+        h[c].load(reinterpret_cast<const T*>(p.h) + row * p.h_ld + (t + c * TPR) * V);
+        g[c].load(reinterpret_cast<const T*>(p.dy) + row * p.cols + (t + c * TPR) * V);
+      }
+    }
+    if (p.dh != nullptr && p.dx != nullptr) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (t + c * TPR < pieces) d[c].load(reinterpret_cast<const T*>(p.dh) + row * p.cols + (t + c * TPR) * V);
+    }
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (t + c * TPR < pieces) {
+        float w[V];
+        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          s[0] = fmaf(h[c].get(i), h[c].get(i), s[0]);
+          s[1] = fmaf(w[i] * g[c].get(i), h[c].get(i), s[1]);
+        }
+      }
+    }
+    join_row<Sum, 2, TPR>(s, sh[turn]);  // the other half is still read by threads that are a row behind
+    const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
+    const float k = inv * inv * (s[1] / (float)p.cols);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (t + c * TPR < pieces) {
+        float w[V];
+        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
+        Piece<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float hv = h[c].get(i), gv = g[c].get(i);
+          dw[c][i] = fmaf(gv, hv * inv, dw[c][i]);
+          float v = inv * (w[i] * gv - hv * k);
+          if (p.dh != nullptr && p.dx != nullptr) v += d[c].get(i);
+          o.set(i, v);
+        }
+        if (p.dx != nullptr) o.store(reinterpret_cast<T*>(p.dx) + row * p.cols + (t + c * TPR) * V);
+      }
+    }
+  }
+  if (p.partial == nullptr) return;
+  if constexpr (RPB > 1) {  // several rows at a time: their threads' sums meet in shared memory, in order
+    __shared__ float acc[TPR * CH * V];
+    for (int r = 0; r < RPB; ++r) {
+      if ((int)threadIdx.x / TPR == r) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float* a = acc + (t + c * TPR) * V + i;
+            *a = r == 0 ? dw[c][i] : *a + dw[c][i];
+          }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < p.cols; i += BLOCK) p.partial[(int64_t)blockIdx.x * p.cols + i] = acc[i];
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (t + c * TPR < pieces) p.partial[(int64_t)blockIdx.x * p.cols + (t + c * TPR) * V + i] = dw[c][i];
+  }
+}
+
+// dw[col] = sum over the blocks' partial sums, in order: 32 columns per block, 32 threads to a column.
+template <typename W>
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int parts, int cols, W* __restrict__ dw) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sh[32][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+  float s = 0.0f;
+  if (col < cols) {
+#pragma unroll 4
+    for (int i = r; i < parts; i += 32) s += partial[(int64_t)i * cols + col];
+  }
+  sh[r][threadIdx.x & 31] = s;
+  __syncthreads();
+  s = sh[threadIdx.x & 31][r];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, off);
+  const int out = blockIdx.x * 32 + r;
+  if ((threadIdx.x & 31) == 0 && out < cols) dw[out] = from_f32<W>(s);
+}
+
+// Any row length: dx with the rows read twice, r of every row kept for the columns' kernel behind.
+template <typename T>
+__global__ void __launch_bounds__(256) rms_norm_grad_any_kernel(const Backward p, float* __restrict__ inv_rms) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sh[16];
+  const int64_t row = blockIdx.x;
+  const T* h = reinterpret_cast<const T*>(p.h) + row * p.h_ld;
+  const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.cols;
+  auto weight = [&](int i) {
+    return p.w_f32 ? reinterpret_cast<const float*>(p.weight)[i] : ToF32<T>::get(reinterpret_cast<const T*>(p.weight)[i]);
+  };
+  float s[2] = {0.0f, 0.0f};
+  for (int i = threadIdx.x; i < p.cols; i += 256) {
+    const float hv = ToF32<T>::get(h[i]);
+    s[0] = fmaf(hv, hv, s[0]);
+    s[1] = fmaf(weight(i) * ToF32<T>::get(dy[i]), hv, s[1]);
+  }
+  join_row<Sum, 2, 256>(s, sh);
+  const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
+  const float k = inv * inv * (s[1] / (float)p.cols);
+  if (inv_rms != nullptr && threadIdx.x == 0) inv_rms[row] = inv;
+  if (p.dx == nullptr) return;
+  for (int i = threadIdx.x; i < p.cols; i += 256) {
+    float v = inv * (weight(i) * ToF32<T>::get(dy[i]) - ToF32<T>::get(h[i]) * k);
+    if (p.dh != nullptr) v += ToF32<T>::get(reinterpret_cast<const T*>(p.dh)[row * p.cols + i]);
+    reinterpret_cast<T*>(p.dx)[row * p.cols + i] = from_f32<T>(v);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) weight_grad_any_kernel(const Backward p, const float* __restrict__ inv_rms) {
+  pdl_wait();
+  pdl_trigger();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col >= p.cols) return;
+  float s = 0.0f;
+  for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y)
+    s = fmaf(ToF32<T>::get(reinterpret_cast<const T*>(p.dy)[row * p.cols + col]),
+             ToF32<T>::get(reinterpret_cast<const T*>(p.h)[row * p.h_ld + col]) * inv_rms[row], s);
+  p.partial[(int64_t)blockIdx.y * p.cols + col] = s;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool pieces16(const void* p, int64_t ld, int size) { return aligned16(p) && ld * size % 16 == 0; }
+
+// How a row is shared out: threads to a row and pieces to a thread; 0 threads = the kernel for any row.
+struct Split { int threads, chunks; };
+Split split_of(int pieces, bool vector) {
+  if (pieces <= 32 * 4) return {32, 4};
+  if (pieces <= 256) return {vector ? 32 : 256, vector ? 8 : 4};
+  if (pieces <= 256 * 4) return {256, 4};
+  if (pieces <= 512 * 4) return {512, 4};
+  if (!vector && pieces <= 1024 * 8) return {1024, 8};
+  return {0, 0};
+}
+
+template <typename T, bool QUANT>
+int launch_forward(const Forward& p, bool vector, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const Split s = split_of(vector ? p.cols / VEC : p.cols, vector);
+#define MOE_RN(V, TPR, CH)                                                                                                 \
+  launch_pdl(rms_norm_kernel<T, V, TPR, CH, QUANT>, dim3((unsigned)((p.rows + (TPR > 128 ? 1 : 128 / TPR) - 1) / (TPR > 128 ? 1 : 128 / TPR))), \
+             TPR > 128 ? TPR : 128, 0, 1, st, "rms_norm", p)
+  // groups of a power of two of pieces within a warp, or whole rows, are quantised from registers
+  const int lanes = QUANT ? p.group / (vector ? VEC : 1) : 0;
+  const bool held = !QUANT || p.group == p.cols || (p.group % (vector ? VEC : 1) == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0);
+  if (s.threads == 0 || !held) return launch_pdl(rms_norm_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm", p);
+  if (vector) {
+    if (s.threads == 32) return s.chunks == 4 ? MOE_RN(VEC, 32, 4) : MOE_RN(VEC, 32, 8);
+    return s.threads == 256 ? MOE_RN(VEC, 256, 4) : MOE_RN(VEC, 512, 4);
+  }
+  if (s.threads == 32) return MOE_RN(1, 32, 4);
+  if (s.threads == 256) return MOE_RN(1, 256, 4);
+  return s.threads == 512 ? MOE_RN(1, 512, 4) : MOE_RN(1, 1024, 8);
+#undef MOE_RN
+}
+
+int forward(const Forward& p, int dtype, bool quant, cudaStream_t st) {
+  const int size = dtype == MOE_F32 ? 4 : 2, vec = 16 / size;
+  const bool vector = p.cols % vec == 0 && pieces16(p.x, p.x_ld, size) && (!p.residual || pieces16(p.residual, p.residual_ld, size)) &&
+                      (!p.h || pieces16(p.h, p.h_ld, size)) && (!p.y || pieces16(p.y, p.y_ld, size)) && aligned16(p.weight) &&
+                      (!p.q || aligned16(p.q));
+  switch (dtype) {
+    case MOE_F32: return quant ? launch_forward<float, true>(p, vector, st) : launch_forward<float, false>(p, vector, st);
+    case MOE_F16: return quant ? launch_forward<__half, true>(p, vector, st) : launch_forward<__half, false>(p, vector, st);
+    default: return quant ? launch_forward<__nv_bfloat16, true>(p, vector, st) : launch_forward<__nv_bfloat16, false>(p, vector, st);
+  }
+}
+
+constexpr int64_t kMaxRows = 0x7FFFFFFF;  // blocks of a grid
+constexpr int kPartsPerSm = 2;            // blocks of the gradient, each with its part of dw
+
+// Checks that both forward entry points share.
+int check_forward(const char* who, const void* x, int dtype, int weight_dtype, const void* residual, const void* weight, int64_t rows,
+                  int64_t cols, float eps, int64_t x_ld, int64_t residual_ld, void* h, int64_t h_ld) {
+  if (rows < 0 || cols <= 0 || cols > (1 << 24)) return fail(MOE_E_BADARG, "%s: bad extent", who);
+  if (rows > kMaxRows) return fail(MOE_E_TOOBIG, "%s: too many rows", who);
+  if (dtype != MOE_F32 && dtype != MOE_F16 && dtype != MOE_BF16) return fail(MOE_E_DTYPE, "%s: unsupported dtype %d", who, dtype);
+  if (weight_dtype != dtype && weight_dtype != MOE_F32) return fail(MOE_E_DTYPE, "%s: the weight is fp32 or of the rows' type", who);
+  if (!(eps >= 0.0f) || !(eps < 3.0e38f)) return fail(MOE_E_BADARG, "%s: eps must be finite and not negative", who);
+  if (rows == 0) return 0;
+  if (!x || !weight || (residual && !h)) return fail(MOE_E_BADARG, "%s: null pointer", who);
+  if (x_ld < 0 || (residual && (residual_ld < 0 || (h_ld < cols && rows > 1)))) return fail(MOE_E_BADARG, "%s: bad row distance", who);
+  return 0;
+}
+
+int grad_blocks(int64_t rows) {
+  const int64_t most = (int64_t)sm_count() * kPartsPerSm;
+  return (int)(rows < most ? rows : most);
+}
+
+template <typename T>
+int launch_backward(const Backward& p, bool vector, int parts, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const Split s = split_of(vector ? p.cols / VEC : p.cols, vector);
+#define MOE_RG(V, TPR, CH) launch_pdl(rms_norm_grad_kernel<T, V, TPR, CH>, dim3((unsigned)parts), TPR > 128 ? TPR : 128, 0, 1, st, "rms_norm_grad", p)
+  if (s.threads == 0 || s.threads == 1024) {
+    float* inv = p.partial ? p.partial + (int64_t)parts * p.cols : nullptr;
+    int rc = launch_pdl(rms_norm_grad_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm_grad", p, inv);
+    if (rc || !p.partial) return rc;
+    return launch_pdl(weight_grad_any_kernel<T>, dim3((unsigned)((p.cols + 255) / 256), (unsigned)parts), 256, 0, 1, st, "rms_norm_grad", p,
+                      (const float*)inv);
+  }
+  if (vector) {
+    if (s.threads == 32) return s.chunks == 4 ? MOE_RG(VEC, 32, 4) : MOE_RG(VEC, 32, 8);
+    return s.threads == 256 ? MOE_RG(VEC, 256, 4) : MOE_RG(VEC, 512, 4);
+  }
+  if (s.threads == 32) return MOE_RG(1, 32, 4);
+  return s.threads == 256 ? MOE_RG(1, 256, 4) : MOE_RG(1, 512, 4);
+#undef MOE_RG
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_rms_norm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const void* weight, int dtype,
+                            int weight_dtype, int64_t rows, int64_t cols, float eps, void* y, int64_t y_ld, void* residual_out,
+                            int64_t residual_out_ld, void* stream) {
+  using namespace moe;
+  const int rc = check_forward("rms_norm", x, dtype, weight_dtype, residual, weight, rows, cols, eps, x_ld, residual_ld, residual_out,
+                               residual_out_ld);
+  if (rc || rows == 0) return rc;
+  if (!y || (y_ld < cols && rows > 1)) return fail(MOE_E_BADARG, "rms_norm: bad output");
+  if (!residual && y == x) return fail(MOE_E_BADARG, "rms_norm: the output may lie over the input only with a residual");
+  Forward p = {};
+  p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = residual ? residual_out : nullptr;
+  p.x_ld = x_ld; p.residual_ld = residual_ld; p.y_ld = y_ld; p.h_ld = residual_out_ld; p.rows = rows;
+  p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps; p.group = (int)cols;
+  return forward(p, dtype, false, (cudaStream_t)stream);
+}
+
+extern "C" int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const void* weight, int dtype,
+                                  int weight_dtype, int64_t rows, int64_t cols, float eps, int format, int group, float quant_eps,
+                                  int scale_flags, void* q, float* scales, int64_t scale_ld, void* y, void* residual_out, void* stream) {
+  using namespace moe;
+  const int rc = check_forward("rms_norm_quant", x, dtype, weight_dtype, residual, weight, rows, cols, eps, x_ld, residual_ld,
+                               residual_out, cols);
+  if (rc) return rc;
+  if (format < kE4M3 || format > kInt8) return fail(MOE_E_DTYPE, "rms_norm_quant: unknown 8-bit format %d", format);
+  if (group <= 0 || cols % group != 0) return fail(MOE_E_SHAPE, "rms_norm_quant: the row must be a multiple of the group size %d", group);
+  if (!(quant_eps >= 0.0f) || !(quant_eps < 3.0e38f)) return fail(MOE_E_BADARG, "rms_norm_quant: quant_eps must be finite and not negative");
+  if ((scale_flags & 2) && format == kInt8) return fail(MOE_E_BADARG, "rms_norm_quant: power-of-two scales are for the 8-bit floats");
+  if (rows == 0) return 0;
+  if (!q || !scales || ((scale_flags & 1) && scale_ld < rows)) return fail(MOE_E_BADARG, "rms_norm_quant: bad output");
+  if (y && y == x) return fail(MOE_E_BADARG, "rms_norm_quant: the norm is written to memory of its own");
+  Forward p = {};
+  p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = residual ? residual_out : nullptr;
+  p.x_ld = x_ld; p.residual_ld = residual_ld; p.y_ld = cols; p.h_ld = cols; p.rows = rows;
+  p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps;
+  p.q = (uint8_t*)q; p.scales = scales; p.scale_ld = scale_ld; p.group = group; p.format = format;
+  p.transposed = scale_flags & 1; p.ue8m0 = (scale_flags >> 1) & 1; p.quant_eps = quant_eps;
+  return forward(p, dtype, true, (cudaStream_t)stream);
+}
+
+extern "C" int moe_rms_norm_grad_workspace(int64_t rows, int64_t cols, int64_t* bytes) {
+  using namespace moe;
+  if (rows < 0 || cols <= 0 || cols > (1 << 24) || !bytes) return fail(MOE_E_BADARG, "rms_norm_grad: bad extent");
+  if (rows > kMaxRows) return fail(MOE_E_TOOBIG, "rms_norm_grad: too many rows");
+  *bytes = 4 * ((int64_t)grad_blocks(rows) * cols + rows);
+  return 0;
+}
+
+extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, const void* h, int64_t h_ld, const void* weight, int dtype,
+                                 int weight_dtype, int64_t rows, int64_t cols, float eps, void* dx, void* dweight, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  using namespace moe;
+  int rc = check_forward("rms_norm_grad", h, dtype, weight_dtype, nullptr, weight, rows, cols, eps, h_ld, 0, nullptr, 0);
+  if (rc) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (rows == 0) {
+    if (!dweight) return 0;
+    const cudaError_t ce = cudaMemsetAsync(dweight, 0, (size_t)cols * (weight_dtype == MOE_F32 ? 4 : 2), st);
+    return ce == cudaSuccess ? 0 : fail((int)ce, "rms_norm_grad: %s", cudaGetErrorString(ce));
+  }
+  if (!dy || (!dx && !dweight)) return fail(MOE_E_BADARG, "rms_norm_grad: null pointer");
+  const int parts = grad_blocks(rows);
+  if (dweight && (!workspace || workspace_bytes < 4 * ((int64_t)parts * cols + rows) || !aligned16(workspace)))
+    return fail(MOE_E_BADARG, "rms_norm_grad: workspace too small");
+  Backward p = {};
+  p.dy = dy; p.dh = dresidual_out; p.h = h; p.weight = weight; p.dx = dx; p.partial = dweight ? (float*)workspace : nullptr;
+  p.h_ld = h_ld; p.rows = rows; p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps;
+  const int size = dtype == MOE_F32 ? 4 : 2;
+  const bool vector = cols % (16 / size) == 0 && pieces16(h, h_ld, size) && aligned16(dy) && aligned16(dresidual_out) && aligned16(dx) &&
+                      aligned16(weight);
+  rc = dtype == MOE_F32 ? launch_backward<float>(p, vector, parts, st)
+       : dtype == MOE_F16 ? launch_backward<__half>(p, vector, parts, st)
+                          : launch_backward<__nv_bfloat16>(p, vector, parts, st);
+  if (rc || !dweight) return rc;
+  const dim3 grid((unsigned)((cols + 31) / 32));
+  const float* partial = (const float*)workspace;
+  switch (weight_dtype) {
+    case MOE_F32: return launch_pdl(weight_grad_kernel<float>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, (int)cols, (float*)dweight);
+    case MOE_F16: return launch_pdl(weight_grad_kernel<__half>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, (int)cols, (__half*)dweight);
+    default:
+      return launch_pdl(weight_grad_kernel<__nv_bfloat16>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, (int)cols,
+                        (__nv_bfloat16*)dweight);
+  }
+}

@@ -40,15 +40,6 @@ __global__ void __launch_bounds__(kThreads) zero_padding_kernel(const int4* __re
     scales_t[(int64_t)(i / padding) * scale_ld + d.x + occupied + i % padding] = 0.0f;
 }
 
-// v / s, correctly rounded, for |v| <= 448 s (1 + ulp) from the rounded reciprocal of s: one correction step by the exact
-// remainder (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990).  Where the quotient is
-// so small that the remainder is not exact it rounds to zero in e4m3 all the same: over every pair of finite bf16 or f16
-// values (amax, |v| <= amax) the e4m3 bytes are those of the division.  The sign is v's, of a zero too.
-__device__ __forceinline__ float div_by_scale(float v, float s, float inv) {
-  const float q = v * inv;
-  return copysignf(fmaf(fmaf(-q, s, v), inv, q), v);
-}
-
 // EARLY (below): the token is read and quantised while the route plan is still being made.
 // Block (c, m): P x blockDim.x / 8 128-groups of token m, eight lanes per group, 16 elements per lane.  The bytes and scales
 // are those of the stand-alone quantiser (quant.cu).  With a division per element the kernel was bound by its instructions.

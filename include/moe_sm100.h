@@ -468,6 +468,51 @@ int moe_layer(int mode, int act_dtype, const void* x, int64_t num_tokens, int to
               int quant_kind2, const float* quant_scale2, void* ws_plan, void* ws_x, void* ws_act, void* ws_y, int stages,
               int32_t* status, void* stream);
 
+/* RMS norm of the residual stream (no counterpart among the reference's files of this path; what stands in front of a layer):
+ *   h = round(x + residual), or x without a residual;   y = round(weight h / sqrt(mean(h^2) + eps))
+ * x, residual [rows, cols] with rows `*_ld` elements apart (0 = the same row for all), weight [cols] of the rows' dtype or
+ * fp32; y and residual_out (null without a residual) with `*_ld` >= cols.  With a residual y may be x and residual_out may be
+ * residual (same memory, same row distance); other overlaps are the caller's error.  Any cols up to 2^24; rows made of
+ * 16-byte pieces are read in such pieces. */
+int moe_rms_norm(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const void* weight, int dtype,
+                 int weight_dtype, int64_t rows, int64_t cols, float eps, void* y, int64_t y_ld, void* residual_out,
+                 int64_t residual_out_ld, void* stream);
+
+/* The same with y in 8 bits: per `group` consecutive columns (cols = one group per row)
+ *   s = max(amax |y|, quant_eps) / qmax;   q = round(y / s)
+ * of the fp32 value of y.  format: 0 e4m3 (qmax 448), 1 e5m2 (57344), 2 int8 (127).  scale_flags: 1 = scales [cols / group,
+ * scale_ld] instead of [rows, cols / group]; 2 = s rounded up to a power of two (8-bit floats).  A NaN in a group makes its
+ * scale NaN.  q, y (null = not wanted) and residual_out are [rows, cols] without gaps. */
+int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const void* weight, int dtype,
+                       int weight_dtype, int64_t rows, int64_t cols, float eps, int format, int group, float quant_eps,
+                       int scale_flags, void* q, float* scales, int64_t scale_ld, void* y, void* residual_out, void* stream);
+
+/* Gradient of moe_rms_norm from h: dx (also the residual's; null = not wanted) = d y / d h applied to dy, plus
+ * dresidual_out (null = none); dweight (null = not wanted) summed in fp32 over the rows in a fixed order and rounded to
+ * weight_dtype.  dy, dresidual_out, dx [rows, cols] without gaps.  The workspace is needed for dweight. */
+int moe_rms_norm_grad_workspace(int64_t rows, int64_t cols, int64_t* bytes /* host */);
+int moe_rms_norm_grad(const void* dy, const void* dresidual_out, const void* h, int64_t h_ld, const void* weight, int dtype,
+                      int weight_dtype, int64_t rows, int64_t cols, float eps, void* dx, void* dweight, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Balance loss of a router and tokens per expert (no counterpart in the reference, which does not train):
+ *   p_t = softmax(logits_t), or (sigmoid != 0) the sigmoids of the row divided by their sum
+ *   per sequence of N > 0 tokens that are not padding: counts_e = its routes to e, loss_s = sum_e (E counts_e / (topk N)) mean_t p_te
+ *   loss = mean of loss_s over those sequences (0 if there is none)
+ * logits [tokens, experts], rows `ld` elements apart; topk_ids [tokens, topk] int32 / int64 (negative = no route; >= experts:
+ * skipped, MOE_ST_BAD_EXPERT_ID); cu_seqlens [sequences + 1] int32 or null (one sequence of all rows); is_padding [tokens] or
+ * null.  Rows in no sequence count for nothing.  cu_seqlens that decrease or leave [0, tokens]: loss NaN, counts 0,
+ * MOE_ST_BAD_ROW.  counts [sequences, experts]; saved: what the gradient needs.  At most 1024 experts, 32 routes per token,
+ * 65535 sequences.  bytes[0] of the workspace, bytes[1] of saved. */
+int moe_balance_loss_workspace(int64_t tokens, int experts, int topk, int sequences, int64_t* bytes /* host [2] */);
+int moe_balance_loss(const void* logits, int64_t ld, int dtype, int64_t tokens, int experts, const void* topk_ids, int ids_int64,
+                     int topk, int sigmoid, const int32_t* cu_seqlens, int sequences, const uint8_t* is_padding, float* loss,
+                     int32_t* counts, void* saved, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+/* dlogits [tokens, experts] without gaps, of the logits' dtype; the counts are held.  Rows that count for nothing get zeros. */
+int moe_balance_loss_grad(const void* logits, int64_t ld, int dtype, int64_t tokens, int experts, int topk, int sigmoid,
+                          const int32_t* cu_seqlens, int sequences, const uint8_t* is_padding, const void* saved,
+                          const float* dloss, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,7 +11,7 @@
 // is left of two nearly equal sums when the experts are nearly even is exact to fp32.  A row whose logits are all -inf has
 // p = 0 and no gradient.
 //
-// Two launches forward.  Each block of the first takes a run of rows and, for every sequence in it, sums p and counts routes
+// Two launches forward, one where a block holds all rows.  Each block of the first takes a run of rows and, for every sequence in it, sums p and counts routes
 // in registers and shared memory; sequence s in block c goes to slot c + s, which no other pair has (a walk along the rows
 // adds one to c or to s at every step).  The second adds the slots in order, so that results are the same bits in every run.
 // Bound: memory, one pass over the logits forward and one backward; the launches for a few thousand tokens.
@@ -20,7 +20,7 @@
 namespace moe {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBlocksPerSm = 2;
 
 struct Balance {
   const void* logits;
@@ -51,11 +51,16 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int sequences, int
   return lo;
 }
 
+// Tokens that a lane has in hand at once: their loads and the two sums over the lanes of each run beside one another.
+__host__ __device__ constexpr int tokens_in_hand(int values) { return values >= 32 ? 1 : values >= 16 ? 2 : 4; }
+
 template <typename T, int V, int CH>
 __device__ __forceinline__ void load_row(const T* row, int at, int lanes, int experts, bool live, float (&l)[CH][V]) {
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int e = (at + c * lanes) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[c][i] = -INFINITY;
     if (live && e < experts) {
       if constexpr (V == 1) {
         l[c][0] = ToF32<T>::get(row[e]);
@@ -64,53 +69,103 @@ __device__ __forceinline__ void load_row(const T* row, int at, int lanes, int ex
 #pragma unroll
         for (int i = 0; i < V; ++i) l[c][i] = ToF32<T>::get(reinterpret_cast<const T*>(&raw)[i]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) l[c][i] = -INFINITY;
     }
   }
 }
 
-// l -> p, over the `lanes` lanes of a token (all lanes of the warp call it).
-template <int V, int CH>
-__device__ __forceinline__ void scores(const float (&l)[CH][V], int lanes, bool sigmoid, float (&p)[CH][V]) {
-  float m = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      p[c][i] = sigmoid ? fminf(l[c][i], 0.0f) - log1pf(expf(-fabsf(l[c][i]))) : l[c][i];
-      if (!(l[c][i] == l[c][i])) p[c][i] = l[c][i];  // fminf drops a NaN
-      m = max_nan(m, p[c][i]);
-    }
-  for (int off = lanes / 2; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
-  float sum = 0.0f;
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      // the difference first: with the type's lowest value in every place it is zero
-      p[c][i] = m == -INFINITY ? 0.0f : exp2f((p[c][i] - m) * 1.4426950408889634f);
-      sum += p[c][i];
-    }
-  for (int off = lanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) p[c][i] *= inv;
+// 2^x; what is below 2^-126 is zero.
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
+// l -> e of U tokens, each over `lanes` lanes (all lanes of the warp call it); the scores are p = e inv.
+template <int V, int CH, int U>
+__device__ __forceinline__ void scores(const float (&l)[U][CH][V], int lanes, bool sigmoid, float (&e)[U][CH][V], float (&inv)[U]) {
+  if (sigmoid) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float x = l[u][c][i];
+          e[u][c][i] = x == x ? fminf(x, 0.0f) - log1pf(expf(-fabsf(x))) : x;  // fminf drops a NaN
+        }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[u][c][i] = l[u][c][i];
+  }
+  float m[U], sum[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    m[u] = -INFINITY;
+    sum[u] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) m[u] = max_nan(m[u], e[u][c][i]);
+  }
+  for (int off = lanes / 2; off > 0; off >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) m[u] = max_nan(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], off));
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float at = m[u] == -INFINITY ? 0.0f : m[u];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        // the difference first: with the type's lowest value in every place it is zero
+        e[u][c][i] = exp2_ftz((e[u][c][i] - at) * 1.4426950408889634f);
+        sum[u] += e[u][c][i];
+      }
+  }
+  for (int off = lanes / 2; off > 0; off >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xFFFFFFFFu, sum[u], off);
+#pragma unroll
+  for (int u = 0; u < U; ++u) inv[u] = sum[u] == 0.0f ? 0.0f : 1.0f / sum[u];  // the sum is at least 1, or the row has no score
+}
+
+// Sum over the block, the same in every thread and run; `sh` holds a value per warp.
+template <typename X>
+__device__ __forceinline__ X block_sum(X v, X* sh) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  v = lane < (int)blockDim.x / 32 ? sh[lane] : X(0);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+  return v;
+}
+
+// What the call gives back; null in the first of two launches.
+struct Result {
+  int32_t *counts, *saved;
+  float* loss;
+};
+
 template <typename T, int V, int CH>
-__global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b, const Slots out, int32_t* __restrict__ status) {
+__global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b, const Slots out, const Result result, int32_t* __restrict__ status) {
   pdl_wait();
   pdl_trigger();
+  constexpr int U = tokens_in_hand(V * CH);
   extern __shared__ float sh[];  // [warps, experts] of p, [experts] of routes, tokens
+  __shared__ double sh_sum[kWarps];
   int32_t* hist = reinterpret_cast<int32_t*>(sh + kWarps * b.experts);
   int32_t* live_tokens = hist + b.experts;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, step = kWarps * groups;
   const int64_t r0 = (int64_t)blockIdx.x * b.rows, r1 = min(b.tokens, r0 + b.rows);
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && result.loss == nullptr) {
     int bad = 0;
     if (b.cu != nullptr)
       for (int s = threadIdx.x; s < b.sequences; s += kThreads) bad |= b.cu[s] < 0 || b.cu[s + 1] < b.cu[s] || b.cu[s + 1] > b.tokens;
@@ -133,25 +188,39 @@ __global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b,
     for (int e = threadIdx.x; e <= b.experts; e += kThreads) hist[e] = 0;  // and the tokens behind
     __syncthreads();
     const uint32_t routes = (uint32_t)(last * b.topk);  // check(): all routes are below 2^31
-    for (uint32_t i = (uint32_t)(first * b.topk) + threadIdx.x; i < routes; i += kThreads) {
-      if (b.padding != nullptr && b.padding[i / (uint32_t)b.topk]) continue;
-      const int64_t id = b.ids64 ? reinterpret_cast<const int64_t*>(b.ids)[i] : (int64_t) reinterpret_cast<const int32_t*>(b.ids)[i];
-      if (id >= 0 && id < b.experts) atomicAdd(hist + id, 1);
-      else bad_id |= id >= b.experts;
+    for (uint32_t i0 = (uint32_t)(first * b.topk) + threadIdx.x; i0 < routes; i0 += 4 * kThreads) {
+      int64_t id[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t i = i0 + j * kThreads;
+        id[j] = -1;
+        if (i < routes && (b.padding == nullptr || !b.padding[i / (uint32_t)b.topk]))
+          id[j] = b.ids64 ? reinterpret_cast<const int64_t*>(b.ids)[i] : (int64_t) reinterpret_cast<const int32_t*>(b.ids)[i];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (id[j] >= 0 && id[j] < b.experts) atomicAdd(hist + id[j], 1);
+        else bad_id |= id[j] >= b.experts;
+      }
     }
     float acc[CH][V] = {};
     int mine = 0;
-    for (int64_t t0 = first + warp * groups; t0 < last; t0 += kWarps * groups) {
-      const int64_t t = t0 + lane / b.lanes;
-      const bool live = t < last && (b.padding == nullptr || !b.padding[t]);
-      float l[CH][V], p[CH][V];
-      load_row<T, V, CH>(reinterpret_cast<const T*>(b.logits) + t * b.ld, lane % b.lanes, b.lanes, b.experts, live, l);
-      scores<V, CH>(l, b.lanes, b.sigmoid, p);
-      mine += live && lane % b.lanes == 0;
+    for (int64_t t0 = first + warp * groups; t0 < last; t0 += U * step) {
+      float l[U][CH][V], p[U][CH][V], inv[U];
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
+      for (int u = 0; u < U; ++u) {
+        const int64_t t = t0 + u * step + lane / b.lanes;
+        const bool live = t < last && (b.padding == nullptr || !b.padding[t]);
+        load_row<T, V, CH>(reinterpret_cast<const T*>(b.logits) + t * b.ld, lane % b.lanes, b.lanes, b.experts, live, l[u]);
+        mine += live && lane % b.lanes == 0;
+      }
+      scores<V, CH, U>(l, b.lanes, b.sigmoid, p, inv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[c][i] += p[c][i];
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[c][i] = fmaf(p[u][c][i], inv[u], acc[c][i]);
     }
     for (int off = 16; off >= b.lanes; off >>= 1)
 #pragma unroll
@@ -171,35 +240,37 @@ __global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b,
     }
     __syncthreads();
     const int64_t slot = (int64_t)blockIdx.x + s;
+    double part = 0.0;
     for (int e = threadIdx.x; e < b.experts; e += kThreads) {
       float m = sh[e];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) m += sh[w * b.experts + e];
-      out.mass[slot * b.experts + e] = m;
-      out.count[slot * b.experts + e] = hist[e];
+      if (result.loss != nullptr) {
+        result.counts[e] = result.saved[e] = hist[e];
+        part += (double)hist[e] * (double)m;
+      } else {
+        out.mass[slot * b.experts + e] = m;
+        out.count[slot * b.experts + e] = hist[e];
+      }
     }
-    if (threadIdx.x == 0) out.tokens[slot] = *live_tokens;
+    if (result.loss != nullptr) {  // one block, one sequence: this was all
+      const int live = *live_tokens;
+      part = block_sum(part, sh_sum);
+      if (threadIdx.x == 0) {
+        result.saved[b.experts] = live;
+        result.saved[b.experts + 1] = live > 0;
+        *result.loss = live > 0 ? (float)(part * (double)b.experts / ((double)b.topk * (double)live * (double)live)) : 0.0f;
+      }
+    } else if (threadIdx.x == 0) {
+      out.tokens[slot] = *live_tokens;
+    }
     __syncthreads();
   }
   if (bad_id) set_status(status, MOE_ST_BAD_EXPERT_ID);
 }
 
-// Sum over the block, the same in every thread and run; `sh` holds a value per warp.
-template <typename X>
-__device__ __forceinline__ X block_sum(X v, X* sh) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int w = 1; w < (int)blockDim.x / 32; ++w) v += sh[w];
-  return v;
-}
-
-// Block (sequence, 32 experts): a lane per expert, the warps share the slots.  The block that is last to end adds up the loss.
-__global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, const Slots in, int32_t* __restrict__ counts,
-                                                            int32_t* __restrict__ saved, float* __restrict__ loss) {
+// Block (32 experts, sequence): a lane per expert, the warps share the slots.  The block that is last to end adds up the loss.
+__global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, const Slots in, const Result out) {
   pdl_wait();
   pdl_trigger();
   __shared__ float mass[32][33];
@@ -208,40 +279,59 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
   __shared__ int shi[32], is_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
   const int s = blockIdx.y, e = blockIdx.x * 32 + lane;
-  const bool bad = in.flags[0] != 0;
+  const int bad = in.flags[0];
   int64_t first = 0, last = b.tokens;
-  if (b.cu != nullptr) { first = b.cu[s]; last = b.cu[s + 1]; }
-  int64_t c0 = 0, c1 = 0;  // blocks that hold rows of the sequence
-  if (!bad && first < last) { c0 = first / b.rows; c1 = (last - 1) / b.rows + 1; }
+  if (b.cu != nullptr) {  // within the rows whatever they are: what is read for bad ones is not used
+    first = min(max((int64_t)b.cu[s], (int64_t)0), b.tokens);
+    last = min(max((int64_t)b.cu[s + 1], first), b.tokens);
+  }
+  const int c0 = (int)(first / b.rows), c1 = first < last ? (int)((last - 1) / b.rows) + 1 : c0;  // blocks that hold its rows
   float m = 0.0f;
   int n = 0, live = 0;
-#pragma unroll 4
-  for (int64_t c = c0 + warp; c < c1; c += warps) {
-    if (e < b.experts) {
-      m += in.mass[(c + s) * b.experts + e];
-      n += in.count[(c + s) * b.experts + e];
+  for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) live += in.tokens[c + s];
+  for (int c = c0 + warp; c < c1; c += 10 * warps) {  // ten slots in flight: two a multiprocessor are one round of 32 warps
+    float mv[10];
+    int nv[10];
+#pragma unroll
+    for (int j = 0; j < 10; ++j) {
+      const bool there = e < b.experts && c + j * warps < c1;
+      const int64_t at = (int64_t)(c + j * warps + s) * b.experts + e;
+      mv[j] = there ? in.mass[at] : 0.0f;
+      nv[j] = there ? in.count[at] : 0;
     }
-    if (lane == 0) live += in.tokens[c + s];
+#pragma unroll
+    for (int j = 0; j < 10; ++j) { m += mv[j]; n += nv[j]; }
   }
   mass[warp][lane] = m;
   count[warp][lane] = n;
-  live = block_sum(live, shi);  // its barriers stand between the writes above and the reads below
+  live = __reduce_add_sync(0xFFFFFFFFu, live);
+  if (lane == 0) shi[warp] = live;
+  __syncthreads();
+  live = __reduce_add_sync(0xFFFFFFFFu, lane < warps ? shi[lane] : 0);
+  if (bad) live = 0;
   double part = 0.0;
-  if (warp == 0) {
-    double total = 0.0;
-    n = 0;
-    for (int w = 0; w < warps; ++w) { total += (double)mass[w][lane]; n += count[w][lane]; }
-    if (e < b.experts) {
-      counts[(int64_t)s * b.experts + e] = n;
-      saved[(int64_t)s * b.experts + e] = n;
-      if (live > 0) part = (double)n * total;
+  for (int r = warp; r < 32; r += warps) {  // a warp per expert
+    double total = lane < warps ? (double)mass[lane][r] : 0.0;
+    n = lane < warps && !bad ? count[lane][r] : 0;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    const int expert = blockIdx.x * 32 + r;
+    if (lane == 0 && expert < b.experts) {
+      out.counts[(int64_t)s * b.experts + expert] = n;
+      out.saved[(int64_t)s * b.experts + expert] = n;
+      part += (double)n * total;
     }
+  }
+  if (lane == 0) shd[warp] = part;
+  __syncthreads();
+  if (warp == 0) {
+    part = lane < warps ? shd[lane] : 0.0;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, off);
-    if (live > 0) part *= (double)b.experts / ((double)b.topk * (double)live * (double)live);
     if (lane == 0) {
-      in.part[(int64_t)s * gridDim.x + blockIdx.x] = part;
-      if (blockIdx.x == 0) saved[(int64_t)b.sequences * b.experts + s] = live;
+      in.part[(int64_t)s * gridDim.x + blockIdx.x] = live > 0 ? part * (double)b.experts / ((double)b.topk * (double)live * (double)live) : 0.0;
+      if (blockIdx.x == 0) out.saved[(int64_t)b.sequences * b.experts + s] = live;
       __threadfence();
       is_last = atomicAdd(in.flags + 1, 1) == (int)(gridDim.x * gridDim.y) - 1;
     }
@@ -252,12 +342,12 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
   double sum = 0.0;
   int filled = 0;
   for (int64_t i = threadIdx.x; i < (int64_t)b.sequences * gridDim.x; i += blockDim.x) sum += __ldcg(in.part + i);
-  for (int i = threadIdx.x; i < b.sequences; i += blockDim.x) filled += __ldcg(saved + (int64_t)b.sequences * b.experts + i) > 0;
+  for (int i = threadIdx.x; i < b.sequences; i += blockDim.x) filled += __ldcg(out.saved + (int64_t)b.sequences * b.experts + i) > 0;
   sum = block_sum(sum, shd);
   filled = block_sum(filled, shi);
   if (threadIdx.x == 0) {
-    saved[(int64_t)b.sequences * (b.experts + 1)] = filled;
-    *loss = bad ? __uint_as_float(0x7FC00000u) : (float)(sum / (filled > 0 ? filled : 1));
+    out.saved[(int64_t)b.sequences * (b.experts + 1)] = filled;
+    *out.loss = bad ? __uint_as_float(0x7FC00000u) : (float)(sum / (filled > 0 ? filled : 1));
   }
 }
 
@@ -266,57 +356,75 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Balance b,
                                                                 const float* __restrict__ dloss, T* __restrict__ dlogits) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, at = lane % b.lanes;
+  constexpr int U = tokens_in_hand(V * CH);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, at = lane % b.lanes, step = kWarps * groups;
   const int64_t r0 = (int64_t)blockIdx.x * b.rows, r1 = min(b.tokens, r0 + b.rows);
   const int32_t* live_tokens = saved + (int64_t)b.sequences * b.experts;
   const double scale = (double)*dloss / (double)max(1, live_tokens[b.sequences]);
   int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0 + warp * groups + lane / b.lanes), held = -1;
   float a[CH][V] = {};
-  for (int64_t t0 = r0 + warp * groups; t0 < r1; t0 += kWarps * groups) {
-    const int64_t t = t0 + lane / b.lanes;
-    bool live = t < r1 && (b.padding == nullptr || !b.padding[t]);
-    if (b.cu != nullptr) {
-      while (s < b.sequences && b.cu[s + 1] <= t) ++s;
-      live = live && s < b.sequences && b.cu[s] <= t;
+  for (int64_t t0 = r0 + warp * groups; t0 < r1; t0 += U * step) {
+    float l[U][CH][V], p[U][CH][V], inv[U];
+    int own[U];  // the token's sequence, -1 = its gradient is zero
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = t0 + u * step + lane / b.lanes;
+      bool live = t < r1 && (b.padding == nullptr || !b.padding[t]);
+      if (b.cu != nullptr) {
+        while (s < b.sequences && b.cu[s + 1] <= t) ++s;
+        live = live && s < b.sequences && b.cu[s] <= t;
+      }
+      own[u] = live ? s : -1;
+      load_row<T, V, CH>(reinterpret_cast<const T*>(b.logits) + t * b.ld, at, b.lanes, b.experts, live, l[u]);
     }
-    float l[CH][V], p[CH][V];
-    load_row<T, V, CH>(reinterpret_cast<const T*>(b.logits) + t * b.ld, at, b.lanes, b.experts, live, l);
-    if (live && s != held) {
-      held = s;
-      const double n = (double)max(1, live_tokens[s]);
-      const float k = (float)(scale / ((double)b.topk * n * n));
-      const int64_t even = (int64_t)b.topk * live_tokens[s];
+    scores<V, CH, U>(l, b.lanes, b.sigmoid, p, inv);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (own[u] >= 0 && own[u] != held) {
+        held = own[u];
+        const double n = (double)max(1, live_tokens[held]);
+        const float k = (float)(scale / ((double)b.topk * n * n));
+        const int64_t even = (int64_t)b.topk * live_tokens[held];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const int e = (at + c * b.lanes) * V + i;
+            a[c][i] = e < b.experts ? k * (float)((int64_t)b.experts * saved[(int64_t)held * b.experts + e] - even) : 0.0f;
+          }
+      }
+      float mean = 0.0f;
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int e = (at + c * b.lanes) * V + i;
-          a[c][i] = e < b.experts ? k * (float)((int64_t)b.experts * saved[(int64_t)s * b.experts + e] - even) : 0.0f;
-        }
-    }
-    scores<V, CH>(l, b.lanes, b.sigmoid, p);
-    float mean = 0.0f;
+        for (int i = 0; i < V; ++i) mean = fmaf(p[u][c][i], a[c][i], mean);
+      for (int off = b.lanes / 2; off > 0; off >>= 1) mean += __shfl_xor_sync(0xFFFFFFFFu, mean, off);
+      mean *= inv[u];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int i = 0; i < V; ++i) mean = fmaf(p[c][i], a[c][i], mean);
-    for (int off = b.lanes / 2; off > 0; off >>= 1) mean += __shfl_xor_sync(0xFFFFFFFFu, mean, off);
-    if (t >= r1) continue;
+        for (int i = 0; i < V; ++i) p[u][c][i] = p[u][c][i] * inv[u] * (a[c][i] - mean);
+      if (b.sigmoid) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int e = (at + c * b.lanes) * V;
-      if (e >= b.experts) continue;
-      uint4 raw;
-      T* o = reinterpret_cast<T*>(&raw);
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float d = p[c][i] * (a[c][i] - mean);
-        if (b.sigmoid) d /= 1.0f + expf(l[c][i]);
-        o[i] = from_f32<T>(live ? d : 0.0f);
+          for (int i = 0; i < V; ++i) p[u][c][i] /= 1.0f + expf(l[u][c][i]);
       }
-      T* dst = dlogits + t * b.experts + e;
-      if constexpr (V == 1) *dst = o[0];
-      else *reinterpret_cast<uint4*>(dst) = raw;
+      const int64_t t = t0 + u * step + lane / b.lanes;
+      if (t < r1) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int e = (at + c * b.lanes) * V;
+          if (e >= b.experts) continue;
+          uint4 raw;
+          T* o = reinterpret_cast<T*>(&raw);
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] = from_f32<T>(own[u] >= 0 ? p[u][c][i] : 0.0f);
+          T* dst = dlogits + t * b.experts + e;
+          if constexpr (V == 1) *dst = o[0];
+          else *reinterpret_cast<uint4*>(dst) = raw;
+        }
+      }
     }
   }
 }
@@ -324,23 +432,24 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Balance b,
 constexpr int kMaxExperts = 1024, kMaxTopk = 32;
 constexpr int64_t kMaxTokens = 0x7FFFFFFF;
 
-// Rows of a block: four blocks to a multiprocessor, but four turns for every warp.
-int rows_of_block(int64_t tokens, int lanes) {
-  const int64_t spread = (int64_t)sm_count() * 4, least = 4 * kWarps * (32 / lanes);
-  const int64_t rows = (tokens + spread - 1) / spread;
-  return (int)(rows > least ? rows : least);
-}
-
-struct Plan { bool vector; int lanes, rows; int64_t blocks; };
+// How the rows are shared out.  A turn of a block takes the tokens that its lanes have in hand; calls of up to four turns are
+// one block's, larger ones are spread over the multiprocessors.
+struct Plan { bool vector; int pieces, lanes, rows; int64_t blocks; };
 Plan plan_of(const void* logits, int64_t ld, const void* other, int dtype, int64_t tokens, int experts) {
   Plan p;
   const int size = dtype == MOE_F32 ? 4 : 2, vec = 16 / size;
   p.vector = experts % vec == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)other & 15) == 0 && ld * size % 16 == 0;
-  const int pieces = p.vector ? experts / vec : experts;
+  const int width = p.vector ? vec : 1, pieces = experts / width;
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes < pieces) p.lanes *= 2;
-  p.rows = rows_of_block(tokens, p.lanes);
-  p.blocks = (tokens + p.rows - 1) / p.rows;
+  // pieces of a lane, as the kernels are built for them
+  p.pieces = p.vector ? (pieces <= 32 ? 1 : pieces <= 64 ? 2 : 32 / vec) : (pieces <= 64 ? 2 : pieces <= 256 ? 8 : 32);
+  const int64_t turn = (int64_t)kWarps * (32 / p.lanes) * tokens_in_hand(p.pieces * width), spread = (int64_t)sm_count() * kBlocksPerSm;
+  int64_t rows = (tokens + spread - 1) / spread;
+  if (rows < turn) rows = turn;
+  if (tokens <= 4 * turn) rows = tokens;
+  p.rows = (int)rows;
+  p.blocks = (tokens + rows - 1) / rows;
   return p;
 }
 
@@ -357,9 +466,9 @@ int64_t lay_out(int64_t tokens, int experts, int sequences, int64_t blocks, void
   if (out) *out = Slots{(float*)mass, (int32_t*)count, (int32_t*)tok, (int32_t*)flags, (double*)part};
   return at;
 }
-int64_t most_blocks(int64_t tokens) {  // least rows of a block: one token to a warp
-  const int64_t rows = rows_of_block(tokens, 32);
-  return (tokens + rows - 1) / rows;
+int64_t most_blocks(int64_t tokens) {
+  const int64_t turns = (tokens + kWarps - 1) / kWarps, spread = (int64_t)sm_count() * kBlocksPerSm;
+  return turns < spread ? turns : spread;
 }
 
 int check(const char* who, int64_t tokens, int experts, int topk, int sequences, int dtype, int64_t ld) {
@@ -373,14 +482,14 @@ int check(const char* who, int64_t tokens, int experts, int topk, int sequences,
 }  // namespace
 }  // namespace moe
 
-// Calls F(T, V, CH) for the kernels of a plan: CH pieces per lane.
-#define MOE_BALANCE_PIECES(F, T, VEC, plan, experts)                                       \
-  ((plan).vector ? ((experts) <= 32 * VEC ? F(T, VEC, 1) : (experts) <= 64 * VEC ? F(T, VEC, 2) : F(T, VEC, (32 / VEC))) \
-                 : ((experts) <= 64 ? F(T, 1, 2) : (experts) <= 256 ? F(T, 1, 8) : F(T, 1, 32)))
-#define MOE_BALANCE_DISPATCH(F, dtype, plan, experts)                                      \
-  ((dtype) == MOE_F32 ? MOE_BALANCE_PIECES(F, float, 4, plan, experts)                     \
-   : (dtype) == MOE_F16 ? MOE_BALANCE_PIECES(F, __half, 8, plan, experts)                  \
-                        : MOE_BALANCE_PIECES(F, __nv_bfloat16, 8, plan, experts))
+// Calls F(T, V, CH) for the kernel of a plan.
+#define MOE_BALANCE_PIECES(F, T, VEC, plan)                                                                       \
+  ((plan).vector ? ((plan).pieces == 1 ? F(T, VEC, 1) : (plan).pieces == 2 ? F(T, VEC, 2) : F(T, VEC, (32 / VEC))) \
+                 : ((plan).pieces == 2 ? F(T, 1, 2) : (plan).pieces == 8 ? F(T, 1, 8) : F(T, 1, 32)))
+#define MOE_BALANCE_DISPATCH(F, dtype, plan)                         \
+  ((dtype) == MOE_F32 ? MOE_BALANCE_PIECES(F, float, 4, plan)        \
+   : (dtype) == MOE_F16 ? MOE_BALANCE_PIECES(F, __half, 8, plan)     \
+                        : MOE_BALANCE_PIECES(F, __nv_bfloat16, 8, plan))
 
 extern "C" int moe_balance_loss_workspace(int64_t tokens, int experts, int topk, int sequences, int64_t* bytes) {
   using namespace moe;
@@ -414,14 +523,17 @@ extern "C" int moe_balance_loss(const void* logits, int64_t ld, int dtype, int64
   const Balance b = {logits, ld, topk_ids, cu_seqlens, is_padding, tokens, experts, topk, sequences, ids_int64 != 0, sigmoid != 0,
                      plan.rows, plan.lanes};
   const size_t smem = 4 * ((size_t)(kWarps + 1) * experts + 1);
-#define MOE_BL(T, V, CH) \
-  launch_pdl(balance_sums_kernel<T, V, CH>, dim3((unsigned)plan.blocks), kThreads, smem, 1, st, "balance_loss", b, slots, status)
-  rc = MOE_BALANCE_DISPATCH(MOE_BL, dtype, plan, experts);
+  const Result result = {counts, (int32_t*)saved, loss}, later = {};
+  const bool whole = plan.blocks == 1 && !cu_seqlens;
+#define MOE_BL(T, V, CH)                                                                                                            \
+  launch_pdl(balance_sums_kernel<T, V, CH>, dim3((unsigned)plan.blocks), kThreads, smem, 1, st, "balance_loss", b, slots, whole ? result : later, \
+             status)
+  rc = MOE_BALANCE_DISPATCH(MOE_BL, dtype, plan);
 #undef MOE_BL
-  if (rc) return rc;
+  if (rc || whole) return rc;
   // one sequence has its rows in all blocks, several have few each
   return launch_pdl(balance_loss_kernel, dim3((unsigned)((experts + 31) / 32), (unsigned)sequences), sequences == 1 ? 1024 : 256, 0, 1, st,
-                    "balance_loss (sum)", b, slots, counts, (int32_t*)saved, loss);
+                    "balance_loss (sum)", b, slots, result);
 }
 
 extern "C" int moe_balance_loss_grad(const void* logits, int64_t ld, int dtype, int64_t tokens, int experts, int topk, int sigmoid,
@@ -437,6 +549,6 @@ extern "C" int moe_balance_loss_grad(const void* logits, int64_t ld, int dtype, 
 #define MOE_BG(T, V, CH)                                                                                                               \
   launch_pdl(balance_grad_kernel<T, V, CH>, dim3((unsigned)plan.blocks), kThreads, 0, 1, st, "balance_loss_grad", b, (const int32_t*)saved, \
              dloss, (T*)dlogits)
-  return MOE_BALANCE_DISPATCH(MOE_BG, dtype, plan, experts);
+  return MOE_BALANCE_DISPATCH(MOE_BG, dtype, plan);
 #undef MOE_BG
 }

@@ -16,22 +16,53 @@
 namespace moe {
 namespace {
 
+// Two 16-bit values as fp32 and back, an instruction or less per value: element by element the norm took 21 instructions per
+// element and its gradient 30, and both waited for the integer pipe.
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // V consecutive elements that one thread moves at once: 16 bytes, or a single element where rows are not made of such pieces.
 template <typename T, int V> struct Piece {
-  uint4 raw;
+  uint4 raw = {0, 0, 0, 0};
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
-  __device__ __forceinline__ void clear() { raw = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ float get(int i) const { return ToF32<T>::get(reinterpret_cast<const T*>(&raw)[i]); }
-  __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (V == 4) {
+        v[i] = __uint_as_float(w[i]);
+      } else {
+        const float2 f = unpack2<T>(w[i]);
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[V]) {
+    if constexpr (V == 4)
+      raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    else
+      raw = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  }
 };
 template <typename T> struct Piece<T, 1> {
-  T raw;
+  T raw = from_f32<T>(0.0f);
   __device__ __forceinline__ void load(const T* p) { raw = *p; }
   __device__ __forceinline__ void store(T* p) const { *p = raw; }
-  __device__ __forceinline__ void clear() { raw = from_f32<T>(0.0f); }
-  __device__ __forceinline__ float get(int) const { return ToF32<T>::get(raw); }
-  __device__ __forceinline__ void set(int, float v) { raw = from_f32<T>(v); }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = ToF32<T>::get(raw); }
+  __device__ __forceinline__ void set(const float (&v)[1]) { raw = from_f32<T>(v[0]); }
 };
 
 // The V weights from element `at` on; the weight has the type of the rows or is fp32.
@@ -51,8 +82,7 @@ __device__ __forceinline__ void load_weight(const void* w, bool w_f32, int at, f
   } else {
     Piece<T, V> p;
     p.load(reinterpret_cast<const T*>(w) + at);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = p.get(i);
+    p.get(v);
   }
 }
 
@@ -60,8 +90,9 @@ struct Sum { static __device__ __forceinline__ float join(float a, float b) { re
 struct Max { static __device__ __forceinline__ float join(float a, float b) { return max_nan(a, b); } };
 
 // N values joined over the TPR threads of a row; every thread gets the same bits (fixed order).  `sh` holds N floats per
-// warp of the block; a caller that comes again puts a barrier between.
-template <class Op, int N, int TPR>
+// warp of the block; a caller that comes again puts a barrier between.  WHOLE: the block has no other rows at the time (else
+// the row's threads meet at a barrier of their own).
+template <class Op, int N, int TPR, bool WHOLE = true>
 __device__ __forceinline__ void join_row(float (&v)[N], float* sh) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1)
@@ -72,7 +103,8 @@ __device__ __forceinline__ void join_row(float (&v)[N], float* sh) {
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int n = 0; n < N; ++n) sh[warp * N + n] = v[n];
-    __syncthreads();
+    if constexpr (WHOLE) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(first / (TPR / 32) + 1), "n"(TPR) : "memory");
 #pragma unroll
     for (int n = 0; n < N; ++n) v[n] = sh[first * N + n];
 #pragma unroll
@@ -102,19 +134,37 @@ __device__ __forceinline__ uint8_t to_8bit(float v, int format) {  // fp8 conver
   return (uint8_t)(int8_t)max(-128, min(127, __float2int_rn(v)));  // NaN gives 0; its scale is NaN
 }
 
+// Four values rounded to the nearest whole number, halves to even, and cut to [-128, 127].
+__device__ __forceinline__ uint32_t pack_int8(float a, float b, float c, float d) {
+  uint32_t hi, out;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(__float2int_rn(d)), "r"(__float2int_rn(c)));
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(out) : "r"(__float2int_rn(b)), "r"(__float2int_rn(a)), "r"(hi));
+  return out;
+}
+
 // V quotients of one piece as bytes.
 template <int V>
 __device__ __forceinline__ void quantise(const float (&y)[V], float s, int format, uint8_t* dst) {
-  const bool plain = s > 1e-30f && s < 1e30f;  // where the reciprocal and its remainders stay normal numbers
-  const float inv = 1.0f / s;
   float d[V];
+  if (s > 1e-30f && s < 1e30f) {  // where the reciprocal and its remainders stay normal numbers
+    const float inv = 1.0f / s;
 #pragma unroll
-  for (int i = 0; i < V; ++i) d[i] = plain ? div_by_scale(y[i], s, inv) : y[i] / s;
+    for (int i = 0; i < V; ++i) d[i] = div_by_scale(y[i], s, inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = y[i] / s;
+  }
   uint32_t w[(V + 3) / 4] = {};
-  if (format == kE4M3 && V % 2 == 0) {
+  if (format == kE4M3 && V % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i + 1 < V; i += 2)
-      w[i / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(d[i], d[i + 1]), __NV_SATFINITE, __NV_E4M3) << (8 * (i & 3));
+    for (int i = 0; i + 3 < V; i += 4) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(d[i], d[i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(d[i + 2], d[i + 3]), __NV_SATFINITE, __NV_E4M3);
+      w[i / 4] = lo | hi << 16;
+    }
+  } else if (format == kInt8 && V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i + 3 < V; i += 4) w[i / 4] = pack_int8(d[i], d[i + 1], d[i + 2], d[i + 3]);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) w[i / 4] |= (uint32_t)to_8bit(d[i], format) << (8 * (i & 3));
@@ -153,72 +203,62 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
   const int t = threadIdx.x % TPR, pieces = p.cols / V;
   const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
   if (TPR <= 32 && row >= p.rows) return;  // wider rows fill their block, and the grid has no block too many
-  Piece<T, V> h[CH];
+  float h[CH][V];  // the stream, then its norm
   {
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_ld;
+    Piece<T, V> a[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      h[c].clear();
-      if (t + c * TPR < pieces) h[c].load(x + (t + c * TPR) * V);
-    }
+    for (int c = 0; c < CH; ++c)
+      if (t + c * TPR < pieces) a[c].load(x + (t + c * TPR) * V);
     if (p.residual != nullptr) {
       const T* r = reinterpret_cast<const T*>(p.residual) + row * p.residual_ld;
-      Piece<T, V> a[CH];
+      Piece<T, V> b[CH];
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        a[c].clear();
-        if (t + c * TPR < pieces) a[c].load(r + (t + c * TPR) * V);
-      }
+      for (int c = 0; c < CH; ++c)
+        if (t + c * TPR < pieces) b[c].load(r + (t + c * TPR) * V);
       T* out = reinterpret_cast<T*>(p.h) + row * p.h_ld;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
+        float u[V], v[V];
+        a[c].get(u);
+        b[c].get(v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[c].set(i, h[c].get(i) + a[c].get(i));
-        if (t + c * TPR < pieces) h[c].store(out + (t + c * TPR) * V);
+        for (int i = 0; i < V; ++i) u[i] += v[i];
+        a[c].set(u);
+        if (t + c * TPR < pieces) a[c].store(out + (t + c * TPR) * V);
       }
     }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) a[c].get(h[c]);
   }
   float ss[1] = {0.0f};
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int i = 0; i < V; ++i) ss[0] = fmaf(h[c].get(i), h[c].get(i), ss[0]);
+    for (int i = 0; i < V; ++i) ss[0] = fmaf(h[c][i], h[c][i], ss[0]);
   join_row<Sum, 1, TPR>(ss, sh[0]);
   const float inv = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps);
-  if constexpr (!QUANT) {
-    T* out = reinterpret_cast<T*>(p.y) + row * p.y_ld;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      if (t + c * TPR < pieces) {
-        float w[V];
-        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
+  for (int c = 0; c < CH; ++c) {
+    if (t + c * TPR < pieces) {
+      float w[V];
+      load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[c].set(i, h[c].get(i) * inv * w[i]);
-        h[c].store(out + (t + c * TPR) * V);
+      for (int i = 0; i < V; ++i) h[c][i] = h[c][i] * inv * w[i];
+      if (!QUANT || p.y != nullptr) {
+        Piece<T, V> o;
+        o.set(h[c]);
+        o.store(reinterpret_cast<T*>(p.y) + row * p.y_ld + (t + c * TPR) * V);
       }
     }
-  } else {
-    float y[CH][V], amax[CH];
+  }
+  if constexpr (QUANT) {
+    float amax[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       amax[c] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) y[c][i] = 0.0f;
-      if (t + c * TPR < pieces) {
-        float w[V];
-        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          y[c][i] = h[c].get(i) * inv * w[i];
-          amax[c] = max_nan(amax[c], fabsf(y[c][i]));
-        }
-        if (p.y != nullptr) {
-          Piece<T, V> o;
-#pragma unroll
-          for (int i = 0; i < V; ++i) o.set(i, y[c][i]);
-          o.store(reinterpret_cast<T*>(p.y) + row * p.y_ld + (t + c * TPR) * V);
-        }
-      }
+      for (int i = 0; i < V; ++i) amax[c] = max_nan(amax[c], fabsf(h[c][i]));  // zero beyond the row
     }
     uint8_t* q = p.q + row * p.cols;
     if (p.group == p.cols) {
@@ -230,18 +270,19 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
       if (t == 0) *scale_at(p, row, 0) = s;
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        if (t + c * TPR < pieces) quantise<V>(y[c], s, p.format, q + (t + c * TPR) * V);
+        if (t + c * TPR < pieces) quantise<V>(h[c], s, p.format, q + (t + c * TPR) * V);
     } else {
       const int lanes = p.group / V;  // a power of two up to 32: the pieces of a group lie in one warp
+      for (int off = lanes / 2; off > 0; off >>= 1)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) amax[c] = max_nan(amax[c], __shfl_xor_sync(0xFFFFFFFFu, amax[c], off));
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        float m = amax[c];
-        for (int off = lanes / 2; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
         const int piece = t + c * TPR;
         if (piece < pieces) {
-          const float s = group_scale(m, p.quant_eps, p.format, p.ue8m0);
-          if (piece % lanes == 0) *scale_at(p, row, piece / lanes) = s;
-          quantise<V>(y[c], s, p.format, q + piece * V);
+          const float s = group_scale(amax[c], p.quant_eps, p.format, p.ue8m0);
+          if ((piece & (lanes - 1)) == 0) *scale_at(p, row, piece / lanes) = s;
+          quantise<V>(h[c], s, p.format, q + piece * V);
         }
       }
     }
@@ -313,91 +354,179 @@ struct Backward {
   float eps;
 };
 
-// Rows dealt out to the blocks in turn; a thread keeps its columns' part of dw in registers over all of them.
-template <typename T, int V, int TPR, int CH, int BLOCK = (TPR > 128 ? TPR : 128)>
-__global__ void __launch_bounds__(BLOCK) rms_norm_grad_kernel(const Backward p) {
+// 16 bytes into shared memory behind the thread's back.
+__device__ __forceinline__ void copy16(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+// Rows made of 16-byte pieces: TPR threads to a row, 512 / TPR rows of a block at a time, dealt out in turn; a thread keeps its
+// columns' part of dw in registers over all of them.  The rows to come are on their way into shared memory meanwhile.  A thread
+// fetches the pieces that it reads itself, so the copies need no barrier, only the thread's own wait: per row there is the one
+// barrier of the two sums.  STAGES rows of dy, h and dh per group of threads make up to 196 KB in flight on a multiprocessor.
+constexpr int kGradThreads = 512;
+template <typename T, int TPR, int CH, int STAGES>
+__global__ void __launch_bounds__(kGradThreads, 1) rms_norm_grad_kernel(const Backward p) {
+  constexpr int V = 16 / sizeof(T), GROUPS = kGradThreads / TPR;
+  extern __shared__ uint4 ring[];  // [STAGES][3][CH][threads]
+  __shared__ float sh[2][kGradThreads / 32 * 2];
   pdl_wait();
   pdl_trigger();
-  constexpr int RPB = BLOCK / TPR;
-  __shared__ float sh[2][BLOCK / 32 * 2];
-  const int t = threadIdx.x % TPR, pieces = p.cols / V;
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, pieces = p.cols / V;
+  const int64_t row0 = (int64_t)group * gridDim.x + blockIdx.x, step = (int64_t)GROUPS * gridDim.x;
+  const bool with_dh = p.dh != nullptr && p.dx != nullptr;
+  auto slot = [&](int stage, int n, int c) { return ring + ((stage * 3 + n) * CH + c) * kGradThreads + threadIdx.x; };
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < p.rows) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int at = t + c * TPR;
+        if (at < pieces) {
+          copy16(slot(stage, 0, c), reinterpret_cast<const T*>(p.h) + row * p.h_ld + at * V);
+          copy16(slot(stage, 1, c), reinterpret_cast<const T*>(p.dy) + row * p.cols + at * V);
+          if (with_dh) copy16(slot(stage, 2, c), reinterpret_cast<const T*>(p.dh) + row * p.cols + at * V);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   float dw[CH][V];
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[c][i] = 0.0f;
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB, turn ^= 1) {
-    Piece<T, V> h[CH], g[CH], d[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      h[c].clear(); g[c].clear();
-      if (t + c * TPR < pieces) {
-        h[c].load(reinterpret_cast<const T*>(p.h) + row * p.h_ld + (t + c * TPR) * V);
-        g[c].load(reinterpret_cast<const T*>(p.dy) + row * p.cols + (t + c * TPR) * V);
-      }
-    }
-    if (p.dh != nullptr && p.dx != nullptr) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (t + c * TPR < pieces) d[c].load(reinterpret_cast<const T*>(p.dh) + row * p.cols + (t + c * TPR) * V);
-    }
+  for (int i = 0; i < STAGES; ++i) fetch(row0 + i * step, i);
+  int stage = 0, turn = 0;
+  for (int64_t row = row0; row < p.rows; row += step, turn ^= 1) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (t + c * TPR < pieces) {
-        float w[V];
+        Piece<T, V> a;
+        float h[V], g[V], w[V];
+        a.raw = *slot(stage, 0, c);
+        a.get(h);
+        a.raw = *slot(stage, 1, c);
+        a.get(g);
         load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          s[0] = fmaf(h[c].get(i), h[c].get(i), s[0]);
-          s[1] = fmaf(w[i] * g[c].get(i), h[c].get(i), s[1]);
+          s[0] = fmaf(h[i], h[i], s[0]);
+          s[1] = fmaf(w[i] * g[i], h[i], s[1]);
         }
       }
     }
-    join_row<Sum, 2, TPR>(s, sh[turn]);  // the other half is still read by threads that are a row behind
+    join_row<Sum, 2, TPR, TPR == kGradThreads>(s, sh[turn]);  // the other half is still read by threads that are a row behind
+    const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
+    const float k = inv * (s[1] / (float)p.cols);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (t + c * TPR < pieces) {
+        Piece<T, V> a;
+        float h[V], g[V], d[V], w[V];  // read again: kept in registers beside dw they would spill
+        a.raw = *slot(stage, 0, c);
+        a.get(h);
+        a.raw = *slot(stage, 1, c);
+        a.get(g);
+        a.raw = with_dh ? *slot(stage, 2, c) : make_uint4(0, 0, 0, 0);
+        a.get(d);
+        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float x = h[i] * inv;
+          dw[c][i] = fmaf(g[i], x, dw[c][i]);
+          d[i] = fmaf(inv, fmaf(-x, k, w[i] * g[i]), d[i]);
+        }
+        if (p.dx != nullptr) {
+          a.set(d);
+          a.store(reinterpret_cast<T*>(p.dx) + row * p.cols + (t + c * TPR) * V);
+        }
+      }
+    }
+    fetch(row + STAGES * step, stage);  // over what this thread alone has read, and used
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  if (p.partial == nullptr) return;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  // the groups' sums meet in shared memory, in order
+  float* acc = reinterpret_cast<float*>(ring);
+  for (int r = 0; r < GROUPS; ++r) {
+    __syncthreads();
+    if (group == r) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (t + c * TPR < pieces) {
+            float* a = acc + (t + c * TPR) * V + i;
+            *a = r == 0 ? dw[c][i] : *a + dw[c][i];
+          }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.cols; i += kGradThreads) p.partial[(int64_t)blockIdx.x * p.cols + i] = acc[i];
+}
+
+// Rows that are not: element by element, straight into registers.
+template <typename T, int TPR, int CH, int BLOCK = (TPR > 128 ? TPR : 128)>
+__global__ void __launch_bounds__(BLOCK) rms_norm_grad_single_kernel(const Backward p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int RPB = BLOCK / TPR;
+  __shared__ float sh[2][BLOCK / 32 * 2];
+  const int t = threadIdx.x % TPR;
+  float dw[CH] = {};
+  int turn = 0;
+  auto weight = [&](int i) {
+    return p.w_f32 ? reinterpret_cast<const float*>(p.weight)[i] : ToF32<T>::get(reinterpret_cast<const T*>(p.weight)[i]);
+  };
+  for (int64_t row = (int64_t)(threadIdx.x / TPR) * gridDim.x + blockIdx.x; row < p.rows; row += (int64_t)gridDim.x * RPB, turn ^= 1) {
+    float h[CH], g[CH], d[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = t + c * TPR;
+      h[c] = g[c] = d[c] = 0.0f;
+      if (at < p.cols) {
+        h[c] = ToF32<T>::get(reinterpret_cast<const T*>(p.h)[row * p.h_ld + at]);
+        g[c] = ToF32<T>::get(reinterpret_cast<const T*>(p.dy)[row * p.cols + at]);
+        if (p.dh != nullptr) d[c] = ToF32<T>::get(reinterpret_cast<const T*>(p.dh)[row * p.cols + at]);
+      }
+    }
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (t + c * TPR < p.cols) {
+        s[0] = fmaf(h[c], h[c], s[0]);
+        s[1] = fmaf(weight(t + c * TPR) * g[c], h[c], s[1]);
+      }
+    }
+    join_row<Sum, 2, TPR>(s, sh[turn]);
     const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
     const float k = inv * inv * (s[1] / (float)p.cols);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      if (t + c * TPR < pieces) {
-        float w[V];
-        load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
-        Piece<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float hv = h[c].get(i), gv = g[c].get(i);
-          dw[c][i] = fmaf(gv, hv * inv, dw[c][i]);
-          float v = inv * (w[i] * gv - hv * k);
-          if (p.dh != nullptr && p.dx != nullptr) v += d[c].get(i);
-          o.set(i, v);
-        }
-        if (p.dx != nullptr) o.store(reinterpret_cast<T*>(p.dx) + row * p.cols + (t + c * TPR) * V);
+      const int at = t + c * TPR;
+      if (at < p.cols) {
+        dw[c] = fmaf(g[c], h[c] * inv, dw[c]);
+        if (p.dx != nullptr) reinterpret_cast<T*>(p.dx)[row * p.cols + at] = from_f32<T>(fmaf(inv, weight(at) * g[c] - h[c] * k, d[c]));
       }
     }
   }
   if (p.partial == nullptr) return;
-  if constexpr (RPB > 1) {  // several rows at a time: their threads' sums meet in shared memory, in order
-    __shared__ float acc[TPR * CH * V];
-    for (int r = 0; r < RPB; ++r) {
-      if ((int)threadIdx.x / TPR == r) {
+  __shared__ float acc[RPB > 1 ? TPR * CH : 1];
+  for (int r = 0; r < RPB; ++r) {  // the rows at a time of a block: their threads' sums meet in order
+    if (RPB > 1) __syncthreads();
+    if ((int)threadIdx.x / TPR == r) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float* a = acc + (t + c * TPR) * V + i;
-            *a = r == 0 ? dw[c][i] : *a + dw[c][i];
-          }
+      for (int c = 0; c < CH; ++c) {
+        const int at = t + c * TPR;
+        if (at >= p.cols) continue;
+        const float v = r == 0 ? dw[c] : acc[RPB > 1 ? at : 0] + dw[c];
+        if (r + 1 == RPB) p.partial[(int64_t)blockIdx.x * p.cols + at] = v;
+        else acc[at] = v;
       }
-      __syncthreads();
     }
-    for (int i = threadIdx.x; i < p.cols; i += BLOCK) p.partial[(int64_t)blockIdx.x * p.cols + i] = acc[i];
-  } else {
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (t + c * TPR < pieces) p.partial[(int64_t)blockIdx.x * p.cols + (t + c * TPR) * V + i] = dw[c][i];
   }
 }
 
@@ -409,9 +538,12 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
   __shared__ float sh[32][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
   float s = 0.0f;
-  if (col < cols) {
-#pragma unroll 4
-    for (int i = r; i < parts; i += 32) s += partial[(int64_t)i * cols + col];
+  for (int i = r; i < parts; i += 32 * 5) {  // a part for every multiprocessor in one go
+    float v[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) v[j] = col < cols && i + 32 * j < parts ? partial[(int64_t)(i + 32 * j) * cols + col] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 5; ++j) s += v[j];
   }
   sh[r][threadIdx.x & 31] = s;
   __syncthreads();
@@ -512,7 +644,6 @@ int forward(const Forward& p, int dtype, bool quant, cudaStream_t st) {
 }
 
 constexpr int64_t kMaxRows = 0x7FFFFFFF;  // blocks of a grid
-constexpr int kPartsPerSm = 2;            // blocks of the gradient, each with its part of dw
 
 // Checks that both forward entry points share.
 int check_forward(const char* who, const void* x, int dtype, int weight_dtype, const void* residual, const void* weight, int64_t rows,
@@ -528,29 +659,47 @@ int check_forward(const char* who, const void* x, int dtype, int weight_dtype, c
   return 0;
 }
 
-int grad_blocks(int64_t rows) {
-  const int64_t most = (int64_t)sm_count() * kPartsPerSm;
+// Blocks of the gradient, each with its part of dw: one to a multiprocessor, whose shared memory it fills, or two.
+int grad_blocks(int64_t rows, bool vector) {
+  const int64_t most = (int64_t)sm_count() * (vector ? 1 : 2);
   return (int)(rows < most ? rows : most);
 }
 
 template <typename T>
+int launch_grad_any(const Backward& p, int parts, cudaStream_t st) {
+  float* inv = p.partial ? p.partial + (int64_t)parts * p.cols : nullptr;
+  const int rc = launch_pdl(rms_norm_grad_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm_grad", p, inv);
+  if (rc || !p.partial) return rc;
+  return launch_pdl(weight_grad_any_kernel<T>, dim3((unsigned)((p.cols + 255) / 256), (unsigned)parts), 256, 0, 1, st, "rms_norm_grad", p,
+                    (const float*)inv);
+}
+
+template <typename T, int TPR, int CH, int STAGES>
+int launch_grad_ring(const Backward& p, int parts, cudaStream_t st) {
+  constexpr int smem = STAGES * 3 * CH * kGradThreads * 16;
+  static_assert(smem + 1024 <= 227 * 1024, "the ring fits a multiprocessor");
+  const int rc = allow_smem((const void*)rms_norm_grad_kernel<T, TPR, CH, STAGES>, smem);
+  if (rc) return rc;
+  return launch_pdl(rms_norm_grad_kernel<T, TPR, CH, STAGES>, dim3((unsigned)parts), kGradThreads, smem, 1, st, "rms_norm_grad", p);
+}
+
+template <typename T>
 int launch_backward(const Backward& p, bool vector, int parts, cudaStream_t st) {
-  constexpr int VEC = 16 / sizeof(T);
-  const Split s = split_of(vector ? p.cols / VEC : p.cols, vector);
-#define MOE_RG(V, TPR, CH) launch_pdl(rms_norm_grad_kernel<T, V, TPR, CH>, dim3((unsigned)parts), TPR > 128 ? TPR : 128, 0, 1, st, "rms_norm_grad", p)
-  if (s.threads == 0 || s.threads == 1024) {
-    float* inv = p.partial ? p.partial + (int64_t)parts * p.cols : nullptr;
-    int rc = launch_pdl(rms_norm_grad_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm_grad", p, inv);
-    if (rc || !p.partial) return rc;
-    return launch_pdl(weight_grad_any_kernel<T>, dim3((unsigned)((p.cols + 255) / 256), (unsigned)parts), 256, 0, 1, st, "rms_norm_grad", p,
-                      (const float*)inv);
-  }
   if (vector) {
-    if (s.threads == 32) return s.chunks == 4 ? MOE_RG(VEC, 32, 4) : MOE_RG(VEC, 32, 8);
-    return s.threads == 256 ? MOE_RG(VEC, 256, 4) : MOE_RG(VEC, 512, 4);
+    const int pieces = p.cols / (16 / (int)sizeof(T));
+    if (pieces <= 32 * 4) return launch_grad_ring<T, 32, 4, 2>(p, parts, st);
+    if (pieces <= 64 * 4) return launch_grad_ring<T, 64, 4, 2>(p, parts, st);
+    if (pieces <= 128 * 4) return launch_grad_ring<T, 128, 4, 2>(p, parts, st);
+    if (pieces <= 256 * 4) return launch_grad_ring<T, 256, 4, 2>(p, parts, st);
+    if (pieces <= 512 * 4) return launch_grad_ring<T, 512, 4, 2>(p, parts, st);
+    return launch_grad_any<T>(p, parts, st);
   }
-  if (s.threads == 32) return MOE_RG(1, 32, 4);
-  return s.threads == 256 ? MOE_RG(1, 256, 4) : MOE_RG(1, 512, 4);
+#define MOE_RG(TPR, CH) \
+  launch_pdl(rms_norm_grad_single_kernel<T, TPR, CH>, dim3((unsigned)parts), TPR > 128 ? TPR : 128, 0, 1, st, "rms_norm_grad", p)
+  if (p.cols <= 32 * 4) return MOE_RG(32, 4);
+  if (p.cols <= 256 * 4) return MOE_RG(256, 4);
+  if (p.cols <= 512 * 4) return MOE_RG(512, 4);
+  return launch_grad_any<T>(p, parts, st);
 #undef MOE_RG
 }
 
@@ -600,7 +749,7 @@ extern "C" int moe_rms_norm_grad_workspace(int64_t rows, int64_t cols, int64_t* 
   using namespace moe;
   if (rows < 0 || cols <= 0 || cols > (1 << 24) || !bytes) return fail(MOE_E_BADARG, "rms_norm_grad: bad extent");
   if (rows > kMaxRows) return fail(MOE_E_TOOBIG, "rms_norm_grad: too many rows");
-  *bytes = 4 * ((int64_t)grad_blocks(rows) * cols + rows);
+  *bytes = 4 * ((int64_t)grad_blocks(rows, false) * cols + rows);
   return 0;
 }
 
@@ -617,8 +766,7 @@ extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, cons
     return ce == cudaSuccess ? 0 : fail((int)ce, "rms_norm_grad: %s", cudaGetErrorString(ce));
   }
   if (!dy || (!dx && !dweight)) return fail(MOE_E_BADARG, "rms_norm_grad: null pointer");
-  const int parts = grad_blocks(rows);
-  if (dweight && (!workspace || workspace_bytes < 4 * ((int64_t)parts * cols + rows) || !aligned16(workspace)))
+  if (dweight && (!workspace || workspace_bytes < 4 * ((int64_t)grad_blocks(rows, false) * cols + rows) || !aligned16(workspace)))
     return fail(MOE_E_BADARG, "rms_norm_grad: workspace too small");
   Backward p = {};
   p.dy = dy; p.dh = dresidual_out; p.h = h; p.weight = weight; p.dx = dx; p.partial = dweight ? (float*)workspace : nullptr;
@@ -626,6 +774,7 @@ extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, cons
   const int size = dtype == MOE_F32 ? 4 : 2;
   const bool vector = cols % (16 / size) == 0 && pieces16(h, h_ld, size) && aligned16(dy) && aligned16(dresidual_out) && aligned16(dx) &&
                       aligned16(weight);
+  const int parts = grad_blocks(rows, vector);
   rc = dtype == MOE_F32 ? launch_backward<float>(p, vector, parts, st)
        : dtype == MOE_F16 ? launch_backward<__half>(p, vector, parts, st)
                           : launch_backward<__nv_bfloat16>(p, vector, parts, st);

@@ -14,7 +14,7 @@ from . import _lib
 
 logger = logging.getLogger(__name__)
 
-_MAX_EXPERTS, _MAX_TOPK, _MAX_SEQUENCES = 1024, 32, 65535
+_MAX_EXPERTS, _MAX_TOPK, _MAX_SEQUENCES, _MAX_ROUTES = 1024, 32, 65535, 0x7FFF0000
 
 
 def moe_balance_loss(
@@ -55,8 +55,8 @@ def moe_balance_loss(
         raise NotImplementedError(f"moe_balance_loss supports 1 to {_MAX_TOPK} routes per token")
     if ids.dtype not in (torch.int32, torch.int64, torch.uint32):
         raise TypeError("topk_ids must be int32/int64/uint32")
-    if ids.numel() >= 1 << 31:
-        raise ValueError("moe_balance_loss: at most 2^31 - 1 routes")
+    if ids.numel() > _MAX_ROUTES:
+        raise ValueError("moe_balance_loss: at most 2^31 - 2^16 routes")
     if cu_seqlens is not None:
         if cu_seqlens.ndim != 1 or cu_seqlens.dtype != torch.int32 or cu_seqlens.numel() < 2:
             raise ValueError("cu_seqlens must be int32 [sequences + 1] with at least one sequence")

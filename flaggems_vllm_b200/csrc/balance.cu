@@ -20,7 +20,8 @@
 namespace moe {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBlocksPerSm = 2;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kSumBlocks = 3, kGradBlocks = 2;  // of a multiprocessor, as their registers allow: one wave
 
 struct Balance {
   const void* logits;
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b,
   int32_t* hist = reinterpret_cast<int32_t*>(sh + kWarps * b.experts);
   int32_t* live_tokens = hist + b.experts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, step = kWarps * groups;
+  const int group = lane / b.lanes, at = lane % b.lanes;
   const int64_t r0 = (int64_t)blockIdx.x * b.rows, r1 = min(b.tokens, r0 + b.rows);
   if (blockIdx.x == 0 && result.loss == nullptr) {
     int bad = 0;
@@ -205,14 +207,16 @@ __global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b,
     }
     float acc[CH][V] = {};
     int mine = 0;
-    for (int64_t t0 = first + warp * groups; t0 < last; t0 += U * step) {
+    const T* row = reinterpret_cast<const T*>(b.logits) + (first + warp * groups + group) * b.ld;
+    const int64_t apart = step * b.ld;
+    for (int t0 = (int)first + warp * groups + group; t0 - group < (int)last; t0 += U * step, row += U * apart) {
       float l[U][CH][V], p[U][CH][V], inv[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t t = t0 + u * step + lane / b.lanes;
-        const bool live = t < last && (b.padding == nullptr || !b.padding[t]);
-        load_row<T, V, CH>(reinterpret_cast<const T*>(b.logits) + t * b.ld, lane % b.lanes, b.lanes, b.experts, live, l[u]);
-        mine += live && lane % b.lanes == 0;
+        const int t = t0 + u * step;
+        const bool live = t < (int)last && (b.padding == nullptr || !b.padding[t]);
+        load_row<T, V, CH>(row + u * apart, at, b.lanes, b.experts, live, l[u]);
+        mine += live && at == 0;
       }
       scores<V, CH, U>(l, b.lanes, b.sigmoid, p, inv);
 #pragma unroll
@@ -289,18 +293,18 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
   float m = 0.0f;
   int n = 0, live = 0;
   for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) live += in.tokens[c + s];
-  for (int c = c0 + warp; c < c1; c += 10 * warps) {  // ten slots in flight: two a multiprocessor are one round of 32 warps
-    float mv[10];
-    int nv[10];
+  for (int c = c0 + warp; c < c1; c += 14 * warps) {  // as many in flight: three slots a multiprocessor are one round of 32 warps
+    float mv[14];
+    int nv[14];
 #pragma unroll
-    for (int j = 0; j < 10; ++j) {
+    for (int j = 0; j < 14; ++j) {
       const bool there = e < b.experts && c + j * warps < c1;
       const int64_t at = (int64_t)(c + j * warps + s) * b.experts + e;
       mv[j] = there ? in.mass[at] : 0.0f;
       nv[j] = there ? in.count[at] : 0;
     }
 #pragma unroll
-    for (int j = 0; j < 10; ++j) { m += mv[j]; n += nv[j]; }
+    for (int j = 0; j < 14; ++j) { m += mv[j]; n += nv[j]; }
   }
   mass[warp][lane] = m;
   count[warp][lane] = n;
@@ -352,30 +356,35 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
 }
 
 template <typename T, int V, int CH>
-__global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Balance b, const int32_t* __restrict__ saved,
+__global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_kernel(const Balance b, const int32_t* __restrict__ saved,
                                                                 const float* __restrict__ dloss, T* __restrict__ dlogits) {
   pdl_wait();
   pdl_trigger();
   constexpr int U = tokens_in_hand(V * CH);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, at = lane % b.lanes, step = kWarps * groups;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, step = kWarps * groups;
+  const int group = lane / b.lanes, at = lane % b.lanes;
   const int64_t r0 = (int64_t)blockIdx.x * b.rows, r1 = min(b.tokens, r0 + b.rows);
   const int32_t* live_tokens = saved + (int64_t)b.sequences * b.experts;
   const double scale = (double)*dloss / (double)max(1, live_tokens[b.sequences]);
-  int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0 + warp * groups + lane / b.lanes), held = -1;
+  int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0 + warp * groups + group), held = -1;
   float a[CH][V] = {};
-  for (int64_t t0 = r0 + warp * groups; t0 < r1; t0 += U * step) {
+  const T* row = reinterpret_cast<const T*>(b.logits) + (r0 + warp * groups + group) * b.ld;
+  T* drow = dlogits + (r0 + warp * groups + group) * b.experts;
+  const int64_t apart = step * b.ld;
+  const int dapart = step * b.experts;
+  for (int t0 = (int)r0 + warp * groups + group; t0 - group < (int)r1; t0 += U * step, row += U * apart, drow += U * dapart) {
     float l[U][CH][V], p[U][CH][V], inv[U];
     int own[U];  // the token's sequence, -1 = its gradient is zero
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t t = t0 + u * step + lane / b.lanes;
-      bool live = t < r1 && (b.padding == nullptr || !b.padding[t]);
+      const int t = t0 + u * step;
+      bool live = t < (int)r1 && (b.padding == nullptr || !b.padding[t]);
       if (b.cu != nullptr) {
         while (s < b.sequences && b.cu[s + 1] <= t) ++s;
         live = live && s < b.sequences && b.cu[s] <= t;
       }
       own[u] = live ? s : -1;
-      load_row<T, V, CH>(reinterpret_cast<const T*>(b.logits) + t * b.ld, at, b.lanes, b.experts, live, l[u]);
+      load_row<T, V, CH>(row + u * apart, at, b.lanes, b.experts, live, l[u]);
     }
     scores<V, CH, U>(l, b.lanes, b.sigmoid, p, inv);
 #pragma unroll
@@ -410,8 +419,7 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Balance b,
 #pragma unroll
           for (int i = 0; i < V; ++i) p[u][c][i] /= 1.0f + expf(l[u][c][i]);
       }
-      const int64_t t = t0 + u * step + lane / b.lanes;
-      if (t < r1) {
+      if (t0 + u * step < (int)r1) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const int e = (at + c * b.lanes) * V;
@@ -420,7 +428,7 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Balance b,
           T* o = reinterpret_cast<T*>(&raw);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] = from_f32<T>(own[u] >= 0 ? p[u][c][i] : 0.0f);
-          T* dst = dlogits + t * b.experts + e;
+          T* dst = drow + u * dapart + e;
           if constexpr (V == 1) *dst = o[0];
           else *reinterpret_cast<uint4*>(dst) = raw;
         }
@@ -430,21 +438,21 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Balance b,
 }
 
 constexpr int kMaxExperts = 1024, kMaxTopk = 32;
-constexpr int64_t kMaxTokens = 0x7FFFFFFF;
+constexpr int64_t kMaxRoutes = 0x7FFF0000;  // a turn behind the last token is an int too
 
 // How the rows are shared out.  A turn of a block takes the tokens that its lanes have in hand; calls of up to four turns are
 // one block's, larger ones are spread over the multiprocessors.
 struct Plan { bool vector; int pieces, lanes, rows; int64_t blocks; };
-Plan plan_of(const void* logits, int64_t ld, const void* other, int dtype, int64_t tokens, int experts) {
+Plan plan_of(const void* logits, int64_t ld, const void* other, int dtype, int64_t tokens, int experts, int blocks_per_sm) {
   Plan p;
   const int size = dtype == MOE_F32 ? 4 : 2, vec = 16 / size;
   p.vector = experts % vec == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)other & 15) == 0 && ld * size % 16 == 0;
   const int width = p.vector ? vec : 1, pieces = experts / width;
+  // 16 values to a lane: the sums over its lanes and all else that is done once per token count half of what they do at eight
+  p.pieces = (experts <= 512 ? 16 : 32) / width;
   p.lanes = 1;
-  while (p.lanes < 32 && p.lanes < pieces) p.lanes *= 2;
-  // pieces of a lane, as the kernels are built for them
-  p.pieces = p.vector ? (pieces <= 32 ? 1 : pieces <= 64 ? 2 : 32 / vec) : (pieces <= 64 ? 2 : pieces <= 256 ? 8 : 32);
-  const int64_t turn = (int64_t)kWarps * (32 / p.lanes) * tokens_in_hand(p.pieces * width), spread = (int64_t)sm_count() * kBlocksPerSm;
+  while (p.lanes * p.pieces < pieces) p.lanes *= 2;
+  const int64_t turn = (int64_t)kWarps * (32 / p.lanes) * tokens_in_hand(p.pieces * width), spread = (int64_t)sm_count() * blocks_per_sm;
   int64_t rows = (tokens + spread - 1) / spread;
   if (rows < turn) rows = turn;
   if (tokens <= 4 * turn) rows = tokens;
@@ -467,15 +475,15 @@ int64_t lay_out(int64_t tokens, int experts, int sequences, int64_t blocks, void
   return at;
 }
 int64_t most_blocks(int64_t tokens) {
-  const int64_t turns = (tokens + kWarps - 1) / kWarps, spread = (int64_t)sm_count() * kBlocksPerSm;
+  const int64_t turns = (tokens + kWarps - 1) / kWarps, spread = (int64_t)sm_count() * kSumBlocks;
   return turns < spread ? turns : spread;
 }
 
 int check(const char* who, int64_t tokens, int experts, int topk, int sequences, int dtype, int64_t ld) {
   if (tokens < 0 || experts <= 0 || topk <= 0 || sequences < 1 || ld < 0) return fail(MOE_E_BADARG, "%s: bad extent", who);
   if (dtype != MOE_F32 && dtype != MOE_F16 && dtype != MOE_BF16) return fail(MOE_E_DTYPE, "%s: unsupported dtype %d", who, dtype);
-  if (experts > kMaxExperts || topk > kMaxTopk || tokens > kMaxTokens || tokens * topk > kMaxTokens || sequences > 65535)
-    return fail(MOE_E_TOOBIG, "%s: at most %d experts, %d routes per token, 65535 sequences and 2^31 - 1 routes", who, kMaxExperts, kMaxTopk);
+  if (experts > kMaxExperts || topk > kMaxTopk || tokens * topk > kMaxRoutes || sequences > 65535)
+    return fail(MOE_E_TOOBIG, "%s: at most %d experts, %d routes per token, 65535 sequences and 2^31 - 2^16 routes", who, kMaxExperts, kMaxTopk);
   return 0;
 }
 
@@ -483,9 +491,9 @@ int check(const char* who, int64_t tokens, int experts, int topk, int sequences,
 }  // namespace moe
 
 // Calls F(T, V, CH) for the kernel of a plan.
-#define MOE_BALANCE_PIECES(F, T, VEC, plan)                                                                       \
-  ((plan).vector ? ((plan).pieces == 1 ? F(T, VEC, 1) : (plan).pieces == 2 ? F(T, VEC, 2) : F(T, VEC, (32 / VEC))) \
-                 : ((plan).pieces == 2 ? F(T, 1, 2) : (plan).pieces == 8 ? F(T, 1, 8) : F(T, 1, 32)))
+#define MOE_BALANCE_PIECES(F, T, VEC, plan)                                               \
+  ((plan).vector ? ((plan).pieces == 16 / VEC ? F(T, VEC, (16 / VEC)) : F(T, VEC, (32 / VEC))) \
+                 : ((plan).pieces == 16 ? F(T, 1, 16) : F(T, 1, 32)))
 #define MOE_BALANCE_DISPATCH(F, dtype, plan)                         \
   ((dtype) == MOE_F32 ? MOE_BALANCE_PIECES(F, float, 4, plan)        \
    : (dtype) == MOE_F16 ? MOE_BALANCE_PIECES(F, __half, 8, plan)     \
@@ -516,7 +524,7 @@ extern "C" int moe_balance_loss(const void* logits, int64_t ld, int dtype, int64
     return ce == cudaSuccess ? 0 : fail((int)ce, "balance_loss: %s", cudaGetErrorString(ce));
   }
   if (!logits || !topk_ids || !workspace) return fail(MOE_E_BADARG, "balance_loss: null pointer");
-  const Plan plan = plan_of(logits, ld, nullptr, dtype, tokens, experts);
+  const Plan plan = plan_of(logits, ld, nullptr, dtype, tokens, experts, kSumBlocks);
   Slots slots;
   if (((uintptr_t)workspace & 15) || lay_out(tokens, experts, sequences, plan.blocks, workspace, &slots) > workspace_bytes)
     return fail(MOE_E_BADARG, "balance_loss: workspace too small");
@@ -543,7 +551,7 @@ extern "C" int moe_balance_loss_grad(const void* logits, int64_t ld, int dtype, 
   const int rc = check("balance_loss_grad", tokens, experts, topk, sequences, dtype, ld);
   if (rc || tokens == 0) return rc;
   if (!logits || !saved || !dloss || !dlogits || (!cu_seqlens && sequences != 1)) return fail(MOE_E_BADARG, "balance_loss_grad: bad argument");
-  const Plan plan = plan_of(logits, ld, dlogits, dtype, tokens, experts);
+  const Plan plan = plan_of(logits, ld, dlogits, dtype, tokens, experts, kGradBlocks);
   const Balance b = {logits, ld, nullptr, cu_seqlens, is_padding, tokens, experts, topk, sequences, 0, sigmoid != 0, plan.rows, plan.lanes};
   cudaStream_t st = (cudaStream_t)stream;
 #define MOE_BG(T, V, CH)                                                                                                               \

@@ -565,7 +565,7 @@ bool balance_args(const at::Tensor& l, const at::Tensor& ids, const at::Tensor* 
   p->sequences = 1;
   if (p->code < 0 || !p->status || p->experts <= 0 || p->experts > 1024 || p->topk <= 0 || p->topk > 32 || !cuda_dense(ids, p->dev) ||
       (!p->ids64 && ids.scalar_type() != at::kInt) || !rows_of(l, &p->tokens, &p->ld) || ids.size(0) != p->tokens ||
-      p->tokens * p->topk > 0x7FFFFFFF)
+      p->tokens * p->topk > 0x7FFF0000)
     return false;
   if (cu) {
     if (!cuda_dense(*cu, p->dev) || cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->numel() < 2 || cu->numel() > 65536) return false;

@@ -105,17 +105,27 @@ __device__ __forceinline__ void join_row(float (&v)[N], float* sh) {
       for (int n = 0; n < N; ++n) sh[warp * N + n] = v[n];
     if constexpr (WHOLE) __syncthreads();
     else asm volatile("bar.sync %0, %1;" ::"r"(first / (TPR / 32) + 1), "n"(TPR) : "memory");
+    // every warp joins the warps' values again, a lane each: a dozen instructions where reading them all took four times as many
+    constexpr int W = TPR / 32;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = sh[first * N + n];
+    for (int n = 0; n < N; ++n) v[n] = sh[(first + (lane & (W - 1))) * N + n];
 #pragma unroll
-    for (int i = 1; i < TPR / 32; ++i)
+    for (int off = W / 2; off > 0; off >>= 1)
 #pragma unroll
-      for (int n = 0; n < N; ++n) v[n] = Op::join(v[n], sh[(first + i) * N + n]);
+      for (int n = 0; n < N; ++n) v[n] = Op::join(v[n], __shfl_xor_sync(0xFFFFFFFFu, v[n], off));
   }
 }
 
-enum { kE4M3 = 0, kE5M2 = 1, kInt8 = 2 };
-__device__ __forceinline__ float quant_max(int format) { return format == kE4M3 ? 448.0f : format == kE5M2 ? 57344.0f : 127.0f; }
+// 1 / sqrt(x): the approximation and one step of Newton's method, within two roundings; 0 for infinity, NaN for NaN.
+__device__ __forceinline__ float inverse_root(float x) {
+  const float r = rsqrtf(x);
+  const float better = r * fmaf(-0.5f * x * r, r, 1.5f);
+  return x > 1e-30f && x < 1e30f ? better : r;
+}
+
+enum { kNone = -1, kE4M3 = 0, kE5M2 = 1, kInt8 = 2 };
+__device__ __forceinline__ constexpr float quant_max(int format) { return format == kE4M3 ? 448.0f : format == kE5M2 ? 57344.0f : 127.0f; }
 
 // The scale of a group from its largest magnitude.  A NaN in the group makes the scale NaN, as it makes the values it stands for.
 __device__ __forceinline__ float group_scale(float amax, float eps, int format, bool ue8m0) {
@@ -179,30 +189,30 @@ struct Forward {
   void *y, *h;                        // y: null = not wanted; h: null without a residual
   int64_t x_ld, residual_ld, y_ld, h_ld, rows;
   int cols, w_f32;
-  float eps;
+  float eps, mean;  // mean: 1 / cols
   // 8-bit output
   uint8_t* q;
   float* scales;
   int64_t scale_ld;  // of the transposed layout
-  int group, format, transposed, ue8m0;
+  int group, groups, format, transposed, ue8m0;
   float quant_eps;
 };
 
 __device__ __forceinline__ float* scale_at(const Forward& p, int64_t row, int group_index) {
-  return p.transposed ? p.scales + (int64_t)group_index * p.scale_ld + row
-                      : p.scales + row * (p.cols / p.group) + group_index;
+  return p.transposed ? p.scales + (int64_t)group_index * p.scale_ld + row : p.scales + row * p.groups + group_index;
 }
 
 // One row per TPR threads, kept in registers: CH pieces of V elements per thread.  x and y (residual and h) may be the same
 // memory: a thread has read its pieces before it writes them, and nobody else reads them.
-template <typename T, int V, int TPR, int CH, bool QUANT, int BLOCK = (TPR > 128 ? TPR : 128)>
+template <typename T, int V, int TPR, int CH, int FORMAT, int BLOCK = (TPR > 128 ? TPR : 128)>
 __global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
+  constexpr bool QUANT = FORMAT != kNone;
   pdl_wait();
   pdl_trigger();
   __shared__ float sh[2][BLOCK / 32];
   const int t = threadIdx.x % TPR, pieces = p.cols / V;
   const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
-  if (TPR <= 32 && row >= p.rows) return;  // wider rows fill their block, and the grid has no block too many
+  if (row >= p.rows) return;  // whole warps, and all threads of a row: no barrier is left short
   float h[CH][V];  // the stream, then its norm
   {
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_ld;
@@ -236,8 +246,8 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int i = 0; i < V; ++i) ss[0] = fmaf(h[c][i], h[c][i], ss[0]);
-  join_row<Sum, 1, TPR>(ss, sh[0]);
-  const float inv = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps);
+  join_row<Sum, 1, TPR, TPR == BLOCK>(ss, sh[0]);
+  const float inv = inverse_root(fmaf(ss[0], p.mean, p.eps));
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     if (t + c * TPR < pieces) {
@@ -265,14 +275,17 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
       float m[1] = {amax[0]};
 #pragma unroll
       for (int c = 1; c < CH; ++c) m[0] = max_nan(m[0], amax[c]);
-      join_row<Max, 1, TPR>(m, sh[1]);
-      const float s = group_scale(m[0], p.quant_eps, p.format, p.ue8m0);
+      join_row<Max, 1, TPR, TPR == BLOCK>(m, sh[1]);
+      const float s = group_scale(m[0], p.quant_eps, FORMAT, p.ue8m0);
       if (t == 0) *scale_at(p, row, 0) = s;
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        if (t + c * TPR < pieces) quantise<V>(h[c], s, p.format, q + (t + c * TPR) * V);
+        if (t + c * TPR < pieces) quantise<V>(h[c], s, FORMAT, q + (t + c * TPR) * V);
     } else {
-      const int lanes = p.group / V;  // a power of two up to 32: the pieces of a group lie in one warp
+      // the pieces of a group, a power of two up to 32, lie in one warp
+      const int lanes = p.group / V, shift = 31 - __clz(lanes);
+      float* scales = scale_at(p, row, 0);
+      const int64_t apart = p.transposed ? p.scale_ld : 1;
       for (int off = lanes / 2; off > 0; off >>= 1)
 #pragma unroll
         for (int c = 0; c < CH; ++c) amax[c] = max_nan(amax[c], __shfl_xor_sync(0xFFFFFFFFu, amax[c], off));
@@ -280,9 +293,9 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_kernel(const Forward p) {
       for (int c = 0; c < CH; ++c) {
         const int piece = t + c * TPR;
         if (piece < pieces) {
-          const float s = group_scale(amax[c], p.quant_eps, p.format, p.ue8m0);
-          if ((piece & (lanes - 1)) == 0) *scale_at(p, row, piece / lanes) = s;
-          quantise<V>(h[c], s, p.format, q + piece * V);
+          const float s = group_scale(amax[c], p.quant_eps, FORMAT, p.ue8m0);
+          if ((piece & (lanes - 1)) == 0) scales[(piece >> shift) * apart] = s;
+          quantise<V>(h[c], s, FORMAT, q + piece * V);
         }
       }
     }
@@ -312,7 +325,7 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(const Forward p) {
     for (int i = threadIdx.x; i < p.cols; i += 256) ss[0] = fmaf(ToF32<T>::get(x[i]), ToF32<T>::get(x[i]), ss[0]);
   }
   join_row<Sum, 1, 256>(ss, sh[0]);  // its barrier also makes h visible to the block
-  const float inv = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps);
+  const float inv = inverse_root(fmaf(ss[0], p.mean, p.eps));
   auto norm = [&](int i) {
     const float w = p.w_f32 ? reinterpret_cast<const float*>(p.weight)[i] : ToF32<T>::get(reinterpret_cast<const T*>(p.weight)[i]);
     return ToF32<T>::get(src[i]) * inv * w;
@@ -328,7 +341,7 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(const Forward p) {
       for (int i = threadIdx.x; i < p.cols; i += 256) q[i] = to_8bit(norm(i) / s, p.format);
     } else {  // a warp per group
       const int lane = threadIdx.x & 31;
-      for (int g = threadIdx.x >> 5; g < p.cols / p.group; g += 8) {
+      for (int g = threadIdx.x >> 5; g < p.groups; g += 8) {
         float m[1] = {0.0f};
         for (int i = lane; i < p.group; i += 32) m[0] = max_nan(m[0], fabsf(norm(g * p.group + i)));
         join_row<Max, 1, 32>(m, nullptr);
@@ -351,7 +364,7 @@ struct Backward {
   float* partial;                    // [blocks, cols] sums of dw; null = not wanted
   int64_t h_ld, rows;
   int cols, w_f32;
-  float eps;
+  float eps, mean;  // mean: 1 / cols
 };
 
 // 16 bytes into shared memory behind the thread's back.
@@ -359,22 +372,22 @@ __device__ __forceinline__ void copy16(uint4* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 
-// Rows made of 16-byte pieces: TPR threads to a row, 512 / TPR rows of a block at a time, dealt out in turn; a thread keeps its
+// Rows made of 16-byte pieces: TPR threads to a row, THREADS / TPR rows of a block at a time, dealt out in turn; a thread keeps its
 // columns' part of dw in registers over all of them.  The rows to come are on their way into shared memory meanwhile.  A thread
 // fetches the pieces that it reads itself, so the copies need no barrier, only the thread's own wait: per row there is the one
 // barrier of the two sums.  STAGES rows of dy, h and dh per group of threads make up to 196 KB in flight on a multiprocessor.
-constexpr int kGradThreads = 512;
-template <typename T, int TPR, int CH, int STAGES>
-__global__ void __launch_bounds__(kGradThreads, 1) rms_norm_grad_kernel(const Backward p) {
-  constexpr int V = 16 / sizeof(T), GROUPS = kGradThreads / TPR;
+template <typename T, int TPR, int CH, int STAGES, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backward p) {
+  constexpr int V = 16 / sizeof(T), GROUPS = THREADS / TPR;
+  static_assert(TPR == 32 || GROUPS <= 15, "a named barrier for each group beside the block's own");
   extern __shared__ uint4 ring[];  // [STAGES][3][CH][threads]
-  __shared__ float sh[2][kGradThreads / 32 * 2];
+  __shared__ float sh[2][THREADS / 32 * 2];
   pdl_wait();
   pdl_trigger();
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, pieces = p.cols / V;
   const int64_t row0 = (int64_t)group * gridDim.x + blockIdx.x, step = (int64_t)GROUPS * gridDim.x;
   const bool with_dh = p.dh != nullptr && p.dx != nullptr;
-  auto slot = [&](int stage, int n, int c) { return ring + ((stage * 3 + n) * CH + c) * kGradThreads + threadIdx.x; };
+  auto slot = [&](int stage, int n, int c) { return ring + ((stage * 3 + n) * CH + c) * THREADS + threadIdx.x; };
   auto fetch = [&](int64_t row, int stage) {
     if (row < p.rows) {
 #pragma unroll
@@ -417,9 +430,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) rms_norm_grad_kernel(const Ba
         }
       }
     }
-    join_row<Sum, 2, TPR, TPR == kGradThreads>(s, sh[turn]);  // the other half is still read by threads that are a row behind
-    const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
-    const float k = inv * (s[1] / (float)p.cols);
+    join_row<Sum, 2, TPR, TPR == THREADS>(s, sh[turn]);  // the other half is still read by threads that are a row behind
+    const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
+    const float k = inv * (s[1] * p.mean);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (t + c * TPR < pieces) {
@@ -465,7 +478,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) rms_norm_grad_kernel(const Ba
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < p.cols; i += kGradThreads) p.partial[(int64_t)blockIdx.x * p.cols + i] = acc[i];
+  for (int i = threadIdx.x; i < p.cols; i += THREADS) p.partial[(int64_t)blockIdx.x * p.cols + i] = acc[i];
 }
 
 // Rows that are not: element by element, straight into registers.
@@ -502,8 +515,8 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_grad_single_kernel(const Backw
       }
     }
     join_row<Sum, 2, TPR>(s, sh[turn]);
-    const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
-    const float k = inv * inv * (s[1] / (float)p.cols);
+    const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
+    const float k = inv * inv * (s[1] * p.mean);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = t + c * TPR;
@@ -573,8 +586,8 @@ __global__ void __launch_bounds__(256) rms_norm_grad_any_kernel(const Backward p
     s[1] = fmaf(weight(i) * ToF32<T>::get(dy[i]), hv, s[1]);
   }
   join_row<Sum, 2, 256>(s, sh);
-  const float inv = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
-  const float k = inv * inv * (s[1] / (float)p.cols);
+  const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
+  const float k = inv * inv * (s[1] * p.mean);
   if (inv_rms != nullptr && threadIdx.x == 0) inv_rms[row] = inv;
   if (p.dx == nullptr) return;
   for (int i = threadIdx.x; i < p.cols; i += 256) {
@@ -599,47 +612,65 @@ __global__ void __launch_bounds__(256) weight_grad_any_kernel(const Backward p, 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool pieces16(const void* p, int64_t ld, int size) { return aligned16(p) && ld * size % 16 == 0; }
 
-// How a row is shared out: threads to a row and pieces to a thread; 0 threads = the kernel for any row.
-struct Split { int threads, chunks; };
-Split split_of(int pieces, bool vector) {
-  if (pieces <= 32 * 4) return {32, 4};
-  if (pieces <= 256) return {vector ? 32 : 256, vector ? 8 : 4};
-  if (pieces <= 256 * 4) return {256, 4};
-  if (pieces <= 512 * 4) return {512, 4};
-  if (!vector && pieces <= 1024 * 8) return {1024, 8};
-  return {0, 0};
+// Threads to a row that give each up to four pieces, all in flight at once; 0 = the kernel for any row.
+int threads_of(int pieces, bool vector) {
+  if (pieces <= 32 * 4) return 32;
+  if (pieces <= 64 * 4 && vector) return 64;
+  if (pieces <= 128 * 4 && vector) return 128;
+  if (pieces <= 256 * 4) return 256;
+  if (pieces <= 512 * 4) return 512;
+  return !vector && pieces <= 1024 * 8 ? 1024 : 0;
 }
 
-template <typename T, bool QUANT>
+template <typename T, int V, int TPR, int CH, int FORMAT>
+int launch_rows(const Forward& p, cudaStream_t st) {
+  constexpr int block = TPR > 128 ? TPR : 128, at_a_time = block / TPR;
+  return launch_pdl(rms_norm_kernel<T, V, TPR, CH, FORMAT>, dim3((unsigned)((p.rows + at_a_time - 1) / at_a_time)), block, 0, 1, st, "rms_norm", p);
+}
+
+template <typename T, int FORMAT>
 int launch_forward(const Forward& p, bool vector, cudaStream_t st) {
   constexpr int VEC = 16 / sizeof(T);
-  const Split s = split_of(vector ? p.cols / VEC : p.cols, vector);
-#define MOE_RN(V, TPR, CH)                                                                                                 \
-  launch_pdl(rms_norm_kernel<T, V, TPR, CH, QUANT>, dim3((unsigned)((p.rows + (TPR > 128 ? 1 : 128 / TPR) - 1) / (TPR > 128 ? 1 : 128 / TPR))), \
-             TPR > 128 ? TPR : 128, 0, 1, st, "rms_norm", p)
+  const int width = vector ? VEC : 1, threads = threads_of(p.cols / width, vector), lanes = p.group / width;
   // groups of a power of two of pieces within a warp, or whole rows, are quantised from registers
-  const int lanes = QUANT ? p.group / (vector ? VEC : 1) : 0;
-  const bool held = !QUANT || p.group == p.cols || (p.group % (vector ? VEC : 1) == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0);
-  if (s.threads == 0 || !held) return launch_pdl(rms_norm_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm", p);
+  const bool held = FORMAT == kNone || p.group == p.cols || (p.group % width == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0);
+  if (threads == 0 || !held) return launch_pdl(rms_norm_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm", p);
   if (vector) {
-    if (s.threads == 32) return s.chunks == 4 ? MOE_RN(VEC, 32, 4) : MOE_RN(VEC, 32, 8);
-    return s.threads == 256 ? MOE_RN(VEC, 256, 4) : MOE_RN(VEC, 512, 4);
+    switch (threads) {
+      case 32: return launch_rows<T, VEC, 32, 4, FORMAT>(p, st);
+      case 64: return launch_rows<T, VEC, 64, 4, FORMAT>(p, st);
+      case 128: return launch_rows<T, VEC, 128, 4, FORMAT>(p, st);
+      case 256: return launch_rows<T, VEC, 256, 4, FORMAT>(p, st);
+      default: return launch_rows<T, VEC, 512, 4, FORMAT>(p, st);
+    }
   }
-  if (s.threads == 32) return MOE_RN(1, 32, 4);
-  if (s.threads == 256) return MOE_RN(1, 256, 4);
-  return s.threads == 512 ? MOE_RN(1, 512, 4) : MOE_RN(1, 1024, 8);
-#undef MOE_RN
+  switch (threads) {
+    case 32: return launch_rows<T, 1, 32, 4, FORMAT>(p, st);
+    case 256: return launch_rows<T, 1, 256, 4, FORMAT>(p, st);
+    case 512: return launch_rows<T, 1, 512, 4, FORMAT>(p, st);
+    default: return launch_rows<T, 1, 1024, 8, FORMAT>(p, st);
+  }
 }
 
-int forward(const Forward& p, int dtype, bool quant, cudaStream_t st) {
+template <typename T>
+int launch_format(const Forward& p, bool vector, cudaStream_t st) {
+  if (p.q == nullptr) return launch_forward<T, kNone>(p, vector, st);
+  switch (p.format) {
+    case kE4M3: return launch_forward<T, kE4M3>(p, vector, st);
+    case kE5M2: return launch_forward<T, kE5M2>(p, vector, st);
+    default: return launch_forward<T, kInt8>(p, vector, st);
+  }
+}
+
+int forward(const Forward& p, int dtype, cudaStream_t st) {
   const int size = dtype == MOE_F32 ? 4 : 2, vec = 16 / size;
   const bool vector = p.cols % vec == 0 && pieces16(p.x, p.x_ld, size) && (!p.residual || pieces16(p.residual, p.residual_ld, size)) &&
                       (!p.h || pieces16(p.h, p.h_ld, size)) && (!p.y || pieces16(p.y, p.y_ld, size)) && aligned16(p.weight) &&
                       (!p.q || aligned16(p.q));
   switch (dtype) {
-    case MOE_F32: return quant ? launch_forward<float, true>(p, vector, st) : launch_forward<float, false>(p, vector, st);
-    case MOE_F16: return quant ? launch_forward<__half, true>(p, vector, st) : launch_forward<__half, false>(p, vector, st);
-    default: return quant ? launch_forward<__nv_bfloat16, true>(p, vector, st) : launch_forward<__nv_bfloat16, false>(p, vector, st);
+    case MOE_F32: return launch_format<float>(p, vector, st);
+    case MOE_F16: return launch_format<__half>(p, vector, st);
+    default: return launch_format<__nv_bfloat16>(p, vector, st);
   }
 }
 
@@ -674,24 +705,24 @@ int launch_grad_any(const Backward& p, int parts, cudaStream_t st) {
                     (const float*)inv);
 }
 
-template <typename T, int TPR, int CH, int STAGES>
+template <typename T, int TPR, int CH, int STAGES, int THREADS>
 int launch_grad_ring(const Backward& p, int parts, cudaStream_t st) {
-  constexpr int smem = STAGES * 3 * CH * kGradThreads * 16;
+  constexpr int smem = STAGES * 3 * CH * THREADS * 16;
   static_assert(smem + 1024 <= 227 * 1024, "the ring fits a multiprocessor");
-  const int rc = allow_smem((const void*)rms_norm_grad_kernel<T, TPR, CH, STAGES>, smem);
+  const int rc = allow_smem((const void*)rms_norm_grad_kernel<T, TPR, CH, STAGES, THREADS>, smem);
   if (rc) return rc;
-  return launch_pdl(rms_norm_grad_kernel<T, TPR, CH, STAGES>, dim3((unsigned)parts), kGradThreads, smem, 1, st, "rms_norm_grad", p);
+  return launch_pdl(rms_norm_grad_kernel<T, TPR, CH, STAGES, THREADS>, dim3((unsigned)parts), THREADS, smem, 1, st, "rms_norm_grad", p);
 }
 
 template <typename T>
 int launch_backward(const Backward& p, bool vector, int parts, cudaStream_t st) {
   if (vector) {
     const int pieces = p.cols / (16 / (int)sizeof(T));
-    if (pieces <= 32 * 4) return launch_grad_ring<T, 32, 4, 2>(p, parts, st);
-    if (pieces <= 64 * 4) return launch_grad_ring<T, 64, 4, 2>(p, parts, st);
-    if (pieces <= 128 * 4) return launch_grad_ring<T, 128, 4, 2>(p, parts, st);
-    if (pieces <= 256 * 4) return launch_grad_ring<T, 256, 4, 2>(p, parts, st);
-    if (pieces <= 512 * 4) return launch_grad_ring<T, 512, 4, 2>(p, parts, st);
+    if (pieces <= 32 * 4) return launch_grad_ring<T, 32, 4, 2, 512>(p, parts, st);
+    if (pieces <= 128 * 2) return launch_grad_ring<T, 128, 2, 2, 1024>(p, parts, st);
+    if (pieces <= 256 * 2) return launch_grad_ring<T, 256, 2, 2, 1024>(p, parts, st);
+    if (pieces <= 512 * 2) return launch_grad_ring<T, 512, 2, 2, 1024>(p, parts, st);
+    if (pieces <= 1024 * 2) return launch_grad_ring<T, 1024, 2, 2, 1024>(p, parts, st);
     return launch_grad_any<T>(p, parts, st);
   }
 #define MOE_RG(TPR, CH) \
@@ -718,8 +749,8 @@ extern "C" int moe_rms_norm(const void* x, int64_t x_ld, const void* residual, i
   Forward p = {};
   p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = residual ? residual_out : nullptr;
   p.x_ld = x_ld; p.residual_ld = residual_ld; p.y_ld = y_ld; p.h_ld = residual_out_ld; p.rows = rows;
-  p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps; p.group = (int)cols;
-  return forward(p, dtype, false, (cudaStream_t)stream);
+  p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps; p.mean = 1.0f / (float)cols; p.group = (int)cols; p.groups = 1;
+  return forward(p, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const void* weight, int dtype,
@@ -739,10 +770,10 @@ extern "C" int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* resid
   Forward p = {};
   p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = residual ? residual_out : nullptr;
   p.x_ld = x_ld; p.residual_ld = residual_ld; p.y_ld = cols; p.h_ld = cols; p.rows = rows;
-  p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps;
-  p.q = (uint8_t*)q; p.scales = scales; p.scale_ld = scale_ld; p.group = group; p.format = format;
+  p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps; p.mean = 1.0f / (float)cols;
+  p.q = (uint8_t*)q; p.scales = scales; p.scale_ld = scale_ld; p.group = group; p.groups = (int)(cols / group); p.format = format;
   p.transposed = scale_flags & 1; p.ue8m0 = (scale_flags >> 1) & 1; p.quant_eps = quant_eps;
-  return forward(p, dtype, true, (cudaStream_t)stream);
+  return forward(p, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int moe_rms_norm_grad_workspace(int64_t rows, int64_t cols, int64_t* bytes) {
@@ -770,7 +801,7 @@ extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, cons
     return fail(MOE_E_BADARG, "rms_norm_grad: workspace too small");
   Backward p = {};
   p.dy = dy; p.dh = dresidual_out; p.h = h; p.weight = weight; p.dx = dx; p.partial = dweight ? (float*)workspace : nullptr;
-  p.h_ld = h_ld; p.rows = rows; p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps;
+  p.h_ld = h_ld; p.rows = rows; p.cols = (int)cols; p.w_f32 = weight_dtype == MOE_F32; p.eps = eps; p.mean = 1.0f / (float)cols;
   const int size = dtype == MOE_F32 ? 4 : 2;
   const bool vector = cols % (16 / size) == 0 && pieces16(h, h_ld, size) && aligned16(dy) && aligned16(dresidual_out) && aligned16(dx) &&
                       aligned16(weight);

@@ -503,7 +503,7 @@ int moe_rms_norm_grad(const void* dy, const void* dresidual_out, const void* h, 
  * skipped, MOE_ST_BAD_EXPERT_ID); cu_seqlens [sequences + 1] int32 or null (one sequence of all rows); is_padding [tokens] or
  * null.  Rows in no sequence count for nothing.  cu_seqlens that decrease or leave [0, tokens]: loss NaN, counts 0,
  * MOE_ST_BAD_ROW.  counts [sequences, experts]; saved: what the gradient needs.  At most 1024 experts, 32 routes per token,
- * 65535 sequences.  bytes[0] of the workspace, bytes[1] of saved. */
+ * 65535 sequences, 2^31 - 2^16 routes.  bytes[0] of the workspace, bytes[1] of saved. */
 int moe_balance_loss_workspace(int64_t tokens, int experts, int topk, int sequences, int64_t* bytes /* host [2] */);
 int moe_balance_loss(const void* logits, int64_t ld, int dtype, int64_t tokens, int experts, const void* topk_ids, int ids_int64,
                      int topk, int sigmoid, const int32_t* cu_seqlens, int sequences, const uint8_t* is_padding, float* loss,

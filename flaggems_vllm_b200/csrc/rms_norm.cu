@@ -388,17 +388,23 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
   const int64_t row0 = (int64_t)group * gridDim.x + blockIdx.x, step = (int64_t)GROUPS * gridDim.x;
   const bool with_dh = p.dh != nullptr && p.dx != nullptr;
   auto slot = [&](int stage, int n, int c) { return ring + ((stage * 3 + n) * CH + c) * THREADS + threadIdx.x; };
+  const T *h_next = reinterpret_cast<const T*>(p.h) + row0 * p.h_ld + t * V,  // this thread's pieces of the next row to fetch
+          *dy_next = reinterpret_cast<const T*>(p.dy) + row0 * p.cols + t * V, *dh_next = reinterpret_cast<const T*>(p.dh) + row0 * p.cols + t * V;
+  T* dx = reinterpret_cast<T*>(p.dx) + row0 * p.cols + t * V;
+  const int64_t h_step = step * p.h_ld, step_elements = step * p.cols;
   auto fetch = [&](int64_t row, int stage) {
     if (row < p.rows) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int at = t + c * TPR;
-        if (at < pieces) {
-          copy16(slot(stage, 0, c), reinterpret_cast<const T*>(p.h) + row * p.h_ld + at * V);
-          copy16(slot(stage, 1, c), reinterpret_cast<const T*>(p.dy) + row * p.cols + at * V);
-          if (with_dh) copy16(slot(stage, 2, c), reinterpret_cast<const T*>(p.dh) + row * p.cols + at * V);
+        if (t + c * TPR < pieces) {
+          copy16(slot(stage, 0, c), h_next + c * TPR * V);
+          copy16(slot(stage, 1, c), dy_next + c * TPR * V);
+          if (with_dh) copy16(slot(stage, 2, c), dh_next + c * TPR * V);
         }
       }
+      h_next += h_step;
+      dy_next += step_elements;
+      dh_next += step_elements;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -408,7 +414,12 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[c][i] = 0.0f;
 #pragma unroll
-  for (int i = 0; i < STAGES; ++i) fetch(row0 + i * step, i);
+  for (int i = 0; i < STAGES; ++i) {
+    if (!with_dh)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) *slot(i, 2, c) = make_uint4(0, 0, 0, 0);  // and it stays so: nothing is added
+    fetch(row0 + i * step, i);
+  }
   int stage = 0, turn = 0;
   for (int64_t row = row0; row < p.rows; row += step, turn ^= 1) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
@@ -442,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
         a.get(h);
         a.raw = *slot(stage, 1, c);
         a.get(g);
-        a.raw = with_dh ? *slot(stage, 2, c) : make_uint4(0, 0, 0, 0);
+        a.raw = *slot(stage, 2, c);
         a.get(d);
         load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
 #pragma unroll
@@ -453,10 +464,11 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
         }
         if (p.dx != nullptr) {
           a.set(d);
-          a.store(reinterpret_cast<T*>(p.dx) + row * p.cols + (t + c * TPR) * V);
+          a.store(dx + c * TPR * V);
         }
       }
     }
+    dx += step_elements;
     fetch(row + STAGES * step, stage);  // over what this thread alone has read, and used
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }

@@ -480,7 +480,17 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
-// fused_add_rms_norm(x, residual, weight, eps) -> True when done, in place (the caller has looked at overlaps)
+// Whether rows of `cols` elements of two tensors share memory.  Two windows of one buffer's columns do not.
+bool rows_meet(const at::Tensor& a, int64_t a_rows, int64_t a_ld, const at::Tensor& b, int64_t b_rows, int64_t b_ld, int64_t cols) {
+  const uintptr_t a0 = (uintptr_t)a.const_data_ptr(), b0 = (uintptr_t)b.const_data_ptr();
+  const uintptr_t a_size = a.element_size(), b_size = b.element_size();
+  if (a0 >= b0 + ((b_rows - 1) * b_ld + cols) * b_size || b0 >= a0 + ((a_rows - 1) * a_ld + cols) * a_size) return false;
+  if (a_ld != b_ld || a_size != b_size || (a0 - b0) % a_size != 0) return true;
+  const int64_t apart = (int64_t)((a0 > b0 ? a0 - b0 : b0 - a0) / a_size) % a_ld;
+  return apart < cols || a_ld - apart < cols;
+}
+
+// fused_add_rms_norm(x, residual, weight, eps) -> True when done, in place
 PyObject* fused_add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   double eps;
   if (n != 4 || !is_tensor(a[0]) || !is_tensor(a[1]) || !is_tensor(a[2]) || !as_double(a[3], &eps)) MOE_NONE;
@@ -488,9 +498,9 @@ PyObject* fused_add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NormArgs p;
   if (!(eps >= 0.0 && eps < 3e38) || !norm_args(x, w, &residual, &p) || wants_grad({&x, &residual, &w})) MOE_NONE;
   if (p.rows > 1 && (p.x_ld < p.cols || p.residual_ld < p.cols)) MOE_NONE;
-  const char *x0 = (const char*)x.const_data_ptr(), *r0 = (const char*)residual.const_data_ptr();
-  const int64_t size = x.element_size(), x_bytes = ((p.rows - 1) * p.x_ld + p.cols) * size, r_bytes = ((p.rows - 1) * p.residual_ld + p.cols) * size;
-  if (p.rows > 0 && x0 < r0 + r_bytes && r0 < x0 + x_bytes) MOE_NONE;  // the two share memory
+  if (p.rows > 0 && (rows_meet(x, p.rows, p.x_ld, residual, p.rows, p.residual_ld, p.cols) ||
+                     rows_meet(x, p.rows, p.x_ld, w, 1, p.cols, p.cols) || rows_meet(residual, p.rows, p.residual_ld, w, 1, p.cols, p.cols)))
+    MOE_NONE;
   {
     Unlocked unlocked;
     c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);

@@ -144,6 +144,9 @@ __device__ __forceinline__ uint8_t to_8bit(float v, int format) {  // fp8 conver
   return (uint8_t)(int8_t)max(-128, min(127, __float2int_rn(v)));  // NaN gives 0; its scale is NaN
 }
 
+// A scale of zero (no floor under it, and nothing in the group) stands over zeros.
+__device__ __forceinline__ float quotient(float y, float s) { return s == 0.0f ? 0.0f : y / s; }
+
 // Four values rounded to the nearest whole number, halves to even, and cut to [-128, 127].
 __device__ __forceinline__ uint32_t pack_int8(float a, float b, float c, float d) {
   uint32_t hi, out;
@@ -162,7 +165,7 @@ __device__ __forceinline__ void quantise(const float (&y)[V], float s, int forma
     for (int i = 0; i < V; ++i) d[i] = div_by_scale(y[i], s, inv);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) d[i] = y[i] / s;
+    for (int i = 0; i < V; ++i) d[i] = quotient(y[i], s);
   }
   uint32_t w[(V + 3) / 4] = {};
   if (format == kE4M3 && V % 4 == 0) {
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(const Forward p) {
       join_row<Max, 1, 256>(m, sh[1]);
       const float s = group_scale(m[0], p.quant_eps, p.format, p.ue8m0);
       if (threadIdx.x == 0) *scale_at(p, row, 0) = s;
-      for (int i = threadIdx.x; i < p.cols; i += 256) q[i] = to_8bit(norm(i) / s, p.format);
+      for (int i = threadIdx.x; i < p.cols; i += 256) q[i] = to_8bit(quotient(norm(i), s), p.format);
     } else {  // a warp per group
       const int lane = threadIdx.x & 31;
       for (int g = threadIdx.x >> 5; g < p.groups; g += 8) {
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(const Forward p) {
         join_row<Max, 1, 32>(m, nullptr);
         const float s = group_scale(m[0], p.quant_eps, p.format, p.ue8m0);
         if (lane == 0) *scale_at(p, row, g) = s;
-        for (int i = lane; i < p.group; i += 32) q[g * p.group + i] = to_8bit(norm(g * p.group + i) / s, p.format);
+        for (int i = lane; i < p.group; i += 32) q[g * p.group + i] = to_8bit(quotient(norm(g * p.group + i), s), p.format);
       }
     }
   }

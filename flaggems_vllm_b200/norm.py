@@ -18,7 +18,7 @@ from .quant import SUPPORTED_FP8_DTYPE
 logger = logging.getLogger(__name__)
 
 _FORMATS = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1, torch.int8: 2}
-_MAX_COLS = 1 << 24
+_MAX_COLS, _MAX_ROWS = 1 << 24, 0x7FFFFFFF
 
 
 def _check(x, weight, eps, residual, what):
@@ -27,6 +27,8 @@ def _check(x, weight, eps, residual, what):
     _lib.dtype_code(x.dtype)  # ValueError("Unsupported dtype")
     if x.shape[-1] > _MAX_COLS:
         raise ValueError(f"{what}: rows of at most {_MAX_COLS} elements")
+    if x.numel() // x.shape[-1] > _MAX_ROWS:
+        raise ValueError(f"{what}: at most {_MAX_ROWS} rows")
     if weight.ndim != 1 or weight.shape[0] != x.shape[-1]:
         raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {list(weight.shape)}")
     if weight.dtype not in (x.dtype, torch.float32):
@@ -78,7 +80,7 @@ def fused_add_rms_norm(
     """In place: ``residual`` becomes the stream ``x + residual``, ``x`` its norm; returns (x, residual).
 
     Values are those of ``rms_norm(x, weight, eps, residual)``.  The rows of both may lie in wider buffers, whose other
-    columns stay as they are; the two may not share memory.  Not differentiable: refused where a gradient is wanted."""
+    columns stay as they are; neither may share memory with the other or with the weight.  Not differentiable: refused where a gradient is wanted."""
     logger.debug("GEMS FUSED ADD RMS NORM")
     if not x.is_cuda or not _lib.host().fused_add_rms_norm(x, residual, weight, eps):
         what, eps = "fused_add_rms_norm", float(eps)
@@ -86,7 +88,8 @@ def fused_add_rms_norm(
         if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad):
             raise RuntimeError(f"{what} works in place and has no gradient: use rms_norm, or torch.no_grad()")
         if not _lib.host().fused_add_rms_norm(x, residual, weight.contiguous(), eps):
-            raise ValueError(f"{what}: x and residual must be rows of contiguous elements that share no memory")
+            raise ValueError(f"{what}: x and residual must be rows of contiguous elements that share no memory with each other "
+                             "or the weight")
     return x, residual
 
 
@@ -107,7 +110,8 @@ def rms_norm_quant(
 
     ``x_s`` holds one scale per ``group_size`` elements of a row (None: one per row), shape
     ``x.shape[:-1] + (cols / group_size,)``, column-major in memory when ``column_major_scales``;
-    ``x_s = max(amax, quant_eps) / qmax``, rounded up to a power of two with ``scale_ue8m0``.  ``dtype`` is
+    ``x_s = max(amax, quant_eps) / qmax``, rounded up to a power of two with ``scale_ue8m0``; a scale of zero
+    (``quant_eps=0``) stands over zeros.  ``dtype`` is
     float8_e4m3fn (default), float8_e5m2 or int8.  The fp32 value of the norm is quantised, not its 16-bit rounding.
     A NaN makes its group's scale NaN.  Not differentiable: refused where a gradient is wanted."""
     logger.debug("GEMS RMS NORM QUANT")

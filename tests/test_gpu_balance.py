@@ -86,7 +86,7 @@ def check(logits, ids, scoring, cu=None, pad=None, dloss=1.0):
 
 
 @pytest.mark.parametrize("E,k", [(1, 1), (2, 1), (3, 2), (8, 2), (60, 4), (64, 6), (100, 8), (128, 8), (160, 6), (256, 8), (257, 8),
-                                 (384, 8), (512, 10), (1000, 8), (1024, 32)])
+                                 (384, 8), (511, 4), (512, 10), (516, 4), (520, 4), (1000, 8), (1023, 7), (1024, 32)])
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_every_number_of_experts(E, k, scoring):
     for dtype in (torch.float32, torch.bfloat16, torch.float16):

@@ -55,7 +55,8 @@ def check_norm(y, want, cols, dtype):
 
 
 ROWS = [1, 2, 5, 37, 300]
-COLS = [1, 7, 8, 33, 64, 100, 128, 256, 1000, 1023, 1024, 1032, 2048, 2056, 4096, 7168, 8192, 8200, 16384, 16392, 20001]
+COLS = [1, 7, 8, 33, 64, 100, 128, 256, 1000, 1023, 1024, 1032, 1999, 2048, 2056, 4096, 4104, 5001, 7168, 8191, 8192, 8200, 16384,
+        16392, 20001]
 
 
 @pytest.mark.parametrize("cols", COLS)
@@ -149,6 +150,19 @@ def test_in_place():
             assert bx._version > versions[0] and br._version > versions[1]
 
 
+def test_in_place_in_two_windows_of_one_buffer():
+    for H in (64, 65):
+        both = torch.randn(8, 2 * H + 6, device=DEV).bfloat16()
+        w = torch.randn(H, device=DEV).bfloat16()
+        x, r, rest = both[:, :H], both[:, H + 6:], both[:, H:H + 6].clone()
+        y, h = fg.rms_norm(x, w, EPS, r)
+        fg.fused_add_rms_norm(x, r, w, EPS)
+        assert torch.equal(x, y) and torch.equal(r, h) and torch.equal(both[:, H:H + 6], rest)
+        y, h = fg.rms_norm(r, w, EPS, x)
+        fg.fused_add_rms_norm(r, x, w, EPS)
+        assert torch.equal(r, y) and torch.equal(x, h)
+
+
 def test_in_place_refusals():
     x, r, w, _ = make(8, 64, torch.bfloat16)
     with pytest.raises(ValueError, match="share no memory"):
@@ -158,6 +172,13 @@ def test_in_place_refusals():
         fg.fused_add_rms_norm(buf[:8], buf[1:], w)
     with pytest.raises(ValueError, match="share no memory"):
         fg.fused_add_rms_norm(x[:1].expand(8, 64), r, w)  # every row is the same memory
+    with pytest.raises(ValueError, match="share no memory"):
+        fg.fused_add_rms_norm(x, r, x[3])
+    with pytest.raises(ValueError, match="share no memory"):
+        fg.fused_add_rms_norm(x, r, r[0])
+    both = torch.randn(8, 130, device=DEV).bfloat16()
+    with pytest.raises(ValueError, match="share no memory"):
+        fg.fused_add_rms_norm(both[:, :66], both[:, 64:], torch.ones(66, device=DEV).bfloat16())
     with pytest.raises(ValueError, match="rows of contiguous elements"):
         fg.fused_add_rms_norm(x.t().contiguous().t(), r, w)
     with pytest.raises(RuntimeError, match="no gradient"):
@@ -193,7 +214,8 @@ def check_grads(x, r, w, dy, dh, dx, dw, eps=EPS):
         assert ((dw.double() - terms.sum(0)).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("cols", [1, 7, 64, 100, 128, 1000, 1023, 1024, 2048, 2056, 4096, 7168, 8200, 16384, 16392, 20001])
+@pytest.mark.parametrize("cols", [1, 7, 64, 100, 128, 1000, 1023, 1024, 1032, 1999, 2048, 2056, 4096, 4104, 7168, 8200, 16384, 16392,
+                                  20001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_gradients(cols, dtype):
     for M in (1, 3, 333):
@@ -390,8 +412,11 @@ def test_quant_options():
     assert d[1].shape == (6, 2) and d[1].stride() == (1, 6) and torch.equal(d[1], c[1].view(6, 2))
     big = fg.rms_norm_quant(x, w, EPS, group_size=128, quant_eps=1e4)
     assert torch.equal(big[1], torch.full_like(big[1], 1e4) * torch.tensor(1 / 448, dtype=torch.float32, device=DEV))
-    zero = fg.rms_norm_quant(torch.zeros_like(x), w, EPS, quant_eps=0.0)
-    assert (zero[1] == 0).all()  # nothing to scale: the caller asked for no floor
+    for cols in (256, 250):  # nothing to scale and no floor under it
+        for dtype in QMAX:
+            for group in (None, 2, cols):
+                q, s = fg.rms_norm_quant(x[:, :cols] * 0, w[:cols], EPS, quant_eps=0.0, dtype=dtype, group_size=group)
+                assert (s == 0).all() and (q.float() == 0).all()
     with pytest.raises(RuntimeError, match="no gradient"):
         fg.rms_norm_quant(x.clone().requires_grad_(), w)
 

@@ -59,7 +59,7 @@ def _host_ext_cmd() -> list:
             "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
             "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
             os.path.join(CSRC, "host_ext.cpp"), "-o", HOST_EXT, "-L" + HERE, "-l:libmoe_sm100.so",
-            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
             "-Wl,-rpath,$ORIGIN"]
 
 

@@ -10,7 +10,11 @@
 // gradient, which has only h, is that of the same function.  y itself is rounded once: the quantiser takes its fp32 value.
 // The gradient computes r again (the row is in registers anyway), so nothing but h is kept between the two passes.
 //
-// Bound: memory.  A row is read once: it stays in the registers of the threads that share it.
+// Bound: memory.  A row is read once: it stays in the registers of the threads that share it, 32 values to a thread so that four
+// blocks of 256 threads, and their loads, are on a multiprocessor.  us on the device, 8192 x 7168 bf16 with a residual (470 MB: 72
+// at the rate of a copy): norm 69.5; e4m3 in groups of 128 70.4 (411 MB: 63), with the norm itself 82 (528 MB: 81); int8 per row
+// 68; gradient 84, of which 4 for the weight's (470 MB: 72).  16 or 64 values to a thread
+// instead: 3 to 6 % slower.  One token of 7168: 2.7, a launch and one round of loads.
 #include "moe_common.cuh"
 
 namespace moe {
@@ -33,28 +37,47 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// V consecutive elements that one thread moves at once: 16 bytes, or a single element where rows are not made of such pieces.
+// V consecutive elements that one thread moves at once: 32 or 16 bytes, or a single element where rows are not made of such
+// pieces.  Loads and stores of 32 bytes are sm_100's own.
 template <typename T, int V> struct Piece {
-  uint4 raw = {0, 0, 0, 0};
-  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = raw; }
+  static constexpr int W = V * (int)sizeof(T) / 4;
+  static_assert(W == 8 || W == 4, "16 or 32 bytes");
+  uint32_t raw[W] = {};
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (W == 8) {
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7])
+                   : "l"(p));
+    } else {
+      set_raw(*reinterpret_cast<const uint4*>(p));
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (W == 8)
+      asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(raw[0]), "r"(raw[1]), "r"(raw[2]), "r"(raw[3]), "r"(raw[4]),
+                   "r"(raw[5]), "r"(raw[6]), "r"(raw[7]), "l"(p)
+                   : "memory");
+    else
+      *reinterpret_cast<uint4*>(p) = make_uint4(raw[0], raw[1], raw[2], raw[3]);
+  }
+  __device__ __forceinline__ void set_raw(uint4 v) { raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w; }
   __device__ __forceinline__ void get(float (&v)[V]) const {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (V == 4) {
-        v[i] = __uint_as_float(w[i]);
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(raw[i]);
       } else {
-        const float2 f = unpack2<T>(w[i]);
+        const float2 f = unpack2<T>(raw[i]);
         v[2 * i] = f.x; v[2 * i + 1] = f.y;
       }
     }
   }
   __device__ __forceinline__ void set(const float (&v)[V]) {
-    if constexpr (V == 4)
-      raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    else
-      raw = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) raw[i] = __float_as_uint(v[i]);
+      else raw[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
   }
 };
 template <typename T> struct Piece<T, 1> {
@@ -182,7 +205,8 @@ __device__ __forceinline__ void quantise(const float (&y)[V], float s, int forma
 #pragma unroll
     for (int i = 0; i < V; ++i) w[i / 4] |= (uint32_t)to_8bit(d[i], format) << (8 * (i & 3));
   }
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  if constexpr (V == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
   else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
   else *dst = (uint8_t)w[0];
 }
@@ -432,9 +456,9 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
       if (t + c * TPR < pieces) {
         Piece<T, V> a;
         float h[V], g[V], w[V];
-        a.raw = *slot(stage, 0, c);
+        a.set_raw(*slot(stage, 0, c));
         a.get(h);
-        a.raw = *slot(stage, 1, c);
+        a.set_raw(*slot(stage, 1, c));
         a.get(g);
         load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
 #pragma unroll
@@ -452,11 +476,11 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
       if (t + c * TPR < pieces) {
         Piece<T, V> a;
         float h[V], g[V], d[V], w[V];  // read again: kept in registers beside dw they would spill
-        a.raw = *slot(stage, 0, c);
+        a.set_raw(*slot(stage, 0, c));
         a.get(h);
-        a.raw = *slot(stage, 1, c);
+        a.set_raw(*slot(stage, 1, c));
         a.get(g);
-        a.raw = *slot(stage, 2, c);
+        a.set_raw(*slot(stage, 2, c));
         a.get(d);
         load_weight<T, V>(p.weight, p.w_f32, (t + c * TPR) * V, w);
 #pragma unroll
@@ -627,14 +651,11 @@ __global__ void __launch_bounds__(256) weight_grad_any_kernel(const Backward p, 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool pieces16(const void* p, int64_t ld, int size) { return aligned16(p) && ld * size % 16 == 0; }
 
-// Threads to a row that give each up to four pieces, all in flight at once; 0 = the kernel for any row.
-int threads_of(int pieces, bool vector) {
-  if (pieces <= 32 * 4) return 32;
-  if (pieces <= 64 * 4 && vector) return 64;
-  if (pieces <= 128 * 4 && vector) return 128;
-  if (pieces <= 256 * 4) return 256;
-  if (pieces <= 512 * 4) return 512;
-  return !vector && pieces <= 1024 * 8 ? 1024 : 0;
+// Threads to a row that give each all pieces that it holds, `held` of them in flight at once; 0 = the kernel for any row.
+int threads_of(int pieces, int held) {
+  for (int threads = 32; threads <= 512; threads *= 2)
+    if (pieces <= threads * held) return threads;
+  return 0;
 }
 
 template <typename T, int V, int TPR, int CH, int FORMAT>
@@ -643,49 +664,56 @@ int launch_rows(const Forward& p, cudaStream_t st) {
   return launch_pdl(rms_norm_kernel<T, V, TPR, CH, FORMAT>, dim3((unsigned)((p.rows + at_a_time - 1) / at_a_time)), block, 0, 1, st, "rms_norm", p);
 }
 
-template <typename T, int FORMAT>
-int launch_forward(const Forward& p, bool vector, cudaStream_t st) {
-  constexpr int VEC = 16 / sizeof(T);
-  const int width = vector ? VEC : 1, threads = threads_of(p.cols / width, vector), lanes = p.group / width;
+template <typename T, int V, int CH, int FORMAT>
+int launch_pieces(const Forward& p, cudaStream_t st) {
+  const int threads = threads_of(p.cols / V, CH), lanes = p.group / V;
   // groups of a power of two of pieces within a warp, or whole rows, are quantised from registers
-  const bool held = FORMAT == kNone || p.group == p.cols || (p.group % width == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0);
-  if (threads == 0 || !held) return launch_pdl(rms_norm_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm", p);
-  if (vector) {
-    switch (threads) {
-      case 32: return launch_rows<T, VEC, 32, 4, FORMAT>(p, st);
-      case 64: return launch_rows<T, VEC, 64, 4, FORMAT>(p, st);
-      case 128: return launch_rows<T, VEC, 128, 4, FORMAT>(p, st);
-      case 256: return launch_rows<T, VEC, 256, 4, FORMAT>(p, st);
-      default: return launch_rows<T, VEC, 512, 4, FORMAT>(p, st);
-    }
+  const bool held = FORMAT == kNone || p.group == p.cols || (p.group % V == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0);
+  switch (held ? threads : 0) {
+    case 32: return launch_rows<T, V, 32, CH, FORMAT>(p, st);
+    case 64: return launch_rows<T, V, 64, CH, FORMAT>(p, st);
+    case 128: return launch_rows<T, V, 128, CH, FORMAT>(p, st);
+    case 256: return launch_rows<T, V, 256, CH, FORMAT>(p, st);
+    case 512: return launch_rows<T, V, 512, CH, FORMAT>(p, st);
   }
-  switch (threads) {
-    case 32: return launch_rows<T, 1, 32, 4, FORMAT>(p, st);
-    case 256: return launch_rows<T, 1, 256, 4, FORMAT>(p, st);
-    case 512: return launch_rows<T, 1, 512, 4, FORMAT>(p, st);
-    default: return launch_rows<T, 1, 1024, 8, FORMAT>(p, st);
-  }
+  if (V == 1 && held && p.cols <= 1024 * 8) return launch_rows<T, 1, 1024, 8, FORMAT>(p, st);
+  return launch_pdl(rms_norm_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm", p);
+}
+
+// `piece`: bytes that rows and pointers are made of, 32 or 16, or fewer.  With 32 each lane's part of a group is twice as long (its
+// largest value, scale and reciprocal are half the work per value) and half as many loads and stores are issued: 8192 x 7168 bf16
+// in groups of 128 in 70.4 us, 77.7 in pieces of 16; the norm alone 69.5 and 71.0.
+template <typename T, int FORMAT>
+int launch_forward(const Forward& p, int piece, cudaStream_t st) {
+  constexpr int S = sizeof(T);
+  if (piece == 32 && p.group % (32 / S) == 0) return launch_pieces<T, 32 / S, 2, FORMAT>(p, st);
+  if (piece >= 16) return launch_pieces<T, 16 / S, 4, FORMAT>(p, st);
+  return launch_pieces<T, 1, 4, FORMAT>(p, st);
 }
 
 template <typename T>
-int launch_format(const Forward& p, bool vector, cudaStream_t st) {
-  if (p.q == nullptr) return launch_forward<T, kNone>(p, vector, st);
+int launch_format(const Forward& p, int piece, cudaStream_t st) {
+  if (p.q == nullptr) return launch_forward<T, kNone>(p, piece, st);
   switch (p.format) {
-    case kE4M3: return launch_forward<T, kE4M3>(p, vector, st);
-    case kE5M2: return launch_forward<T, kE5M2>(p, vector, st);
-    default: return launch_forward<T, kInt8>(p, vector, st);
+    case kE4M3: return launch_forward<T, kE4M3>(p, piece, st);
+    case kE5M2: return launch_forward<T, kE5M2>(p, piece, st);
+    default: return launch_forward<T, kInt8>(p, piece, st);
   }
 }
 
 int forward(const Forward& p, int dtype, cudaStream_t st) {
-  const int size = dtype == MOE_F32 ? 4 : 2, vec = 16 / size;
-  const bool vector = p.cols % vec == 0 && pieces16(p.x, p.x_ld, size) && (!p.residual || pieces16(p.residual, p.residual_ld, size)) &&
-                      (!p.h || pieces16(p.h, p.h_ld, size)) && (!p.y || pieces16(p.y, p.y_ld, size)) && aligned16(p.weight) &&
-                      (!p.q || aligned16(p.q));
+  const int size = dtype == MOE_F32 ? 4 : 2;
+  uint64_t bits = (uint64_t)p.cols * size | (uintptr_t)p.x | (uintptr_t)p.weight | (uintptr_t)p.y | (uintptr_t)p.q;
+  if (p.rows > 1) bits |= (uint64_t)p.x_ld * size | (p.y ? (uint64_t)p.y_ld * size : 0);
+  if (p.residual) {
+    bits |= (uintptr_t)p.residual | (uintptr_t)p.h;
+    if (p.rows > 1) bits |= (uint64_t)(p.residual_ld | p.h_ld) * size;
+  }
+  const int piece = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 1;
   switch (dtype) {
-    case MOE_F32: return launch_format<float>(p, vector, st);
-    case MOE_F16: return launch_format<__half>(p, vector, st);
-    default: return launch_format<__nv_bfloat16>(p, vector, st);
+    case MOE_F32: return launch_format<float>(p, piece, st);
+    case MOE_F16: return launch_format<__half>(p, piece, st);
+    default: return launch_format<__nv_bfloat16>(p, piece, st);
   }
 }
 

@@ -429,6 +429,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     if (!dy.defined()) {  // only the stream was used: its gradient passes through
       if (want_x && dh.defined()) out[0] = dh;
       if (has_residual) out[2] = out[0];
+      if (want_w) out[1] = at::zeros_like(w);
       return once(out, "rms_norm");
     }
     NormArgs p;

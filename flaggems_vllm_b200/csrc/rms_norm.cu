@@ -789,6 +789,9 @@ extern "C" int moe_rms_norm(const void* x, int64_t x_ld, const void* residual, i
   if (rc || rows == 0) return rc;
   if (!y || (y_ld < cols && rows > 1)) return fail(MOE_E_BADARG, "rms_norm: bad output");
   if (!residual && y == x) return fail(MOE_E_BADARG, "rms_norm: the output may lie over the input only with a residual");
+  const bool shifted = (y == x && y_ld != x_ld) || (residual && residual_out == residual && residual_out_ld != residual_ld);
+  if (residual && (y == residual_out || (shifted && rows > 1)))
+    return fail(MOE_E_BADARG, "rms_norm: outputs over the inputs have their row distance, and lie apart");
   Forward p = {};
   p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = residual ? residual_out : nullptr;
   p.x_ld = x_ld; p.residual_ld = residual_ld; p.y_ld = y_ld; p.h_ld = residual_out_ld; p.rows = rows;
@@ -809,7 +812,9 @@ extern "C" int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* resid
   if ((scale_flags & 2) && format == kInt8) return fail(MOE_E_BADARG, "rms_norm_quant: power-of-two scales are for the 8-bit floats");
   if (rows == 0) return 0;
   if (!q || !scales || ((scale_flags & 1) && scale_ld < rows)) return fail(MOE_E_BADARG, "rms_norm_quant: bad output");
-  if (y && y == x) return fail(MOE_E_BADARG, "rms_norm_quant: the norm is written to memory of its own");
+  if (y && (y == x || y == residual || y == residual_out)) return fail(MOE_E_BADARG, "rms_norm_quant: the norm is written to memory of its own");
+  if (residual && residual_out == residual && residual_ld != cols && rows > 1)
+    return fail(MOE_E_BADARG, "rms_norm_quant: a stream over the residual has its row distance");
   Forward p = {};
   p.x = x; p.residual = residual; p.weight = weight; p.y = y; p.h = residual ? residual_out : nullptr;
   p.x_ld = x_ld; p.residual_ld = residual_ld; p.y_ld = cols; p.h_ld = cols; p.rows = rows;

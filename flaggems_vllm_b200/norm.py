@@ -84,6 +84,8 @@ def fused_add_rms_norm(
     logger.debug("GEMS FUSED ADD RMS NORM")
     if not x.is_cuda or not _lib.host().fused_add_rms_norm(x, residual, weight, eps):
         what, eps = "fused_add_rms_norm", float(eps)
+        if residual is None:
+            raise ValueError(f"{what}: there must be a residual")
         _check(x, weight, eps, residual, what)
         if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad):
             raise RuntimeError(f"{what} works in place and has no gradient: use rms_norm, or torch.no_grad()")

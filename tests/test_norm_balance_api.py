@@ -31,6 +31,8 @@ def test_norm_refusals():
         if "residual" in bad or "eps" in bad:
             with pytest.raises(ValueError, match=match):
                 fg.fused_add_rms_norm(**{"residual": x.clone(), **args})
+    with pytest.raises(ValueError, match="there must be a residual"):
+        fg.fused_add_rms_norm(x, None, w)
     for call in (lambda: fg.rms_norm(x, w), lambda: fg.rms_norm(x, w, residual=x), lambda: fg.fused_add_rms_norm(x, x, w),
                  lambda: fg.rms_norm_quant(x, w, group_size=32)):
         with pytest.raises(RuntimeError, match="no CPU path"):
@@ -80,16 +82,18 @@ def test_c_entry_points_reject_bad_arguments():
 
     assert norm(rows=0) == 0
     for bad in (dict(rows=-1), dict(cols=0), dict(cols=(1 << 24) + 1), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(w=None),
-                dict(y=None), dict(y_ld=63), dict(r=P), dict(r=P, h=P, h_ld=8), dict(x_ld=-1), dict(y=P)):
+                dict(y=None), dict(y_ld=63), dict(r=P), dict(r=P, h=P, h_ld=8), dict(x_ld=-1), dict(y=P), dict(r=3 * P, h=2 * P),
+                dict(r=3 * P, h=4 * P, y=P, y_ld=72), dict(r=3 * P, h=3 * P, h_ld=72)):
         assert norm(**bad) == -1, bad
     assert norm(rows=1 << 31) == -5
     assert norm(dtype=3) == -2 and norm(dtype=1, wdtype=2) == -2
 
-    def quant(fmt=0, group=32, qeps=1e-10, flags=0, q=P, s=P, s_ld=4, y=None):
-        return lib.moe_rms_norm_quant(P, 64, None, 64, P, 0, 0, 4, 64, 1e-6, fmt, group, qeps, flags, q, s, s_ld, y, None, None)
+    def quant(fmt=0, group=32, qeps=1e-10, flags=0, q=P, s=P, s_ld=4, y=None, r=None, r_ld=64, h=None):
+        return lib.moe_rms_norm_quant(P, 64, r, r_ld, P, 0, 0, 4, 64, 1e-6, fmt, group, qeps, flags, q, s, s_ld, y, h, None)
 
     for bad, code in ((dict(fmt=3), -2), (dict(group=0), -3), (dict(group=48), -3), (dict(qeps=-1.0), -1), (dict(flags=2, fmt=2), -1),
-                      (dict(q=None), -1), (dict(s=None), -1), (dict(flags=1, s_ld=3), -1), (dict(y=P), -1)):
+                      (dict(q=None), -1), (dict(s=None), -1), (dict(flags=1, s_ld=3), -1), (dict(y=P), -1),
+                      (dict(r=2 * P, h=2 * P, r_ld=72), -1), (dict(r=2 * P, h=3 * P, y=3 * P), -1), (dict(r=2 * P, h=3 * P, y=2 * P), -1)):
         assert quant(**bad) == code, bad
 
     need = ctypes.c_int64()

@@ -14,7 +14,9 @@
 // Two launches forward, one where a block holds all rows.  Each block of the first takes a run of rows and, for every sequence in it, sums p and counts routes
 // in registers and shared memory; sequence s in block c goes to slot c + s, which no other pair has (a walk along the rows
 // adds one to c or to s at every step).  The second adds the slots in order, so that results are the same bits in every run.
-// Bound: memory, one pass over the logits forward and one backward; the launches for a few thousand tokens.
+// Bound: the logits are read once forward and once backward; up to some ten thousand tokens it is the launches and the chain of
+// loads in a block.  us on the device, forward and backward: 64 x 8 fp32 4.0 + 2.8 (one launch forward), 4096 x 128 bf16 10.7 + 4.4,
+// 8192 x 256 fp32 11.5 + 5.6, the same in 23 padded sequences of sigmoid scores 18.7 + 9.5, 65536 x 256 fp32 21 + 27.6 (floor 10 + 20).
 #include "moe_common.cuh"
 
 namespace moe {
@@ -42,12 +44,16 @@ struct Slots {
   double* part;  // [sequences, slices] of the loss
 };
 
-// The first sequence that ends behind row t (their number if none does).
+// The first sequence that ends behind row t (their number if none does), the same in every lane: 32 edges are looked at a time,
+// as a search by halves waits for the memory at every step.
 __device__ __forceinline__ int sequence_of(const int32_t* cu, int sequences, int64_t t) {
-  int lo = 0, hi = sequences;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (cu[mid + 1] > t) hi = mid; else lo = mid + 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = sequences;  // it is one of lo .. lo + n
+  while (n > 0) {
+    const int step = (n + 31) / 32, i = (lane + 1) * step - 1;
+    const int passed = __popc(__ballot_sync(0xFFFFFFFFu, i < n && cu[lo + i + 1] <= t));
+    lo += passed * step;
+    n = min(step - 1, n - passed * step);
   }
   return lo;
 }
@@ -81,6 +87,12 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   return y;
 }
 
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // l -> e of U tokens, each over `lanes` lanes (all lanes of the warp call it); the scores are p = e inv.
 template <int V, int CH, int U>
 __device__ __forceinline__ void scores(const float (&l)[U][CH][V], int lanes, bool sigmoid, float (&e)[U][CH][V], float (&inv)[U]) {
@@ -92,7 +104,8 @@ __device__ __forceinline__ void scores(const float (&l)[U][CH][V], int lanes, bo
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float x = l[u][c][i];
-          e[u][c][i] = x == x ? fminf(x, 0.0f) - log1pf(expf(-fabsf(x))) : x;  // fminf drops a NaN
+          // off by 2^-22 of one, as little as the score is then off by itself; fminf drops a NaN
+          e[u][c][i] = x == x ? fmaf(log2_approx(1.0f + expf(-fabsf(x))), -0.6931471805599453f, fminf(x, 0.0f)) : x;
         }
   } else {
 #pragma unroll
@@ -156,7 +169,7 @@ struct Result {
 };
 
 template <typename T, int V, int CH>
-__global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b, const Slots out, const Result result, int32_t* __restrict__ status) {
+__global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : kSumBlocks) balance_sums_kernel(const Balance b, const Slots out, const Result result, int32_t* __restrict__ status) {
   pdl_wait();
   pdl_trigger();
   constexpr int U = tokens_in_hand(V * CH);
@@ -167,64 +180,92 @@ __global__ void __launch_bounds__(kThreads) balance_sums_kernel(const Balance b,
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / b.lanes, step = kWarps * groups;
   const int group = lane / b.lanes, at = lane % b.lanes;
   const int64_t r0 = (int64_t)blockIdx.x * b.rows, r1 = min(b.tokens, r0 + b.rows);
-  if (blockIdx.x == 0 && result.loss == nullptr) {
+  if (b.cu != nullptr && blockIdx.x == gridDim.x - 1) {  // a block more, which looks at the edges
     int bad = 0;
-    if (b.cu != nullptr)
-      for (int s = threadIdx.x; s < b.sequences; s += kThreads) bad |= b.cu[s] < 0 || b.cu[s + 1] < b.cu[s] || b.cu[s + 1] > b.tokens;
+    for (int s = threadIdx.x; s < b.sequences; s += kThreads) bad |= b.cu[s] < 0 || b.cu[s + 1] < b.cu[s] || b.cu[s + 1] > b.tokens;
     bad = __syncthreads_or(bad);
     if (threadIdx.x == 0) {
       out.flags[0] = bad;
       out.flags[1] = 0;
       if (bad) set_status(status, MOE_ST_BAD_ROW);
     }
+    return;
   }
+  if (b.cu == nullptr && result.loss == nullptr && blockIdx.x == 0 && threadIdx.x < 2) out.flags[threadIdx.x] = 0;
   bool bad_id = false;
-  for (int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0); s < b.sequences; ++s) {
+  int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0);
+  int64_t edge = b.cu == nullptr ? 0 : b.cu[s];
+  for (; s < b.sequences; ++s) {
     int64_t first = r0, last = r1;
     if (b.cu != nullptr) {
-      if (b.cu[s] >= r1) break;
-      first = max(r0, (int64_t)b.cu[s]);
-      last = min(r1, (int64_t)b.cu[s + 1]);
+      if (edge >= r1) break;
+      first = max(r0, edge);
+      edge = b.cu[s + 1];
+      last = min(r1, edge);
       if (first >= last) continue;
     }
-    for (int e = threadIdx.x; e <= b.experts; e += kThreads) hist[e] = 0;  // and the tokens behind
-    __syncthreads();
+    // What a sequence's part needs is asked for at once: routes, padding, the first tokens.  One load behind another, and the
+    // routes before the tokens, a block of two sequences took 13 us where one of one took 7.7.
     const uint32_t routes = (uint32_t)(last * b.topk);  // check(): all routes are below 2^31
-    for (uint32_t i0 = (uint32_t)(first * b.topk) + threadIdx.x; i0 < routes; i0 += 4 * kThreads) {
-      int64_t id[4];
+    uint32_t i0 = (uint32_t)(first * b.topk) + threadIdx.x;
+    int id[4];
+    auto load_ids = [&] {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t i = i0 + j * kThreads;
         id[j] = -1;
-        if (i < routes && (b.padding == nullptr || !b.padding[i / (uint32_t)b.topk]))
-          id[j] = b.ids64 ? reinterpret_cast<const int64_t*>(b.ids)[i] : (int64_t) reinterpret_cast<const int32_t*>(b.ids)[i];
+        if (i >= routes) continue;
+        const bool pad = b.padding != nullptr && b.padding[i / (uint32_t)b.topk];
+        const int64_t v = b.ids64 ? reinterpret_cast<const int64_t*>(b.ids)[i] : (int64_t) reinterpret_cast<const int32_t*>(b.ids)[i];
+        id[j] = pad || v < 0 ? -1 : v < b.experts ? (int)v : b.experts;
       }
+    };
+    auto count_ids = [&] {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (id[j] >= 0 && id[j] < b.experts) atomicAdd(hist + id[j], 1);
-        else bad_id |= id[j] >= b.experts;
+        bad_id |= id[j] == b.experts;
       }
-    }
+    };
+    load_ids();
+    for (int e = threadIdx.x; e <= b.experts; e += kThreads) hist[e] = 0;  // and the tokens behind
+    __syncthreads();
     float acc[CH][V] = {};
     int mine = 0;
     const T* row = reinterpret_cast<const T*>(b.logits) + (first + warp * groups + group) * b.ld;
     const int64_t apart = step * b.ld;
     for (int t0 = (int)first + warp * groups + group; t0 - group < (int)last; t0 += U * step, row += U * apart) {
       float l[U][CH][V], p[U][CH][V], inv[U];
+      bool live[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int t = t0 + u * step;
-        const bool live = t < (int)last && (b.padding == nullptr || !b.padding[t]);
-        load_row<T, V, CH>(row + u * apart, at, b.lanes, b.experts, live, l[u]);
-        mine += live && at == 0;
+        live[u] = t < (int)last;
+        load_row<T, V, CH>(row + u * apart, at, b.lanes, b.experts, live[u], l[u]);
+        if (b.padding != nullptr && live[u]) live[u] = !b.padding[t];
+      }
+      if (b.padding != nullptr) {  // whatever padding holds
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) l[u][c][i] = live[u] ? l[u][c][i] : -INFINITY;
       }
       scores<V, CH, U>(l, b.lanes, b.sigmoid, p, inv);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        mine += live[u] && at == 0;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
           for (int i = 0; i < V; ++i) acc[c][i] = fmaf(p[u][c][i], inv[u], acc[c][i]);
+      }
+    }
+    count_ids();
+    for (i0 += 4 * kThreads; i0 - threadIdx.x < routes; i0 += 4 * kThreads) {
+      load_ids();
+      count_ids();
     }
     for (int off = 16; off >= b.lanes; off >>= 1)
 #pragma unroll
@@ -366,7 +407,12 @@ __global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_ke
   const int64_t r0 = (int64_t)blockIdx.x * b.rows, r1 = min(b.tokens, r0 + b.rows);
   const int32_t* live_tokens = saved + (int64_t)b.sequences * b.experts;
   const double scale = (double)*dloss / (double)max(1, live_tokens[b.sequences]);
-  int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0 + warp * groups + group), held = -1;
+  int s = b.cu == nullptr ? 0 : sequence_of(b.cu, b.sequences, r0 + warp * groups), held = -1;
+  int begin = 0, end = INT32_MAX;  // of sequence s
+  if (b.cu != nullptr) {
+    begin = b.cu[s];
+    end = s < b.sequences ? b.cu[s + 1] : INT32_MAX;
+  }
   float a[CH][V] = {};
   const T* row = reinterpret_cast<const T*>(b.logits) + (r0 + warp * groups + group) * b.ld;
   T* drow = dlogits + (r0 + warp * groups + group) * b.experts;
@@ -378,13 +424,15 @@ __global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_ke
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int t = t0 + u * step;
-      bool live = t < (int)r1 && (b.padding == nullptr || !b.padding[t]);
-      if (b.cu != nullptr) {
-        while (s < b.sequences && b.cu[s + 1] <= t) ++s;
-        live = live && s < b.sequences && b.cu[s] <= t;
-      }
-      own[u] = live ? s : -1;
+      bool live = t < (int)r1;
       load_row<T, V, CH>(row + u * apart, at, b.lanes, b.experts, live, l[u]);
+      if (b.padding != nullptr && live) live = !b.padding[t];
+      while (end <= t) {  // ends behind the last sequence at the latest
+        begin = end;
+        ++s;
+        end = s < b.sequences ? b.cu[s + 1] : INT32_MAX;
+      }
+      own[u] = live && s < b.sequences && begin <= t ? s : -1;  // what the row holds is then of no account
     }
     scores<V, CH, U>(l, b.lanes, b.sigmoid, p, inv);
 #pragma unroll
@@ -417,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_ke
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-          for (int i = 0; i < V; ++i) p[u][c][i] /= 1.0f + expf(l[u][c][i]);
+          for (int i = 0; i < V; ++i) p[u][c][i] = __fdividef(p[u][c][i], 1.0f + expf(l[u][c][i]));  // 0 where the sum overflows
       }
       if (t0 + u * step < (int)r1) {
 #pragma unroll
@@ -534,7 +582,7 @@ extern "C" int moe_balance_loss(const void* logits, int64_t ld, int dtype, int64
   const Result result = {counts, (int32_t*)saved, loss}, later = {};
   const bool whole = plan.blocks == 1 && !cu_seqlens;
 #define MOE_BL(T, V, CH)                                                                                                            \
-  launch_pdl(balance_sums_kernel<T, V, CH>, dim3((unsigned)plan.blocks), kThreads, smem, 1, st, "balance_loss", b, slots, whole ? result : later, \
+  launch_pdl(balance_sums_kernel<T, V, CH>, dim3((unsigned)plan.blocks + (cu_seqlens != nullptr)), kThreads, smem, 1, st, "balance_loss", b, slots, whole ? result : later, \
              status)
   rc = MOE_BALANCE_DISPATCH(MOE_BL, dtype, plan);
 #undef MOE_BL

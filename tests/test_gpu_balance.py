@@ -1,7 +1,7 @@
 """moe_balance_loss against its definition in 64 bits, and the run from a layer's output to the experts.
 
 Tolerances: a score is exp2((u - max) log2 e) over its sum.  The argument is off by 3 roundings of itself, u of the sigmoid
-form by some 4 of its own, exp2 by 2, the sum over a row and the quotient by 40 roundings at most; a mean over tokens by one
+form by some 4 of its own and 4 of one, exp2 by 2, the sum over a row and the quotient by 40 roundings at most; a mean over tokens by one
 for each addition."""
 
 import pytest

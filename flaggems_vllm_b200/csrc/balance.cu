@@ -15,8 +15,8 @@
 // in registers and shared memory; sequence s in block c goes to slot c + s, which no other pair has (a walk along the rows
 // adds one to c or to s at every step).  The second adds the slots in order, so that results are the same bits in every run.
 // Bound: the logits are read once forward and once backward; up to some ten thousand tokens it is the launches and the chain of
-// loads in a block.  us on the device, forward and backward: 64 x 8 fp32 4.0 + 2.8 (one launch forward), 4096 x 128 bf16 10.7 + 4.4,
-// 8192 x 256 fp32 11.5 + 5.6, the same in 23 padded sequences of sigmoid scores 18.7 + 9.5, 65536 x 256 fp32 21 + 27.6 (floor 10 + 20).
+// loads in a block.  us on the device, forward and backward: 64 x 8 fp32 4.0 + 2.8 (one launch forward), 4096 x 128 bf16 9.8 + 4.4,
+// 8192 x 256 fp32 10.6 + 5.6, the same in 23 padded sequences of sigmoid scores 18.7 + 9.5, 65536 x 256 fp32 21 + 27.6 (floor 10 + 20).
 #include "moe_common.cuh"
 
 namespace moe {
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
   if (bad) live = 0;
   double part = 0.0;
   for (int r = warp; r < 32; r += warps) {  // a warp per expert
-    double total = lane < warps ? (double)mass[lane][r] : 0.0;
+    float total = lane < warps ? mass[lane][r] : 0.0f;
     n = lane < warps && !bad ? count[lane][r] : 0;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
     if (lane == 0 && expert < b.experts) {
       out.counts[(int64_t)s * b.experts + expert] = n;
       out.saved[(int64_t)s * b.experts + expert] = n;
-      part += (double)n * total;
+      part += (double)n * (double)total;
     }
   }
   if (lane == 0) shd[warp] = part;
@@ -386,13 +386,23 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
   __threadfence();
   double sum = 0.0;
   int filled = 0;
-  for (int64_t i = threadIdx.x; i < (int64_t)b.sequences * gridDim.x; i += blockDim.x) sum += __ldcg(in.part + i);
-  for (int i = threadIdx.x; i < b.sequences; i += blockDim.x) filled += __ldcg(out.saved + (int64_t)b.sequences * b.experts + i) > 0;
-  sum = block_sum(sum, shd);
-  filled = block_sum(filled, shi);
+  const int parts = b.sequences * (int)gridDim.x;
+  if (parts <= 32) {  // a warp's work: no barriers
+    if (warp != 0) return;
+    sum = lane < parts ? __ldcg(in.part + lane) : 0.0;
+    filled = lane < b.sequences && __ldcg(out.saved + (int64_t)b.sequences * b.experts + lane) > 0;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+    filled = __reduce_add_sync(0xFFFFFFFFu, filled);
+  } else {
+    for (int i = threadIdx.x; i < parts; i += blockDim.x) sum += __ldcg(in.part + i);
+    for (int i = threadIdx.x; i < b.sequences; i += blockDim.x) filled += __ldcg(out.saved + (int64_t)b.sequences * b.experts + i) > 0;
+    sum = block_sum(sum, shd);
+    filled = block_sum(filled, shi);
+  }
   if (threadIdx.x == 0) {
     out.saved[(int64_t)b.sequences * (b.experts + 1)] = filled;
-    *out.loss = bad ? __uint_as_float(0x7FC00000u) : (float)(sum / (filled > 0 ? filled : 1));
+    *out.loss = bad ? __uint_as_float(0x7FC00000u) : (float)(filled > 1 ? sum / filled : sum);
   }
 }
 

@@ -653,7 +653,7 @@ bool pieces16(const void* p, int64_t ld, int size) { return aligned16(p) && ld *
 
 // Threads to a row that give each all pieces that it holds, `held` of them in flight at once; 0 = the kernel for any row.
 int threads_of(int pieces, int held) {
-  for (int threads = 32; threads <= 512; threads *= 2)
+  for (int threads = 32; threads <= 1024; threads *= 2)
     if (pieces <= threads * held) return threads;
   return 0;
 }
@@ -675,6 +675,7 @@ int launch_pieces(const Forward& p, cudaStream_t st) {
     case 128: return launch_rows<T, V, 128, CH, FORMAT>(p, st);
     case 256: return launch_rows<T, V, 256, CH, FORMAT>(p, st);
     case 512: return launch_rows<T, V, 512, CH, FORMAT>(p, st);
+    case 1024: return launch_rows<T, V, 1024, CH, FORMAT>(p, st);
   }
   if (V == 1 && held && p.cols <= 1024 * 8) return launch_rows<T, 1, 1024, 8, FORMAT>(p, st);
   return launch_pdl(rms_norm_any_kernel<T>, dim3((unsigned)p.rows), 256, 0, 1, st, "rms_norm", p);
@@ -766,6 +767,7 @@ int launch_backward(const Backward& p, bool vector, int parts, cudaStream_t st) 
     if (pieces <= 256 * 2) return launch_grad_ring<T, 256, 2, 2, 1024>(p, parts, st);
     if (pieces <= 512 * 2) return launch_grad_ring<T, 512, 2, 2, 1024>(p, parts, st);
     if (pieces <= 1024 * 2) return launch_grad_ring<T, 1024, 2, 2, 1024>(p, parts, st);
+    if (pieces <= 1024 * 4) return launch_grad_ring<T, 1024, 4, 1, 1024>(p, parts, st);  // one row fills the ring
     return launch_grad_any<T>(p, parts, st);
   }
 #define MOE_RG(TPR, CH) \

@@ -56,7 +56,7 @@ def check_norm(y, want, cols, dtype):
 
 ROWS = [1, 2, 5, 37, 300]
 COLS = [1, 7, 8, 33, 64, 100, 128, 256, 1000, 1023, 1024, 1032, 1999, 2048, 2056, 4096, 4104, 5001, 7168, 8191, 8192, 8200, 16384,
-        16392, 20001]
+        16392, 20001, 20480, 33000]
 
 
 @pytest.mark.parametrize("cols", COLS)
@@ -134,7 +134,8 @@ def test_bad_values_stay_in_their_row(cols):
 
 def test_in_place():
     for cols, dtype, gap in ((64, torch.bfloat16, 0), (7168, torch.bfloat16, 0), (2048, torch.float16, 16), (1023, torch.float32, 3),
-                             (16392, torch.bfloat16, 0), (20001, torch.float32, 1)):
+                             (16392, torch.bfloat16, 0), (20001, torch.float32, 1),
+                             (33000, torch.bfloat16, 0)):
         for M in (1, 5, 200):
             bx = torch.randn(M, cols + gap, device=DEV).to(dtype)
             br = torch.randn(M, cols + gap, device=DEV).to(dtype)
@@ -215,7 +216,7 @@ def check_grads(x, r, w, dy, dh, dx, dw, eps=EPS):
 
 
 @pytest.mark.parametrize("cols", [1, 7, 64, 100, 128, 1000, 1023, 1024, 1032, 1999, 2048, 2056, 4096, 4104, 7168, 8200, 16384, 16392,
-                                  20001])
+                                  20001, 20480, 33000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_gradients(cols, dtype):
     for M in (1, 3, 333):
@@ -365,7 +366,7 @@ def check_quant(q, s, want, group, dtype, quant_eps, ue8m0, cols):
 
 @pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2, torch.int8])
 @pytest.mark.parametrize("cols,groups", [(128, (None, 128, 64, 8)), (512, (None, 256, 512, 1)), (1000, (None, 8, 40, 125)),
-                                         (2048, (None, 128)), (7168, (None, 128, 64)), (16384, (None, 128)), (16896, (None, 128, 96)), (1032, (None, 8, 24)), (5000, (None, 8)), (1040, (None, 16)),
+                                         (2048, (None, 128)), (7168, (None, 128, 64)), (16384, (None, 128)), (16896, (None, 128, 96)), (1032, (None, 8, 24)), (5000, (None, 8)), (1040, (None, 16)), (20480, (None, 128)), (33024, (None, 128)),
                                          (777, (None, 7))])
 def test_quant(dtype, cols, groups):
     for in_dtype in (torch.bfloat16, torch.float32):

@@ -265,6 +265,23 @@ def test_large_and_repeatable():
     check(logits, ids, "sigmoid", cu, torch.rand(T, device=DEV) < 0.2)
 
 
+def test_offsets_beyond_32_bits():
+    """Rows that begin more than 2^31 elements into their buffer."""
+    ld, E = 1 << 28, 96
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("not enough free memory")
+    buf = torch.empty(9 * ld, dtype=torch.bfloat16, device=DEV).view(9, ld)
+    logits, ids = make(9, E, 4, torch.bfloat16)
+    far = buf[:, 64:64 + E]
+    far.copy_(logits)
+    for scoring in ("softmax", "sigmoid"):
+        near = check(logits, ids, scoring)
+        leaf = far.detach().requires_grad_()
+        loss, counts = fg.moe_balance_loss(leaf, ids, scoring)
+        assert torch.equal(loss, near[0]) and torch.equal(counts, near[1])
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], near[2])
+
+
 def test_counts_are_the_callers():
     logits, ids = make(100, 16, 2)
     leaf = logits.clone().requires_grad_()

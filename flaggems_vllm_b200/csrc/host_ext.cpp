@@ -594,18 +594,20 @@ bool balance_args(const at::Tensor& l, const at::Tensor& ids, const at::Tensor* 
 const int32_t* cu_pointer(const at::Tensor* cu) { return cu ? cu->const_data_ptr<int32_t>() : nullptr; }
 const uint8_t* pad_pointer(const at::Tensor* pad) { return pad ? (const uint8_t*)pad->const_data_ptr() : nullptr; }
 
-// loss, counts, and what the gradient needs
+// loss, counts, and what the gradient needs (where `keep`; else it lies in the workspace: an allocation less)
 std::array<at::Tensor, 3> balance_forward(const at::Tensor& l, const at::Tensor& ids, const at::Tensor* cu, const at::Tensor* pad,
-                                          bool sigmoid, const BalanceArgs& p) {
+                                          bool sigmoid, const BalanceArgs& p, bool keep) {
   c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
   int64_t bytes[2];
   must(moe_balance_loss_workspace(p.tokens, (int)p.experts, (int)p.topk, p.sequences, bytes));
   at::Tensor loss = fresh({}, at::kFloat, p.dev);
   at::Tensor counts = cu ? fresh({p.sequences, p.experts}, at::kInt, p.dev) : fresh({p.experts}, at::kInt, p.dev);
-  at::Tensor saved = fresh({bytes[1]}, at::kByte, p.dev), ws = fresh({bytes[0]}, at::kByte, p.dev);
+  at::Tensor saved, ws = fresh({bytes[0] + (keep ? 0 : bytes[1])}, at::kByte, p.dev);  // bytes[0] is a multiple of 16
+  if (keep) saved = fresh({bytes[1]}, at::kByte, p.dev);
   must(moe_balance_loss(l.const_data_ptr(), p.ld, p.code, p.tokens, (int)p.experts, ids.const_data_ptr(), p.ids64, (int)p.topk, sigmoid,
                         cu_pointer(cu), p.sequences, pad_pointer(pad), loss.mutable_data_ptr<float>(), counts.mutable_data_ptr<int32_t>(),
-                        saved.mutable_data_ptr(), ws.mutable_data_ptr(), bytes[0], p.status, stream_on(p.dev)));
+                        keep ? saved.mutable_data_ptr() : (char*)ws.mutable_data_ptr() + bytes[0], ws.mutable_data_ptr(), bytes[0], p.status,
+                        stream_on(p.dev)));
   return {loss, counts, saved};
 }
 
@@ -615,7 +617,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     BalanceArgs p;
     const at::Tensor *c = cu ? &*cu : nullptr, *m = pad ? &*pad : nullptr;
     if (!balance_args(l, ids, c, m, &p)) throw KernelError("moe_balance_loss: unsupported operands");
-    auto out = balance_forward(l, ids, c, m, sigmoid, p);
+    auto out = balance_forward(l, ids, c, m, sigmoid, p, true);
     ctx->save_for_backward({l, out[2], c ? *c : at::Tensor(), m ? *m : at::Tensor()});
     ctx->saved_data["sigmoid"] = sigmoid;
     ctx->saved_data["topk"] = p.topk;
@@ -669,7 +671,7 @@ PyObject* balance_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
       loss = out[0];
       counts = out[1];
     } else {
-      auto out = balance_forward(l, ids, cu, pad, sigmoid, p);
+      auto out = balance_forward(l, ids, cu, pad, sigmoid, p, false);
       loss = out[0];
       counts = out[1];
     }

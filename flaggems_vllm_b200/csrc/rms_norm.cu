@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_grad_single_kernel(const Backw
         s[1] = fmaf(weight(t + c * TPR) * g[c], h[c], s[1]);
       }
     }
-    join_row<Sum, 2, TPR>(s, sh[turn]);
+    join_row<Sum, 2, TPR, TPR == BLOCK>(s, sh[turn]);
     const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
     const float k = inv * inv * (s[1] * p.mean);
 #pragma unroll
@@ -582,20 +582,21 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_grad_single_kernel(const Backw
   }
 }
 
-// dw[col] = sum over the blocks' partial sums, in order: 32 columns per block, 32 threads to a column.
-template <typename W>
+// dw[col] = sum over the blocks' partial sums, in order: 32 columns per block, 32 threads to a column, N parts of each in flight
+// (with 5 a part of every multiprocessor is one round).
+template <typename W, int N>
 __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int parts, int cols, W* __restrict__ dw) {
   pdl_wait();
   pdl_trigger();
   __shared__ float sh[32][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
   float s = 0.0f;
-  for (int i = r; i < parts; i += 32 * 5) {  // a part for every multiprocessor in one go
-    float v[5];
+  for (int i = r; i < parts; i += 32 * N) {
+    float v[N];
 #pragma unroll
-    for (int j = 0; j < 5; ++j) v[j] = col < cols && i + 32 * j < parts ? partial[(int64_t)(i + 32 * j) * cols + col] : 0.0f;
+    for (int j = 0; j < N; ++j) v[j] = col < cols && i + 32 * j < parts ? partial[(int64_t)(i + 32 * j) * cols + col] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 5; ++j) s += v[j];
+    for (int j = 0; j < N; ++j) s += v[j];
   }
   sh[r][threadIdx.x & 31] = s;
   __syncthreads();
@@ -734,10 +735,18 @@ int check_forward(const char* who, const void* x, int dtype, int weight_dtype, c
   return 0;
 }
 
-// Blocks of the gradient, each with its part of dw: one to a multiprocessor, whose shared memory it fills, or two.
-int grad_blocks(int64_t rows, bool vector) {
-  const int64_t most = (int64_t)sm_count() * (vector ? 1 : 2);
+// Blocks of the gradient, each with its part of dw: one to a multiprocessor, whose shared memory it fills, or, element by element,
+// as many as make 1024 threads (8192 x 501 bf16: 28 us with two of 256 threads, 17 with eight of 128).
+int grad_blocks(int64_t rows, int64_t cols, bool vector) {
+  const int64_t most = (int64_t)sm_count() * (vector ? 1 : cols <= 128 * 4 ? 8 : cols <= 256 * 4 ? 4 : 2);
   return (int)(rows < most ? rows : most);
+}
+
+template <typename W>
+int sum_parts(const float* partial, int parts, int cols, W* dw, cudaStream_t st) {
+  const dim3 grid((unsigned)((cols + 31) / 32));
+  return parts <= 32 * 5 ? launch_pdl(weight_grad_kernel<W, 5>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, cols, dw)
+                         : launch_pdl(weight_grad_kernel<W, 10>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, cols, dw);
 }
 
 template <typename T>
@@ -773,6 +782,8 @@ int launch_backward(const Backward& p, bool vector, int parts, cudaStream_t st) 
 #define MOE_RG(TPR, CH) \
   launch_pdl(rms_norm_grad_single_kernel<T, TPR, CH>, dim3((unsigned)parts), TPR > 128 ? TPR : 128, 0, 1, st, "rms_norm_grad", p)
   if (p.cols <= 32 * 4) return MOE_RG(32, 4);
+  if (p.cols <= 64 * 4) return MOE_RG(64, 4);
+  if (p.cols <= 128 * 4) return MOE_RG(128, 4);
   if (p.cols <= 256 * 4) return MOE_RG(256, 4);
   if (p.cols <= 512 * 4) return MOE_RG(512, 4);
   return launch_grad_any<T>(p, parts, st);
@@ -830,7 +841,7 @@ extern "C" int moe_rms_norm_grad_workspace(int64_t rows, int64_t cols, int64_t* 
   using namespace moe;
   if (rows < 0 || cols <= 0 || cols > (1 << 24) || !bytes) return fail(MOE_E_BADARG, "rms_norm_grad: bad extent");
   if (rows > kMaxRows) return fail(MOE_E_TOOBIG, "rms_norm_grad: too many rows");
-  *bytes = 4 * ((int64_t)grad_blocks(rows, false) * cols + rows);
+  *bytes = 4 * ((int64_t)grad_blocks(rows, cols, false) * cols + rows);
   return 0;
 }
 
@@ -847,7 +858,7 @@ extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, cons
     return ce == cudaSuccess ? 0 : fail((int)ce, "rms_norm_grad: %s", cudaGetErrorString(ce));
   }
   if (!dy || (!dx && !dweight)) return fail(MOE_E_BADARG, "rms_norm_grad: null pointer");
-  if (dweight && (!workspace || workspace_bytes < 4 * ((int64_t)grad_blocks(rows, false) * cols + rows) || !aligned16(workspace)))
+  if (dweight && (!workspace || workspace_bytes < 4 * ((int64_t)grad_blocks(rows, cols, false) * cols + rows) || !aligned16(workspace)))
     return fail(MOE_E_BADARG, "rms_norm_grad: workspace too small");
   Backward p = {};
   p.dy = dy; p.dh = dresidual_out; p.h = h; p.weight = weight; p.dx = dx; p.partial = dweight ? (float*)workspace : nullptr;
@@ -855,18 +866,13 @@ extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, cons
   const int size = dtype == MOE_F32 ? 4 : 2;
   const bool vector = cols % (16 / size) == 0 && pieces16(h, h_ld, size) && aligned16(dy) && aligned16(dresidual_out) && aligned16(dx) &&
                       aligned16(weight);
-  const int parts = grad_blocks(rows, vector);
+  const int parts = grad_blocks(rows, cols, vector);
   rc = dtype == MOE_F32 ? launch_backward<float>(p, vector, parts, st)
        : dtype == MOE_F16 ? launch_backward<__half>(p, vector, parts, st)
                           : launch_backward<__nv_bfloat16>(p, vector, parts, st);
   if (rc || !dweight) return rc;
-  const dim3 grid((unsigned)((cols + 31) / 32));
   const float* partial = (const float*)workspace;
-  switch (weight_dtype) {
-    case MOE_F32: return launch_pdl(weight_grad_kernel<float>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, (int)cols, (float*)dweight);
-    case MOE_F16: return launch_pdl(weight_grad_kernel<__half>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, (int)cols, (__half*)dweight);
-    default:
-      return launch_pdl(weight_grad_kernel<__nv_bfloat16>, grid, 1024, 0, 1, st, "rms_norm_grad (weight)", partial, parts, (int)cols,
-                        (__nv_bfloat16*)dweight);
-  }
+  return weight_dtype == MOE_F32   ? sum_parts(partial, parts, (int)cols, (float*)dweight, st)
+         : weight_dtype == MOE_F16 ? sum_parts(partial, parts, (int)cols, (__half*)dweight, st)
+                                   : sum_parts(partial, parts, (int)cols, (__nv_bfloat16*)dweight, st);
 }

@@ -108,10 +108,15 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return (g / (1.0f + expf(-g))) * u;
 }
 
-// v / s, correctly rounded, for |v| <= 448 s (1 + ulp) from the rounded reciprocal of s: one correction step by the exact
-// remainder (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990).  Where the quotient is
-// so small that the remainder is not exact it rounds to zero in e4m3 all the same: over every pair of finite bf16 or f16
-// values (amax, |v| <= amax) the e4m3 bytes are those of the division.  The sign is v's, of a zero too.
+// v / s from the rounded reciprocal of s: one correction step by the exact remainder (P. Markstein, Computation of elementary
+// functions on the IBM RISC System/6000, 1990).  The sign is v's, of a zero too.
+//
+// For e4m3, e5m2 and int8, fp32 v of any size in the format's reach and 1e-20 < s < 1e30 the bytes are those of the division.
+// They can differ at the format's borders only, and there they were compared for each of the 2^23 mantissas of s, all borders
+// and the nine fp32 values of v around each, with s near 2^-66, 2^-40, 1, 2^60 and 2^99: not one quotient differs.  Quotients
+// below the smallest border round to zero either way.  Far below 1e-20 the remainder of a small quotient is a subnormal that
+// has lost its last bits: with s near 2^-88 two bytes of e5m2 differ, near 2^-99 some 5500 of them and 54 of e4m3.  In e4m3 with
+// the scale's floor at 1e-10 / 448, as the layer has it, every pair of finite bf16 or f16 values (amax, |v| <= amax) agrees.
 __device__ __forceinline__ float div_by_scale(float v, float s, float inv) {
   const float q = v * inv;
   return copysignf(fmaf(fmaf(-q, s, v), inv, q), v);

@@ -182,7 +182,7 @@ __device__ __forceinline__ uint32_t pack_int8(float a, float b, float c, float d
 template <int V>
 __device__ __forceinline__ void quantise(const float (&y)[V], float s, int format, uint8_t* dst) {
   float d[V];
-  if (s > 1e-30f && s < 1e30f) {  // where the reciprocal and its remainders stay normal numbers
+  if (s > 1e-20f && s < 1e30f) {  // where div_by_scale() gives the bytes of the division
     const float inv = 1.0f / s;
 #pragma unroll
     for (int i = 0; i < V; ++i) d[i] = div_by_scale(y[i], s, inv);

@@ -354,6 +354,12 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// A tangent of forward mode would be dropped (a dual tensor wants no gradient by itself) or, in place, be left on other values.
+void no_tangent(std::initializer_list<const at::Tensor*> ts, const char* who) {
+  for (const at::Tensor* t : ts)
+    if (t && t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(who) + " has no derivative in forward mode");
+}
+
 // Gradients that a second differentiation would go through end in an error there, not in silence.
 variable_list once(variable_list grads, const char* who) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -467,6 +473,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 4 || !is_tensor(a[0]) || !is_tensor(a[1]) || !as_double(a[2], &eps) || (a[3] != Py_None && !is_tensor(a[3]))) MOE_NONE;
   const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]);
   const at::Tensor* residual = a[3] == Py_None ? nullptr : &tensor(a[3]);
+  no_tangent({&x, &w, residual}, "rms_norm");
   NormArgs p;
   if (!(eps >= 0.0 && eps < 3e38) || !norm_args(x, w, residual, &p)) MOE_NONE;
   at::Tensor y, h;
@@ -502,6 +509,7 @@ PyObject* fused_add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   double eps;
   if (n != 4 || !is_tensor(a[0]) || !is_tensor(a[1]) || !is_tensor(a[2]) || !as_double(a[3], &eps)) MOE_NONE;
   const at::Tensor &x = tensor(a[0]), &residual = tensor(a[1]), &w = tensor(a[2]);
+  no_tangent({&x, &residual, &w}, "fused_add_rms_norm");
   NormArgs p;
   if (!(eps >= 0.0 && eps < 3e38) || !norm_args(x, w, &residual, &p) || wants_grad({&x, &residual, &w})) MOE_NONE;
   if (p.rows > 1 && (p.x_ld < p.cols || p.residual_ld < p.cols)) MOE_NONE;
@@ -528,6 +536,7 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
     MOE_NONE;
   const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]);
   const at::Tensor* residual = a[3] == Py_None ? nullptr : &tensor(a[3]);
+  no_tangent({&x, &w, residual}, "rms_norm_quant");
   NormArgs p;
   if (!(eps >= 0.0 && eps < 3e38) || !(quant_eps >= 0.0 && quant_eps < 3e38) || !norm_args(x, w, residual, &p) ||
       wants_grad({&x, &w, residual}))
@@ -659,6 +668,7 @@ PyObject* balance_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     MOE_NONE;
   const at::Tensor &l = tensor(a[0]), &ids = tensor(a[1]);
   const at::Tensor *cu = a[3] == Py_None ? nullptr : &tensor(a[3]), *pad = a[4] == Py_None ? nullptr : &tensor(a[4]);
+  no_tangent({&l}, "moe_balance_loss");
   BalanceArgs p;
   if (!balance_args(l, ids, cu, pad, &p)) MOE_NONE;
   const bool sigmoid = truth(a[2]);

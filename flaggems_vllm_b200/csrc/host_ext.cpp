@@ -374,6 +374,9 @@ variable_list once(variable_list grads, const char* who) {
   return grads;
 }
 
+// A hook on saved tensors may hand back anything: another layout is served, another device, type or size refused.
+constexpr char kChanged[] = ": what was saved for the backward pass came back with another device, type or size";
+
 cudaStream_t stream_on(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 
 struct NormArgs {
@@ -425,8 +428,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const variable_list saved = ctx->get_saved_variables();
     const bool has_residual = ctx->saved_data["residual"].toBool();
     const double eps = ctx->saved_data["eps"].toDouble();
-    at::Tensor h = saved[0];
-    const at::Tensor& w = saved[1];
+    at::Tensor h = saved[0], w = saved[1];
     const at::Tensor dy = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
     const at::Tensor dh = has_residual && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
     const bool want_w = ctx->needs_input_grad(1);
@@ -441,8 +443,12 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     NormArgs p;
     if (!norm_args(h, w, nullptr, &p)) {  // a hook may have handed back another layout
       h = h.contiguous();
-      if (!norm_args(h, w, nullptr, &p)) throw KernelError("rms_norm: unsupported operands in the backward pass");
+      w = w.contiguous();
+      if (!norm_args(h, w, nullptr, &p)) throw KernelError(std::string("rms_norm") + kChanged);
     }
+    for (const at::Tensor* t : {&dy, &dh})  // the engine holds them against the outputs, nobody holds those against what was saved
+      if (t->defined() && (!t->is_cuda() || t->get_device() != p.dev || t->scalar_type() != h.scalar_type() || !t->sizes().equals(h.sizes())))
+        throw KernelError(std::string("rms_norm") + kChanged);
     {
       at::AutoDispatchBelowADInplaceOrView below;  // the buffers are no part of a graph
       c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
@@ -639,13 +645,21 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     variable_list out(5);
     if (!grads[0].defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
-    at::Tensor l = saved[0];
-    const at::Tensor *cu = saved[2].defined() ? &saved[2] : nullptr, *pad = saved[3].defined() ? &saved[3] : nullptr;
+    at::Tensor l = saved[0], counts = saved[1], cu = saved[2], pad = saved[3];
+    const int64_t sequences = ctx->saved_data["sequences"].toInt();
+    if (!l.is_cuda() || l.dim() != 2 || float_code(l) < 0) throw KernelError(std::string("moe_balance_loss") + kChanged);
     int64_t tokens, ld;
     if (!rows_of(l, &tokens, &ld)) {
       l = l.contiguous();
       rows_of(l, &tokens, &ld);
     }
+    auto dense = [&](at::Tensor& t, at::ScalarType type, int64_t numel) {
+      if (t.defined()) t = t.contiguous();
+      return !t.defined() || (cuda_dense(t, l.get_device()) && t.scalar_type() == type && t.numel() == numel);
+    };
+    if (!counts.defined() || !dense(counts, at::kByte, 4 * (sequences * (l.size(1) + 1) + 1)) || !dense(cu, at::kInt, sequences + 1) ||
+        !dense(pad, at::kBool, tokens))
+      throw KernelError(std::string("moe_balance_loss") + kChanged);
     const at::Tensor dloss = grads[0].to(at::kFloat).contiguous();
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -653,8 +667,8 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
       c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
       out[0] = fresh(l.sizes(), l.scalar_type(), dev);
       must(moe_balance_loss_grad(l.const_data_ptr(), ld, float_code(l), tokens, (int)l.size(1), (int)ctx->saved_data["topk"].toInt(),
-                                 ctx->saved_data["sigmoid"].toBool(), cu_pointer(cu), (int)ctx->saved_data["sequences"].toInt(),
-                                 pad_pointer(pad), saved[1].const_data_ptr(), dloss.const_data_ptr<float>(), out[0].mutable_data_ptr(),
+                                 ctx->saved_data["sigmoid"].toBool(), cu_pointer(cu.defined() ? &cu : nullptr), (int)sequences,
+                                 pad_pointer(pad.defined() ? &pad : nullptr), counts.const_data_ptr(), dloss.const_data_ptr<float>(), out[0].mutable_data_ptr(),
                                  stream_on(dev)));
     }
     return once(out, "moe_balance_loss");

@@ -1,4 +1,5 @@
-"""What the norms and the balance loss do with the rest of torch's differentiation: forward mode is refused, not lost."""
+"""What the norms and the balance loss do with the rest of torch's differentiation: forward mode is refused, not lost, and hooks on
+saved tensors may hand back another layout, nothing else."""
 
 import pytest
 import torch
@@ -51,3 +52,67 @@ def test_forward_mode_of_the_balance_loss_is_refused(strided):
             fg.moe_balance_loss(fwad.make_dual(l, torch.ones_like(l)), ids)
         inside = fg.moe_balance_loss(logits, ids)
     assert torch.equal(inside[0], fg.moe_balance_loss(logits, ids)[0])
+
+
+def hooks(change, which=None):
+    """Saved tensors come back changed, all of them or the one that was saved as the `which`-th."""
+    saved = []
+
+    def pack(t):
+        saved.append(t)
+        return len(saved) - 1, t
+
+    def unpack(item):
+        return change(item[1]) if which is None or item[0] == which else item[1]
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, unpack)
+
+
+def apart(t):
+    return torch.stack([t, t], -1)[..., 0]
+
+
+def norm_grads(residual=True):
+    x, w, r = (t.requires_grad_() for t in rows(torch.bfloat16))
+    out = fg.rms_norm(x, w, 1e-6, r if residual else None)
+    leaves = (x, w, r) if residual else (x, w)
+    return lambda: torch.autograd.grad([t.float().square().sum() for t in (out if residual else [out])], leaves)
+
+
+def balance_grads():
+    g = torch.Generator(device=DEV)
+    g.manual_seed(0)
+    l = torch.randn((50, 16), generator=g, device=DEV).requires_grad_()
+    ids = torch.randint(0, 16, (50, 2), generator=g, device=DEV)
+    cu = torch.tensor([0, 20, 45], dtype=torch.int32, device=DEV)
+    loss, _ = fg.moe_balance_loss(l, ids, "softmax", cu, torch.rand((50,), generator=g, device=DEV) < 0.2)
+    return lambda: torch.autograd.grad(loss, l)
+
+
+@pytest.mark.parametrize("make", [norm_grads, lambda: norm_grads(False), balance_grads], ids=["norm", "norm alone", "balance"])
+@pytest.mark.parametrize("change", [lambda t: t.cpu().cuda(), apart, lambda t: t.clone()], ids=["moved", "strided", "copied"])
+def test_saved_tensors_in_another_layout(make, change):
+    want = make()()
+    with hooks(change):
+        grads = make()
+    assert all(torch.equal(a, b) for a, b in zip(grads(), want))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+@pytest.mark.parametrize("change", [lambda t: t.cpu(), lambda t: t[:-1], lambda t: torch.cat([t, t]), lambda t: t.to(torch.float64)],
+                         ids=["on the host", "shorter", "longer", "another type"])
+def test_saved_tensors_that_changed_are_refused(which, change):
+    for make in (norm_grads, balance_grads):
+        if make is norm_grads and which > 1:
+            continue
+        with hooks(change, which):
+            grads = make()
+        with pytest.raises((RuntimeError, ValueError)):  # a row more or less without sequences or padding is the engine's to refuse
+            grads()
+
+
+def test_a_stream_of_another_type_is_refused():
+    with hooks(lambda t: t.float()):  # the norm's own types, but not those of the gradient that comes in
+        grads = norm_grads()
+    with pytest.raises(RuntimeError, match="came back"):
+        grads()

@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) rms_norm_grad_kernel(const Backwar
     }
     join_row<Sum, 2, TPR, TPR == THREADS>(s, sh[turn]);  // the other half is still read by threads that are a row behind
     const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
-    const float k = inv * (s[1] * p.mean);
+    const float k = inv * (s[1] * p.mean);  // r^2 itself is infinite for rows below 5e-20 where eps is zero
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (t + c * TPR < pieces) {
@@ -555,13 +555,14 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_grad_single_kernel(const Backw
     }
     join_row<Sum, 2, TPR, TPR == BLOCK>(s, sh[turn]);
     const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
-    const float k = inv * inv * (s[1] * p.mean);
+    const float k = inv * (s[1] * p.mean);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = t + c * TPR;
       if (at < p.cols) {
-        dw[c] = fmaf(g[c], h[c] * inv, dw[c]);
-        if (p.dx != nullptr) reinterpret_cast<T*>(p.dx)[row * p.cols + at] = from_f32<T>(fmaf(inv, weight(at) * g[c] - h[c] * k, d[c]));
+        const float x = h[c] * inv;
+        dw[c] = fmaf(g[c], x, dw[c]);
+        if (p.dx != nullptr) reinterpret_cast<T*>(p.dx)[row * p.cols + at] = from_f32<T>(fmaf(inv, fmaf(-x, k, weight(at) * g[c]), d[c]));
       }
     }
   }
@@ -627,13 +628,13 @@ __global__ void __launch_bounds__(256) rms_norm_grad_any_kernel(const Backward p
   }
   join_row<Sum, 2, 256>(s, sh);
   const float inv = inverse_root(fmaf(s[0], p.mean, p.eps));
-  const float k = inv * inv * (s[1] * p.mean);
+  const float k = inv * (s[1] * p.mean);
   if (inv_rms != nullptr && threadIdx.x == 0) inv_rms[row] = inv;
   if (p.dx == nullptr) return;
   for (int i = threadIdx.x; i < p.cols; i += 256) {
-    float v = inv * (weight(i) * ToF32<T>::get(dy[i]) - ToF32<T>::get(h[i]) * k);
-    if (p.dh != nullptr) v += ToF32<T>::get(reinterpret_cast<const T*>(p.dh)[row * p.cols + i]);
-    reinterpret_cast<T*>(p.dx)[row * p.cols + i] = from_f32<T>(v);
+    const float d = p.dh != nullptr ? ToF32<T>::get(reinterpret_cast<const T*>(p.dh)[row * p.cols + i]) : 0.0f;
+    const float x = ToF32<T>::get(h[i]) * inv;
+    reinterpret_cast<T*>(p.dx)[row * p.cols + i] = from_f32<T>(fmaf(inv, fmaf(-x, k, weight(i) * ToF32<T>::get(dy[i])), d));
   }
 }
 template <typename T>

@@ -1,0 +1,40 @@
+"""Norms and their gradients where fp32 itself is the limit: rows of tiny numbers and rows of millions of equal ones."""
+
+import pytest
+import torch
+
+import flaggems_vllm_b200 as fg
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32 = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [64, 100, 1000, 1001, 1999, 2048, 2049, 4097, 7168, 20001, 33024])
+def test_gradient_of_tiny_rows_without_eps(cols, dtype):
+    """Rows of some 2^-65: the squares are normal numbers (2^-130 is a subnormal of 19 bits), the square of the root's inverse is
+    infinite.  Alignment and length do not matter."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(cols)
+    sign = torch.randint(0, 2, (5, cols), generator=g, device=DEV) * 2 - 1
+    x = ((1.0 + torch.rand((5, cols), generator=g, device=DEV)) * sign * 2.0 ** -65).to(dtype)
+    w = (1.0 + 0.5 * torch.rand((cols,), generator=g, device=DEV)).to(dtype)
+    dy = torch.randn((5, cols), generator=g, device=DEV).to(dtype)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = fg.rms_norm(xl, wl, 0.0)
+    dx, dw = torch.autograd.grad(y, (xl, wl), dy)
+    xd, wd, dyd = x.double(), w.double(), dy.double()
+    inv = 1.0 / xd.square().mean(-1, keepdim=True).sqrt()
+    n = xd * inv
+    mean = (wd * dyd * n).mean(-1, keepdim=True)
+    want = inv * (wd * dyd - n * mean)
+    # squares are off by 2^-19 at most, their root by half of that, and so is what is made of it; each sum adds its additions'
+    off = 2.0 ** -20 + (cols // 256 + 80) * F32
+    half = torch.finfo(dtype).eps / 2
+    assert ((y.double() - n * wd).abs() <= (n * wd).abs() * (half + off)).all()
+    size = inv * ((wd * dyd).abs() + n.abs() * (wd * dyd * n).abs().mean(-1, keepdim=True) * 2)
+    assert ((dx.double() - want).abs() <= want.abs() * half + size * 2 * off).all()
+    dww = (dyd * n).sum(0)
+    assert ((dw.double() - dww).abs() <= dww.abs() * half + (dyd * n).abs().sum(0) * (off + 16 * F32) + 1e-38).all()

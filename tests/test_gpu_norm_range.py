@@ -38,3 +38,30 @@ def test_gradient_of_tiny_rows_without_eps(cols, dtype):
     assert ((dx.double() - want).abs() <= want.abs() * half + size * 2 * off).all()
     dww = (dyd * n).sum(0)
     assert ((dw.double() - dww).abs() <= dww.abs() * half + (dyd * n).abs().sum(0) * (off + 16 * F32) + 1e-38).all()
+
+
+@pytest.mark.parametrize("cols", [33024, (1 << 20) + 8, (1 << 22) + 1, 1 << 24])
+@pytest.mark.parametrize("residual", [False, True])
+def test_long_rows_of_equal_numbers(cols, residual):
+    """The errors of additions do not cancel here; those of a row's sums must not grow with its length: at most 32 terms and a
+    tree of 8 additions are fp32, and each product, quotient, root and rounding counts one."""
+    value = 1.1
+    x = torch.full((1, cols), value, device=DEV)
+    r = torch.full((1, cols), 0.0, device=DEV) if residual else None
+    w = torch.full((cols,), 1.3, device=DEV)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    out = fg.rms_norm(*leaves, 0.0, r)
+    y = out[0] if residual else out
+    sums = 32 + 8 + 2
+    want = float(w.detach()[0].double())  # x / |x| times the weight
+    assert abs(y.double() - want).max().item() <= want * (sums / 2 + 5) * F32
+    # dy = 1 in one half, 3 in the other: dx = r w (dy - 2), where the mean of dy is 2 but for the odd column
+    dy = torch.ones_like(y)
+    dy[:, cols // 2:] = 3.0
+    dx, _ = torch.autograd.grad(y, leaves, dy)
+    mean = 1.0 + 2.0 * (cols - cols // 2) / cols
+    inv = 1.0 / float(x.detach()[0, 0].double())
+    exact = (inv * want * (dy.double() - mean))
+    # terms of the size r w dy and r w mean, each off by its own share: half the first sum's for r, three halves and the second sum's
+    off = inv * want * (3.0 * (sums / 2 + 5) + mean * (2.5 * sums + 12)) * F32
+    assert (dx.double() - exact).abs().max().item() <= off

@@ -335,16 +335,27 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, int dev) {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Rows of the last dimension and how far apart they are; false where that is no single distance.
+// Rows of the last dimension, whatever is in front of it, and how far apart they are; false where that is no single distance.
 bool rows_of(const at::Tensor& t, int64_t* rows, int64_t* ld) {
   if (t.dim() < 1) return false;
   const int64_t H = t.size(-1);
   *rows = H == 0 ? 0 : t.numel() / H;
   *ld = H;
   if (t.is_contiguous()) return true;
-  if (t.dim() != 2 || t.stride(1) != 1 || t.stride(0) < 0) return false;
-  *ld = t.stride(0);
-  return true;
+  if (H > 1 && t.stride(-1) != 1) return false;
+  int64_t inner = 0;  // rows of the dimensions behind
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (inner == 0) {
+      *ld = t.stride(d);
+      inner = t.size(d);
+    } else if (t.stride(d) == *ld * inner) {
+      inner *= t.size(d);
+    } else {
+      return false;
+    }
+  }
+  return *ld >= 0;
 }
 
 bool wants_grad(std::initializer_list<const at::Tensor*> ts) {

@@ -516,6 +516,8 @@ bool rows_meet(const at::Tensor& a, int64_t a_rows, int64_t a_ld, const at::Tens
   const uintptr_t a0 = (uintptr_t)a.const_data_ptr(), b0 = (uintptr_t)b.const_data_ptr();
   const uintptr_t a_size = a.element_size(), b_size = b.element_size();
   if (a0 >= b0 + ((b_rows - 1) * b_ld + cols) * b_size || b0 >= a0 + ((a_rows - 1) * a_ld + cols) * a_size) return false;
+  if (a_rows == 1) a_ld = b_ld;  // a single row has any distance
+  if (b_rows == 1) b_ld = a_ld;
   if (a_ld != b_ld || a_size != b_size || (a0 - b0) % a_size != 0) return true;
   const int64_t apart = (int64_t)((a0 > b0 ? a0 - b0 : b0 - a0) / a_size) % a_ld;
   return apart < cols || a_ld - apart < cols;

@@ -65,3 +65,16 @@ def test_rows_without_a_single_distance():
         with pytest.raises(ValueError, match="rows of contiguous elements"):
             fg.fused_add_rms_norm(x, torch.randn(x.shape, device=DEV), w)
         assert torch.equal(base, keep)
+
+
+def test_a_weight_between_the_rows():
+    for dtype, off in ((torch.bfloat16, 64), (torch.bfloat16, 70), (torch.float32, 64)):
+        buf = torch.randn(4, 160, device=DEV).to(dtype)
+        x, w = buf[:, :64], buf[2, off:off + 64]
+        r = torch.randn(4, 64, device=DEV).to(dtype)
+        want = fg.rms_norm(x, w, 1e-6, r)
+        fg.fused_add_rms_norm(x, r, w)
+        assert torch.equal(x, want[0]) and torch.equal(r, want[1])
+        for meets in (buf[2, 63:127], buf.view(-1)[160 + 97:160 + 161], buf.view(-1)[160 + 120:160 + 184]):
+            with pytest.raises(ValueError, match="share no memory"):
+                fg.fused_add_rms_norm(x, r, meets)

@@ -7,7 +7,6 @@ projections that ``per_token_group_quant_fp8`` feeds otherwise."""
 from __future__ import annotations
 
 import logging
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -18,7 +17,7 @@ from .quant import SUPPORTED_FP8_DTYPE
 logger = logging.getLogger(__name__)
 
 _FORMATS = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1, torch.int8: 2}
-_MAX_COLS, _MAX_ROWS = 1 << 24, 0x7FFFFFFF
+_MAX_COLS, _MAX_ROWS, _MAX_EPS = 1 << 24, 0x7FFFFFFF, 3e38
 
 
 def _check(x, weight, eps, residual, what):
@@ -33,8 +32,8 @@ def _check(x, weight, eps, residual, what):
         raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {list(weight.shape)}")
     if weight.dtype not in (x.dtype, torch.float32):
         raise ValueError(f"{what}: weight must be of the type of x or float32, got {weight.dtype}")
-    if not (math.isfinite(eps) and eps >= 0.0):
-        raise ValueError(f"{what}: eps must be finite and not negative")
+    if not 0.0 <= eps < _MAX_EPS:
+        raise ValueError(f"{what}: eps must be finite in fp32 and not negative")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"{what}: residual must have the shape and type of x")
     _lib.require_cuda(x, what)
@@ -149,5 +148,5 @@ def _check_quant(x, group_size, dtype, column_major_scales, scale_ue8m0, quant_e
         raise ValueError(f"{what}: column-major scales need a 2-D input")
     if scale_ue8m0 and dtype == torch.int8:
         raise ValueError(f"{what}: power-of-two scales are for the 8-bit floats")
-    if not (math.isfinite(quant_eps) and quant_eps >= 0.0):
-        raise ValueError(f"{what}: quant_eps must be finite and not negative")
+    if not 0.0 <= quant_eps < _MAX_EPS:
+        raise ValueError(f"{what}: quant_eps must be finite in fp32 and not negative")

@@ -142,6 +142,8 @@ def _check_quant(x, group_size, dtype, column_major_scales, scale_ue8m0, quant_e
     if group_size is not None:
         if group_size <= 0:
             raise ValueError(f"{what}: group_size must be positive")
+        if group_size % 1 != 0:
+            raise ValueError(f"{what}: group_size must be a whole number")
         if x.ndim >= 1 and x.shape[-1] % group_size != 0:
             raise ValueError(f"{what}: the last dimension of x {x.shape[-1]} must be divisible by group_size {group_size}")
     if column_major_scales and x.ndim != 2:

@@ -15,3 +15,17 @@ def test_eps_beyond_fp32(value):
             call()
     with pytest.raises(ValueError, match="quant_eps"):
         fg.rms_norm_quant(x, w, quant_eps=value)
+
+
+@pytest.mark.parametrize("group", [0.5, 2.5, 64 / 3])
+def test_group_sizes_that_are_no_whole_number(group):
+    """The row may well be a multiple of them: they used to be cut to whole numbers, 0.5 to the whole row."""
+    x, w = torch.zeros(4, 64 if group != 2.5 else 10), torch.ones(64 if group != 2.5 else 10)
+    with pytest.raises(ValueError, match="whole number"):
+        fg.rms_norm_quant(x, w, group_size=group)
+
+
+@pytest.mark.parametrize("group", [32, 32.0, np.int64(32)])
+def test_group_sizes_that_are_one(group):
+    with pytest.raises(RuntimeError, match="no CPU path"):  # past every other check
+        fg.rms_norm_quant(torch.zeros(4, 64), torch.ones(64), group_size=group)

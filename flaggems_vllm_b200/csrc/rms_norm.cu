@@ -882,6 +882,8 @@ extern "C" int moe_rms_norm_grad(const void* dy, const void* dresidual_out, cons
     return ce == cudaSuccess ? 0 : fail((int)ce, "rms_norm_grad: %s", cudaGetErrorString(ce));
   }
   if (!dy || (!dx && !dweight)) return fail(MOE_E_BADARG, "rms_norm_grad: null pointer");
+  if (dx && (dx == dy || dx == h || dx == dresidual_out))  // long rows are read again for dweight when dx is written
+    return fail(MOE_E_BADARG, "rms_norm_grad: dx lies apart from what it is made of");
   if (dweight && (!workspace || workspace_bytes < 4 * ((int64_t)grad_blocks(rows, cols, false) * cols + rows) || !aligned16(workspace)))
     return fail(MOE_E_BADARG, "rms_norm_grad: workspace too small");
   Backward p = {};

@@ -489,7 +489,8 @@ int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* residual, int64_
 
 /* Gradient of moe_rms_norm from h: dx (also the residual's; null = not wanted) = d y / d h applied to dy, plus
  * dresidual_out (null = none); dweight (null = not wanted) summed in fp32 over the rows in a fixed order and rounded to
- * weight_dtype.  dy, dresidual_out, dx [rows, cols] without gaps.  The workspace is needed for dweight. */
+ * weight_dtype.  dy, dresidual_out, dx [rows, cols] without gaps; dx lies apart from the others.  The workspace is needed for
+ * dweight. */
 int moe_rms_norm_grad_workspace(int64_t rows, int64_t cols, int64_t* bytes /* host */);
 int moe_rms_norm_grad(const void* dy, const void* dresidual_out, const void* h, int64_t h_ld, const void* weight, int dtype,
                       int weight_dtype, int64_t rows, int64_t cols, float eps, void* dx, void* dweight, void* workspace,

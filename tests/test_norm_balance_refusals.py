@@ -29,3 +29,14 @@ def test_group_sizes_that_are_no_whole_number(group):
 def test_group_sizes_that_are_one(group):
     with pytest.raises(RuntimeError, match="no CPU path"):  # past every other check
         fg.rms_norm_quant(torch.zeros(4, 64), torch.ones(64), group_size=group)
+
+
+def test_c_gradient_over_its_inputs():
+    """Rows of more than 64 KB are read again for the weight's gradient when dx has been written.  No call gets as far as a launch."""
+    from flaggems_vllm_b200 import _lib
+
+    P, before = 1 << 20, _lib.LAUNCHES
+    for dy, dh, h, dx in ((P, None, 2 * P, P), (P, None, 2 * P, 2 * P), (P, 3 * P, 2 * P, 3 * P)):
+        rc = _lib.lib().moe_rms_norm_grad(dy, dh, h, 64, 4 * P, 0, 0, 4, 64, 1e-6, dx, 5 * P, 6 * P, 1 << 30, None)
+        assert rc == -1 and b"apart" in _lib.lib().moe_last_error()
+    assert _lib.LAUNCHES == before

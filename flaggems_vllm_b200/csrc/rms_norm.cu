@@ -760,9 +760,12 @@ int check_forward(const char* who, const void* x, int dtype, int weight_dtype, c
 }
 
 // Blocks of the gradient, each with its part of dw: one to a multiprocessor, whose shared memory it fills, or, element by element,
-// as many as make 1024 threads (8192 x 501 bf16: 28 us with two of 256 threads, 17 with eight of 128).
+// as many as make 1024 threads (8192 x 501 bf16: 28 us with two of 256 threads, 17 with eight of 128).  The parts of long rows take
+// 256 MB at most, or 16 rows: two to a multiprocessor would be 20 GB for 2^24 columns, whose columns alone fill the device.
 int grad_blocks(int64_t rows, int64_t cols, bool vector) {
-  const int64_t most = (int64_t)sm_count() * (vector ? 1 : cols <= 128 * 4 ? 8 : cols <= 256 * 4 ? 4 : 2);
+  int64_t most = (int64_t)sm_count() * (vector ? 1 : cols <= 128 * 4 ? 8 : cols <= 256 * 4 ? 4 : 2);
+  const int64_t room = (int64_t)(256 << 20) / 4 / cols;
+  if (most > room) most = room > 16 ? room : 16;
   return (int)(rows < most ? rows : most);
 }
 

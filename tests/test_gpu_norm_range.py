@@ -65,3 +65,25 @@ def test_long_rows_of_equal_numbers(cols, residual):
     # terms of the size r w dy and r w mean, each off by its own share: half the first sum's for r, three halves and the second sum's
     off = inv * want * (3.0 * (sums / 2 + 5) + mean * (2.5 * sums + 12)) * F32
     assert (dx.double() - exact).abs().max().item() <= off
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 1 << 22), (40, (1 << 22) + 1), (70, (1 << 20) + 3)])
+def test_gradient_of_more_rows_than_parts(rows, cols):
+    """Long rows share 16 parts of the weight's gradient, or as many as 256 MB hold."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows)
+    x = torch.randn((rows, cols), generator=g, device=DEV).bfloat16()
+    dy = torch.randn((rows, cols), generator=g, device=DEV).bfloat16()
+    xl, wl = x.clone().requires_grad_(), torch.ones(cols, device=DEV, requires_grad=True)
+    dx, dw = torch.autograd.grad(fg.rms_norm(xl, wl), (xl, wl), dy)
+    want, terms = torch.zeros(cols, dtype=torch.float64, device=DEV), torch.zeros(cols, dtype=torch.float64, device=DEV)
+    off = (32 + 8 + 2) / 2 + 6 + rows  # a row's sum and root, its products; then every row behind one another at most
+    for i in range(rows):
+        n = x[i].double() / (x[i].double().square().mean() + 1e-6).sqrt()
+        want += n * dy[i].double()
+        terms += (n * dy[i].double()).abs()
+        exact = (dy[i].double() - n * (n * dy[i].double()).mean()) / (x[i].double().square().mean() + 1e-6).sqrt()
+        # a mean of products of random signs; its error is counted on their magnitudes
+        tol = exact.abs() * 2.0 ** -8 + (dy[i].double().abs() + n.abs()) * 2 * (off + 64) * F32
+        assert ((dx[i].double() - exact).abs() <= tol).all()
+    assert ((dw.double() - want).abs() <= terms * off * F32 + 1e-38).all()

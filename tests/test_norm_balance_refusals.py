@@ -40,3 +40,16 @@ def test_c_gradient_over_its_inputs():
         rc = _lib.lib().moe_rms_norm_grad(dy, dh, h, 64, 4 * P, 0, 0, 4, 64, 1e-6, dx, 5 * P, 6 * P, 1 << 30, None)
         assert rc == -1 and b"apart" in _lib.lib().moe_last_error()
     assert _lib.LAUNCHES == before
+
+
+@pytest.mark.parametrize("cols", [64, 8192, 1 << 16, 1 << 20, 1 << 22, 1 << 24])
+def test_workspace_of_the_gradient_does_not_outgrow_its_rows(cols):
+    """256 MB of partial sums, or those of 16 rows, and a number per row."""
+    import ctypes
+
+    from flaggems_vllm_b200 import _lib
+
+    need = ctypes.c_int64()
+    for rows in (1, 16, 300, 5000):
+        _lib.check(_lib.lib().moe_rms_norm_grad_workspace(rows, cols, ctypes.addressof(need)))
+        assert need.value <= 4 * rows + max(256 << 20, 4 * 16 * cols)

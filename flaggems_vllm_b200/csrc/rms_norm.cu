@@ -10,11 +10,12 @@
 // gradient, which has only h, is that of the same function.  y itself is rounded once: the quantiser takes its fp32 value.
 // The gradient computes r again (the row is in registers anyway), so nothing but h is kept between the two passes.
 //
-// Bound: memory.  A row is read once: it stays in the registers of the threads that share it, 32 values to a thread so that four
-// blocks of 256 threads, and their loads, are on a multiprocessor.  us on the device, 8192 x 7168 bf16 with a residual (470 MB: 72
-// at the rate of a copy): norm 69.5; e4m3 in groups of 128 70.4 (411 MB: 63), with the norm itself 82 (528 MB: 81); int8 per row
-// 68; gradient 84, of which 4 for the weight's (470 MB: 72).  16 or 64 values to a thread
-// instead: 3 to 6 % slower.  One token of 7168: 2.7, a launch and one round of loads.
+// Bound: memory.  A row is read once: it stays in the registers of the threads that share it, 64 bytes to a thread (32 values of 16
+// bits, 16 of fp32; four or eight where rows are not made of 16-byte pieces) so that four blocks of 256 threads, and their loads,
+// are on a multiprocessor.  us on the device, 8192 x 7168 bf16 with a residual (470 MB: 72 at the rate of a copy): norm 69.5; e4m3
+// in groups of 128 70.4 (411 MB: 63), with the norm itself 82 (528 MB: 81); int8 per row 68; gradient 84, of which 4 for the
+// weight's (470 MB: 72).  16 or 64 values of bf16 to a thread instead: 3 to 6 % slower.  One token of 7168: 2.7, a launch and one
+// round of loads.
 #include "moe_common.cuh"
 
 namespace moe {
@@ -153,7 +154,7 @@ __device__ __forceinline__ constexpr float quant_max(int format) { return format
 // The scale of a group from its largest magnitude.  A NaN in the group makes the scale NaN, as it makes the values it stands for.
 __device__ __forceinline__ float group_scale(float amax, float eps, int format, bool ue8m0) {
   float s = max_nan(amax, eps) * (1.0f / quant_max(format));
-  if (ue8m0 && s < INFINITY) {  // the smallest power of two that is not below it
+  if (ue8m0 && s < INFINITY) {  // the smallest power of two that is not below it, nor below 1e-10: the stand-alone quantiser's rule
     s = fmaxf(s, 1e-10f);
     const uint32_t b = __float_as_uint(s);
     s = __uint_as_float((b + 0x7FFFFFu) & 0x7F800000u);

@@ -56,8 +56,9 @@ def rms_norm(
     residual (it, h).
 
     ``h`` is ``x``, or ``x + residual`` rounded to their type: the stream as the next layer finds it.  ``weight`` has the
-    type of ``x`` or float32.  Differentiable once in all three; the weight's gradient is summed in fp32, in the same
-    order in every run."""
+    type of ``x`` or float32.  Differentiable once in all three, backwards; the weight's gradient is summed in fp32, in the
+    same order in every run.  The mean square is an fp32 number: rows whose mean square is beyond it are normed to zero, and
+    below 2^-130 (with ``eps`` of no more) it loses bits."""
     logger.debug("GEMS RMS NORM")
     out = _lib.host().rms_norm(x, weight, eps, residual) if x.is_cuda else None
     if out is None:
@@ -79,7 +80,8 @@ def fused_add_rms_norm(
     """In place: ``residual`` becomes the stream ``x + residual``, ``x`` its norm; returns (x, residual).
 
     Values are those of ``rms_norm(x, weight, eps, residual)``.  The rows of both may lie in wider buffers, whose other
-    columns stay as they are; neither may share memory with the other or with the weight.  Not differentiable: refused where a gradient is wanted."""
+    columns stay as they are, with any number of dimensions in front at one row distance; neither may share memory with the
+    other or with the weight.  Not differentiable: refused where a gradient is wanted."""
     logger.debug("GEMS FUSED ADD RMS NORM")
     if not x.is_cuda or not _lib.host().fused_add_rms_norm(x, residual, weight, eps):
         what, eps = "fused_add_rms_norm", float(eps)
@@ -111,10 +113,11 @@ def rms_norm_quant(
 
     ``x_s`` holds one scale per ``group_size`` elements of a row (None: one per row), shape
     ``x.shape[:-1] + (cols / group_size,)``, column-major in memory when ``column_major_scales``;
-    ``x_s = max(amax, quant_eps) / qmax``, rounded up to a power of two with ``scale_ue8m0``; a scale of zero
-    (``quant_eps=0``) stands over zeros.  ``dtype`` is
-    float8_e4m3fn (default), float8_e5m2 or int8.  The fp32 value of the norm is quantised, not its 16-bit rounding.
-    A NaN makes its group's scale NaN.  Not differentiable: refused where a gradient is wanted."""
+    ``x_s = max(amax, quant_eps) / qmax``; a scale of zero (``quant_eps=0``) stands over zeros.  ``scale_ue8m0`` raises
+    scales below 1e-10 to it and rounds up to a power of two, as ``per_token_group_quant_fp8`` does: the smallest is
+    2^-33, whatever ``quant_eps``.  ``dtype`` is float8_e4m3fn (default), float8_e5m2 or int8.  The fp32 value of the norm
+    is quantised, not its 16-bit rounding.  A NaN makes its group's scale NaN.  Not differentiable: refused where a
+    gradient is wanted."""
     logger.debug("GEMS RMS NORM QUANT")
     what = "rms_norm_quant"
     dtype = SUPPORTED_FP8_DTYPE if dtype is None else dtype

@@ -481,8 +481,8 @@ int moe_rms_norm(const void* x, int64_t x_ld, const void* residual, int64_t resi
 /* The same with y in 8 bits: per `group` consecutive columns (cols = one group per row)
  *   s = max(amax |y|, quant_eps) / qmax;   q = round(y / s)
  * of the fp32 value of y.  format: 0 e4m3 (qmax 448), 1 e5m2 (57344), 2 int8 (127).  scale_flags: 1 = scales [cols / group,
- * scale_ld] instead of [rows, cols / group]; 2 = s rounded up to a power of two (8-bit floats).  A NaN in a group makes its
- * scale NaN.  q, y (null = not wanted) and residual_out are [rows, cols] without gaps. */
+ * scale_ld] instead of [rows, cols / group]; 2 = max(s, 1e-10) rounded up to a power of two (8-bit floats; 2^-33 at least,
+ * whatever quant_eps).  A NaN in a group makes its scale NaN; a scale of zero stands over zeros.  q, y (null = not wanted) and residual_out are [rows, cols] without gaps. */
 int moe_rms_norm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, const void* weight, int dtype,
                        int weight_dtype, int64_t rows, int64_t cols, float eps, int format, int group, float quant_eps,
                        int scale_flags, void* q, float* scales, int64_t scale_ld, void* y, void* residual_out, void* stream);

@@ -73,3 +73,17 @@ def test_scales_of_any_size(dtype, lo, hi):
         w = shift(s * edge[at], torch.randint(-4, 5, (n, GROUP), generator=g, device=DEV, dtype=torch.int32))
         w[:, :1] = s * QMAX[dtype]  # the largest of the group
         check(w, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("cols", [256, 250])
+def test_power_of_two_scales_have_a_floor(dtype, cols):
+    """2^-33, the first power of two that is not below 1e-10, as the stand-alone quantiser has it, whatever quant_eps."""
+    x = torch.ones(3, cols, device=DEV)
+    for value in (0.0, 1e-30, 1e-10 * QMAX[dtype], 1.2e-10 * QMAX[dtype]):
+        w = torch.full((cols,), value, device=DEV)
+        want = 2.0 ** -32 if value == 1.2e-10 * QMAX[dtype] else 2.0 ** -33
+        for quant_eps in (0.0, 1e-10 * value):
+            q, s = fg.rms_norm_quant(x, w, 0.0, quant_eps=quant_eps, dtype=dtype, scale_ue8m0=True, group_size=cols // 2)
+            assert (s == want).all()
+            assert torch.equal(q.view(torch.uint8), bytes_of((w / want).expand_as(x), dtype).view(torch.uint8))

@@ -498,10 +498,13 @@ __global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_ke
 constexpr int kMaxExperts = 1024, kMaxTopk = 32;
 constexpr int64_t kMaxRoutes = 0x7FFF0000;  // a turn behind the last token is an int too
 
-// How the rows are shared out.  A turn of a block takes the tokens that its lanes have in hand; calls of up to four turns are
-// one block's, larger ones are spread over the multiprocessors.
+// How the rows are shared out: a turn of a block takes the tokens that its lanes have in hand, and turns are spread over the
+// multiprocessors.  `whole`: one block that has all rows ends the call, without a second launch, so it takes up to four turns (us
+// forward, 2048 x 8 fp32 8.6, 2049 x 8 in five blocks 8.8).  Where there is no launch to save it only works alone, so it is not
+// for sequences (2000 x 8 in 64 of them: 151 in one block, 48 in four) nor for the gradient (2048 x 8: 7.4 and 3.4, 128 x 256: 9.8
+// and 4.2).
 struct Plan { bool vector; int pieces, lanes, rows; int64_t blocks; };
-Plan plan_of(const void* logits, int64_t ld, const void* other, int dtype, int64_t tokens, int experts, int blocks_per_sm) {
+Plan plan_of(const void* logits, int64_t ld, const void* other, int dtype, int64_t tokens, int experts, int blocks_per_sm, bool whole) {
   Plan p;
   const int size = dtype == MOE_F32 ? 4 : 2, vec = 16 / size;
   p.vector = experts % vec == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)other & 15) == 0 && ld * size % 16 == 0;
@@ -513,7 +516,7 @@ Plan plan_of(const void* logits, int64_t ld, const void* other, int dtype, int64
   const int64_t turn = (int64_t)kWarps * (32 / p.lanes) * tokens_in_hand(p.pieces * width), spread = (int64_t)sm_count() * blocks_per_sm;
   int64_t rows = (tokens + spread - 1) / spread;
   if (rows < turn) rows = turn;
-  if (tokens <= 4 * turn) rows = tokens;
+  if (whole && tokens <= 4 * turn) rows = tokens;
   p.rows = (int)rows;
   p.blocks = (tokens + rows - 1) / rows;
   return p;
@@ -582,7 +585,7 @@ extern "C" int moe_balance_loss(const void* logits, int64_t ld, int dtype, int64
     return ce == cudaSuccess ? 0 : fail((int)ce, "balance_loss: %s", cudaGetErrorString(ce));
   }
   if (!logits || !topk_ids || !workspace) return fail(MOE_E_BADARG, "balance_loss: null pointer");
-  const Plan plan = plan_of(logits, ld, nullptr, dtype, tokens, experts, kSumBlocks);
+  const Plan plan = plan_of(logits, ld, nullptr, dtype, tokens, experts, kSumBlocks, !cu_seqlens);
   Slots slots;
   if (((uintptr_t)workspace & 15) || lay_out(tokens, experts, sequences, plan.blocks, workspace, &slots) > workspace_bytes)
     return fail(MOE_E_BADARG, "balance_loss: workspace too small");
@@ -609,7 +612,7 @@ extern "C" int moe_balance_loss_grad(const void* logits, int64_t ld, int dtype, 
   const int rc = check("balance_loss_grad", tokens, experts, topk, sequences, dtype, ld);
   if (rc || tokens == 0) return rc;
   if (!logits || !saved || !dloss || !dlogits || (!cu_seqlens && sequences != 1)) return fail(MOE_E_BADARG, "balance_loss_grad: bad argument");
-  const Plan plan = plan_of(logits, ld, dlogits, dtype, tokens, experts, kGradBlocks);
+  const Plan plan = plan_of(logits, ld, dlogits, dtype, tokens, experts, kGradBlocks, false);
   const Balance b = {logits, ld, nullptr, cu_seqlens, is_padding, tokens, experts, topk, sequences, 0, sigmoid != 0, plan.rows, plan.lanes};
   cudaStream_t st = (cudaStream_t)stream;
 #define MOE_BG(T, V, CH)                                                                                                               \

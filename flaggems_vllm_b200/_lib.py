@@ -180,7 +180,12 @@ def status_word(device) -> torch.Tensor:
     if key is None:
         key = torch.cuda.current_device()
     if key not in _status:
-        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        # as part of a graph the word would hold anything before the first replay, and every replay would clear what other
+        # calls reported
+        if torch.cuda.is_current_stream_capturing():
+            word = host().word_beside_capture(key)
+        else:
+            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
         host().set_status(key, word.data_ptr())
         _status[key] = word
     return _status[key]

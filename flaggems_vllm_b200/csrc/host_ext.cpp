@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <Python.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -325,6 +326,23 @@ PyObject* set_error(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_INCREF(a[0]);
   g_error = a[0];  // lives as long as the module
   MOE_NONE;
+}
+
+// word_beside_capture(device) -> int32 [1] of zero, complete on return, no part of the graph that the current stream captures:
+// allocated and cleared on another stream, in the mode that lets this thread do so meanwhile.
+PyObject* word_beside_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  long long dev;
+  if (n != 1 || !as_int(a[0], &dev)) MOE_NONE;
+  at::Tensor word;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    const c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)dev);
+    c10::cuda::CUDAStreamGuard guard(side);
+    word = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev));
+    side.synchronize();
+  }
+  return THPVariable_Wrap(word);
 }
 
 // Memory without the dispatcher's way to it, half of an allocation's 1.3 us: an operator of a decode step takes up to four.
@@ -745,7 +763,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 #define MOE_FN(name) {#name, (PyCFunction)(void (*)(void))guarded<name>, METH_FASTCALL, nullptr}
 #define MOE_OP(name) {#name, (PyCFunction)(void (*)(void))raising<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MOE_FN(set_status), MOE_FN(fused_experts), MOE_FN(grouped_topk), MOE_FN(topk_route),
-                         MOE_FN(router_gemm), MOE_FN(align), MOE_FN(set_error), MOE_OP(rms_norm), MOE_OP(fused_add_rms_norm),
+                         MOE_FN(router_gemm), MOE_FN(align), MOE_FN(set_error), MOE_OP(word_beside_capture), MOE_OP(rms_norm), MOE_OP(fused_add_rms_norm),
                          MOE_OP(rms_norm_quant), MOE_OP(balance_loss), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ext", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

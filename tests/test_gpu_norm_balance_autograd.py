@@ -4,6 +4,7 @@ saved tensors may hand back another layout, nothing else."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
+import torch.utils.checkpoint
 
 import flaggems_vllm_b200 as fg
 
@@ -116,3 +117,45 @@ def test_a_stream_of_another_type_is_refused():
         grads = norm_grads()
     with pytest.raises(RuntimeError, match="came back"):
         grads()
+
+
+def test_inference_mode():
+    x, w, r = rows(torch.bfloat16)
+    want = fg.rms_norm(x, w, 1e-6, r)
+    with torch.inference_mode():
+        y, h = fg.rms_norm(x, w.requires_grad_(), 1e-6, r)
+        assert y.is_inference() and torch.equal(y, want[0]) and torch.equal(h, want[1])
+        q = fg.rms_norm_quant(y, w, 1e-6, h)
+        assert torch.equal(q[2], (y.float() + h.float()).bfloat16())
+        bx, br = x.clone(), r.clone()
+        fg.fused_add_rms_norm(bx, br, w)
+        assert torch.equal(bx, y) and torch.equal(br, h)
+        loss, counts = fg.moe_balance_loss(torch.zeros(4, 8, device=DEV), torch.zeros(4, 1, device=DEV, dtype=torch.int32))
+        assert counts[0].item() == 4 and abs(loss.item() - 1.0) <= 64 * 2.0 ** -24
+    w.requires_grad_(False)
+    fg.fused_add_rms_norm(x, r, w)
+    assert torch.equal(x, want[0]) and torch.equal(r, want[1])
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpoint_computes_the_same_again(reentrant):
+    x, w, r = (t.requires_grad_() for t in rows())
+    gate = torch.randn(8, 64, device=DEV, requires_grad=True)
+    ids = torch.randint(0, 8, (6, 2), device=DEV)
+
+    def block(x, w, r, gate):
+        y, h = fg.rms_norm(x, w, 1e-6, r)
+        loss, _ = fg.moe_balance_loss((y.unsqueeze(1) * gate).sum(-1), ids)
+        return y, h, loss
+
+    leaves = (x, w, r, gate)
+
+    def grads(outs):
+        for t in leaves:
+            t.grad = None
+        sum(t.square().sum() for t in outs).backward()
+        return [t.grad.clone() for t in leaves]
+
+    want = grads(block(*leaves))
+    got = grads(torch.utils.checkpoint.checkpoint(block, *leaves, use_reentrant=reentrant))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -11,12 +11,14 @@
 // is left of two nearly equal sums when the experts are nearly even is exact to fp32.  A row whose logits are all -inf has
 // p = 0 and no gradient.
 //
-// Two launches forward, one where a block holds all rows.  Each block of the first takes a run of rows and, for every sequence in it, sums p and counts routes
-// in registers and shared memory; sequence s in block c goes to slot c + s, which no other pair has (a walk along the rows
-// adds one to c or to s at every step).  The second adds the slots in order, so that results are the same bits in every run.
+// Two launches forward, one where a block holds all rows.  Each block of the first takes a run of rows and, for every sequence in
+// it, sums p and counts routes in registers and shared memory; sequence s in block c goes to slot c + s, which no other pair has (a
+// walk along the rows adds one to c or to s at every step).  The second adds the slots in order, so that results are the same bits
+// in every run.
 // Bound: the logits are read once forward and once backward; up to some ten thousand tokens it is the launches and the chain of
-// loads in a block.  us on the device, forward and backward: 64 x 8 fp32 4.0 + 2.8 (one launch forward), 4096 x 128 bf16 9.8 + 4.4,
-// 8192 x 256 fp32 10.6 + 5.6, the same in 23 padded sequences of sigmoid scores 18.7 + 9.5, 65536 x 256 fp32 21 + 27.6 (floor 10 + 20).
+// loads in a block, with many short sequences that chain once for each.  us on the device, logits not in L2, forward and backward:
+// 64 x 8 fp32 3.8 + 2.8 (one launch forward), 4096 x 128 bf16 9.5 + 4.7, 8192 x 256 fp32 10.6 + 6.1, the same in 23 sequences of
+// sigmoid scores 22.7 + 10.0, in 700 94 + 10.9, 65536 x 256 fp32 22.8 + 27.9 (floor 10 + 20).
 #include "moe_common.cuh"
 
 namespace moe {

@@ -12,10 +12,10 @@
 //
 // Bound: memory.  A row is read once: it stays in the registers of the threads that share it, 64 bytes to a thread (32 values of 16
 // bits, 16 of fp32; four or eight where rows are not made of 16-byte pieces) so that four blocks of 256 threads, and their loads,
-// are on a multiprocessor.  us on the device, 8192 x 7168 bf16 with a residual (470 MB: 72 at the rate of a copy): norm 69.5; e4m3
-// in groups of 128 70.4 (411 MB: 63), with the norm itself 82 (528 MB: 81); int8 per row 68; gradient 84, of which 4 for the
-// weight's (470 MB: 72).  16 or 64 values of bf16 to a thread instead: 3 to 6 % slower.  One token of 7168: 2.7, a launch and one
-// round of loads.
+// are on a multiprocessor.  us on the device, 8192 x 7168 bf16 with a residual (470 MB: 72 at the rate of a copy): norm 69.7; e4m3
+// in groups of 128 70.7 (411 MB: 63), e5m2 73.2, with the norm itself 82 (528 MB: 81); int8 per row 68.6; gradient 85, of which 5
+// for the weight's (470 MB: 72).  16 or 64 values of bf16 to a thread instead: 3 to 6 % slower.  One token of 7168: 2.4, a launch
+// and one round of loads.
 #include "moe_common.cuh"
 
 namespace moe {

@@ -408,9 +408,11 @@ __global__ void __launch_bounds__(1024) balance_loss_kernel(const Balance b, con
   }
 }
 
+// saved and dloss may be the work of the kernel in front, which still runs when this one starts: no __restrict__, whose loads the
+// compiler may take for read-only as long as the kernel lives.
 template <typename T, int V, int CH>
-__global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_kernel(const Balance b, const int32_t* __restrict__ saved,
-                                                                const float* __restrict__ dloss, T* __restrict__ dlogits) {
+__global__ void __launch_bounds__(kThreads, V * CH > 16 ? 1 : 2) balance_grad_kernel(const Balance b, const int32_t* saved,
+                                                                const float* dloss, T* dlogits) {
   pdl_wait();
   pdl_trigger();
   constexpr int U = tokens_in_hand(V * CH);

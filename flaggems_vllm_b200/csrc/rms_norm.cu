@@ -608,9 +608,10 @@ __global__ void __launch_bounds__(BLOCK) rms_norm_grad_single_kernel(const Backw
 }
 
 // dw[col] = sum over the blocks' partial sums, in order: 32 columns per block, 32 threads to a column, N parts of each in flight
-// (with 5 a part of every multiprocessor is one round).
+// (with 5 a part of every multiprocessor is one round).  What the kernel in front writes has no __restrict__: this one may have
+// started meanwhile, and loads that the compiler takes for read-only need not stay behind the wait.
 template <typename W, int N>
-__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int parts, int cols, W* __restrict__ dw) {
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* partial, int parts, int cols, W* __restrict__ dw) {
   pdl_wait();
   pdl_trigger();
   __shared__ float sh[32][33];
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(256) rms_norm_grad_any_kernel(const Backward p
   }
 }
 template <typename T>
-__global__ void __launch_bounds__(256) weight_grad_any_kernel(const Backward p, const float* __restrict__ inv_rms) {
+__global__ void __launch_bounds__(256) weight_grad_any_kernel(const Backward p, const float* inv_rms) {
   pdl_wait();
   pdl_trigger();
   const int col = blockIdx.x * 256 + threadIdx.x;

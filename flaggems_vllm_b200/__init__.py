@@ -16,6 +16,7 @@ from .fused_moe import (  # noqa: F401
     inplace_fused_experts,
     outplace_fused_experts,
 )
+from .linear import fused_linear  # noqa: F401
 from .norm import fused_add_rms_norm, rms_norm, rms_norm_quant  # noqa: F401
 from .quant import SUPPORTED_FP8_DTYPE, moe_sum, per_token_group_quant_fp8  # noqa: F401
 from .router_gemm import (  # noqa: F401
@@ -39,4 +40,5 @@ __all__ = [
     "per_token_group_quant_fp8", "SUPPORTED_FP8_DTYPE", "read_status", "MoeKernelError", "topk_softmax",
     "topk_sigmoid", "router_gemm", "fp32_router_gemm", "supports_fp32_router_gemm", "router_gemm_grouped_topk",
     "silu_and_mul", "silu_and_mul_out", "rms_norm", "fused_add_rms_norm", "rms_norm_quant", "moe_balance_loss",
+    "fused_linear",
 ]

@@ -737,6 +737,161 @@ PyObject* balance_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
+struct LinearArgs {
+  int code, bias_code, dev, act;
+  int64_t M, N, W, K, x_ld, w_ld, residual_ld;  // W: rows of the weights, 2 N for the gated activation
+  int32_t* status;
+};
+bool linear_args(const at::Tensor& x, const at::Tensor& w, const at::Tensor* bias, const at::Tensor* residual, int act, LinearArgs* p) {
+  if (!x.is_cuda() || x.dim() < 1 || w.dim() != 2 || act < MOE_LIN_NONE || act > MOE_LIN_SILU_MUL) return false;
+  p->dev = x.get_device();
+  p->act = act;
+  p->code = float_code(x);
+  p->status = status_of(p->dev);
+  p->K = x.size(-1);
+  p->W = w.size(0);
+  p->N = act == MOE_LIN_SILU_MUL ? p->W / 2 : p->W;
+  if (p->code < 0 || !p->status || p->K <= 0 || p->N <= 0 || (act == MOE_LIN_SILU_MUL && p->W % 2 != 0) || w.size(1) != p->K ||
+      !w.is_cuda() || w.get_device() != p->dev || w.scalar_type() != x.scalar_type() || p->K > 0x3FFFFFFF || p->N > 0x1FFFFFFF)
+    return false;
+  int64_t rows;
+  if (!rows_of(x, &p->M, &p->x_ld) || !rows_of(w, &rows, &p->w_ld) || p->M > 0x3FFFFFFF) return false;
+  if (p->M == 1) p->x_ld = p->K;  // a single row has any distance
+  if (p->W == 1) p->w_ld = p->K;
+  if (p->x_ld < p->K || p->w_ld < p->K) return false;
+  p->bias_code = p->code;
+  if (bias) {
+    p->bias_code = float_code(*bias);
+    if (!cuda_dense(*bias, p->dev) || bias->dim() != 1 || bias->size(0) != p->W || (p->bias_code != p->code && p->bias_code != MOE_F32)) return false;
+  }
+  p->residual_ld = p->N;
+  if (residual) {
+    if (!residual->is_cuda() || residual->get_device() != p->dev || residual->scalar_type() != x.scalar_type() || residual->dim() != x.dim() ||
+        residual->size(-1) != p->N || !residual->sizes().slice(0, x.dim() - 1).equals(x.sizes().slice(0, x.dim() - 1)) ||
+        !rows_of(*residual, &rows, &p->residual_ld))
+      return false;
+    if (p->M == 1) p->residual_ld = p->N;
+    if (p->residual_ld < p->N) return false;
+  }
+  return true;
+}
+
+// y, and z where `keep`
+std::pair<at::Tensor, at::Tensor> linear_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor* bias, const at::Tensor* residual,
+                                                 const LinearArgs& p, bool keep) {
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)p.dev);
+  c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = p.N;
+  at::Tensor y = fresh(sizes, x.scalar_type(), p.dev), z, ws;
+  if (keep) z = fresh({p.M, p.W}, x.scalar_type(), p.dev);
+  int64_t bytes = 0;
+  must(moe_fused_linear_workspace(x.const_data_ptr(), p.x_ld, w.const_data_ptr(), p.w_ld, p.code, p.M, p.N, p.K, p.act, &bytes));
+  if (bytes) ws = fresh({bytes}, at::kByte, p.dev);
+  must(moe_fused_linear(x.const_data_ptr(), p.x_ld, w.const_data_ptr(), p.w_ld, bias ? bias->const_data_ptr() : nullptr, p.bias_code,
+                        residual ? residual->const_data_ptr() : nullptr, p.residual_ld, p.code, p.M, p.N, p.K, p.act, y.mutable_data_ptr(), p.N,
+                        keep ? z.mutable_data_ptr() : nullptr, p.W, bytes ? ws.mutable_data_ptr() : nullptr, bytes, p.status, stream_on(p.dev)));
+  return {y, z};
+}
+
+struct FusedLinear : torch::autograd::Function<FusedLinear> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
+                               const std::optional<at::Tensor>& residual, int64_t act) {
+    LinearArgs p;
+    const at::Tensor *b = bias ? &*bias : nullptr, *r = residual ? &*residual : nullptr;
+    if (!linear_args(x, w, b, r, (int)act, &p)) throw KernelError("fused_linear: unsupported operands");
+    const bool want_x = x.requires_grad(), want_w = w.requires_grad(), want_b = b && b->requires_grad();
+    auto [y, z] = linear_forward(x, w, b, r, p, act != MOE_LIN_NONE && (want_x || want_w || want_b));
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["K"] = p.K;
+    ctx->saved_data["W"] = p.W;
+    ctx->saved_data["bias"] = b ? (int64_t)p.bias_code : (int64_t)-1;
+    ctx->saved_data["residual"] = r != nullptr;
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({want_w ? x : at::Tensor(), want_x ? w : at::Tensor(), z});
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t K = ctx->saved_data["K"].toInt(), W = ctx->saved_data["W"].toInt(), act = ctx->saved_data["act"].toInt();
+    const int64_t bias_code = ctx->saved_data["bias"].toInt(), N = act == MOE_LIN_SILU_MUL ? W / 2 : W;
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = bias_code >= 0 && ctx->needs_input_grad(2);
+    if (ctx->saved_data["residual"].toBool()) out[3] = grads[0];  // y = ... + residual
+    if (!want_x && !want_w && !want_b) return once(out, "fused_linear");
+    const at::Tensor dy = grads[0].contiguous();
+    const int dev = dy.get_device(), code = float_code(dy);
+    const int64_t M = dy.numel() / N;
+    at::Tensor x = saved[0], w = saved[1], z = saved[2];
+    int64_t x_ld = K, w_ld = K;
+    // the engine holds dy against y, nobody holds what a hook handed back against what was saved
+    auto held = [&](at::Tensor& t, int64_t rows, int64_t cols, int64_t* ld) {
+      if (!t.defined() || !t.is_cuda() || t.get_device() != dev || t.scalar_type() != dy.scalar_type() || t.dim() < 1 || t.size(-1) != cols ||
+          t.numel() != rows * cols)
+        throw KernelError(std::string("fused_linear") + kChanged);
+      int64_t n;
+      if (!rows_of(t, &n, ld) || (*ld < cols && n > 1)) {
+        t = t.contiguous();
+        *ld = cols;
+      }
+      if (n == 1) *ld = cols;
+    };
+    if (code < 0) throw KernelError(std::string("fused_linear") + kChanged);
+    if (want_w) held(x, M, K, &x_ld);
+    if (want_x) held(w, W, K, &w_ld);
+    int64_t z_ld = W;
+    if (act != MOE_LIN_NONE) held(z, M, W, &z_ld);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;  // the buffers are no part of a graph
+      c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+      const auto bias_type = bias_code == MOE_F32 ? at::kFloat : dy.scalar_type();
+      at::Tensor ws;
+      if (want_x) out[0] = fresh(ctx->saved_data["sizes"].toIntVector(), dy.scalar_type(), dev);
+      if (M == 0) {
+        const auto like = dy.options();
+        if (want_w) out[1] = at::zeros({W, K}, like);
+        if (want_b) out[2] = at::zeros({W}, like.dtype(bias_type));
+        return once(out, "fused_linear");
+      }
+      if (want_w) out[1] = fresh({W, K}, dy.scalar_type(), dev);
+      if (want_b) out[2] = fresh({W}, bias_type, dev);
+      int64_t bytes = 0;
+      must(moe_fused_linear_grad_workspace(want_w ? x.const_data_ptr() : nullptr, x_ld, want_x ? w.const_data_ptr() : nullptr, w_ld, code, M, N, K,
+                                           (int)act, &bytes));
+      ws = fresh({bytes}, at::kByte, dev);
+      must(moe_fused_linear_grad(dy.const_data_ptr(), z.defined() ? z.const_data_ptr() : nullptr, z_ld, want_w ? x.const_data_ptr() : nullptr, x_ld,
+                                 want_x ? w.const_data_ptr() : nullptr, w_ld, code, M, N, K, (int)act, want_x ? out[0].mutable_data_ptr() : nullptr,
+                                 want_w ? out[1].mutable_data_ptr() : nullptr, want_b ? out[2].mutable_data_ptr() : nullptr,
+                                 want_b ? (int)bias_code : code, ws.mutable_data_ptr(), bytes, status_of(dev), stream_on(dev)));
+    }
+    return once(out, "fused_linear");
+  }
+};
+
+// fused_linear(x, weight, bias, activation, residual) -> y; activation: its MOE_LIN_ number
+PyObject* fused_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  long long act;
+  if (n != 5 || !is_tensor(a[0]) || !is_tensor(a[1]) || (a[2] != Py_None && !is_tensor(a[2])) || !as_int(a[3], &act) ||
+      (a[4] != Py_None && !is_tensor(a[4])))
+    MOE_NONE;
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]);
+  const at::Tensor *bias = a[2] == Py_None ? nullptr : &tensor(a[2]), *residual = a[4] == Py_None ? nullptr : &tensor(a[4]);
+  no_tangent({&x, &w, bias, residual}, "fused_linear");
+  LinearArgs p;
+  if (!linear_args(x, w, bias, residual, (int)act, &p)) MOE_NONE;
+  at::Tensor y;
+  {
+    Unlocked unlocked;
+    if (wants_grad({&x, &w, bias, residual}))
+      y = FusedLinear::apply(x, w, bias ? std::optional<at::Tensor>(*bias) : std::nullopt,
+                             residual ? std::optional<at::Tensor>(*residual) : std::nullopt, (int64_t)act)[0];
+    else
+      y = linear_forward(x, w, bias, residual, p, false).first;
+  }
+  return THPVariable_Wrap(y);
+}
+
 // Exceptions of the operators above become Python's: a failed launch MoeKernelError, torch's own as torch raises them.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* raising(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -764,7 +919,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 #define MOE_OP(name) {#name, (PyCFunction)(void (*)(void))raising<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MOE_FN(set_status), MOE_FN(fused_experts), MOE_FN(grouped_topk), MOE_FN(topk_route),
                          MOE_FN(router_gemm), MOE_FN(align), MOE_FN(set_error), MOE_OP(word_beside_capture), MOE_OP(rms_norm), MOE_OP(fused_add_rms_norm),
-                         MOE_OP(rms_norm_quant), MOE_OP(balance_loss), {nullptr, nullptr, 0, nullptr}};
+                         MOE_OP(rms_norm_quant), MOE_OP(balance_loss), MOE_OP(fused_linear), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ext", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

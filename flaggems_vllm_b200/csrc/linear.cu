@@ -1,0 +1,1019 @@
+// Dense products with a fused epilogue, and their gradients:
+//
+//     z = x W^T + b,   y = act(z) + residual          x [M, K], W [N', K], y [M, N]
+//     dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum over rows of dz
+//
+// N' = N, or 2 N for the gated activation silu(z[:, :N]) * z[:, N:].  Sums, bias, activation and residual are fp32, y is rounded
+// once.  z is kept for the backward pass in the operands' type: its rounding reaches the gradients through act' only, and dz has
+// to be rounded to that type anyway, because it is an operand of two products; the bias' gradient sums dz before its rounding.
+//
+// All products are one form, D[r, c] = sum_k A[r, k] B[c, k], in which each operand may lie either way in memory: rows of k
+// ("K-major": x and W forward, dz for dx) or rows of r or c ("MN-major": W for dx, dz and x for dW).  The tensor core takes both
+// from 128-byte swizzled tiles, so nothing is transposed on the way: a box of 64 x 64 elements lands as 8 KB in both cases and
+// only its descriptor differs.  Two kernels:
+//
+//   pair_kernel   256 x 256 (or 256 x 128) tiles by a CTA pair (cta_group::2), persistent, two accumulators, so that a tile's
+//                 epilogue runs under the next tile's products: products that fill the GPU.
+//   tile_kernel   128 x BN tiles, K divided over a cluster whose partial sums are added through distributed shared memory in
+//                 rank order: few rows (the weights are then the 128 side, "swapped", and what counts is how many SMs stream
+//                 them), and products of few tiles.
+//
+// Both are deterministic.  fp32 operands run on f32_kernel (CUDA cores: the tensor core has no fp32 products).
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+#include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace moe {
+namespace {
+using namespace tc;
+
+// What happens to a finished sum.  m: row of y, n: column of y.
+struct Epilogue {
+  const void* bias;      // [N'], in the operands' type or (bias_f32) fp32; null = none
+  const void* residual;  // [M, N], rows residual_ld apart; null = none
+  void* y;               // [M, N]
+  void* z;               // [M, N'], null = not kept
+  int64_t residual_ld, y_ld, z_ld;
+  int64_t M;
+  int N, act, bias_f32;
+};
+
+__device__ __forceinline__ float act_value(int act, float z) {
+  switch (act) {
+    case MOE_LIN_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
+    case MOE_LIN_SILU: return z / (1.0f + expf(-z));
+    case MOE_LIN_GELU: return z * normcdff(z);
+    case MOE_LIN_GELU_TANH: return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z)));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(int act, float z) {
+  switch (act) {
+    case MOE_LIN_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+    case MOE_LIN_SILU: {
+      const float s = 1.0f / (1.0f + expf(-z));
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case MOE_LIN_GELU: return normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z));
+    case MOE_LIN_GELU_TANH: {
+      const float t = tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z));
+      return 0.5f * (1.0f + t) + 0.5f * z * (1.0f - t * t) * (0.7978845608028654f * (1.0f + 0.134145f * z * z));
+    }
+    default: return 1.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float bias_at(const Epilogue& E, int n) {
+  if (E.bias == nullptr) return 0.0f;
+  return E.bias_f32 ? reinterpret_cast<const float*>(E.bias)[n] : ToF32<T>::get(reinterpret_cast<const T*>(E.bias)[n]);
+}
+// the sum(s) of output (m, n) -> y and z; z1: the gate's partner
+template <typename T>
+__device__ __forceinline__ void finish(const Epilogue& E, int64_t m, int n, float z0, float z1) {
+  z0 += bias_at<T>(E, n);
+  float v;
+  if (E.act == MOE_LIN_SILU_MUL) {
+    z1 += bias_at<T>(E, E.N + n);
+    v = silu_mul(z0, z1);
+    if (E.z) {
+      T* z = reinterpret_cast<T*>(E.z) + m * E.z_ld + n;
+      z[0] = from_f32<T>(z0);
+      z[E.N] = from_f32<T>(z1);
+    }
+  } else {
+    v = act_value(E.act, z0);
+    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(z0);
+  }
+  if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
+  reinterpret_cast<T*>(E.y)[m * E.y_ld + n] = from_f32<T>(v);
+}
+
+// ------------------------------------------------------------------ operand tiles
+constexpr int BOX = 64 * 128;  // bytes of a box: 64 rows of 128 bytes, swizzled, either way round
+
+// descriptor of a tile of such boxes: K-major rows follow each other; MN-major boxes are 64 rows (columns of D) each, the
+// eight-k groups of a box 1024 bytes apart
+__device__ __forceinline__ uint64_t box_desc(uint32_t saddr, bool mn) {
+  uint64_t d = make_smem_desc(saddr);
+  if (mn) d = (d & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(BOX >> 4) << 16);
+  return d;
+}
+// what 16 elements of k are in a descriptor's address field
+__device__ __forceinline__ uint64_t k_step(bool mn) { return mn ? 2048 >> 4 : 32 >> 4; }
+
+struct Product {
+  int64_t rows, cols;  // of D
+  int KB;              // steps of 64 k
+  int a_mn, b_mn;
+  int gate;            // distance of the up rows from the gate rows in the weights (N of a gated call), else 0
+  int swapped;         // rows of D are columns of y
+  int split, BN;       // tile_kernel
+  int group;           // pair_kernel: row tiles that walk the column tiles together
+  int32_t* status;
+  unsigned long long wait_ns;
+};
+
+// ------------------------------------------------------------------ tile_kernel
+constexpr int TTHREADS = 256;
+struct TAux {
+  uint64_t full[12], empty[12], done;
+  uint32_t tmem_base;
+};
+constexpr int kTileRing = 196608;
+__host__ __device__ constexpr int tile_stage(int bn) { return (128 + bn) * 128; }
+__host__ __device__ constexpr int tile_stages(int bn) { return kTileRing / tile_stage(bn) < 12 ? kTileRing / tile_stage(bn) : 12; }
+constexpr size_t kTileSmem = (size_t)kTileRing + 1024 + sizeof(TAux);
+static_assert(128 * 257 * 4 <= kTileRing, "the partial tile takes the ring's place");
+
+__device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* a) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]), "=r"(a[9]),
+        "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// One 128 x BN tile of D by the `split` CTAs of a cluster, each over its share of K.  A gated call's tile is half gate rows and
+// half up rows of the weights, whichever side they are on.
+template <typename T>
+__global__ void __launch_bounds__(TTHREADS, 1)
+tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product P, const Epilogue E) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_1024(smem_raw);
+  TAux* aux = reinterpret_cast<TAux*>(smem + kTileRing);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int BN = P.BN, stage = tile_stage(BN), stages = tile_stages(BN);
+  const bool gate_a = P.gate != 0 && P.swapped, gate_b = P.gate != 0 && !P.swapped;
+  const int out_rows = gate_a ? 64 : 128, out_cols = gate_b ? BN / 2 : BN;  // of D that the tile finishes
+  const int64_t r0 = (int64_t)blockIdx.y * out_rows;
+  const int64_t c0 = (int64_t)(blockIdx.x / P.split) * out_cols;
+  const int kb0 = (int)((int64_t)P.KB * rank / P.split), kb1 = (int)((int64_t)P.KB * (rank + 1) / P.split);
+  const uint32_t cols_alloc = BN < 32 ? 32 : BN;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&aux->full[s], 1); mbar_init(&aux->empty[s], 1); }
+    mbar_init(&aux->done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&aux->tmem_base)), "r"(cols_alloc));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = aux->tmem_base;
+  pdl_wait();  // operands, weights among them, may be the kernel's in front
+  pdl_trigger();
+  if (warp == 0) {
+    const bool leader = elect_lane();
+    const int bbox = gate_b ? (BN / 2 < 64 ? BN / 2 : 64) : (BN < 64 ? BN : 64);  // rows of a box of B
+    const int nb = BN / bbox;
+    for (int kb = kb0, s = 0, ph = 1; kb < kb1; ++kb) {
+      if (!mbar_wait(&aux->empty[s], ph, P.status, P.wait_ns)) break;
+      if (leader) {
+        uint8_t* sA = smem + (size_t)s * stage;
+        mbar_expect_tx(&aux->full[s], stage);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = (int)r0 + (gate_a ? j * P.gate : j * 64);
+          tma_load_2d(&map_a, &aux->full[s], sA + j * BOX, P.a_mn ? r : kb * 64, P.a_mn ? kb * 64 : r);
+        }
+        for (int j = 0; j < nb; ++j) {
+          int c = (int)c0 + j * bbox;
+          if (gate_b && j >= nb / 2) c += P.gate - out_cols;
+          tma_load_2d(&map_b, &aux->full[s], sA + 2 * BOX + j * bbox * 128, P.b_mn ? c : kb * 64, P.b_mn ? kb * 64 : c);
+        }
+      }
+      if (++s == stages) { s = 0; ph ^= 1; }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_lane();
+    constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
+                           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    const uint64_t ka = k_step(P.a_mn), kb_ = k_step(P.b_mn);
+    const uint64_t a0 = box_desc(smem_u32(smem), P.a_mn), b0 = box_desc(smem_u32(smem) + 2 * BOX, P.b_mn);
+    bool first = true;
+    for (int kb = kb0, s = 0, ph = 0; kb < kb1; ++kb) {
+      if (!mbar_wait(&aux->full[s], ph, P.status, P.wait_ns)) break;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t ad = a0 + (uint64_t)(s * (stage >> 4)), bd = b0 + (uint64_t)(s * (stage >> 4));
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) tc_mma<MMA_F16>(tmem, ad + k4 * ka, bd + k4 * kb_, idesc, first && k4 == 0 ? 0u : 1u);
+        tc_commit(&aux->empty[s]);
+      }
+      first = false;
+      if (++s == stages) { s = 0; ph ^= 1; }
+    }
+    if (leader) tc_commit(&aux->done);
+  } else if (warp >= 4) {
+    // every product has finished reading the ring: it now holds the partial tile, rows of BN + 1 floats (a pitch without bank
+    // conflicts down a column as well as along the lanes' rows)
+    const bool ok = warp_agrees(mbar_wait(&aux->done, 0, P.status, P.wait_ns));
+    tc_fence_after();
+    const int row = ((warp & 3) << 5) + lane;
+    float* part = reinterpret_cast<float*>(smem) + (size_t)row * (BN + 1);
+    if (ok) {
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 16) {
+        uint32_t r[16];
+        tmem_ld16_sync(tmem + ((uint32_t)((warp & 3) << 5) << 16) + (uint32_t)c, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[c + i] = __uint_as_float(r[i]);
+      }
+    }
+    tc_fence_before();
+  }
+  if (P.split > 1) cluster.sync();
+  else __syncthreads();
+  {
+    // this CTA's share of the outputs, the fast index along the rows of y
+    const int64_t left_r = P.rows - r0, left_c = P.cols - c0;
+    const int nr = (int)(left_r < out_rows ? left_r : out_rows), nc = (int)(left_c < out_cols ? left_c : out_cols);
+    const int fast = P.swapped ? nr : nc, total = nr * nc;
+    const int lo = (int)((int64_t)total * rank / P.split), hi = (int)((int64_t)total * (rank + 1) / P.split);
+    const float* base = reinterpret_cast<const float*>(smem);
+    for (int i = lo + threadIdx.x; i < hi; i += TTHREADS) {
+      const int slow = i / fast, f = i - slow * fast;
+      const int r = P.swapped ? f : slow, c = P.swapped ? slow : f;
+      const int at = r * (BN + 1) + c, up = gate_a ? 64 * (BN + 1) : BN / 2;
+      float z0 = 0.0f, z1 = 0.0f;
+      if (P.split == 1) {
+        z0 = base[at];
+        if (P.gate) z1 = base[at + up];
+      } else {
+#pragma unroll 8
+        for (int j = 0; j < P.split; ++j) {
+          const float* peer = cluster.map_shared_rank(base, j);
+          z0 += peer[at];
+          if (P.gate) z1 += peer[at + up];
+        }
+      }
+      finish<T>(E, P.swapped ? c0 + c : r0 + r, (int)(P.swapped ? r0 + r : c0 + c), z0, z1);
+    }
+  }
+  tc_fence_before();
+  if (P.split > 1) cluster.sync();  // no CTA leaves while its partial tile may still be read
+  else __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols_alloc));
+  }
+}
+
+// ------------------------------------------------------------------ pair_kernel
+constexpr int PTHREADS = 384, PCONS = 256;
+constexpr int kPairRing = 196608;
+struct PAux {
+  uint64_t full[8], empty[8], tmem_full[2], tmem_empty[2];
+  uint32_t tmem_base;
+};
+constexpr size_t kPairSmem = (size_t)kPairRing + 1024 + sizeof(PAux);
+
+// Tile order: `group` row tiles share a walk over the column tiles, so that the pairs that run at one time read few different
+// operand tiles.
+__device__ __forceinline__ void tile_at(int item, int RT, int CT, int group, int& rt, int& ct) {
+  const int per = group * CT, g = item / per, first = g * group;
+  const int size = RT - first < group ? RT - first : group;
+  const int in = item - g * per;
+  rt = first + in % size;
+  ct = in / size;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_row32(const T* p, bool wide, int n, float (&v)[32]) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float t[8];
+      load8<T>(p + 8 * i, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[8 * i + j] = t[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = i < n ? ToF32<T>::get(p[i]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_row32(T* p, bool wide, bool wide32, int n, const float (&v)[32]) {
+  if (wide) {
+    uint4 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]), pack2<T>(v[8 * i + 4], v[8 * i + 5]),
+                        pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+    store_row_pieces<4>(p, q, wide32);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) p[i] = from_f32<T>(v[i]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PTHREADS, 1)
+pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product P, const Epilogue E) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_1024(smem_raw);
+  PAux* aux = reinterpret_cast<PAux*>(smem + kPairRing);
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int cr = (int)cluster_ctarank();  // 0 leads
+  const int BN = P.BN, stage = 2 * BOX + (BN / 128) * BOX, stages = BN == 256 ? 6 : 8;
+  const int out_cols = P.gate ? BN / 2 : BN;
+  const int RT = (int)((P.rows + 255) / 256), CT = (int)((P.cols + out_cols - 1) / out_cols);
+  const int total = RT * CT, item0 = blockIdx.x / 2, step = gridDim.x / 2;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&aux->full[s], 1); mbar_init(&aux->empty[s], 1); }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&aux->tmem_full[a], 1);
+      mbar_init(&aux->tmem_empty[a], 2 * (PCONS / 32));  // the warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&aux->tmem_base)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before anyone signals across
+  tc_fence_after();
+  const uint32_t tmem_base = aux->tmem_base;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    const bool leader = elect_lane();
+    if (leader) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
+    uint32_t s = 0, ph = 1;
+    bool alive = true;
+    for (int item = item0; item < total && alive; item += step) {
+      int rt, ct;
+      tile_at(item, RT, CT, P.group, rt, ct);
+      const int r = rt * 256 + cr * 128;
+      // the pair's columns, half from each CTA: gate and up of a gated call
+      const int c = P.gate ? ct * out_cols + cr * P.gate : ct * BN + cr * (BN / 2);
+      for (int kb = 0; kb < P.KB; ++kb) {
+        if (!mbar_wait(&aux->empty[s], ph, P.status, P.wait_ns)) { alive = false; break; }
+        if (leader) {
+          if (cr == 0) mbar_expect_tx(&aux->full[s], 2 * stage);  // the peer's bytes may already have been counted
+          uint8_t* sA = smem + (size_t)s * stage;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            tma_load_2d_pair(&map_a, &aux->full[s], sA + j * BOX, P.a_mn ? r + 64 * j : kb * 64, P.a_mn ? kb * 64 : r + 64 * j);
+          for (int j = 0; j < BN / 128; ++j)
+            tma_load_2d_pair(&map_b, &aux->full[s], sA + (2 + j) * BOX, P.b_mn ? c + 64 * j : kb * 64, P.b_mn ? kb * 64 : c + 64 * j);
+        }
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1 && cr == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const bool leader = elect_lane();
+    constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
+                           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+    const uint64_t ka = k_step(P.a_mn), kb_ = k_step(P.b_mn);
+    const uint64_t a0 = box_desc(smem_u32(smem), P.a_mn), b0 = box_desc(smem_u32(smem) + 2 * BOX, P.b_mn);
+    uint64_t ad = a0, bd = b0;
+    uint32_t s = 0, ph = 0, acc_it = 0;
+    bool alive = true;
+    for (int item = item0; item < total && alive; item += step) {
+      const uint32_t a = acc_it & 1, d = tmem_base + a * 256;
+      if (!mbar_wait(&aux->tmem_empty[a], ((acc_it >> 1) & 1) ^ 1, P.status, P.wait_ns)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int kb = 0; kb < P.KB; ++kb) {
+        if (!mbar_wait(&aux->full[s], ph, P.status, P.wait_ns)) { alive = false; break; }
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) tc_mma_pair<MMA_F16>(d, ad + k4 * ka, bd + k4 * kb_, idesc, kb > 0 || k4 > 0 ? 1u : 0u);
+          tc_commit_pair(&aux->empty[s]);
+        }
+        ad += (uint64_t)(stage >> 4);
+        bd += (uint64_t)(stage >> 4);
+        if (++s == (uint32_t)stages) { s = 0; ad = a0; bd = b0; ph ^= 1; }
+      }
+      if (leader && alive) tc_commit_pair(&aux->tmem_full[a]);
+      ++acc_it;
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue: a thread has 32 columns of one row at a time
+    const int h = (warp - 4) >> 2, wq = warp & 3;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(wq << 5) << 16);
+    uint32_t acc_it = 0;
+    const T* res = reinterpret_cast<const T*>(E.residual);
+    T *y = reinterpret_cast<T*>(E.y), *z = reinterpret_cast<T*>(E.z);
+    const bool y16 = ((uintptr_t)y & 15) == 0 && E.y_ld % 8 == 0, y32 = ((uintptr_t)y & 31) == 0 && E.y_ld % 16 == 0;
+    const bool r16 = ((uintptr_t)res & 15) == 0 && E.residual_ld % 8 == 0;
+    const bool z16 = ((uintptr_t)z & 15) == 0 && E.z_ld % 8 == 0 && E.N % 8 == 0;
+    const bool z32 = z16 && ((uintptr_t)z & 31) == 0 && E.z_ld % 16 == 0 && E.N % 16 == 0;
+    for (int item = item0; item < total; item += step) {
+      const uint32_t a = acc_it & 1;
+      if (!warp_agrees(mbar_wait_idle(&aux->tmem_full[a], (acc_it >> 1) & 1, P.status, P.wait_ns))) break;
+      tc_fence_after();
+      int rt, ct;
+      tile_at(item, RT, CT, P.group, rt, ct);
+      const int64_t m = (int64_t)rt * 256 + cr * 128 + wq * 32 + lane;
+      const bool live = m < P.rows;
+      const int span = out_cols / 2;  // columns of this warp
+#pragma unroll 1
+      for (int q = 0; q < span; q += 32) {
+        const int in = h * span + q, n0 = ct * out_cols + in;
+        uint32_t r0[32], r1[32];
+        tmem_ld32_async(t_lane + a * 256 + (uint32_t)in, r0);
+        if (P.gate) tmem_ld32_async(t_lane + a * 256 + (uint32_t)(BN / 2 + in), r1);
+        tmem_wait32(r0);
+        if (P.gate) tmem_wait32(r1);
+        const int n = (int)(P.cols - n0 < 32 ? P.cols - n0 : 32);
+        if (live && n > 0) {
+          float v[32];
+  #pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r0[i]);
+          if (E.bias) {
+  #pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += i < n ? bias_at<T>(E, n0 + i) : 0.0f;
+          }
+          const bool whole = n == 32;
+          if (P.gate) {
+            float u[32];
+  #pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(r1[i]);
+            if (E.bias) {
+  #pragma unroll
+              for (int i = 0; i < 32; ++i) u[i] += i < n ? bias_at<T>(E, E.N + n0 + i) : 0.0f;
+            }
+            if (z) {
+              store_row32<T>(z + m * E.z_ld + n0, whole && z16, z32, n, v);
+              store_row32<T>(z + m * E.z_ld + E.N + n0, whole && z16, z32, n, u);
+            }
+  #pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = silu_mul_fast(v[i], u[i]);
+          } else {
+            if (z) store_row32<T>(z + m * E.z_ld + n0, whole && z16, z32, n, v);
+            switch (E.act) {  // one loop each: the choice is the call's
+              case MOE_LIN_NONE: break;
+              case MOE_LIN_RELU:
+  #pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = act_value(MOE_LIN_RELU, v[i]);
+                break;
+              case MOE_LIN_SILU:
+  #pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = silu_mul_fast(v[i], 1.0f);
+                break;
+              case MOE_LIN_GELU:
+  #pragma unroll 4
+                for (int i = 0; i < 32; ++i) v[i] = act_value(MOE_LIN_GELU, v[i]);
+                break;
+              default:
+  #pragma unroll 4
+                for (int i = 0; i < 32; ++i) v[i] = act_value(MOE_LIN_GELU_TANH, v[i]);
+            }
+          }
+          if (res) {
+            float t[32];
+            load_row32<T>(res + m * E.residual_ld + n0, whole && r16, n, t);
+  #pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += t[i];
+          }
+          store_row32<T>(y + m * E.y_ld + n0, whole && y16, y32, n, v);
+        }
+        __syncwarp();  // the next columns are loaded by the warp as one
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (cr == 1) mbar_arrive_remote(&aux->tmem_empty[a], 0);
+        else mbar_arrive(&aux->tmem_empty[a]);
+      }
+      ++acc_it;
+    }
+  }
+  // -------------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while its partner may still signal its barriers
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
+  }
+}
+
+// ------------------------------------------------------------------ fp32 operands
+// 64 x 64 tiles of D by 256 threads, 4 x 4 outputs each, 16 k at a time through shared memory; either operand either way round.
+struct F32Operand {
+  const float* p;
+  int64_t rs, ks;  // strides of the row (r or c) and of k
+};
+__global__ void __launch_bounds__(256) f32_kernel(F32Operand A, F32Operand B, int64_t rows, int64_t cols, int64_t K, int64_t gate, Epilogue E) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sa[2][16][68], sb[2][16][68];
+  const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
+  const int out_cols = gate ? 32 : 64;
+  const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * out_cols;
+  float acc[4][4] = {};
+  // a thread's four elements of a 64 x 16 tile: neighbouring threads along the contiguous side
+  auto fetch = [&](const F32Operand& X, int64_t base, int64_t end, bool gated, int64_t k0, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = X.ks == 1 ? (t >> 4) + 16 * i : (t & 63), k = X.ks == 1 ? (t & 15) : (t >> 6) + 4 * i;
+      int64_t row = base + r;
+      bool in = row < end;
+      if (gated) {  // first half gate rows, second half up rows
+        row = base + (r & 31);
+        in = row < end;
+        row += r < 32 ? 0 : gate;
+      }
+      v[i] = in && k0 + k < K ? __ldg(X.p + row * X.rs + (k0 + k) * X.ks) : 0.0f;
+    }
+  };
+  auto put = [&](const F32Operand& X, float (*s)[68], const float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = X.ks == 1 ? (t >> 4) + 16 * i : (t & 63), k = X.ks == 1 ? (t & 15) : (t >> 6) + 4 * i;
+      s[k][r] = v[i];
+    }
+  };
+  float va[4], vb[4];
+  fetch(A, r0, rows, false, 0, va);
+  fetch(B, c0, cols, gate != 0, 0, vb);
+  put(A, sa[0], va);
+  put(B, sb[0], vb);
+  __syncthreads();
+  int cur = 0;
+  for (int64_t k0 = 0; k0 < K; k0 += 16) {
+    const bool more = k0 + 16 < K;
+    if (more) {
+      fetch(A, r0, rows, false, k0 + 16, va);
+      fetch(B, c0, cols, gate != 0, k0 + 16, vb);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float4 a = *reinterpret_cast<const float4*>(&sa[cur][k][4 * ty]);
+      float b[4];
+      if (gate) {  // a thread's columns: two gates and their ups
+        b[0] = sb[cur][k][2 * tx]; b[1] = sb[cur][k][2 * tx + 1];
+        b[2] = sb[cur][k][32 + 2 * tx]; b[3] = sb[cur][k][32 + 2 * tx + 1];
+      } else {
+        const float4 q = *reinterpret_cast<const float4*>(&sb[cur][k][4 * tx]);
+        b[0] = q.x; b[1] = q.y; b[2] = q.z; b[3] = q.w;
+      }
+      const float ar[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ar[i], b[j], acc[i][j]);
+    }
+    if (more) {
+      put(A, sa[cur ^ 1], va);
+      put(B, sb[cur ^ 1], vb);
+    }
+    __syncthreads();
+    cur ^= 1;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = r0 + 4 * ty + i;
+    if (m >= rows) continue;
+    if (gate) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (c0 + 2 * tx + j < cols) finish<float>(E, m, (int)(c0 + 2 * tx + j), acc[i][j], acc[i][2 + j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c0 + 4 * tx + j < cols) finish<float>(E, m, (int)(c0 + 4 * tx + j), acc[i][j], 0.0f);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gradient of the activation, and of the bias
+// dz = dy act'(z) element by element, and per block the sums over its rows of dz in fp32, before its rounding.  A warp takes 32 V
+// neighbouring columns, the block's eight warps every eighth row.  HBM-bound.
+struct ActGrad {
+  const void *dy, *z;
+  void* dz;     // null: only sums are wanted
+  float* part;  // [blocks of rows, N'], null: no bias
+  int64_t M, dy_ld, z_ld, dz_ld, rows_per_block;
+  int N, act;
+};
+template <typename T, int V>
+__global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad P) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = (blockIdx.x * 32 + lane) * V;
+  const int64_t m0 = (int64_t)blockIdx.y * P.rows_per_block;
+  const int64_t m1 = m0 + P.rows_per_block < P.M ? m0 + P.rows_per_block : P.M;
+  const bool gated = P.act == MOE_LIN_SILU_MUL, in = n < P.N;
+  float s0[V] = {}, s1[V] = {};
+  auto load = [](const void* base, int64_t at, float (&v)[V]) {
+    const T* p = reinterpret_cast<const T*>(base) + at;
+    if constexpr (V == 8) load8<T>(p, v);
+    else v[0] = ToF32<T>::get(*p);
+  };
+  auto store = [](void* base, int64_t at, const float (&v)[V]) {
+    T* p = reinterpret_cast<T*>(base) + at;
+    if constexpr (V == 8 && sizeof(T) == 2)
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    else
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] = from_f32<T>(v[i]);
+  };
+  if (in) {
+#pragma unroll 2
+    for (int64_t m = m0 + warp; m < m1; m += 8) {
+      float dy[V], z[V];
+      load(P.dy, m * P.dy_ld + n, dy);
+      if (gated) {
+        float u[V], du[V];
+        load(P.z, m * P.z_ld + n, z);
+        load(P.z, m * P.z_ld + P.N + n, u);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float s = 1.0f / (1.0f + expf(-z[i])), d = dy[i];
+          du[i] = d * (z[i] * s);
+          dy[i] = d * u[i] * (s * (1.0f + z[i] * (1.0f - s)));
+          s0[i] += dy[i];
+          s1[i] += du[i];
+        }
+        if (P.dz) {
+          store(P.dz, m * P.dz_ld + n, dy);
+          store(P.dz, m * P.dz_ld + P.N + n, du);
+        }
+      } else {
+        if (P.act != MOE_LIN_NONE) {
+          load(P.z, m * P.z_ld + n, z);
+#pragma unroll
+          for (int i = 0; i < V; ++i) dy[i] *= act_slope(P.act, z[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s0[i] += dy[i];
+        if (P.dz) store(P.dz, m * P.dz_ld + n, dy);
+      }
+    }
+  }
+  if (P.part == nullptr) return;
+  __shared__ float sum[8][32 * V];
+  float* out = P.part + (int64_t)blockIdx.y * (gated ? 2 * P.N : P.N);
+  for (int half = 0; half <= (gated ? 1 : 0); ++half) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[warp][lane * V + i] = half ? s1[i] : s0[i];
+    __syncthreads();
+    const int c = blockIdx.x * 32 * V + threadIdx.x;
+    if (threadIdx.x < 32 * V && c < P.N) {
+      float v = sum[0][threadIdx.x];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) v += sum[w][threadIdx.x];
+      out[half * P.N + c] = v;
+    }
+  }
+}
+// the blocks' sums in order: a warp per 32 columns would read them one behind another, so eight warps take every eighth block
+template <typename BT>
+__global__ void __launch_bounds__(256) bias_grad_kernel(const float* part, int64_t blocks, int64_t cols, BT* db) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sum[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float v = 0.0f;
+  if (c < cols) {
+#pragma unroll 4
+    for (int64_t b = warp; b < blocks; b += 8) v += part[b * cols + c];
+  }
+  sum[warp][lane] = v;
+  __syncthreads();
+  if (warp == 0 && c < cols) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) v += sum[w][lane];
+    db[c] = from_f32<BT>(v);
+  }
+}
+
+// rows of 16-bit elements that TMA cannot read (a pitch that is no multiple of 16 bytes, an odd address) -> rows that it can
+__global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t src_ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t dst_ld) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + warp; r < rows; r += (int64_t)gridDim.x * 8) {
+    const uint16_t* s = src + r * src_ld;
+    uint16_t* d = dst + r * dst_ld;
+#pragma unroll 8
+    for (int64_t c = lane; c < cols; c += 32) d[c] = s[c];
+  }
+}
+
+// ------------------------------------------------------------------ host side
+struct Matrix {  // row-major in memory: `rows` rows of `cols`, `ld` apart
+  const void* p;
+  int64_t rows, cols, ld;
+};
+bool tma_reads(const Matrix& m) { return ((uintptr_t)m.p & 15) == 0 && m.ld % 8 == 0; }
+int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
+int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
+
+// a workspace handed out front to back
+struct Space {
+  uint8_t* at;
+  int64_t left;
+  void* take(int64_t bytes) {
+    bytes = up256(bytes);
+    if (bytes > left) return nullptr;
+    void* p = at;
+    at += bytes;
+    left -= bytes;
+    return p;
+  }
+};
+int readable(Matrix& m, Space& ws, cudaStream_t st) {
+  if (tma_reads(m)) return 0;
+  const int64_t ld = padded(m.cols);
+  void* p = ws.take(m.rows * ld * 2);
+  if (!p) return fail(MOE_E_BADARG, "fused_linear: workspace too small");
+  const int64_t blocks = (m.rows + 7) / 8;
+  const int rc = launch_pdl(pitch_kernel, dim3((unsigned)(blocks < 8 * sm_count() ? blocks : 8 * sm_count())), 256, 0, 1, st,
+                            "fused_linear (pitch)", (const uint16_t*)m.p, m.ld, m.rows, m.cols, (uint16_t*)p, ld);
+  m.p = p;
+  m.ld = ld;
+  return rc;
+}
+
+// Which kernel, tile and split of K.  Costs in clocks of an SM that moves operands at 64 bytes per clock out of L2 and multiplies
+// 128 x BN x 64 in 2 BN; a whole product also moves its bytes through HBM once.
+struct Plan {
+  bool pair, swapped;
+  int BN, split;
+};
+Plan choose(int64_t rows, int64_t cols, int64_t K, bool gated, bool a_mn, bool b_mn, int sms) {
+  Plan best = {false, false, 64, 1};
+  double cost = 1e300;
+  const int64_t kb = (K + 63) / 64;
+  auto consider = [&](Plan p, double c) {
+    if (c < cost) { cost = c; best = p; }
+  };
+  for (int swapped = 0; swapped <= 1; ++swapped) {  // D as it is, or transposed: its columns on the 128 side
+    const int64_t r = swapped ? cols : rows, c = swapped ? rows : (gated ? 2 * cols : cols);
+    const int rt = gated && swapped ? 64 : 128, least = swapped && !a_mn ? 16 : 64;  // a box of MN-major rows is 64 of them
+    if ((r + rt - 1) / rt > 65535) continue;
+    for (int bn = least; bn <= 256 && (bn == least || bn / 2 < c); bn *= 2) {
+      const int64_t tiles = (r + rt - 1) / rt * ((c + bn - 1) / bn);
+      for (int s = 1; s <= 8 && s <= kb; s *= 2) {
+        const double reach = (s == 8 ? 112.0 : (s == 4 ? 132.0 : 148.0)) * sms / 148.0;
+        const double waves = (double)(int64_t)((double)(tiles * s) / reach + 0.9999);
+        const double step = (128 + bn) * 2.0;  // never below the products' 2 bn
+        consider({false, swapped != 0, bn, s}, waves * (((kb + s - 1) / s) * step + 24.0 * bn + 1500.0) + 2500.0 + (s > 1 ? 1500.0 + 8.0 * bn : 0.0));
+      }
+    }
+  }
+  for (int bn = 128; bn <= 256; bn *= 2) {
+    const int ct = gated ? bn / 2 : bn;
+    const int64_t tiles = (rows + 255) / 256 * ((cols + ct - 1) / ct);
+    const double waves = (double)((tiles + sms / 2 - 1) / (sms / 2));
+    consider({true, false, bn, 1}, waves * kb * (bn == 256 ? 512.0 : 300.0) + 4000.0 + 12.0 * bn);
+  }
+  return best;
+}
+
+template <typename T>
+int run_product(Matrix a, Matrix b, bool a_mn, bool b_mn, int64_t rows, int64_t cols, int64_t K, bool gated, const Epilogue& E,
+                int32_t* status, cudaStream_t st) {
+  // a, b: the operands of D [rows, cols]; a_mn: a is [K, rows] in memory.  gated: b has 2 cols rows
+  Plan p = choose(rows, cols, K, gated, a_mn, b_mn, sm_count());
+  const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  Product P = {};
+  P.KB = (int)((K + 63) / 64);
+  P.gate = gated ? (int)cols : 0;
+  P.status = status;
+  P.wait_ns = wait_limit_ns();
+  P.BN = p.BN;
+  P.split = p.split;
+  P.swapped = p.swapped;
+  P.rows = p.swapped ? cols : rows;
+  P.cols = p.swapped ? rows : cols;
+  if (p.swapped) { Matrix t = a; a = b; b = t; const bool q = a_mn; a_mn = b_mn; b_mn = q; }
+  P.a_mn = a_mn;
+  P.b_mn = b_mn;
+  int bbox = 64;
+  if (!p.pair) bbox = gated && !p.swapped ? (p.BN / 2 < 64 ? p.BN / 2 : 64) : (p.BN < 64 ? p.BN : 64);
+  CUtensorMap ma, mb;
+  int rc = make_map(&ma, a.p, dt, 2, (uint64_t)a.rows, (uint64_t)a.cols, 64, p.swapped, 128, (uint64_t)a.ld);
+  if (rc) return rc;
+  rc = make_map(&mb, b.p, dt, 2, (uint64_t)b.rows, (uint64_t)b.cols, b_mn ? 64 : bbox, !p.swapped, 128, (uint64_t)b.ld);
+  if (rc) return rc;
+  if (p.pair) {
+    auto kern = pair_kernel<T>;
+    rc = allow_smem((const void*)kern, (int)kPairSmem);
+    if (rc) return rc;
+    const int ct = gated ? p.BN / 2 : p.BN;
+    const int64_t RT = (rows + 255) / 256, CT = (cols + ct - 1) / ct, tiles = RT * CT;
+    if (tiles >= (1ll << 31)) return fail(MOE_E_TOOBIG, "fused_linear: too many tiles");
+    P.group = 8;
+    const int pairs = sm_count() / 2;
+    return launch_pdl(kern, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), PTHREADS, kPairSmem, 2, st, "fused_linear (pair)", ma, mb, P, E);
+  }
+  auto kern = tile_kernel<T>;
+  rc = allow_smem((const void*)kern, (int)kTileSmem);
+  if (rc) return rc;
+  while (P.split > 1 && max_clusters((const void*)kern, P.split, TTHREADS, kTileSmem) == 0) P.split /= 2;
+  const int rt = gated && p.swapped ? 64 : 128, ct = gated && !p.swapped ? p.BN / 2 : p.BN;
+  const dim3 grid((unsigned)((P.cols + ct - 1) / ct * P.split), (unsigned)((P.rows + rt - 1) / rt));
+  return launch_pdl(kern, grid, TTHREADS, kTileSmem, P.split, st, "fused_linear (tile)", ma, mb, P, E);
+}
+
+int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, bool gated, const Epilogue& E, cudaStream_t st) {
+  const int64_t gx = gated ? (cols + 31) / 32 : (cols + 63) / 64, gy = (rows + 63) / 64;
+  if (gy > 65535) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d rows", 65535 * 64);
+  return launch_pdl(f32_kernel, dim3((unsigned)gx, (unsigned)gy), 256, 0, 1, st, "fused_linear (fp32)", a, b, rows, cols, K,
+                    (int64_t)(gated ? cols : 0), E);
+}
+
+int check_sizes(int64_t M, int64_t N, int64_t K, int dtype, int act) {
+  if (dtype != MOE_BF16 && dtype != MOE_F16 && dtype != MOE_F32) return fail(MOE_E_DTYPE, "fused_linear: unsupported dtype %d", dtype);
+  if (act < MOE_LIN_NONE || act > MOE_LIN_SILU_MUL) return fail(MOE_E_BADARG, "fused_linear: activation %d", act);
+  if (M < 0 || N <= 0 || K <= 0) return fail(MOE_E_BADARG, "fused_linear: bad extent");
+  if (M > 0x3FFFFFFF || N > 0x1FFFFFFF || K > 0x3FFFFFFF) return fail(MOE_E_TOOBIG, "fused_linear: extent beyond 2^29 columns or 2^30 rows");
+  return 0;
+}
+int64_t width(int64_t N, int act) { return act == MOE_LIN_SILU_MUL ? 2 * N : N; }
+// blocks of rows of act_grad_kernel: as many as fill the GPU, at least 32 rows each
+int64_t grad_rows(int64_t M, int64_t N, int V, int sms) {
+  const int64_t cb = (N + 32 * V - 1) / (32 * V);
+  int64_t blocks = (8 * (int64_t)sms + cb - 1) / cb;
+  if (blocks > 512) blocks = 512;
+  int64_t rows = (M + blocks - 1) / blocks;
+  if (rows < 32) rows = 32;
+  return (rows + 7) / 8 * 8;
+}
+template <typename T>
+int run_act_grad(ActGrad G, int V, cudaStream_t st) {
+  const dim3 grid((unsigned)((G.N + 32 * V - 1) / (32 * V)), (unsigned)((G.M + G.rows_per_block - 1) / G.rows_per_block));
+  if (V == 8) return launch_pdl(act_grad_kernel<T, 8>, grid, 256, 0, 1, st, "fused_linear (activation's gradient)", G);
+  return launch_pdl(act_grad_kernel<T, 1>, grid, 256, 0, 1, st, "fused_linear (activation's gradient)", G);
+}
+template <typename BT>
+int run_bias_grad(const float* part, int64_t blocks, int64_t cols, void* db, cudaStream_t st) {
+  return launch_pdl(bias_grad_kernel<BT>, dim3((unsigned)((cols + 31) / 32)), 256, 0, 1, st, "fused_linear (bias' gradient)", part, blocks, cols, (BT*)db);
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_fused_linear_workspace(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M, int64_t N,
+                                          int64_t K, int act, int64_t* bytes) {
+  using namespace moe;
+  if (const int rc = check_sizes(M, N, K, dtype, act)) return rc;
+  if (!bytes) return fail(MOE_E_BADARG, "fused_linear_workspace: null pointer");
+  *bytes = 0;
+  if (dtype == MOE_F32) return 0;
+  if (!tma_reads({x, M, K, x_ld})) *bytes += up256(M * padded(K) * 2);
+  if (!tma_reads({w, width(N, act), K, w_ld})) *bytes += up256(width(N, act) * padded(K) * 2);
+  return 0;
+}
+
+extern "C" int moe_fused_linear(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype,
+                                const void* residual, int64_t residual_ld, int dtype, int64_t M, int64_t N, int64_t K, int act, void* y,
+                                int64_t y_ld, void* z, int64_t z_ld, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                void* stream) {
+  using namespace moe;
+  if (const int rc = check_sizes(M, N, K, dtype, act)) return rc;
+  if (M == 0) return 0;
+  if (!x || !w || !y) return fail(MOE_E_BADARG, "fused_linear: null pointer");
+  if (bias && bias_dtype != dtype && bias_dtype != MOE_F32) return fail(MOE_E_DTYPE, "fused_linear: the bias has the operands' type or fp32");
+  const int64_t W = width(N, act);
+  if (x_ld < K || w_ld < K || y_ld < N || (residual && residual_ld < N) || (z && z_ld < W)) return fail(MOE_E_SHAPE, "fused_linear: rows overlap");
+  cudaStream_t st = (cudaStream_t)stream;
+  Epilogue E = {bias, residual, y, z, residual_ld, y_ld, z_ld, M, (int)N, act, bias_dtype == MOE_F32};
+  const bool gated = act == MOE_LIN_SILU_MUL;
+  if (dtype == MOE_F32) return run_f32({(const float*)x, x_ld, 1}, {(const float*)w, w_ld, 1}, M, N, K, gated, E, st);
+  Space ws = {(uint8_t*)workspace, workspace ? workspace_bytes : 0};
+  Matrix a = {x, M, K, x_ld}, b = {w, W, K, w_ld};
+  if (int rc = readable(a, ws, st)) return rc;
+  if (int rc = readable(b, ws, st)) return rc;
+  return dtype == MOE_BF16 ? run_product<__nv_bfloat16>(a, b, false, false, M, N, K, gated, E, status, st)
+                           : run_product<__half>(a, b, false, false, M, N, K, gated, E, status, st);
+}
+
+namespace moe {
+namespace {
+// the parts of the backward pass' workspace: dz (or dy where TMA cannot read it), x and w likewise, the bias' partial sums
+struct GradPlan {
+  bool need_dz;
+  int V;
+  int64_t rows_per_block, blocks;
+};
+GradPlan grad_plan(const void* dy, const void* z, int64_t z_ld, const void* dz, int dtype, int64_t M, int64_t N, int act, bool products) {
+  GradPlan p;
+  const int64_t W = width(N, act);
+  p.need_dz = products && act != MOE_LIN_NONE;
+  const int eb = dtype == MOE_F32 ? 4 : 2;
+  auto wide = [&](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && ld * eb % 16 == 0; };
+  p.V = N % 8 == 0 && wide(dy, N) && (act == MOE_LIN_NONE || wide(z, z_ld)) && wide(dz, W) ? 8 : 1;
+  p.rows_per_block = grad_rows(M, N, p.V, sm_count());
+  p.blocks = (M + p.rows_per_block - 1) / p.rows_per_block;
+  return p;
+}
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_fused_linear_grad_workspace(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M, int64_t N,
+                                               int64_t K, int act, int64_t* bytes) {
+  using namespace moe;
+  if (const int rc = check_sizes(M, N, K, dtype, act)) return rc;
+  if (!bytes) return fail(MOE_E_BADARG, "fused_linear_grad_workspace: null pointer");
+  const int64_t W = width(N, act);
+  const int eb = dtype == MOE_F32 ? 4 : 2;
+  *bytes = up256(M * padded(W) * eb);  // dz, or dy with another pitch
+  *bytes += up256(((M + 31) / 32 < 512 ? (M + 31) / 32 : 512) * W * 4);
+  if (dtype != MOE_F32) {
+    if (!tma_reads({x, M, K, x_ld})) *bytes += up256(M * padded(K) * 2);
+    if (!tma_reads({w, W, K, w_ld})) *bytes += up256(W * padded(K) * 2);
+  }
+  return 0;
+}
+
+extern "C" int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld, const void* x, int64_t x_ld, const void* w, int64_t w_ld,
+                                     int dtype, int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* db, int db_dtype,
+                                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  using namespace moe;
+  if (const int rc = check_sizes(M, N, K, dtype, act)) return rc;
+  if (M == 0) return fail(MOE_E_BADARG, "fused_linear_grad: no rows");
+  const int64_t W = width(N, act);
+  if (!dy || (act != MOE_LIN_NONE && !z) || (dx && !w) || (dw && !x)) return fail(MOE_E_BADARG, "fused_linear_grad: null pointer");
+  if (db && db_dtype != dtype && db_dtype != MOE_F32) return fail(MOE_E_DTYPE, "fused_linear_grad: the bias has the operands' type or fp32");
+  if ((x && x_ld < K) || (w && w_ld < K) || (z && z_ld < W)) return fail(MOE_E_SHAPE, "fused_linear_grad: rows overlap");
+  cudaStream_t st = (cudaStream_t)stream;
+  Space ws = {(uint8_t*)workspace, workspace ? workspace_bytes : 0};
+  const int eb = dtype == MOE_F32 ? 4 : 2;
+  const bool products = dx || dw;
+  const int64_t dz_ld = act == MOE_LIN_NONE ? N : padded(W);
+  void* own = products && act != MOE_LIN_NONE ? ws.take(M * dz_ld * eb) : nullptr;
+  if (products && act != MOE_LIN_NONE && !own) return fail(MOE_E_BADARG, "fused_linear_grad: workspace too small");
+  GradPlan g = grad_plan(dy, z, z_ld, own, dtype, M, N, act, products);
+  if (own || db) {
+    ActGrad G = {dy, z, own, nullptr, M, N, z_ld, dz_ld, g.rows_per_block, (int)N, act};
+    if (db) {
+      G.part = (float*)ws.take(g.blocks * W * 4);
+      if (!G.part) return fail(MOE_E_BADARG, "fused_linear_grad: workspace too small");
+    }
+    int rc = dtype == MOE_BF16 ? run_act_grad<__nv_bfloat16>(G, g.V, st) : dtype == MOE_F16 ? run_act_grad<__half>(G, g.V, st) : run_act_grad<float>(G, g.V, st);
+    if (rc) return rc;
+    if (db) {
+      rc = db_dtype == MOE_F32 ? run_bias_grad<float>(G.part, g.blocks, W, db, st)
+           : db_dtype == MOE_BF16 ? run_bias_grad<__nv_bfloat16>(G.part, g.blocks, W, db, st) : run_bias_grad<__half>(G.part, g.blocks, W, db, st);
+      if (rc) return rc;
+    }
+  }
+  if (!products) return 0;
+  const void* dz = own ? own : dy;
+  Epilogue E = {};
+  E.act = MOE_LIN_NONE;
+  if (dtype == MOE_F32) {
+    if (dx) {
+      E.y = dx; E.y_ld = K; E.M = M; E.N = (int)K;
+      if (int rc = run_f32({(const float*)dz, dz_ld, 1}, {(const float*)w, 1, w_ld}, M, K, W, false, E, st)) return rc;
+    }
+    if (dw) {
+      E.y = dw; E.y_ld = K; E.M = W; E.N = (int)K;
+      if (int rc = run_f32({(const float*)dz, 1, dz_ld}, {(const float*)x, 1, x_ld}, W, K, M, false, E, st)) return rc;
+    }
+    return 0;
+  }
+  Matrix d = {dz, M, W, dz_ld};
+  if (int rc = readable(d, ws, st)) return rc;
+  auto product = [&](const Matrix& a, const Matrix& b, bool a_mn, int64_t rows, int64_t k) {
+    E.y_ld = K; E.M = rows; E.N = (int)K;
+    return dtype == MOE_BF16 ? run_product<__nv_bfloat16>(a, b, a_mn, true, rows, K, k, false, E, status, st)
+                             : run_product<__half>(a, b, a_mn, true, rows, K, k, false, E, status, st);
+  };
+  if (dx) {
+    Matrix b = {w, W, K, w_ld};
+    if (int rc = readable(b, ws, st)) return rc;
+    E.y = dx;
+    if (int rc = product(d, b, false, M, W)) return rc;
+  }
+  if (dw) {
+    Matrix b = {x, M, K, x_ld};
+    if (int rc = readable(b, ws, st)) return rc;
+    E.y = dw;
+    if (int rc = product(d, b, true, W, M)) return rc;
+  }
+  return 0;
+}

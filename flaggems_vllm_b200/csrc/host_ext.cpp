@@ -783,7 +783,7 @@ std::pair<at::Tensor, at::Tensor> linear_forward(const at::Tensor& x, const at::
   c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = p.N;
   at::Tensor y = fresh(sizes, x.scalar_type(), p.dev), z, ws;
-  if (keep) z = fresh({p.M, p.W}, x.scalar_type(), p.dev);
+  if (keep) z = fresh({p.M, p.W}, p.act == MOE_LIN_SILU_MUL ? at::kFloat : x.scalar_type(), p.dev);
   int64_t bytes = 0;
   must(moe_fused_linear_workspace(x.const_data_ptr(), p.x_ld, w.const_data_ptr(), p.w_ld, p.code, p.M, p.N, p.K, p.act, &bytes));
   if (bytes) ws = fresh({bytes}, at::kByte, p.dev);
@@ -826,8 +826,8 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
     at::Tensor x = saved[0], w = saved[1], z = saved[2];
     int64_t x_ld = K, w_ld = K;
     // the engine holds dy against y, nobody holds what a hook handed back against what was saved
-    auto held = [&](at::Tensor& t, int64_t rows, int64_t cols, int64_t* ld) {
-      if (!t.defined() || !t.is_cuda() || t.get_device() != dev || t.scalar_type() != dy.scalar_type() || t.dim() < 1 || t.size(-1) != cols ||
+    auto held = [&](at::Tensor& t, at::ScalarType type, int64_t rows, int64_t cols, int64_t* ld) {
+      if (!t.defined() || !t.is_cuda() || t.get_device() != dev || t.scalar_type() != type || t.dim() < 1 || t.size(-1) != cols ||
           t.numel() != rows * cols)
         throw KernelError(std::string("fused_linear") + kChanged);
       int64_t n;
@@ -838,10 +838,10 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
       if (n == 1) *ld = cols;
     };
     if (code < 0) throw KernelError(std::string("fused_linear") + kChanged);
-    if (want_w) held(x, M, K, &x_ld);
-    if (want_x) held(w, W, K, &w_ld);
+    if (want_w) held(x, dy.scalar_type(), M, K, &x_ld);
+    if (want_x) held(w, dy.scalar_type(), W, K, &w_ld);
     int64_t z_ld = W;
-    if (act != MOE_LIN_NONE) held(z, M, W, &z_ld);
+    if (act != MOE_LIN_NONE) held(z, act == MOE_LIN_SILU_MUL ? at::kFloat : dy.scalar_type(), M, W, &z_ld);
     {
       at::AutoDispatchBelowADInplaceOrView below;  // the buffers are no part of a graph
       c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);

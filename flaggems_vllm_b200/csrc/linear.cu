@@ -42,26 +42,59 @@ struct Epilogue {
   int N, act, bias_f32;
 };
 
+// Distribution function of the normal distribution, Phi.  fp32 results take CUDA's; 16-bit ones formula 7.1.26 of Abramowitz and
+// Stegun, Handbook of Mathematical Functions, for the complementary error function, whose relative error stays near 1e-6 down
+// the tail because the exponential stands outside: a sixth of the instructions (its own error is below 2^-20, theirs 2^-9 and 2^-12).
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float z) {
+  if constexpr (std::is_same<T, float>::value) {
+    return normcdff(z);
+  } else {
+    const float x = fabsf(z) * 0.7071067811865476f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * __expf(-x * x);
+    return z < 0.0f ? tail : 1.0f - tail;
+  }
+}
+// 1 / (1 + e^-z): fast forms where the result is rounded to 16 bits (a couple of ulp of fp32).  The fast division returns zero for
+// divisors beyond 2^126, which is right here.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (std::is_same<T, float>::value) return 1.0f / (1.0f + expf(-z));
+  else return __fdividef(1.0f, 1.0f + __expf(-z));
+}
+// (1 + tanh(c (z + a z^3))) / 2 is the sigmoid of twice the argument
+template <typename T>
+__device__ __forceinline__ float tanh_gate(float z) {
+  return sigmoid<T>(1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f));
+}
+template <typename T>
 __device__ __forceinline__ float act_value(int act, float z) {
   switch (act) {
     case MOE_LIN_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
-    case MOE_LIN_SILU: return z / (1.0f + expf(-z));
-    case MOE_LIN_GELU: return z * normcdff(z);
-    case MOE_LIN_GELU_TANH: return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z)));
+    case MOE_LIN_SILU: return z * sigmoid<T>(z);
+    case MOE_LIN_GELU: return z * normal_cdf<T>(z);
+    case MOE_LIN_GELU_TANH: return z * tanh_gate<T>(z);
     default: return z;
   }
 }
+template <typename T>
 __device__ __forceinline__ float act_slope(int act, float z) {
   switch (act) {
     case MOE_LIN_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
     case MOE_LIN_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
+      const float s = sigmoid<T>(z);
       return s * (1.0f + z * (1.0f - s));
     }
-    case MOE_LIN_GELU: return normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z));
-    case MOE_LIN_GELU_TANH: {
-      const float t = tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z));
-      return 0.5f * (1.0f + t) + 0.5f * z * (1.0f - t * t) * (0.7978845608028654f * (1.0f + 0.134145f * z * z));
+    case MOE_LIN_GELU: {
+      const float e = std::is_same<T, float>::value ? expf(-0.5f * z * z) : __expf(-0.5f * z * z);
+      return normal_cdf<T>(z) + z * (0.3989422804014327f * e);
+    }
+    case MOE_LIN_GELU_TANH: {  // g = sigmoid(s): (z g)' = g + z g (1 - g) s'
+      const float g = tanh_gate<T>(z);
+      const float h = g * (1.0f - g);
+      return h == 0.0f ? g : g + z * h * (1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f));  // s' overflows far out
     }
     default: return 1.0f;
   }
@@ -71,25 +104,29 @@ __device__ __forceinline__ float bias_at(const Epilogue& E, int n) {
   if (E.bias == nullptr) return 0.0f;
   return E.bias_f32 ? reinterpret_cast<const float*>(E.bias)[n] : ToF32<T>::get(reinterpret_cast<const T*>(E.bias)[n]);
 }
-// the sum(s) of output (m, n) -> y and z; z1: the gate's partner
+// the sum(s) of output (m, n) -> its value, and z where it is kept; z1: the gate's partner
 template <typename T>
-__device__ __forceinline__ void finish(const Epilogue& E, int64_t m, int n, float z0, float z1) {
+__device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, float z0, float z1) {
   z0 += bias_at<T>(E, n);
   float v;
   if (E.act == MOE_LIN_SILU_MUL) {
     z1 += bias_at<T>(E, E.N + n);
-    v = silu_mul(z0, z1);
+    v = z0 * sigmoid<T>(z0) * z1;
     if (E.z) {
-      T* z = reinterpret_cast<T*>(E.z) + m * E.z_ld + n;
-      z[0] = from_f32<T>(z0);
-      z[E.N] = from_f32<T>(z1);
+      float* z = reinterpret_cast<float*>(E.z) + m * E.z_ld + n;
+      z[0] = z0;
+      z[E.N] = z1;
     }
   } else {
-    v = act_value(E.act, z0);
+    v = act_value<T>(E.act, z0);
     if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(z0);
   }
   if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
-  reinterpret_cast<T*>(E.y)[m * E.y_ld + n] = from_f32<T>(v);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void finish(const Epilogue& E, int64_t m, int n, float z0, float z1) {
+  reinterpret_cast<T*>(E.y)[m * E.y_ld + n] = from_f32<T>(value<T>(E, m, n, z0, z1));
 }
 
 // ------------------------------------------------------------------ operand tiles
@@ -127,7 +164,7 @@ constexpr int kTileRing = 196608;
 __host__ __device__ constexpr int tile_stage(int bn) { return (128 + bn) * 128; }
 __host__ __device__ constexpr int tile_stages(int bn) { return kTileRing / tile_stage(bn) < 12 ? kTileRing / tile_stage(bn) : 12; }
 constexpr size_t kTileSmem = (size_t)kTileRing + 1024 + sizeof(TAux);
-static_assert(128 * 257 * 4 <= kTileRing, "the partial tile takes the ring's place");
+static_assert(128 * 260 * 4 <= kTileRing, "the partial tile takes the ring's place");
 
 __device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* a) {
   asm volatile(
@@ -137,6 +174,52 @@ __device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* a) {
         "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
       : "r"(taddr)
       : "memory");
+}
+
+// This CTA's share of the outputs of its cluster's tile, four columns of D at a time: the partial sums of all ranks in flight, added
+// in rank order.  Lanes run along the rows of y.
+template <typename T, int SPLIT>
+__device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t* smem, const Product& P, const Epilogue& E, int rank, int64_t r0,
+                                             int64_t c0, int out_rows, int out_cols) {
+  const int pitch = P.BN + 4, quads = out_cols / 4, share = out_rows * quads / SPLIT;  // all powers of two
+  const int row_bits = __ffs(out_rows) - 1, quad_bits = __ffs(quads) - 1;
+  const int up = P.gate == 0 ? 0 : (P.swapped ? 64 * pitch : P.BN / 2);
+  const float* base[SPLIT];
+#pragma unroll
+  for (int j = 0; j < SPLIT; ++j)
+    base[j] = SPLIT == 1 ? reinterpret_cast<const float*>(smem) : cluster.map_shared_rank(reinterpret_cast<const float*>(smem), j);
+  const bool y8 = !P.swapped && ((uintptr_t)E.y & 7) == 0 && E.y_ld % 4 == 0 && E.z == nullptr;
+  for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += TTHREADS) {
+    const int r = P.swapped ? i & (out_rows - 1) : i >> quad_bits, c = 4 * (P.swapped ? i >> row_bits : i & (quads - 1));
+    if (r0 + r >= P.rows || c0 + c >= P.cols) continue;
+    const int at = r * pitch + c;
+    float4 v[SPLIT], u[SPLIT];
+#pragma unroll
+    for (int j = 0; j < SPLIT; ++j) v[j] = *reinterpret_cast<const float4*>(base[j] + at);
+    if (up) {
+#pragma unroll
+      for (int j = 0; j < SPLIT; ++j) u[j] = *reinterpret_cast<const float4*>(base[j] + at + up);
+    }
+    float z0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, z1[4] = {};
+#pragma unroll
+    for (int j = 1; j < SPLIT; ++j) { z0[0] += v[j].x; z0[1] += v[j].y; z0[2] += v[j].z; z0[3] += v[j].w; }
+    if (up) {
+#pragma unroll
+      for (int j = 0; j < SPLIT; ++j) { z1[0] += u[j].x; z1[1] += u[j].y; z1[2] += u[j].z; z1[3] += u[j].w; }
+    }
+    if (y8 && c0 + c + 4 <= P.cols) {
+      const int64_t m = r0 + r;
+      const int n = (int)(c0 + c);
+      float o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = value<T>(E, m, n + q, z0[q], z1[q]);
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(E.y) + m * E.y_ld + n) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (c0 + c + q < P.cols) finish<T>(E, P.swapped ? c0 + c + q : r0 + r, (int)(P.swapped ? r0 + r : c0 + c + q), z0[q], z1[q]);
+    }
+  }
 }
 
 // One 128 x BN tile of D by the `split` CTAs of a cluster, each over its share of K.  A gated call's tile is half gate rows and
@@ -216,50 +299,30 @@ tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     if (leader) tc_commit(&aux->done);
   } else if (warp >= 4) {
-    // every product has finished reading the ring: it now holds the partial tile, rows of BN + 1 floats (a pitch without bank
-    // conflicts down a column as well as along the lanes' rows)
+    // every product has finished reading the ring: it now holds the partial tile, rows of BN + 4 floats (a pitch that spreads
+    // 16-byte pieces over the banks down a column as well as along the lanes' rows)
     const bool ok = warp_agrees(mbar_wait(&aux->done, 0, P.status, P.wait_ns));
     tc_fence_after();
     const int row = ((warp & 3) << 5) + lane;
-    float* part = reinterpret_cast<float*>(smem) + (size_t)row * (BN + 1);
+    float* part = reinterpret_cast<float*>(smem) + (size_t)row * (BN + 4);
     if (ok) {
 #pragma unroll 1
       for (int c = 0; c < BN; c += 16) {
         uint32_t r[16];
         tmem_ld16_sync(tmem + ((uint32_t)((warp & 3) << 5) << 16) + (uint32_t)c, r);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[c + i] = __uint_as_float(r[i]);
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(part + c)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
       }
     }
     tc_fence_before();
   }
   if (P.split > 1) cluster.sync();
   else __syncthreads();
-  {
-    // this CTA's share of the outputs, the fast index along the rows of y
-    const int64_t left_r = P.rows - r0, left_c = P.cols - c0;
-    const int nr = (int)(left_r < out_rows ? left_r : out_rows), nc = (int)(left_c < out_cols ? left_c : out_cols);
-    const int fast = P.swapped ? nr : nc, total = nr * nc;
-    const int lo = (int)((int64_t)total * rank / P.split), hi = (int)((int64_t)total * (rank + 1) / P.split);
-    const float* base = reinterpret_cast<const float*>(smem);
-    for (int i = lo + threadIdx.x; i < hi; i += TTHREADS) {
-      const int slow = i / fast, f = i - slow * fast;
-      const int r = P.swapped ? f : slow, c = P.swapped ? slow : f;
-      const int at = r * (BN + 1) + c, up = gate_a ? 64 * (BN + 1) : BN / 2;
-      float z0 = 0.0f, z1 = 0.0f;
-      if (P.split == 1) {
-        z0 = base[at];
-        if (P.gate) z1 = base[at + up];
-      } else {
-#pragma unroll 8
-        for (int j = 0; j < P.split; ++j) {
-          const float* peer = cluster.map_shared_rank(base, j);
-          z0 += peer[at];
-          if (P.gate) z1 += peer[at + up];
-        }
-      }
-      finish<T>(E, P.swapped ? c0 + c : r0 + r, (int)(P.swapped ? r0 + r : c0 + c), z0, z1);
-    }
+  switch (P.split) {
+    case 1: finish_share<T, 1>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols); break;
+    case 2: finish_share<T, 2>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols); break;
+    case 4: finish_share<T, 4>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols); break;
+    default: finish_share<T, 8>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols);
   }
   tc_fence_before();
   if (P.split > 1) cluster.sync();  // no CTA leaves while its partial tile may still be read
@@ -277,7 +340,10 @@ struct PAux {
   uint64_t full[8], empty[8], tmem_full[2], tmem_empty[2];
   uint32_t tmem_base;
 };
-constexpr size_t kPairSmem = (size_t)kPairRing + 1024 + sizeof(PAux);
+constexpr int kStagePitch = 33;  // floats of a staged row of 32 columns
+constexpr int kPairStage = PCONS * kStagePitch * 4;
+constexpr size_t kPairSmem = (size_t)kPairRing + kPairStage + 1024 + sizeof(PAux);
+static_assert(kPairSmem <= 232448, "shared memory of one SM");
 
 // Tile order: `group` row tiles share a walk over the column tiles, so that the pairs that run at one time read few different
 // operand tiles.
@@ -289,35 +355,71 @@ __device__ __forceinline__ void tile_at(int item, int RT, int CT, int group, int
   ct = in / size;
 }
 
-template <typename T>
-__device__ __forceinline__ void load_row32(const T* p, bool wide, int n, float (&v)[32]) {
-  if (wide) {
+// 32 columns of 32 rows between a warp's registers (lane = row) and memory.  `wide`: the rows are whole 16-byte pieces, and each
+// lane moves its own; else they go through shared memory, so that the warp reads and writes along the rows (4096 x 4097 outputs:
+// XXX us, XXX with each lane at its own row).
+struct Rows {
+  int64_t m0, end;  // the warp's first row, the first row that is not there
+  int n0, n;        // first column, columns that are there (n > 0)
+  float* stage;     // the warp's own
+  int lane;
+};
+template <typename S>
+__device__ __forceinline__ void load_rows(const S* base, int64_t ld, bool wide, const Rows& R, float (&v)[32]) {
+  if (wide && R.n == 32) {
+    if (R.m0 + R.lane < R.end) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float t[8];
-      load8<T>(p + 8 * i, t);
+      for (int i = 0; i < 4; ++i) {
+        float t[8];
+        load8<S>(base + (R.m0 + R.lane) * ld + R.n0 + 8 * i, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[8 * i + j] = t[j];
+        for (int j = 0; j < 8; ++j) v[8 * i + j] = t[j];
+      }
     }
   } else {
+    __syncwarp();
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      R.stage[r * kStagePitch + R.lane] = R.m0 + r < R.end && R.lane < R.n ? ToF32<S>::get(base[(R.m0 + r) * ld + R.n0 + R.lane]) : 0.0f;
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = i < n ? ToF32<T>::get(p[i]) : 0.0f;
+    for (int i = 0; i < 32; ++i) v[i] = R.stage[R.lane * kStagePitch + i];
   }
 }
-template <typename T>
-__device__ __forceinline__ void store_row32(T* p, bool wide, bool wide32, int n, const float (&v)[32]) {
-  if (wide) {
-    uint4 q[4];
+template <typename S>
+__device__ __forceinline__ void store_rows(S* base, int64_t ld, bool wide, bool wide32, const Rows& R, const float (&v)[32]) {
+  if (wide && R.n == 32) {
+    if (R.m0 + R.lane < R.end) {
+      S* p = base + (R.m0 + R.lane) * ld + R.n0;
+      if constexpr (sizeof(S) == 4) {
+        uint4 q[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      q[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]), pack2<T>(v[8 * i + 4], v[8 * i + 5]),
-                        pack2<T>(v[8 * i + 6], v[8 * i + 7]));
-    store_row_pieces<4>(p, q, wide32);
+        for (int i = 0; i < 8; ++i)
+          q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+        store_row_pieces<8>(p, q, wide32);
+      } else {
+        uint4 q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[i] = make_uint4(pack2<S>(v[8 * i], v[8 * i + 1]), pack2<S>(v[8 * i + 2], v[8 * i + 3]), pack2<S>(v[8 * i + 4], v[8 * i + 5]),
+                            pack2<S>(v[8 * i + 6], v[8 * i + 7]));
+        store_row_pieces<4>(p, q, wide32);
+      }
+    }
   } else {
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) p[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < 32; ++i) R.stage[R.lane * kStagePitch + i] = v[i];
+    __syncwarp();
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (R.m0 + r < R.end && R.lane < R.n) base[(R.m0 + r) * ld + R.n0 + R.lane] = from_f32<S>(R.stage[r * kStagePitch + R.lane]);
   }
+}
+// whole 16 (32) byte pieces, for columns that begin at multiples of 32
+template <typename S>
+__device__ __forceinline__ bool pieces(const S* base, int64_t ld, int bytes) {
+  return ((uintptr_t)base & (bytes - 1)) == 0 && ld * (int64_t)sizeof(S) % bytes == 0;
 }
 
 template <typename T>
@@ -325,7 +427,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product P, const Epilogue E) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_1024(smem_raw);
-  PAux* aux = reinterpret_cast<PAux*>(smem + kPairRing);
+  PAux* aux = reinterpret_cast<PAux*>(smem + kPairRing + kPairStage);
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cr = (int)cluster_ctarank();  // 0 leads
   const int BN = P.BN, stage = 2 * BOX + (BN / 128) * BOX, stages = BN == 256 ? 6 : 8;
@@ -419,81 +521,82 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     uint32_t acc_it = 0;
     const T* res = reinterpret_cast<const T*>(E.residual);
     T *y = reinterpret_cast<T*>(E.y), *z = reinterpret_cast<T*>(E.z);
-    const bool y16 = ((uintptr_t)y & 15) == 0 && E.y_ld % 8 == 0, y32 = ((uintptr_t)y & 31) == 0 && E.y_ld % 16 == 0;
-    const bool r16 = ((uintptr_t)res & 15) == 0 && E.residual_ld % 8 == 0;
-    const bool z16 = ((uintptr_t)z & 15) == 0 && E.z_ld % 8 == 0 && E.N % 8 == 0;
-    const bool z32 = z16 && ((uintptr_t)z & 31) == 0 && E.z_ld % 16 == 0 && E.N % 16 == 0;
+    float* zf = reinterpret_cast<float*>(E.z);  // of a gated call
+    const bool y16 = pieces(y, E.y_ld, 16), y32 = pieces(y, E.y_ld, 32), r16 = pieces(res, E.residual_ld, 16);
+    const bool z16 = P.gate ? pieces(zf, E.z_ld, 16) && E.N % 4 == 0 : pieces(z, E.z_ld, 16);
+    const bool z32 = P.gate ? pieces(zf, E.z_ld, 32) && E.N % 8 == 0 : pieces(z, E.z_ld, 32);
+    Rows R;
+    R.end = P.rows;
+    R.stage = reinterpret_cast<float*>(smem + kPairRing) + (warp - 4) * 32 * kStagePitch;
+    R.lane = lane;
     for (int item = item0; item < total; item += step) {
       const uint32_t a = acc_it & 1;
       if (!warp_agrees(mbar_wait_idle(&aux->tmem_full[a], (acc_it >> 1) & 1, P.status, P.wait_ns))) break;
       tc_fence_after();
       int rt, ct;
       tile_at(item, RT, CT, P.group, rt, ct);
-      const int64_t m = (int64_t)rt * 256 + cr * 128 + wq * 32 + lane;
-      const bool live = m < P.rows;
+      R.m0 = (int64_t)rt * 256 + cr * 128 + wq * 32;
       const int span = out_cols / 2;  // columns of this warp
 #pragma unroll 1
       for (int q = 0; q < span; q += 32) {
-        const int in = h * span + q, n0 = ct * out_cols + in;
+        const int in = h * span + q;
+        R.n0 = ct * out_cols + in;
+        if (R.n0 >= P.cols || R.m0 >= R.end) break;
+        R.n = (int)(P.cols - R.n0 < 32 ? P.cols - R.n0 : 32);
         uint32_t r0[32], r1[32];
         tmem_ld32_async(t_lane + a * 256 + (uint32_t)in, r0);
         if (P.gate) tmem_ld32_async(t_lane + a * 256 + (uint32_t)(BN / 2 + in), r1);
         tmem_wait32(r0);
         if (P.gate) tmem_wait32(r1);
-        const int n = (int)(P.cols - n0 < 32 ? P.cols - n0 : 32);
-        if (live && n > 0) {
-          float v[32];
-  #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r0[i]);
-          if (E.bias) {
-  #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += i < n ? bias_at<T>(E, n0 + i) : 0.0f;
-          }
-          const bool whole = n == 32;
-          if (P.gate) {
-            float u[32];
-  #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(r1[i]);
-            if (E.bias) {
-  #pragma unroll
-              for (int i = 0; i < 32; ++i) u[i] += i < n ? bias_at<T>(E, E.N + n0 + i) : 0.0f;
-            }
-            if (z) {
-              store_row32<T>(z + m * E.z_ld + n0, whole && z16, z32, n, v);
-              store_row32<T>(z + m * E.z_ld + E.N + n0, whole && z16, z32, n, u);
-            }
-  #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = silu_mul_fast(v[i], u[i]);
-          } else {
-            if (z) store_row32<T>(z + m * E.z_ld + n0, whole && z16, z32, n, v);
-            switch (E.act) {  // one loop each: the choice is the call's
-              case MOE_LIN_NONE: break;
-              case MOE_LIN_RELU:
-  #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = act_value(MOE_LIN_RELU, v[i]);
-                break;
-              case MOE_LIN_SILU:
-  #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = silu_mul_fast(v[i], 1.0f);
-                break;
-              case MOE_LIN_GELU:
-  #pragma unroll 4
-                for (int i = 0; i < 32; ++i) v[i] = act_value(MOE_LIN_GELU, v[i]);
-                break;
-              default:
-  #pragma unroll 4
-                for (int i = 0; i < 32; ++i) v[i] = act_value(MOE_LIN_GELU_TANH, v[i]);
-            }
-          }
-          if (res) {
-            float t[32];
-            load_row32<T>(res + m * E.residual_ld + n0, whole && r16, n, t);
-  #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += t[i];
-          }
-          store_row32<T>(y + m * E.y_ld + n0, whole && y16, y32, n, v);
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r0[i]);
+        if (E.bias) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += i < R.n ? bias_at<T>(E, R.n0 + i) : 0.0f;
         }
-        __syncwarp();  // the next columns are loaded by the warp as one
+        if (P.gate) {
+          float u[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(r1[i]);
+          if (E.bias) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] += i < R.n ? bias_at<T>(E, E.N + R.n0 + i) : 0.0f;
+          }
+          if (zf) {
+            store_rows<float>(zf, E.z_ld, z16, z32, R, v);
+            store_rows<float>(zf + E.N, E.z_ld, z16, z32, R, u);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = v[i] * sigmoid<T>(v[i]) * u[i];
+        } else {
+          if (z) store_rows<T>(z, E.z_ld, z16, z32, R, v);
+          switch (E.act) {  // one loop each: the choice is the call's
+            case MOE_LIN_NONE: break;
+            case MOE_LIN_RELU:
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = act_value<T>(MOE_LIN_RELU, v[i]);
+              break;
+            case MOE_LIN_SILU:
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = act_value<T>(MOE_LIN_SILU, v[i]);
+              break;
+            case MOE_LIN_GELU:
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = act_value<T>(MOE_LIN_GELU, v[i]);
+              break;
+            default:
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = act_value<T>(MOE_LIN_GELU_TANH, v[i]);
+          }
+        }
+        if (res) {
+          float t[32];
+          load_rows<T>(res, E.residual_ld, r16, R, t);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += t[i];
+        }
+        store_rows<T>(y, E.y_ld, y16, y32, R, v);
       }
       tc_fence_before();
       __syncwarp();
@@ -623,10 +726,11 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad P) {
   const int64_t m1 = m0 + P.rows_per_block < P.M ? m0 + P.rows_per_block : P.M;
   const bool gated = P.act == MOE_LIN_SILU_MUL, in = n < P.N;
   float s0[V] = {}, s1[V] = {};
-  auto load = [](const void* base, int64_t at, float (&v)[V]) {
-    const T* p = reinterpret_cast<const T*>(base) + at;
-    if constexpr (V == 8) load8<T>(p, v);
-    else v[0] = ToF32<T>::get(*p);
+  auto load = [](auto type, const void* base, int64_t at, float (&v)[V]) {
+    using S = decltype(type);
+    const S* p = reinterpret_cast<const S*>(base) + at;
+    if constexpr (V == 8) load8<S>(p, v);
+    else v[0] = ToF32<S>::get(*p);
   };
   auto store = [](void* base, int64_t at, const float (&v)[V]) {
     T* p = reinterpret_cast<T*>(base) + at;
@@ -640,14 +744,14 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad P) {
 #pragma unroll 2
     for (int64_t m = m0 + warp; m < m1; m += 8) {
       float dy[V], z[V];
-      load(P.dy, m * P.dy_ld + n, dy);
+      load(T(), P.dy, m * P.dy_ld + n, dy);
       if (gated) {
         float u[V], du[V];
-        load(P.z, m * P.z_ld + n, z);
-        load(P.z, m * P.z_ld + P.N + n, u);
+        load(float(), P.z, m * P.z_ld + n, z);
+        load(float(), P.z, m * P.z_ld + P.N + n, u);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float s = 1.0f / (1.0f + expf(-z[i])), d = dy[i];
+          const float s = sigmoid<T>(z[i]), d = dy[i];
           du[i] = d * (z[i] * s);
           dy[i] = d * u[i] * (s * (1.0f + z[i] * (1.0f - s)));
           s0[i] += dy[i];
@@ -659,9 +763,9 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad P) {
         }
       } else {
         if (P.act != MOE_LIN_NONE) {
-          load(P.z, m * P.z_ld + n, z);
+          load(T(), P.z, m * P.z_ld + n, z);
 #pragma unroll
-          for (int i = 0; i < V; ++i) dy[i] *= act_slope(P.act, z[i]);
+          for (int i = 0; i < V; ++i) dy[i] *= act_slope<T>(P.act, z[i]);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) s0[i] += dy[i];
@@ -708,16 +812,27 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const float* part, int64
   }
 }
 
-// rows of 16-bit elements that TMA cannot read (a pitch that is no multiple of 16 bytes, an odd address) -> rows that it can
+// Rows of 16-bit elements that TMA cannot read (a pitch that is no multiple of 16 bytes, an odd address) -> rows that it can.  A
+// thread writes 16 bytes at a time, put together from the aligned words that hold them: the first and the last of them may
+// reach beyond the row, never beyond the words that it touches.
 __global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t src_ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t dst_ld) {
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + warp; r < rows; r += (int64_t)gridDim.x * 8) {
-    const uint16_t* s = src + r * src_ld;
-    uint16_t* d = dst + r * dst_ld;
-#pragma unroll 8
-    for (int64_t c = lane; c < cols; c += 32) d[c] = s[c];
+  const int64_t pieces = dst_ld / 8, total = rows * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / pieces, c = (i - r * pieces) * 8;
+    const uintptr_t at = (uintptr_t)(src + r * src_ld + c);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+    const int left = cols - c < 8 ? (int)(cols - c) : 8;      // elements of this piece, > 0
+    const int words = (left + ((at & 2) ? 1 : 0) + 1) / 2;  // words that hold them
+    uint32_t v[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) v[k] = k < words ? __ldg(w + k) : 0u;
+    if (at & 2) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = __funnelshift_r(v[k], v[k + 1], 16);
+    }
+    *reinterpret_cast<uint4*>(dst + r * dst_ld + c) = make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -748,7 +863,7 @@ int readable(Matrix& m, Space& ws, cudaStream_t st) {
   const int64_t ld = padded(m.cols);
   void* p = ws.take(m.rows * ld * 2);
   if (!p) return fail(MOE_E_BADARG, "fused_linear: workspace too small");
-  const int64_t blocks = (m.rows + 7) / 8;
+  const int64_t blocks = (m.rows * (ld / 8) + 255) / 256;
   const int rc = launch_pdl(pitch_kernel, dim3((unsigned)(blocks < 8 * sm_count() ? blocks : 8 * sm_count())), 256, 0, 1, st,
                             "fused_linear (pitch)", (const uint16_t*)m.p, m.ld, m.rows, m.cols, (uint16_t*)p, ld);
   m.p = p;
@@ -925,7 +1040,8 @@ GradPlan grad_plan(const void* dy, const void* z, int64_t z_ld, const void* dz, 
   p.need_dz = products && act != MOE_LIN_NONE;
   const int eb = dtype == MOE_F32 ? 4 : 2;
   auto wide = [&](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && ld * eb % 16 == 0; };
-  p.V = N % 8 == 0 && wide(dy, N) && (act == MOE_LIN_NONE || wide(z, z_ld)) && wide(dz, W) ? 8 : 1;
+  const bool z_wide = act == MOE_LIN_SILU_MUL ? ((uintptr_t)z & 15) == 0 && z_ld % 4 == 0 : act == MOE_LIN_NONE || wide(z, z_ld);
+  p.V = N % 8 == 0 && wide(dy, N) && z_wide && wide(dz, W) ? 8 : 1;
   p.rows_per_block = grad_rows(M, N, p.V, sm_count());
   p.blocks = (M + p.rows_per_block - 1) / p.rows_per_block;
   return p;

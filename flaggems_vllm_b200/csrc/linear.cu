@@ -178,7 +178,7 @@ __device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* a) {
 
 // This CTA's share of the outputs of its cluster's tile, four columns of D at a time: the partial sums of all ranks in flight, added
 // in rank order.  Lanes run along the rows of y.
-template <typename T, int SPLIT>
+template <typename T, int SPLIT, int THREADS = TTHREADS>
 __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t* smem, const Product& P, const Epilogue& E, int rank, int64_t r0,
                                              int64_t c0, int out_rows, int out_cols) {
   const int pitch = P.BN + 4, quads = out_cols / 4, share = out_rows * quads / SPLIT;  // all powers of two
@@ -188,8 +188,8 @@ __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t
 #pragma unroll
   for (int j = 0; j < SPLIT; ++j)
     base[j] = SPLIT == 1 ? reinterpret_cast<const float*>(smem) : cluster.map_shared_rank(reinterpret_cast<const float*>(smem), j);
-  const bool y8 = !P.swapped && ((uintptr_t)E.y & 7) == 0 && E.y_ld % 4 == 0 && E.z == nullptr;
-  for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += TTHREADS) {
+  const bool wide = !P.swapped && ((uintptr_t)E.y & (4 * sizeof(T) - 1)) == 0 && E.y_ld % 4 == 0;
+  for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += THREADS) {
     const int r = P.swapped ? i & (out_rows - 1) : i >> quad_bits, c = 4 * (P.swapped ? i >> row_bits : i & (quads - 1));
     if (r0 + r >= P.rows || c0 + c >= P.cols) continue;
     const int at = r * pitch + c;
@@ -207,13 +207,15 @@ __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t
 #pragma unroll
       for (int j = 0; j < SPLIT; ++j) { z1[0] += u[j].x; z1[1] += u[j].y; z1[2] += u[j].z; z1[3] += u[j].w; }
     }
-    if (y8 && c0 + c + 4 <= P.cols) {
+    if (wide && c0 + c + 4 <= P.cols) {
       const int64_t m = r0 + r;
       const int n = (int)(c0 + c);
       float o[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[q] = value<T>(E, m, n + q, z0[q], z1[q]);
-      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(E.y) + m * E.y_ld + n) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+      T* y = reinterpret_cast<T*>(E.y) + m * E.y_ld + n;
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
+      else *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
@@ -618,92 +620,134 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // ------------------------------------------------------------------ fp32 operands
-// 64 x 64 tiles of D by 256 threads, 4 x 4 outputs each, 16 k at a time through shared memory; either operand either way round.
+// 8 RM x 64 tiles of D by 64 threads, RM x 8 outputs each, 16 k at a time out of a ring in shared memory that asynchronous copies
+// fill (each element to its place, which transposes operands with rows of k; whole 16-byte pieces where rows of r or c allow it);
+// K divided over a cluster as in tile_kernel.  A gated call's tile has 32 gate columns and the 32 up columns that go with them.
 struct F32Operand {
   const float* p;
-  int64_t rs, ks;  // strides of the row (r or c) and of k
+  int64_t rs, ks;  // strides of the row (r or c) and of k, one of them 1
+  int wide;        // rows of r or c in whole 16-byte pieces
 };
-__global__ void __launch_bounds__(256) f32_kernel(F32Operand A, F32Operand B, int64_t rows, int64_t cols, int64_t K, int64_t gate, Epilogue E) {
+constexpr int FTHREADS = 64, FPITCH = 68, FSTAGES = 4;
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void* src, bool yes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(yes ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// ROWS x 16 elements from (base, k0) on; zeros beyond `end` and `kend`.  gate: rows from ROWS / 2 on lie that far behind the first
+template <int ROWS>
+__device__ __forceinline__ void f32_fill(const F32Operand& X, int64_t base, int64_t end, int64_t gate, int64_t k0, int64_t kend, uint32_t dst) {
+  const int t = threadIdx.x;
+  if (X.ks == 1) {
+    const int k = t & 15;
+    const bool in = k0 + k < kend;
+    dst += (uint32_t)(k * FPITCH + (t >> 4)) * 4;
+    const float* p = X.p + (base + (t >> 4)) * X.rs + k0 + k;
+    int64_t left = end - base - (t >> 4);  // rows that are there from this thread's first on
+#pragma unroll
+    for (int i = 0; i < ROWS / 4; ++i) {
+      if (gate != 0 && i == ROWS / 8) {
+        p += (gate - ROWS / 2) * X.rs;
+        left += ROWS / 2;
+      }
+      const bool yes = in && left > 0;
+      cp_async4_or_zero(dst + 16 * i, yes ? p : X.p, yes);
+      p += 4 * X.rs;
+      left -= 4;
+    }
+  } else if (X.wide) {
+    constexpr int LANES = ROWS / 4, PER = FTHREADS / LANES;  // pieces of a k, k of a round
+#pragma unroll
+    for (int i = 0; i < (16 + PER - 1) / PER; ++i) {
+      const int k = t / LANES + PER * i, r = (t % LANES) * 4;
+      if (k >= 16) break;
+      const int64_t left = k0 + k < kend ? end - base - r : 0;
+      const int bytes = left >= 4 ? 16 : (left > 0 ? (int)left * 4 : 0);
+      cp_async16_or_zero(dst + (uint32_t)(k * FPITCH + r) * 4, bytes ? X.p + (k0 + k) * X.ks + base + r : X.p, bytes);
+    }
+  } else {
+    constexpr int PER = FTHREADS / ROWS;
+    const int r = t % ROWS;
+    const bool in = base + r < end;
+#pragma unroll
+    for (int i = 0; i < 16 / PER; ++i) {
+      const int k = t / ROWS + PER * i;
+      const bool yes = in && k0 + k < kend;
+      cp_async4_or_zero(dst + (uint32_t)(k * FPITCH + r) * 4, yes ? X.p + (k0 + k) * X.ks + base + r : X.p, yes);
+    }
+  }
+}
+template <int RM>
+__global__ void __launch_bounds__(FTHREADS, RM == 8 ? 7 : 10) f32_kernel(const F32Operand A, const F32Operand B, int64_t K, const Product P, const Epilogue E) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];  // FSTAGES x {A, B}[16][FPITCH], then the partial tile
+  float* s_mem = reinterpret_cast<float*>(smem_raw);
+  static_assert(64 * FPITCH <= FSTAGES * 2 * 16 * FPITCH, "the partial tile takes the operands' place");
+  constexpr int TM = 8 * RM, HALF = 16 * FPITCH;  // floats of an operand's tile
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int t = threadIdx.x, tx = t & 7, ty = t >> 3;
+  const int out_cols = P.gate ? 32 : 64;
+  const int64_t r0 = (int64_t)blockIdx.y * TM, c0 = (int64_t)(blockIdx.x / P.split) * out_cols;
+  const int64_t steps = (K + 15) / 16, first = steps * rank / P.split, last = steps * (rank + 1) / P.split;
+  const uint32_t s0 = smem_u32(s_mem);
   pdl_wait();
   pdl_trigger();
-  __shared__ float sa[2][16][68], sb[2][16][68];
-  const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
-  const int out_cols = gate ? 32 : 64;
-  const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * out_cols;
-  float acc[4][4] = {};
-  // a thread's four elements of a 64 x 16 tile: neighbouring threads along the contiguous side
-  auto fetch = [&](const F32Operand& X, int64_t base, int64_t end, bool gated, int64_t k0, float (&v)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = X.ks == 1 ? (t >> 4) + 16 * i : (t & 63), k = X.ks == 1 ? (t & 15) : (t >> 6) + 4 * i;
-      int64_t row = base + r;
-      bool in = row < end;
-      if (gated) {  // first half gate rows, second half up rows
-        row = base + (r & 31);
-        in = row < end;
-        row += r < 32 ? 0 : gate;
-      }
-      v[i] = in && k0 + k < K ? __ldg(X.p + row * X.rs + (k0 + k) * X.ks) : 0.0f;
+  float acc[RM][8] = {};
+  auto fill = [&](int64_t step) {
+    if (step < last) {
+      const uint32_t dst = s0 + (uint32_t)((step - first) % FSTAGES) * (2 * HALF * 4);
+      f32_fill<TM>(A, r0, P.rows, 0, step * 16, K, dst);
+      f32_fill<64>(B, c0, P.cols, P.gate, step * 16, K, dst + HALF * 4);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto put = [&](const F32Operand& X, float (*s)[68], const float (&v)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = X.ks == 1 ? (t >> 4) + 16 * i : (t & 63), k = X.ks == 1 ? (t & 15) : (t >> 6) + 4 * i;
-      s[k][r] = v[i];
-    }
-  };
-  float va[4], vb[4];
-  fetch(A, r0, rows, false, 0, va);
-  fetch(B, c0, cols, gate != 0, 0, vb);
-  put(A, sa[0], va);
-  put(B, sb[0], vb);
-  __syncthreads();
-  int cur = 0;
-  for (int64_t k0 = 0; k0 < K; k0 += 16) {
-    const bool more = k0 + 16 < K;
-    if (more) {
-      fetch(A, r0, rows, false, k0 + 16, va);
-      fetch(B, c0, cols, gate != 0, k0 + 16, vb);
-    }
-#pragma unroll
+#pragma unroll 1
+  for (int s = 0; s < FSTAGES - 1; ++s) fill(first + s);
+#pragma unroll 1
+  for (int64_t step = first; step < last; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(FSTAGES - 2) : "memory");
+    __syncthreads();  // this step's tiles are there, the last one's have been read
+    fill(step + FSTAGES - 1);
+    const float* sa = s_mem + ((step - first) % FSTAGES) * (2 * HALF);
+    const float* sb = sa + HALF;
+#pragma unroll 4
     for (int k = 0; k < 16; ++k) {
-      const float4 a = *reinterpret_cast<const float4*>(&sa[cur][k][4 * ty]);
-      float b[4];
-      if (gate) {  // a thread's columns: two gates and their ups
-        b[0] = sb[cur][k][2 * tx]; b[1] = sb[cur][k][2 * tx + 1];
-        b[2] = sb[cur][k][32 + 2 * tx]; b[3] = sb[cur][k][32 + 2 * tx + 1];
+      const float4 b0 = *reinterpret_cast<const float4*>(sb + k * FPITCH + 4 * tx), b1 = *reinterpret_cast<const float4*>(sb + k * FPITCH + 32 + 4 * tx);
+      float a[RM];
+      if constexpr (RM == 8) {
+        const float4 p = *reinterpret_cast<const float4*>(sa + k * FPITCH + 4 * ty), q = *reinterpret_cast<const float4*>(sa + k * FPITCH + 32 + 4 * ty);
+        a[0] = p.x; a[1] = p.y; a[2] = p.z; a[3] = p.w; a[4] = q.x; a[5] = q.y; a[6] = q.z; a[7] = q.w;
       } else {
-        const float4 q = *reinterpret_cast<const float4*>(&sb[cur][k][4 * tx]);
-        b[0] = q.x; b[1] = q.y; b[2] = q.z; b[3] = q.w;
+        a[0] = sa[k * FPITCH + ty];
       }
-      const float ar[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ar[i], b[j], acc[i][j]);
-    }
-    if (more) {
-      put(A, sa[cur ^ 1], va);
-      put(B, sb[cur ^ 1], vb);
-    }
-    __syncthreads();
-    cur ^= 1;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = r0 + 4 * ty + i;
-    if (m >= rows) continue;
-    if (gate) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (c0 + 2 * tx + j < cols) finish<float>(E, m, (int)(c0 + 2 * tx + j), acc[i][j], acc[i][2 + j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c0 + 4 * tx + j < cols) finish<float>(E, m, (int)(c0 + 4 * tx + j), acc[i][j], 0.0f);
+      for (int i = 0; i < RM; ++i) {
+        acc[i][0] = fmaf(a[i], b0.x, acc[i][0]); acc[i][1] = fmaf(a[i], b0.y, acc[i][1]);
+        acc[i][2] = fmaf(a[i], b0.z, acc[i][2]); acc[i][3] = fmaf(a[i], b0.w, acc[i][3]);
+        acc[i][4] = fmaf(a[i], b1.x, acc[i][4]); acc[i][5] = fmaf(a[i], b1.y, acc[i][5]);
+        acc[i][6] = fmaf(a[i], b1.z, acc[i][6]); acc[i][7] = fmaf(a[i], b1.w, acc[i][7]);
+      }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    float* part = s_mem + (RM == 8 ? (i < 4 ? 4 * ty + i : 28 + 4 * ty + i) : ty) * FPITCH + 4 * tx;
+    *reinterpret_cast<float4*>(part) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    *reinterpret_cast<float4*>(part + 32) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+  }
+  if (P.split > 1) cluster.sync();
+  else __syncthreads();
+  uint8_t* tile = reinterpret_cast<uint8_t*>(s_mem);
+  switch (P.split) {
+    case 1: finish_share<float, 1, FTHREADS>(cluster, tile, P, E, rank, r0, c0, TM, out_cols); break;
+    case 2: finish_share<float, 2, FTHREADS>(cluster, tile, P, E, rank, r0, c0, TM, out_cols); break;
+    case 4: finish_share<float, 4, FTHREADS>(cluster, tile, P, E, rank, r0, c0, TM, out_cols); break;
+    default: finish_share<float, 8, FTHREADS>(cluster, tile, P, E, rank, r0, c0, TM, out_cols);
+  }
+  if (P.split > 1) cluster.sync();  // no CTA leaves while its partial tile may still be read
 }
 
 // ------------------------------------------------------------------ gradient of the activation, and of the bias
@@ -954,10 +998,22 @@ int run_product(Matrix a, Matrix b, bool a_mn, bool b_mn, int64_t rows, int64_t 
 }
 
 int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, bool gated, const Epilogue& E, cudaStream_t st) {
-  const int64_t gx = gated ? (cols + 31) / 32 : (cols + 63) / 64, gy = (rows + 63) / 64;
-  if (gy > 65535) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d rows", 65535 * 64);
-  return launch_pdl(f32_kernel, dim3((unsigned)gx, (unsigned)gy), 256, 0, 1, st, "fused_linear (fp32)", a, b, rows, cols, K,
-                    (int64_t)(gated ? cols : 0), E);
+  for (F32Operand* x : {&a, &b}) x->wide = ((uintptr_t)x->p & 15) == 0 && x->ks % 4 == 0;
+  Product P = {};
+  P.rows = rows;
+  P.cols = cols;
+  P.gate = gated ? (int)cols : 0;
+  P.BN = 64;
+  const int TM = rows <= 8 ? 8 : 64;
+  const int64_t ct = (cols + (gated ? 31 : 63)) / (gated ? 32 : 64), rt = (rows + TM - 1) / TM;
+  if (rt > 65535) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d rows", 65535 * 64);
+  // four blocks an SM hide each other's latency; a share of K stays at 64 or more
+  P.split = 1;
+  while (P.split < 8 && ct * rt * P.split < 4 * (int64_t)sm_count() && K / (2 * P.split) >= 64) P.split *= 2;
+  const dim3 grid((unsigned)(ct * P.split), (unsigned)rt);
+  constexpr size_t smem = FSTAGES * 2 * 16 * FPITCH * 4;  // below the 48 KB that need no leave
+  if (TM == 8) return launch_pdl(f32_kernel<1>, grid, FTHREADS, smem, P.split, st, "fused_linear (fp32)", a, b, K, P, E);
+  return launch_pdl(f32_kernel<8>, grid, FTHREADS, smem, P.split, st, "fused_linear (fp32)", a, b, K, P, E);
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K, int dtype, int act) {
@@ -1017,7 +1073,7 @@ extern "C" int moe_fused_linear(const void* x, int64_t x_ld, const void* w, int6
   cudaStream_t st = (cudaStream_t)stream;
   Epilogue E = {bias, residual, y, z, residual_ld, y_ld, z_ld, M, (int)N, act, bias_dtype == MOE_F32};
   const bool gated = act == MOE_LIN_SILU_MUL;
-  if (dtype == MOE_F32) return run_f32({(const float*)x, x_ld, 1}, {(const float*)w, w_ld, 1}, M, N, K, gated, E, st);
+  if (dtype == MOE_F32) return run_f32({(const float*)x, x_ld, 1, 0}, {(const float*)w, w_ld, 1, 0}, M, N, K, gated, E, st);
   Space ws = {(uint8_t*)workspace, workspace ? workspace_bytes : 0};
   Matrix a = {x, M, K, x_ld}, b = {w, W, K, w_ld};
   if (int rc = readable(a, ws, st)) return rc;
@@ -1104,11 +1160,11 @@ extern "C" int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld
   if (dtype == MOE_F32) {
     if (dx) {
       E.y = dx; E.y_ld = K; E.M = M; E.N = (int)K;
-      if (int rc = run_f32({(const float*)dz, dz_ld, 1}, {(const float*)w, 1, w_ld}, M, K, W, false, E, st)) return rc;
+      if (int rc = run_f32({(const float*)dz, dz_ld, 1, 0}, {(const float*)w, 1, w_ld, 0}, M, K, W, false, E, st)) return rc;
     }
     if (dw) {
       E.y = dw; E.y_ld = K; E.M = W; E.N = (int)K;
-      if (int rc = run_f32({(const float*)dz, 1, dz_ld}, {(const float*)x, 1, x_ld}, W, K, M, false, E, st)) return rc;
+      if (int rc = run_f32({(const float*)dz, 1, dz_ld, 0}, {(const float*)x, 1, x_ld, 0}, W, K, M, false, E, st)) return rc;
     }
     return 0;
   }

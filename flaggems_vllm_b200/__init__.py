@@ -11,6 +11,7 @@ from .align import (  # noqa: F401
     moe_align_block_size_triton,
 )
 from .balance import moe_balance_loss  # noqa: F401
+from .few_tokens import MAX_FEW_TOKENS, fused_moe_few_tokens  # noqa: F401
 from .fused_moe import (  # noqa: F401
     fused_experts_impl,
     inplace_fused_experts,
@@ -40,5 +41,5 @@ __all__ = [
     "per_token_group_quant_fp8", "SUPPORTED_FP8_DTYPE", "read_status", "MoeKernelError", "topk_softmax",
     "topk_sigmoid", "router_gemm", "fp32_router_gemm", "supports_fp32_router_gemm", "router_gemm_grouped_topk",
     "silu_and_mul", "silu_and_mul_out", "rms_norm", "fused_add_rms_norm", "rms_norm_quant", "moe_balance_loss",
-    "fused_linear",
+    "fused_linear", "fused_moe_few_tokens", "MAX_FEW_TOKENS",
 ]

@@ -1,0 +1,714 @@
+// A whole layer of experts for a few tokens (up to 8) in two kernels:
+//
+//     logits = x Wr^T;  u = sigmoid(logits) or softmax(logits);  (w, ids) = group-limited top-k of u + bias (grouped_topk.cu's rule)
+//     h_e = silu(W1_e[:I] x) * (W1_e[I:] x);   out = sum_j w_j W2_e(j) h_e(j)  [+ shared expert]  [+ residual]
+//
+// What it costs is reading the weights of the routed experts once; everything else is latency.  few_router_kernel forms the
+// logits.  few_experts_kernel does the rest with one block per multiprocessor: every block routes the tokens for itself (a
+// warp per token, a few hundred bytes of logits), then the blocks share the rows of W1 of all routed experts and of the shared
+// one, and, when all of h is there, the rows of W2.
+//
+// Rows are shared out singly, so the blocks' parts are equal to one row: 8 experts of 2048 rows are 110.7 rows a block, where
+// tiles of 128 rows would be 128 tiles for 148 multiprocessors.  Weights go straight from HBM to registers, 32 bytes a lane and
+// several KB a warp in flight, and into warp-level mma.sync with 16 weight rows as M and the tokens as N = 8; the order of k inside
+// an instruction is free, so a lane's 32 bytes are contiguous.  (No tcgen05: with 8 columns the tensor core idles either way, and
+// its tiles would have to pass through shared memory.)  W1: a tile is 8 gate rows and the up rows of the same outputs, and the
+// warps of a block divide the run of (tile, k step) evenly, joining partial sums in shared memory in a fixed order.  W2: the warps
+// divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in registers.
+//
+// FP8 (128 x 128 block scales): activations in groups of 128 as per_token_group_quant_fp8 has them, h after its rounding to the
+// activations' type, as in the layer of many tokens; every 128 k are folded with both scales in fp32.
+//
+// A block waits for others once, between W1 and W2.  Work is claimed from counters, and a block waits only for work that some running
+// block has claimed: it needs no co-residency, and two calls on two streams cannot wait for each other.  The wait has the
+// library's limit.
+#include <type_traits>
+
+#include "route_row.cuh"
+#include "tc_common.cuh"
+
+namespace moe {
+namespace {
+using namespace tc;
+
+constexpr int kTokens = 8, kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kMaxSlots = 256;   // routed experts of a call: 8 tokens x 32
+constexpr int kTiles = 120;      // tiles of W1 in a block's run, at most
+constexpr int kMaxExperts = 1024, kMaxHidden = 16384;
+
+struct Few {
+  const void *x, *residual;
+  void* out;
+  const void *w1, *w2, *sw1, *sw2;              // sw: shared expert
+  const float *w1s, *w2s, *sw1s, *sw2s;         // block scales
+  const float *logits, *bias;
+  float* topk_w;
+  int32_t* topk_ids;
+  void* h;                                      // [slots][8][I], then the shared expert's [8][Is]
+  int32_t* counters;                            // claims of W1 and W2, finished runs of W1
+  int64_t x_ld, residual_ld;
+  int M, E, H, I, Is, topk, n_group, topk_group, renormalize, sigmoid;
+  float scaling;
+  int x_pitch, staged;                          // bytes of a token's row in shared memory; whether the rows are there
+  int32_t* status;
+  unsigned long long wait_ns;
+};
+
+__device__ __forceinline__ void mma8(float (&d)[4], std::integral_constant<int, 0>, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], std::integral_constant<int, 1>, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], std::integral_constant<int, 2>, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename T, bool FP8> using Kind = std::integral_constant<int, FP8 ? 2 : (std::is_same<T, __nv_bfloat16>::value ? 0 : 1)>;
+
+struct B32 {  // 32 bytes of a row
+  uint32_t r[8];
+};
+// weights are read once: past L1
+__device__ __forceinline__ void load_weights(B32& v, const void* p) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(v.r[0]), "=r"(v.r[1]), "=r"(v.r[2]), "=r"(v.r[3]), "=r"(v.r[4]), "=r"(v.r[5]), "=r"(v.r[6]), "=r"(v.r[7]) : "l"(p));
+}
+__device__ __forceinline__ void zero(B32& v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v.r[i] = 0;
+}
+__device__ __forceinline__ void load_row(B32& v, const void* p) {  // shared or global memory
+  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+  v.r[0] = a.x; v.r[1] = a.y; v.r[2] = a.z; v.r[3] = a.w; v.r[4] = b.x; v.r[5] = b.y; v.r[6] = b.z; v.r[7] = b.w;
+}
+// 16 rows (lo: this lane's row of the first eight, hi: of the others) times 8 tokens over the 128 bytes that four lanes hold
+template <typename KIND>
+__device__ __forceinline__ void multiply(float (&d)[4], const B32& lo, const B32& hi, const B32& x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mma8(d, KIND{}, lo.r[2 * j], hi.r[2 * j], lo.r[2 * j + 1], hi.r[2 * j + 1], x.r[2 * j], x.r[2 * j + 1]);
+}
+
+__device__ __forceinline__ int claim(int32_t* counter) { return atomicAdd(counter, 1); }
+
+template <typename T> __device__ __forceinline__ float2 widen2(uint32_t v);
+template <> __device__ __forceinline__ float2 widen2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+template <> __device__ __forceinline__ float2 widen2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+
+// 32 values of a lane, 128 of the four lanes of a group: their e4m3 bytes and the group's scale
+template <typename T>
+__device__ __forceinline__ float quantise(const B32 (&v)[2], B32& q) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 f = widen2<T>(v[i >> 3].r[i & 7]);
+    m = max_nan(m, max_nan(fabsf(f.x), fabsf(f.y)));
+  }
+  m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+  m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+  const float s = (m > kQuantEps || m != m ? m : kQuantEps) * (1.0f / kFp8Max), inv = 1.0f / s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 a = widen2<T>(v[i >> 2].r[2 * i & 7]), b = widen2<T>(v[i >> 2].r[(2 * i + 1) & 7]);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(div_by_scale(a.x, s, inv), div_by_scale(a.y, s, inv)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(div_by_scale(b.x, s, inv), div_by_scale(b.y, s, inv)), __NV_SATFINITE, __NV_E4M3);
+    q.r[i] = lo | hi << 16;
+  }
+  return s;
+}
+
+// ------------------------------------------------------------------ logits
+// A block per expert; the sums are formed in the order of router_gemm's row-streaming kernel, whose bits they are.
+template <typename XT, typename WT, int ROWS>
+__global__ void __launch_bounds__(128) few_router_kernel(const XT* __restrict__ x, int64_t x_ld, const WT* __restrict__ w, int M, int E, int K,
+                                                         float* __restrict__ out, int32_t* counters) {
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == 0 && threadIdx.x < 4) counters[threadIdx.x] = 0;
+  const WT* row = w + (int64_t)blockIdx.x * K;
+  float acc[ROWS] = {};
+#pragma unroll(ROWS <= 2 ? 4 : 2)
+  for (int k = threadIdx.x * 8; k < K; k += 1024) {
+    float wv[8];
+    load8<WT>(row + k, wv);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (ROWS == 1 || r < M) {
+        float xv[8];
+        load8<XT>(x + r * x_ld + k, xv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[r] = fmaf(xv[i], wv[i], acc[r]);
+      }
+    }
+  }
+  __shared__ float part[4][ROWS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    float v = acc[r];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+    if (lane == 0) part[warp][r] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < ROWS && threadIdx.x < M) {
+    float v = part[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) v += part[i][threadIdx.x];
+    out[(int64_t)threadIdx.x * E + blockIdx.x] = v;
+  }
+}
+
+// ------------------------------------------------------------------ experts
+struct Shared {
+  float weight[kMaxSlots + 1][kTokens];   // of every routed expert for every token; the shared expert's are 1
+  uint32_t mask[kMaxSlots + 1];           // tokens of the expert
+  int32_t list[kMaxSlots];                // routed experts, ascending
+  uint16_t slot[kMaxExperts];
+  float w[kTokens][32];
+  int32_t id[kTokens][32];
+  int32_t slots, next1, next2;
+};
+constexpr int kPartBytes = (kTiles + kWarps) * 512;  // partial tiles; before them the scores of the tokens, behind them those of W2
+static_assert(2 * kTokens * kMaxExperts * 4 <= kPartBytes && kWarps * 4 * 512 <= kPartBytes, "scratch");
+
+// every token's experts, by a warp each; the list of all of them
+template <int VPT>
+__device__ __forceinline__ void route(const Few& P, Shared& S, float* scratch) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < P.M) {
+    float* u = scratch + warp * P.E;
+    const float* logits = P.logits + (int64_t)warp * P.E;
+    if (P.sigmoid) {
+      for (int e = lane; e < P.E; e += 32) u[e] = (float)(1.0 / (1.0 + exp(-(double)__ldcg(logits + e))));
+    } else {
+      float m = -INFINITY;
+      for (int e = lane; e < P.E; e += 32) {
+        u[e] = __ldcg(logits + e);
+        m = fmaxf(m, u[e]);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+      double sum = 0.0;
+      for (int e = lane; e < P.E; e += 32) sum += exp((double)u[e] - (double)m);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+      for (int e = lane; e < P.E; e += 32) u[e] = (float)(exp((double)u[e] - (double)m) / sum);
+    }
+    float* none = scratch + kTokens * P.E + warp * P.E;  // no bias: zeros
+    if (P.bias == nullptr)
+      for (int e = lane; e < P.E; e += 32) none[e] = 0.0f;
+    __syncwarp();
+    route_row<float, float, VPT>(u, 1, P.bias ? P.bias : none, P.E, P.n_group, P.topk_group, P.topk, P.renormalize, P.scaling, 0, S.w[warp], S.id[warp], lane);
+  }
+  for (int e = threadIdx.x; e < P.E; e += kThreads) S.slot[e] = 0;
+  __syncthreads();
+  const int n = P.M * P.topk;
+  for (int i = threadIdx.x; i < n; i += kThreads) S.slot[S.id[i / P.topk][i % P.topk]] = 1;
+  __syncthreads();
+  if (warp == 0) {
+    int count = 0;
+    for (int e0 = 0; e0 < P.E; e0 += 32) {
+      const int e = e0 + lane;
+      const bool used = e < P.E && S.slot[e] != 0;
+      const uint32_t b = __ballot_sync(0xFFFFFFFFu, used);
+      const int at = count + __popc(b & ((1u << lane) - 1));
+      if (used) {
+        S.list[at] = e;
+        S.slot[e] = (uint16_t)at;
+        S.mask[at] = 0;
+      }
+      count += __popc(b);
+    }
+    if (lane == 0) {
+      S.slots = count;
+      S.mask[count] = (1u << P.M) - 1;
+    }
+    if (lane < kTokens) S.weight[count][lane] = 1.0f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int t = i / P.topk, j = i % P.topk, s = S.slot[S.id[t][j]];
+    S.weight[s][t] = S.w[t][j];
+    atomicOr(&S.mask[s], 1u << t);
+    if (blockIdx.x == 0) {
+      P.topk_w[i] = S.w[t][j];
+      P.topk_ids[i] = S.id[t][j];
+    }
+  }
+  __syncthreads();
+}
+
+// Rows [lo, hi) of all experts' W1, counted in outputs: routed experts one behind another, then the shared one.
+template <typename T, bool FP8>
+__device__ __forceinline__ void first_product(const Few& P, const Shared& S, const uint8_t* xrows, const float* xscale, float* part, int64_t lo, int64_t hi) {
+  constexpr int ES = FP8 ? 1 : 2, D = 4;
+  using KIND = Kind<T, FP8>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int KB = P.H * ES / 128, tiles = (int)((hi - lo + 7) / 8), total = tiles * KB;
+  const int begin = (int)((int64_t)total * warp / kWarps), end = (int)((int64_t)total * (warp + 1) / kWarps);
+  const int64_t routed = (int64_t)S.slots * P.I, row_bytes = (int64_t)P.H * ES;
+  const int sblocks = P.H / 128;
+  struct Row {
+    const uint8_t *gate, *up;
+    const float *gs, *us;  // scales of the rows' blocks
+  };
+  auto row_of = [&](int tile) {
+    Row r = {nullptr, nullptr, nullptr, nullptr};
+    const int64_t o = lo + 8 * tile + g;
+    if (o >= hi) return r;
+    int64_t p;  // output inside the expert
+    const uint8_t* base;
+    const float* scales;
+    int width;
+    if (o < routed) {
+      const int64_t s = o / P.I;
+      p = o - s * P.I;
+      const int64_t e = S.list[s];
+      width = P.I;
+      base = reinterpret_cast<const uint8_t*>(P.w1) + e * 2 * width * row_bytes;
+      scales = FP8 ? P.w1s + e * (2 * width / 128) * sblocks : nullptr;
+    } else {
+      p = o - routed;
+      width = P.Is;
+      base = reinterpret_cast<const uint8_t*>(P.sw1);
+      scales = P.sw1s;
+    }
+    r.gate = base + p * row_bytes + c * 32;
+    r.up = base + (p + width) * row_bytes + c * 32;
+    if constexpr (FP8) {
+      r.gs = scales + p / 128 * sblocks;
+      r.us = scales + (p + width) / 128 * sblocks;
+    }
+    return r;
+  };
+  B32 wg[D], wu[D];
+  float sg[D], su[D];
+  int lt = begin / KB, lk = begin - lt * KB;  // where loading stands
+  Row lr = row_of(lt);
+  auto load = [&](int d) {
+    if (lr.gate != nullptr) {
+      load_weights(wg[d], lr.gate + lk * 128);
+      load_weights(wu[d], lr.up + lk * 128);
+      if constexpr (FP8) {
+        sg[d] = __ldg(lr.gs + lk);
+        su[d] = __ldg(lr.us + lk);
+      }
+    } else {
+      zero(wg[d]);
+      zero(wu[d]);
+      sg[d] = su[d] = 0.0f;
+    }
+    if (++lk == KB) {
+      lk = 0;
+      lr = row_of(++lt);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (begin + d < end) load(d);
+  int tile = begin / KB, kb = begin - tile * KB;
+  float acc[4] = {};
+  const uint8_t* xr = xrows + (int64_t)g * P.x_pitch + c * 32;
+  for (int i = begin; i < end; i += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (i + d < end) {
+        B32 x;
+        if (g < P.M) load_row(x, xr + kb * 128);
+        else zero(x);
+        float p[4] = {};
+        multiply<KIND>(p, wg[d], wu[d], x);
+        if constexpr (FP8) {
+          const float s0 = xscale[(2 * c) * sblocks + kb], s1 = xscale[(2 * c + 1) * sblocks + kb];
+          acc[0] = fmaf(p[0], s0 * sg[d], acc[0]);
+          acc[1] = fmaf(p[1], s1 * sg[d], acc[1]);
+          acc[2] = fmaf(p[2], s0 * su[d], acc[2]);
+          acc[3] = fmaf(p[3], s1 * su[d], acc[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] += p[j];
+        }
+        if (i + d + D < end) load(d);
+        if (++kb == KB || i + d + 1 == end) {
+          reinterpret_cast<float4*>(part)[(tile + warp) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+          kb = 0;
+          ++tile;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // a tile's partial sums, one of each warp that had a part of it, in their order
+  for (int t = warp; t < tiles; t += kWarps) {
+    int w = (int)(((int64_t)t * KB * kWarps) / total);
+    while ((int64_t)total * (w + 1) / kWarps <= (int64_t)t * KB) ++w;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (; w < kWarps && (int64_t)total * w / kWarps < (int64_t)(t + 1) * KB; ++w) {
+      if ((int64_t)total * w / kWarps == (int64_t)total * (w + 1) / kWarps) continue;  // fewer steps than warps: it had none
+      const float4 q = reinterpret_cast<const float4*>(part)[(t + w) * 32 + lane];
+      v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+    }
+    const int64_t o = lo + 8 * t + g;
+    if (o < hi) {
+      T* h;
+      int64_t stride;
+      if (o < routed) {
+        const int64_t s = o / P.I;
+        stride = P.I;
+        h = reinterpret_cast<T*>(P.h) + s * kTokens * stride + (o - s * P.I);
+      } else {
+        stride = P.Is;
+        h = reinterpret_cast<T*>(P.h) + routed * kTokens + (o - routed);
+      }
+      if (2 * c < P.M) h[2 * c * stride] = from_f32<T>(silu_mul(v.x, v.z));
+      if (2 * c + 1 < P.M) h[(2 * c + 1) * stride] = from_f32<T>(silu_mul(v.y, v.w));
+    }
+  }
+}
+
+// Rows [lo, hi) of W2, at most 16 RT, of all experts, and the output columns that they are.  `wait`: returns when h is there
+template <typename T, bool FP8, int RT, typename Wait>
+__device__ __forceinline__ void second_product(const Few& P, const Shared& S, float* part, int lo, int hi, Wait wait) {
+  constexpr int ES = FP8 ? 1 : 2, D = RT == 1 ? (FP8 ? 4 : 6) : (RT == 2 ? 3 : 2), HV = FP8 ? 2 : 1;
+  using KIND = Kind<T, FP8>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int KB = P.I * ES / 128, SB = P.Is * ES / 128, routed = S.slots * KB, total = routed + SB;
+  const int begin = (int)((int64_t)total * warp / kWarps), end = (int)((int64_t)total * (warp + 1) / kWarps);
+  const int block = lo >> 7, blocks = P.H >> 7;
+  struct At {
+    int s, kb, KB;
+    const uint8_t* w;  // this lane's bytes of row lo + g
+    int64_t row;       // bytes of a row
+    const float* ws;
+    const T* h;
+  };
+  auto enter = [&](int s, int kb) {  // expert s, S.slots = the shared one
+    At a;
+    a.s = s;
+    a.kb = kb;
+    const bool shared = s == S.slots;
+    const int width = shared ? P.Is : P.I;
+    a.KB = shared ? SB : KB;
+    a.row = (int64_t)width * ES;
+    const int64_t e = shared ? 0 : S.list[s];
+    a.w = reinterpret_cast<const uint8_t*>(shared ? P.sw2 : P.w2) + (e * P.H + lo + g) * a.row + c * 32;
+    a.ws = FP8 ? (shared ? P.sw2s : P.w2s) + (e * blocks + block) * (int64_t)(width / 128) : nullptr;
+    a.h = reinterpret_cast<const T*>(P.h) + (int64_t)S.slots * kTokens * (shared ? P.I : 0) + (int64_t)(shared ? 0 : s) * kTokens * width +
+          (int64_t)g * width + c * (32 / ES);
+    return a;
+  };
+  auto locate = [&](int i) { return i < routed ? enter(i / KB, i % KB) : enter(S.slots, i - routed); };
+  auto advance = [&](At& a) {
+    if (++a.kb == a.KB && a.s < S.slots && (a.s + 1 < S.slots || SB > 0)) a = enter(a.s + 1, 0);
+  };
+  B32 w[D][RT][2], hv[D][HV];
+  float s0[D], s1[D];
+  auto load = [&](int d, const At& a) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (lo + 16 * t + 8 * j + g < hi) load_weights(w[d][t][j], a.w + (16 * t + 8 * j) * a.row + a.kb * 128);
+        else zero(w[d][t][j]);
+      }
+    if constexpr (FP8) {
+      const int width = (int)(a.row / 128);
+      s0[d] = __ldg(a.ws + a.kb);
+      s1[d] = block + 1 < blocks ? __ldg(a.ws + width + a.kb) : 0.0f;
+    }
+  };
+  auto load_h = [&](int d, const At& a) {  // written by other blocks of this kernel: not through the read-only path
+    if ((S.mask[a.s] >> g) & 1) {
+#pragma unroll
+      for (int i = 0; i < HV; ++i) load_row(hv[d][i], a.h + a.kb * (128 / ES) + 16 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < HV; ++i) zero(hv[d][i]);
+    }
+  };
+  At ld = locate(begin < total ? begin : total - 1), at = ld;
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (begin + d < end) {
+      load(d, ld);
+      advance(ld);
+    }
+  wait();
+  ld = at;
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (begin + d < end) {
+      load_h(d, ld);
+      advance(ld);
+    }
+  float acc[RT][4] = {};
+  for (int i = begin; i < end; i += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (i + d < end) {
+        const uint32_t mask = S.mask[at.s];
+        const bool r0 = (mask >> (2 * c)) & 1, r1 = (mask >> (2 * c + 1)) & 1;
+        float f0 = r0 ? S.weight[at.s][2 * c] : 0.0f, f1 = r1 ? S.weight[at.s][2 * c + 1] : 0.0f;
+        B32 x;
+        if constexpr (FP8) {
+          const float s = quantise<T>(hv[d], x);
+          f0 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c);
+          f1 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c + 4);
+        } else {
+          x = hv[d][0];
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          float p[4] = {};
+          multiply<KIND>(p, w[d][t][0], w[d][t][1], x);
+          float a0 = f0, a1 = f1, b0 = f0, b1 = f1;
+          if constexpr (FP8) {
+            const float wa = (lo + 16 * t + g) >> 7 == block ? s0[d] : s1[d], wb = (lo + 16 * t + 8 + g) >> 7 == block ? s0[d] : s1[d];
+            a0 *= wa; a1 *= wa; b0 *= wb; b1 *= wb;
+          }
+          // a token that is not the expert's takes nothing, whatever the weights hold
+          if (r0) { acc[t][0] = fmaf(p[0], a0, acc[t][0]); acc[t][2] = fmaf(p[2], b0, acc[t][2]); }
+          if (r1) { acc[t][1] = fmaf(p[1], a1, acc[t][1]); acc[t][3] = fmaf(p[3], b1, acc[t][3]); }
+        }
+        advance(at);
+        if (i + d + D < end) {
+          load(d, ld);
+          load_h(d, ld);
+          advance(ld);
+        }
+      }
+    }
+  }
+  __syncthreads();  // `part` may still be read by the first product's last part
+#pragma unroll
+  for (int t = 0; t < RT; ++t) reinterpret_cast<float4*>(part)[(warp * RT + t) * 32 + lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+  __syncthreads();
+  for (int t = warp; t < RT; t += kWarps) {
+    float v[4] = {};
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      const float4 q = reinterpret_cast<const float4*>(part)[(k * RT + t) * 32 + lane];
+      v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = lo + 16 * t + 8 * (j >> 1) + g, m = 2 * c + (j & 1);
+      if (r < hi && m < P.M) {
+        float o = v[j];
+        if (P.residual) o += ToF32<T>::get(reinterpret_cast<const T*>(P.residual)[m * P.residual_ld + r]);
+        reinterpret_cast<T*>(P.out)[(int64_t)m * P.H + r] = from_f32<T>(o);
+      }
+    }
+  }
+}
+
+template <typename T, bool FP8, int RT>
+__global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  Shared& S = *reinterpret_cast<Shared*>(smem);
+  float* part = reinterpret_cast<float*>(smem + (sizeof(Shared) + 127) / 128 * 128);
+  uint8_t* xs = reinterpret_cast<uint8_t*>(part) + kPartBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the tokens, older than the kernel in front: into shared memory, in 8 bits where the weights are
+  const uint8_t* xrows = xs;
+  float* xscale = nullptr;
+  if constexpr (FP8) {
+    const int blocks = P.H / 128;
+    xscale = reinterpret_cast<float*>(xs + P.M * P.x_pitch);
+    for (int i = threadIdx.x; i < (kTokens - P.M) * blocks; i += kThreads) xscale[P.M * blocks + i] = 0.0f;
+    const int groups = P.M * blocks;  // eight of them to a warp, four lanes each
+    for (int i0 = warp * 8; i0 < groups; i0 += 8 * kWarps) {
+      const int i = i0 + (lane >> 2), m = i / blocks, b = i - m * blocks;
+      B32 v[2], q;
+      zero(v[0]);
+      zero(v[1]);
+      if (i < groups) {
+        const T* p = reinterpret_cast<const T*>(P.x) + m * P.x_ld + b * 128 + (lane & 3) * 32;
+        load_row(v[0], p);
+        load_row(v[1], p + 16);
+      }
+      const float s = quantise<T>(v, q);
+      if (i < groups) {
+        uint4* d = reinterpret_cast<uint4*>(xs + m * P.x_pitch + b * 128 + (lane & 3) * 32);
+        d[0] = make_uint4(q.r[0], q.r[1], q.r[2], q.r[3]);
+        d[1] = make_uint4(q.r[4], q.r[5], q.r[6], q.r[7]);
+        if ((lane & 3) == 0) xscale[i] = s;
+      }
+    }
+  } else if (P.staged) {
+    const int pieces = P.H / 8;
+    for (int i = threadIdx.x; i < P.M * pieces; i += kThreads) {
+      const int m = i / pieces, k = i - m * pieces;
+      *reinterpret_cast<uint4*>(xs + m * P.x_pitch + k * 16) = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.x) + m * P.x_ld + k * 8);
+    }
+  } else {
+    xrows = reinterpret_cast<const uint8_t*>(P.x);
+  }
+  pdl_wait();  // logits and cleared counters
+  pdl_trigger();
+  int mine1 = 0, mine2 = 0;  // thread 0: claimed, not begun
+  if (threadIdx.x == 0) {
+    mine1 = claim(P.counters);
+    mine2 = claim(P.counters + 1);
+  }
+  if (P.E <= 256) route<8>(P, S, part);
+  else route<32>(P, S, part);
+
+  const int64_t outputs = (int64_t)S.slots * P.I + P.Is;
+  const int G = gridDim.x;
+  const int64_t runs1 = (outputs + (int64_t)G * kTiles * 8 - 1) / ((int64_t)G * kTiles * 8) * G;
+  for (;;) {
+    if (threadIdx.x == 0) S.next1 = mine1;
+    __syncthreads();
+    const int run = S.next1;
+    if (run >= runs1) break;
+    if (threadIdx.x == 0) mine1 = claim(P.counters);
+    first_product<T, FP8>(P, S, xrows, xscale, part, outputs * run / runs1, outputs * (run + 1) / runs1);
+    __syncthreads();  // all of the run's h is written
+    if (threadIdx.x == 0) {
+      __threadfence();
+      atomicAdd(P.counters + 2, 1);
+    }
+  }
+  bool waited = false;
+  auto wait = [&] {
+    if (waited) return;
+    waited = true;
+    if (threadIdx.x == 0) {
+      unsigned long long t0 = 0;
+      for (uint32_t spins = 1;; ++spins) {
+        int done;
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(P.counters + 2) : "memory");
+        if (done >= runs1) break;
+        if ((spins & 0x3F) == 0 && wait_expired(t0, P.status, P.wait_ns)) break;  // goes on, on whatever is there
+      }
+    }
+    __syncthreads();
+  };
+  const int runs2 = (P.H + 16 * RT - 1) / (16 * RT) > G ? (P.H + 16 * RT - 1) / (16 * RT) : G;
+  for (;;) {
+    if (threadIdx.x == 0) S.next2 = mine2;
+    __syncthreads();
+    const int run = S.next2;
+    if (run >= runs2) break;
+    if (threadIdx.x == 0) mine2 = claim(P.counters + 1);
+    second_product<T, FP8, RT>(P, S, part, (int)((int64_t)P.H * run / runs2), (int)((int64_t)P.H * (run + 1) / runs2), wait);
+  }
+}
+
+static_assert((sizeof(Shared) + 127) / 128 * 128 + kPartBytes + kTokens * (kMaxHidden + 16) + kTokens * (kMaxHidden / 128) * 4 <= 232448,
+              "8-bit tokens fit shared memory");
+
+// ------------------------------------------------------------------ host side
+struct Layout {
+  int64_t logits, h, bytes;  // counters in front
+};
+Layout layout(int64_t M, int E, int64_t I, int64_t Is, int topk) {
+  auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+  Layout l;
+  const int64_t slots = M * topk < E ? M * topk : E;
+  l.logits = 256;
+  l.h = l.logits + up(M * E * 4);
+  l.bytes = l.h + up((slots * I + Is) * kTokens * 2);
+  return l;
+}
+
+template <typename XT, typename WT>
+int run_router(const Few& P, const void* w, cudaStream_t st) {
+#define MOE_FEW_ROUTER(ROWS)                                                                                                             \
+  launch_pdl(few_router_kernel<XT, WT, ROWS>, dim3((unsigned)P.E), 128, 0, 1, st, "fused_moe_few_tokens (router)", (const XT*)P.x, P.x_ld, \
+             (const WT*)w, P.M, P.E, P.H, const_cast<float*>(P.logits), P.counters)
+  if (P.M == 1) return MOE_FEW_ROUTER(1);
+  if (P.M == 2) return MOE_FEW_ROUTER(2);
+  if (P.M <= 4) return MOE_FEW_ROUTER(4);
+  return MOE_FEW_ROUTER(8);
+#undef MOE_FEW_ROUTER
+}
+
+template <typename T, bool FP8>
+int run_experts(Few P, cudaStream_t st) {
+  constexpr int64_t head = (sizeof(Shared) + 127) / 128 * 128 + kPartBytes;
+  P.x_pitch = P.H * (FP8 ? 1 : 2) + 16;  // neighbouring tokens' pieces lie in other banks
+  int64_t smem = head + (int64_t)P.M * P.x_pitch + (FP8 ? kTokens * (P.H / 128) * 4 : 0);
+  P.staged = smem <= 232448;
+  if (!P.staged) {
+    if (FP8) return fail(MOE_E_TOOBIG, "fused_moe_few_tokens: %d tokens of %d elements do not fit shared memory", P.M, P.H);  // kMaxHidden lets none
+    smem = head;  // the rows then come out of L1
+    P.x_pitch = (int)(P.x_ld * 2);
+  }
+  const int G = sm_count();
+  const int rows = (P.H + G - 1) / G;
+  auto go = [&](auto rt) {
+    auto kern = few_experts_kernel<T, FP8, decltype(rt)::value>;
+    const int rc = allow_smem((const void*)kern, 232448);
+    if (rc) return rc;
+    return launch_pdl(kern, dim3((unsigned)G), kThreads, (size_t)smem, 1, st, "fused_moe_few_tokens", P);
+  };
+  if (rows <= 16) return go(std::integral_constant<int, 1>());
+  if (rows <= 32) return go(std::integral_constant<int, 2>());
+  return go(std::integral_constant<int, 4>());
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_few_tokens_workspace(int64_t M, int E, int64_t I, int64_t shared_I, int topk, int64_t* bytes) {
+  using namespace moe;
+  if (M < 0 || M > kTokens || E <= 0 || E > kMaxExperts || I <= 0 || shared_I < 0 || topk <= 0 || topk > 32 || !bytes)
+    return fail(MOE_E_BADARG, "few_tokens_workspace: bad extent");
+  *bytes = layout(M, E, I, shared_I, topk).bytes;
+  return 0;
+}
+
+extern "C" int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void* router, int router_dtype, const float* bias, const void* w1,
+                              const void* w2, const float* w1_scale, const float* w2_scale, const void* shared_w1, const void* shared_w2,
+                              const float* shared_w1_scale, const float* shared_w2_scale, const void* residual, int64_t residual_ld, int64_t M,
+                              int E, int H, int I, int shared_I, int topk, int n_group, int topk_group, int renormalize, float scaling,
+                              int sigmoid, void* out, float* topk_weights, int32_t* topk_ids, void* workspace, int64_t workspace_bytes,
+                              int32_t* status, void* stream) {
+  using namespace moe;
+  const char* who = "fused_moe_few_tokens";
+  if (dtype != MOE_BF16 && dtype != MOE_F16) return fail(MOE_E_DTYPE, "%s: activations are bf16 or f16", who);
+  if (router_dtype != dtype && router_dtype != MOE_F32) return fail(MOE_E_DTYPE, "%s: the router's weights have the activations' type or fp32", who);
+  if (M < 0 || M > kTokens) return fail(MOE_E_TOOBIG, "%s: at most %d tokens", who, kTokens);
+  if (M == 0) return 0;
+  const bool fp8 = w1_scale != nullptr;
+  const int unit = fp8 ? 128 : 64;
+  if (E <= 0 || E > kMaxExperts || H <= 0 || H > kMaxHidden || I <= 0 || shared_I < 0 || H % unit || I % unit || shared_I % unit)
+    return fail(MOE_E_SHAPE, "%s: at most %d experts, hidden sizes up to %d; sizes in multiples of %d", who, kMaxExperts, kMaxHidden, unit);
+  if (topk <= 0 || topk > 32 || topk > E || n_group <= 0 || n_group > 32 || E % n_group || topk_group <= 0 || topk_group > n_group ||
+      (int64_t)topk > (int64_t)E / n_group * topk_group)
+    return fail(MOE_E_SHAPE, "%s: groups and topk do not fit the experts", who);
+  if (!x || !router || !w1 || !w2 || !out || !topk_weights || !topk_ids || !workspace || (shared_I > 0) != (shared_w1 != nullptr) ||
+      (shared_I > 0) != (shared_w2 != nullptr) || fp8 != (w2_scale != nullptr) || (fp8 && shared_I > 0 && (!shared_w1_scale || !shared_w2_scale)))
+    return fail(MOE_E_BADARG, "%s: null pointer", who);
+  if (x_ld < H || x_ld % 8 || (residual && residual_ld < H)) return fail(MOE_E_SHAPE, "%s: rows of x in whole 16-byte pieces", who);
+  for (const void* p : {w1, w2, shared_w1, shared_w2})
+    if ((uintptr_t)p & 31) return fail(MOE_E_BADARG, "%s: weights must be 32-byte aligned", who);
+  for (const void* p : {x, router, (const void*)workspace})
+    if ((uintptr_t)p & 15) return fail(MOE_E_BADARG, "%s: operands must be 16-byte aligned", who);
+  const Layout l = layout(M, E, I, shared_I, topk);
+  if (workspace_bytes < l.bytes) return fail(MOE_E_BADARG, "%s: workspace too small", who);
+  uint8_t* ws = (uint8_t*)workspace;
+  Few P = {};
+  P.x = x; P.x_ld = x_ld; P.residual = residual; P.residual_ld = residual_ld; P.out = out;
+  P.w1 = w1; P.w2 = w2; P.sw1 = shared_w1; P.sw2 = shared_w2;
+  P.w1s = w1_scale; P.w2s = w2_scale; P.sw1s = shared_w1_scale; P.sw2s = shared_w2_scale;
+  P.logits = (const float*)(ws + l.logits); P.bias = bias;
+  P.topk_w = topk_weights; P.topk_ids = topk_ids;
+  P.h = ws + l.h; P.counters = (int32_t*)ws;
+  P.M = (int)M; P.E = E; P.H = H; P.I = I; P.Is = shared_I; P.topk = topk; P.n_group = n_group; P.topk_group = topk_group;
+  P.renormalize = renormalize; P.sigmoid = sigmoid; P.scaling = scaling;
+  P.status = status; P.wait_ns = wait_limit_ns();
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool f32 = router_dtype == MOE_F32;
+  int rc = dtype == MOE_BF16 ? (f32 ? run_router<__nv_bfloat16, float>(P, router, st) : run_router<__nv_bfloat16, __nv_bfloat16>(P, router, st))
+                             : (f32 ? run_router<__half, float>(P, router, st) : run_router<__half, __half>(P, router, st));
+  if (rc) return rc;
+  if (dtype == MOE_BF16) return fp8 ? run_experts<__nv_bfloat16, true>(P, st) : run_experts<__nv_bfloat16, false>(P, st);
+  return fp8 ? run_experts<__half, true>(P, st) : run_experts<__half, false>(P, st);
+}

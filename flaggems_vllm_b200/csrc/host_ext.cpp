@@ -892,6 +892,83 @@ PyObject* fused_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(y);
 }
 
+// few_tokens(x, router, w1, w2, topk, renormalize, sigmoid, n_group, topk_group, scaling, bias, w1_scale, w2_scale, shared_w1, shared_w2,
+//   shared_w1_scale, shared_w2_scale, residual) -> (out, topk_weights, topk_ids)
+PyObject* few_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 18) MOE_NONE;
+  long long topk, n_group, topk_group;
+  double scaling;
+  for (int i = 0; i < 4; ++i)
+    if (!is_tensor(a[i])) MOE_NONE;
+  for (int i = 10; i < 18; ++i)
+    if (a[i] != Py_None && !is_tensor(a[i])) MOE_NONE;
+  if (!as_int(a[4], &topk) || !plain_bool(a[5]) || !plain_bool(a[6]) || !as_int(a[7], &n_group) || !as_int(a[8], &topk_group) ||
+      !as_double(a[9], &scaling))
+    MOE_NONE;
+  const at::Tensor &x = tensor(a[0]), &router = tensor(a[1]), &w1 = tensor(a[2]), &w2 = tensor(a[3]);
+  auto opt = [&](int i) { return a[i] == Py_None ? nullptr : &tensor(a[i]); };
+  const at::Tensor *bias = opt(10), *s1 = opt(11), *s2 = opt(12), *w1x = opt(13), *w2x = opt(14), *s1x = opt(15), *s2x = opt(16), *res = opt(17);
+  no_tangent({&x, &router, &w1, &w2, bias, w1x, w2x, res}, "fused_moe_few_tokens");
+  if (wants_grad({&x, &router, &w1, &w2, bias, s1, s2, w1x, w2x, s1x, s2x, res})) MOE_NONE;  // refused by the Python operator
+  if (!x.is_cuda() || x.dim() != 2 || router.dim() != 2 || w1.dim() != 3 || w2.dim() != 3) MOE_NONE;
+  const int dev = x.get_device(), code = float_code(x), router_code = float_code(router);
+  int32_t* status = status_of(dev);
+  const int64_t M = x.size(0), H = x.size(1), E = router.size(0), I = w2.size(2), Is = w2x ? (w2x->dim() == 2 ? w2x->size(1) : -1) : 0;
+  const bool fp8 = s1 != nullptr;
+  const auto type = fp8 ? at::kFloat8_e4m3fn : x.scalar_type();
+  const int64_t unit = fp8 ? 128 : 64;
+  if (!status || (code != MOE_BF16 && code != MOE_F16) || (router_code != code && router_code != MOE_F32) || M > 8 || M <= 0 || H <= 0 || E <= 0 ||
+      E > 1024 || I <= 0 || Is < 0 || H % unit || I % unit || Is % unit || H > 16384 || I > (1 << 24) || Is > (1 << 24) || topk <= 0 ||
+      topk > 32 || topk > E || n_group <= 0 || n_group > 32 || E % n_group || topk_group <= 0 || topk_group > n_group ||
+      topk > E / n_group * topk_group || !(scaling > -3e38 && scaling < 3e38) || (w1x != nullptr) != (w2x != nullptr) || (s2 != nullptr) != fp8 ||
+      (s1x != nullptr) != (fp8 && w1x) || (s2x != nullptr) != (fp8 && w1x))
+    MOE_NONE;
+  auto dense = [&](const at::Tensor* t, at::ScalarType ty, at::IntArrayRef sizes) {
+    return !t || (cuda_dense(*t, dev) && t->scalar_type() == ty && t->sizes().equals(sizes));
+  };
+  if (!dense(&router, router.scalar_type(), {E, H}) || !dense(&w1, type, {E, 2 * I, H}) || !dense(&w2, type, {E, H, I}) ||
+      !dense(w1x, type, {2 * Is, H}) || !dense(w2x, type, {H, Is}) || !dense(bias, at::kFloat, {E}) ||
+      !dense(s1, at::kFloat, {E, 2 * I / 128, H / 128}) || !dense(s2, at::kFloat, {E, H / 128, I / 128}) ||
+      !dense(s1x, at::kFloat, {2 * Is / 128, H / 128}) || !dense(s2x, at::kFloat, {H / 128, Is / 128}))
+    MOE_NONE;
+  auto at16 = [](const at::Tensor& t) { return ((uintptr_t)t.const_data_ptr() & 15) == 0; };
+  for (const at::Tensor* t : {&w1, &w2, w1x, w2x})
+    if (t && ((uintptr_t)t->const_data_ptr() & 31)) MOE_NONE;
+  int64_t rows, x_ld, res_ld = 0;
+  if (!rows_of(x, &rows, &x_ld) || !at16(x) || !at16(router)) MOE_NONE;
+  if (M == 1) x_ld = H;
+  if (x_ld < H || x_ld % 8) MOE_NONE;
+  if (res) {
+    if (!res->is_cuda() || res->get_device() != dev || res->scalar_type() != x.scalar_type() || !res->sizes().equals(x.sizes()) ||
+        !rows_of(*res, &rows, &res_ld))
+      MOE_NONE;
+    if (M == 1) res_ld = H;
+    if (res_ld < H) MOE_NONE;
+  }
+  at::Tensor out, tw, ti;
+  {
+    Unlocked unlocked;
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    int64_t bytes = 0;
+    must(moe_few_tokens_workspace(M, (int)E, I, Is, (int)topk, &bytes));
+    out = fresh({M, H}, x.scalar_type(), dev);
+    tw = fresh({M, topk}, at::kFloat, dev);
+    ti = fresh({M, topk}, at::kInt, dev);
+    at::Tensor ws = fresh({bytes}, at::kByte, dev);
+    auto ptr = [](const at::Tensor* t) { return t ? t->const_data_ptr() : nullptr; };
+    must(moe_few_tokens(x.const_data_ptr(), x_ld, code, router.const_data_ptr(), router_code, (const float*)ptr(bias), w1.const_data_ptr(),
+                        w2.const_data_ptr(), (const float*)ptr(s1), (const float*)ptr(s2), ptr(w1x), ptr(w2x), (const float*)ptr(s1x),
+                        (const float*)ptr(s2x), ptr(res), res_ld, M, (int)E, (int)H, (int)I, (int)Is, (int)topk, (int)n_group, (int)topk_group,
+                        truth(a[5]), (float)scaling, truth(a[6]), out.mutable_data_ptr(), tw.mutable_data_ptr<float>(), ti.mutable_data_ptr<int32_t>(),
+                        ws.mutable_data_ptr(), bytes, status, stream_on(dev)));
+  }
+  PyObject* r = PyTuple_New(3);
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(tw));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(ti));
+  return r;
+}
+
 // Exceptions of the operators above become Python's: a failed launch MoeKernelError, torch's own as torch raises them.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* raising(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -919,7 +996,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 #define MOE_OP(name) {#name, (PyCFunction)(void (*)(void))raising<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MOE_FN(set_status), MOE_FN(fused_experts), MOE_FN(grouped_topk), MOE_FN(topk_route),
                          MOE_FN(router_gemm), MOE_FN(align), MOE_FN(set_error), MOE_OP(word_beside_capture), MOE_OP(rms_norm), MOE_OP(fused_add_rms_norm),
-                         MOE_OP(rms_norm_quant), MOE_OP(balance_loss), MOE_OP(fused_linear), {nullptr, nullptr, 0, nullptr}};
+                         MOE_OP(rms_norm_quant), MOE_OP(balance_loss), MOE_OP(fused_linear), MOE_OP(few_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ext", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

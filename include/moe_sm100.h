@@ -534,6 +534,22 @@ int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld, const voi
                           int dtype, int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* db, int db_dtype,
                           void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
+/* A whole layer of experts for up to 8 tokens, in two launches (no counterpart in the reference, which runs the operators one
+ * behind another):  logits = x router^T;  u = sigmoid(logits) or softmax;  group-limited top-k of u + bias as moe_grouped_topk;
+ * out = sum_j weight_j w2[id_j] (silu(w1[id_j][:I] x) * (w1[id_j][I:] x)) [+ the same of the shared expert] [+ residual], rounded once.
+ * x, residual [M, H] bf16 / f16, rows their ld apart (x: a multiple of 8); router [E, H] in dtype or fp32; bias [E] fp32 or null;
+ * w1 [E, 2I, H], w2 [E, H, I], shared_w1 [2 shared_I, H], shared_w2 [H, shared_I] in dtype, or, where the scales are given (fp32,
+ * [E, 2I/128, H/128] and so on), e4m3: x and the intermediate are then taken in e4m3 too, in groups of 128.  shared_I = 0: none.
+ * Sizes in multiples of 64, in e4m3 128; at most 1024 experts, topk 32.  Weights 32-byte aligned.  out [M, H], topk_weights fp32 and
+ * topk_ids int32 [M, topk] without gaps.  out shares no memory with an operand. */
+int moe_few_tokens_workspace(int64_t M, int E, int64_t I, int64_t shared_I, int topk, int64_t* bytes /* host */);
+int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void* router, int router_dtype, const float* bias, const void* w1,
+                   const void* w2, const float* w1_scale, const float* w2_scale, const void* shared_w1, const void* shared_w2,
+                   const float* shared_w1_scale, const float* shared_w2_scale, const void* residual, int64_t residual_ld, int64_t M,
+                   int E, int H, int I, int shared_I, int topk, int n_group, int topk_group, int renormalize, float scaling,
+                   int sigmoid, void* out, float* topk_weights, int32_t* topk_ids, void* workspace, int64_t workspace_bytes,
+                   int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,12 +9,12 @@
 // one, and, when all of h is there, the rows of W2.
 //
 // Rows are shared out singly, so the blocks' parts are equal to one row: 8 experts of 2048 rows are 110.7 rows a block, where
-// tiles of 128 rows would be 128 tiles for 148 multiprocessors.  Weights go straight from HBM to registers, 32 bytes a lane and
-// several KB a warp in flight, and into warp-level mma.sync with 16 weight rows as M and the tokens as N = 8; the order of k inside
-// an instruction is free, so a lane's 32 bytes are contiguous.  (No tcgen05: with 8 columns the tensor core idles either way, and
-// its tiles would have to pass through shared memory.)  W1: a tile is 8 gate rows and the up rows of the same outputs, and the
-// warps of a block divide the run of (tile, k step) evenly, joining partial sums in shared memory in a fixed order.  W2: the warps
-// divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in registers.
+// tiles of 128 rows would be 128 tiles for 148 multiprocessors.  Every warp copies its rows asynchronously
+// into a ring of its own in shared memory, in whole lines, 12 KB a warp and 96 KB a multiprocessor in flight, and feeds warp-level mma.sync with 16 weight rows as M and the tokens as N = 8.
+// The order of k inside an instruction is free, so a lane's operand is whole 16-byte pieces of a row.
+// (No tcgen05: with 8 columns the tensor core idles either way.)  W1: a tile is 8 gate rows and the up rows of the same outputs,
+// and the warps of a block divide the run of (tile, k step) evenly, joining the tiles that they share in a fixed order.  W2: the
+// warps divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in registers.
 //
 // FP8 (128 x 128 block scales): activations in groups of 128 as per_token_group_quant_fp8 has them, h after its rounding to the
 // activations' type, as in the layer of many tokens; every 128 k are folded with both scales in fp32.
@@ -33,8 +33,8 @@ using namespace tc;
 
 constexpr int kTokens = 8, kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxSlots = 256;   // routed experts of a call: 8 tokens x 32
-constexpr int kTiles = 120;      // tiles of W1 in a block's run, at most
-constexpr int kMaxExperts = 1024, kMaxHidden = 16384;
+constexpr int kRunTiles = 4096;  // tiles of W1 in a block's run, at most
+constexpr int kMaxExperts = 1024, kMaxHidden = 16384, kMaxHidden8 = 8192, kMaxWidth = 1 << 22;
 
 struct Few {
   const void *x, *residual;
@@ -71,17 +71,14 @@ template <typename T, bool FP8> using Kind = std::integral_constant<int, FP8 ? 2
 struct B32 {  // 32 bytes of a row
   uint32_t r[8];
 };
-// weights are read once: past L1
-__device__ __forceinline__ void load_weights(B32& v, const void* p) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-      : "=r"(v.r[0]), "=r"(v.r[1]), "=r"(v.r[2]), "=r"(v.r[3]), "=r"(v.r[4]), "=r"(v.r[5]), "=r"(v.r[6]), "=r"(v.r[7]) : "l"(p));
-}
 __device__ __forceinline__ void zero(B32& v) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v.r[i] = 0;
 }
-__device__ __forceinline__ void load_row(B32& v, const void* p) {  // shared or global memory
-  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+// 16 bytes from p on and 16 from p + APART on, in shared or global memory
+template <int APART>
+__device__ __forceinline__ void load_row(B32& v, const void* p) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + APART);
   v.r[0] = a.x; v.r[1] = a.y; v.r[2] = a.z; v.r[3] = a.w; v.r[4] = b.x; v.r[5] = b.y; v.r[6] = b.z; v.r[7] = b.w;
 }
 // 16 rows (lo: this lane's row of the first eight, hi: of the others) times 8 tokens over the 128 bytes that four lanes hold
@@ -89,6 +86,29 @@ template <typename KIND>
 __device__ __forceinline__ void multiply(float (&d)[4], const B32& lo, const B32& hi, const B32& x) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) mma8(d, KIND{}, lo.r[2 * j], hi.r[2 * j], lo.r[2 * j + 1], hi.r[2 * j + 1], x.r[2 * j], x.r[2 * j + 1]);
+}
+
+// A slot holds rows of 128 bytes in pieces of 16; those of odd rows change halves, so that the eight lanes that read together (four
+// pieces of two neighbouring rows) meet in no bank.  Lane 8 r + q copies piece q of rows r, r + 4, ..: whole lines.
+__device__ __forceinline__ uint32_t place(int row, int piece) { return (uint32_t)(row * 128 + (piece ^ (row & 1) * 4) * 16); }
+__device__ __forceinline__ void copy16(uint32_t at, const void* p) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(at), "l"(p) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t at, const void* p) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(p) : "memory");
+}
+__device__ __forceinline__ void take16(uint32_t* r, uint32_t at) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// pieces c and c + 4 of a row: what lane (row, c) multiplies
+__device__ __forceinline__ void take(B32& v, uint32_t slot, int row, int c) {
+  take16(v.r, slot + place(row, c));
+  take16(v.r + 4, slot + place(row, c + 4));
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING> __device__ __forceinline__ void wait_copies() {  // of all lanes
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+  __syncwarp();
 }
 
 __device__ __forceinline__ int claim(int32_t* counter) { return atomicAdd(counter, 1); }
@@ -171,8 +191,16 @@ struct Shared {
   int32_t id[kTokens][32];
   int32_t slots, next1, next2;
 };
-constexpr int kPartBytes = (kTiles + kWarps) * 512;  // partial tiles; before them the scores of the tokens, behind them those of W2
-static_assert(2 * kTokens * kMaxExperts * 4 <= kPartBytes && kWarps * 4 * 512 <= kPartBytes, "scratch");
+constexpr int kPartBytes = kWarps * 4 * 512;  // partial sums: two tiles of W1 a warp, four of W2
+// W1's ring: a unit is a tile's 128 bytes of k, 2 KB, and in 8 bits its scales
+template <bool FP8> struct Ring1 {
+  static constexpr int UNITS = 7, SLOT = 2048 + (FP8 ? 64 : 0), BYTES = UNITS * SLOT;
+};
+// W2's: a unit is 16 rows' 128 bytes of k; a step's h (and scales) come with its first unit.  As many as fit
+template <bool FP8, int RT> struct Ring2 {
+  static constexpr int UNITS = RT == 1 ? (FP8 ? 5 : 7) : (RT == 2 && FP8 ? 6 : 8), STEPS = (UNITS + RT - 1) / RT + 1;
+  static constexpr int H_SLOT = FP8 ? 2048 + 16 : 1024, BYTES = UNITS * 2048 + STEPS * H_SLOT;
+};
 
 // every token's experts, by a warp each; the list of all of them
 template <int VPT>
@@ -243,29 +271,35 @@ __device__ __forceinline__ void route(const Few& P, Shared& S, float* scratch) {
 
 // Rows [lo, hi) of all experts' W1, counted in outputs: routed experts one behind another, then the shared one.
 template <typename T, bool FP8>
-__device__ __forceinline__ void first_product(const Few& P, const Shared& S, const uint8_t* xrows, const float* xscale, float* part, int64_t lo, int64_t hi) {
-  constexpr int ES = FP8 ? 1 : 2, D = 4;
+__device__ __forceinline__ void first_product(const Few& P, const Shared& S, const uint8_t* xrows, const float* xscale, float* part, uint32_t ring,
+                                              int64_t lo, int64_t hi) {
+  using R = Ring1<FP8>;
+  constexpr int ES = FP8 ? 1 : 2;
   using KIND = Kind<T, FP8>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int KB = P.H * ES / 128, tiles = (int)((hi - lo + 7) / 8), total = tiles * KB;
-  const int begin = (int)((int64_t)total * warp / kWarps), end = (int)((int64_t)total * (warp + 1) / kWarps);
+  auto bound = [&](int w) { return (int)((int64_t)total * w / kWarps); };
+  const int begin = bound(warp), end = bound(warp + 1);
   const int64_t routed = (int64_t)S.slots * P.I, row_bytes = (int64_t)P.H * ES;
   const int sblocks = P.H / 128;
+  ring += (uint32_t)warp * R::BYTES;
+  const int cr = lane >> 3, cq = lane & 7;  // what this lane copies: piece cq of rows cr and cr + 4
+  // output o of all experts': its gate row, and how far behind it the up row is
   struct Row {
-    const uint8_t *gate, *up;
+    const uint8_t* gate;
+    int64_t up;
     const float *gs, *us;  // scales of the rows' blocks
   };
-  auto row_of = [&](int tile) {
-    Row r = {nullptr, nullptr, nullptr, nullptr};
-    const int64_t o = lo + 8 * tile + g;
+  auto row_of = [&](int64_t o) {
+    Row r = {nullptr, 0, nullptr, nullptr};
     if (o >= hi) return r;
     int64_t p;  // output inside the expert
     const uint8_t* base;
     const float* scales;
     int width;
     if (o < routed) {
-      const int64_t s = o / P.I;
-      p = o - s * P.I;
+      const int s = (int)((uint32_t)o / (uint32_t)P.I);
+      p = o - (int64_t)s * P.I;
       const int64_t e = S.list[s];
       width = P.I;
       base = reinterpret_cast<const uint8_t*>(P.w1) + e * 2 * width * row_bytes;
@@ -276,90 +310,61 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
       base = reinterpret_cast<const uint8_t*>(P.sw1);
       scales = P.sw1s;
     }
-    r.gate = base + p * row_bytes + c * 32;
-    r.up = base + (p + width) * row_bytes + c * 32;
+    r.gate = base + p * row_bytes;
+    r.up = width * row_bytes;
     if constexpr (FP8) {
       r.gs = scales + p / 128 * sblocks;
       r.us = scales + (p + width) / 128 * sblocks;
     }
     return r;
   };
-  B32 wg[D], wu[D];
-  float sg[D], su[D];
-  int lt = begin / KB, lk = begin - lt * KB;  // where loading stands
-  Row lr = row_of(lt);
-  auto load = [&](int d) {
-    if (lr.gate != nullptr) {
-      load_weights(wg[d], lr.gate + lk * 128);
-      load_weights(wu[d], lr.up + lk * 128);
-      if constexpr (FP8) {
-        sg[d] = __ldg(lr.gs + lk);
-        su[d] = __ldg(lr.us + lk);
-      }
-    } else {
-      zero(wg[d]);
-      zero(wu[d]);
-      sg[d] = su[d] = 0.0f;
+  int lt = begin / KB, lk = begin - lt * KB;  // where copying stands
+  const uint8_t* src[2];
+  int64_t up[2];
+  const float* scale = nullptr;
+  auto enter = [&] {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const Row r = row_of(lo + 8 * (int64_t)lt + cr + 4 * j);
+      src[j] = r.gate;
+      up[j] = r.up;
     }
-    if (++lk == KB) {
-      lk = 0;
-      lr = row_of(++lt);
+    if constexpr (FP8) {  // lanes 0 to 15: of the eight gate and the eight up rows
+      const Row r = row_of(lo + 8 * (int64_t)lt + cq);
+      scale = lane < 8 ? r.gs : (lane < 16 ? r.us : nullptr);
     }
   };
+  enter();
+  auto copy = [&](uint32_t slot) {
 #pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (begin + d < end) load(d);
-  int tile = begin / KB, kb = begin - tile * KB;
-  float acc[4] = {};
-  const uint8_t* xr = xrows + (int64_t)g * P.x_pitch + c * 32;
-  for (int i = begin; i < end; i += D) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (i + d < end) {
-        B32 x;
-        if (g < P.M) load_row(x, xr + kb * 128);
-        else zero(x);
-        float p[4] = {};
-        multiply<KIND>(p, wg[d], wu[d], x);
-        if constexpr (FP8) {
-          const float s0 = xscale[(2 * c) * sblocks + kb], s1 = xscale[(2 * c + 1) * sblocks + kb];
-          acc[0] = fmaf(p[0], s0 * sg[d], acc[0]);
-          acc[1] = fmaf(p[1], s1 * sg[d], acc[1]);
-          acc[2] = fmaf(p[2], s0 * su[d], acc[2]);
-          acc[3] = fmaf(p[3], s1 * su[d], acc[3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] += p[j];
-        }
-        if (i + d + D < end) load(d);
-        if (++kb == KB || i + d + 1 == end) {
-          reinterpret_cast<float4*>(part)[(tile + warp) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-          acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-          kb = 0;
-          ++tile;
-        }
+    for (int j = 0; j < 2; ++j) {
+      if (src[j] != nullptr) {  // rows that are not there leave the slot as it was, and nobody looks at their outputs
+        const uint8_t* p = src[j] + lk * 128 + cq * 16;
+        copy16(slot + place(cr + 4 * j, cq), p);
+        copy16(slot + 1024 + place(cr + 4 * j, cq), p + up[j]);
       }
     }
-  }
-  __syncthreads();
-  // a tile's partial sums, one of each warp that had a part of it, in their order
-  for (int t = warp; t < tiles; t += kWarps) {
-    int w = (int)(((int64_t)t * KB * kWarps) / total);
-    while ((int64_t)total * (w + 1) / kWarps <= (int64_t)t * KB) ++w;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (; w < kWarps && (int64_t)total * w / kWarps < (int64_t)(t + 1) * KB; ++w) {
-      if ((int64_t)total * w / kWarps == (int64_t)total * (w + 1) / kWarps) continue;  // fewer steps than warps: it had none
-      const float4 q = reinterpret_cast<const float4*>(part)[(t + w) * 32 + lane];
-      v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+    if (FP8 && scale != nullptr) copy4(slot + 2048 + lane * 4, scale + lk);
+    if (++lk == KB) {
+      lk = 0;
+      ++lt;
+      enter();
     }
-    const int64_t o = lo + 8 * t + g;
+  };
+#pragma unroll 1
+  for (int d = 0; d < R::UNITS - 1; ++d) {
+    if (begin + d < end) copy(ring + d * R::SLOT);
+    commit_copies();
+  }
+  auto finish = [&](int tile, const float4& v) {
+    const int64_t o = lo + 8 * (int64_t)tile + g;
     if (o < hi) {
       T* h;
       int64_t stride;
       if (o < routed) {
-        const int64_t s = o / P.I;
+        const int s = (int)((uint32_t)o / (uint32_t)P.I);
         stride = P.I;
-        h = reinterpret_cast<T*>(P.h) + s * kTokens * stride + (o - s * P.I);
+        h = reinterpret_cast<T*>(P.h) + s * kTokens * stride + (o - s * stride);
       } else {
         stride = P.Is;
         h = reinterpret_cast<T*>(P.h) + routed * kTokens + (o - routed);
@@ -367,25 +372,85 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
       if (2 * c < P.M) h[2 * c * stride] = from_f32<T>(silu_mul(v.x, v.z));
       if (2 * c + 1 < P.M) h[(2 * c + 1) * stride] = from_f32<T>(silu_mul(v.y, v.w));
     }
+  };
+  int tile = begin / KB, kb = begin - tile * KB;
+  int to = R::UNITS - 1, at = 0;  // slots
+  float acc[4] = {};
+  const uint8_t* xr = xrows + (int64_t)g * P.x_pitch + c * 16;
+#pragma unroll 1
+  for (int i = begin; i < end; ++i) {
+    wait_copies<R::UNITS - 2>();
+    if (i + R::UNITS - 1 < end) copy(ring + to * R::SLOT);  // the slot that the last step has read
+    commit_copies();
+    if (++to == R::UNITS) to = 0;
+    const uint32_t slot = ring + at * R::SLOT;
+    if (++at == R::UNITS) at = 0;
+    B32 x, wg, wu;
+    take(wg, slot, g, c);
+    take(wu, slot + 1024, g, c);
+    if (g < P.M) load_row<64>(x, xr + kb * 128);
+    else zero(x);
+    float p[4] = {};
+    multiply<KIND>(p, wg, wu, x);
+    if constexpr (FP8) {
+      const float s0 = xscale[(2 * c) * sblocks + kb], s1 = xscale[(2 * c + 1) * sblocks + kb];
+      float sg, su;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sg) : "r"(slot + 2048 + g * 4) : "memory");
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(su) : "r"(slot + 2080 + g * 4) : "memory");
+      acc[0] = fmaf(p[0], s0 * sg, acc[0]);
+      acc[1] = fmaf(p[1], s1 * sg, acc[1]);
+      acc[2] = fmaf(p[2], s0 * su, acc[2]);
+      acc[3] = fmaf(p[3], s1 * su, acc[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += p[j];
+    }
+    if (++kb == KB || i + 1 == end) {
+      const float4 v = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      const bool from_start = tile * KB >= begin;
+      if (from_start && kb == KB) finish(tile, v);  // the warp had all of the tile
+      else reinterpret_cast<float4*>(part)[(warp * 2 + from_start) * 32 + lane] = v;
+      acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+      kb = 0;
+      ++tile;
+    }
+  }
+  __syncthreads();
+  // a shared tile: the warp that has its start adds what the warps behind it hold, in their order
+  if (end > begin && end % KB != 0) {
+    const int t = end / KB;
+    if (t * KB >= begin) {
+      float4 v = reinterpret_cast<const float4*>(part)[(warp * 2 + 1) * 32 + lane];
+      for (int w = warp + 1; w < kWarps && bound(w) < (t + 1) * KB; ++w) {
+        if (bound(w) == bound(w + 1)) continue;
+        const float4 q = reinterpret_cast<const float4*>(part)[w * 2 * 32 + lane];
+        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+      }
+      finish(t, v);
+    }
   }
 }
 
 // Rows [lo, hi) of W2, at most 16 RT, of all experts, and the output columns that they are.  `wait`: returns when h is there
 template <typename T, bool FP8, int RT, typename Wait>
-__device__ __forceinline__ void second_product(const Few& P, const Shared& S, float* part, int lo, int hi, Wait wait) {
-  constexpr int ES = FP8 ? 1 : 2, D = RT == 1 ? (FP8 ? 4 : 6) : (RT == 2 ? 3 : 2), HV = FP8 ? 2 : 1;
+__device__ __forceinline__ void second_product(const Few& P, const Shared& S, float* part, uint32_t ring, int lo, int hi, Wait wait) {
+  using R = Ring2<FP8, RT>;
+  constexpr int ES = FP8 ? 1 : 2, HV = FP8 ? 2 : 1;
   using KIND = Kind<T, FP8>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int KB = P.I * ES / 128, SB = P.Is * ES / 128, routed = S.slots * KB, total = routed + SB;
   const int begin = (int)((int64_t)total * warp / kWarps), end = (int)((int64_t)total * (warp + 1) / kWarps);
   const int block = lo >> 7, blocks = P.H >> 7;
+  ring += (uint32_t)warp * R::BYTES;
+  const uint32_t hring = ring + R::UNITS * 2048;
   struct At {
     int s, kb, KB;
-    const uint8_t* w;  // this lane's bytes of row lo + g
+    const uint8_t* w;  // this lane's piece of row lo + cr
     int64_t row;       // bytes of a row
     const float* ws;
-    const T* h;
+    const T* h;        // the expert's
   };
+  const int cr = lane >> 3, cq = lane & 7;  // what this lane copies: piece cq of rows cr, cr + 4, ..
   auto enter = [&](int s, int kb) {  // expert s, S.slots = the shared one
     At a;
     a.s = s;
@@ -395,95 +460,139 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     a.KB = shared ? SB : KB;
     a.row = (int64_t)width * ES;
     const int64_t e = shared ? 0 : S.list[s];
-    a.w = reinterpret_cast<const uint8_t*>(shared ? P.sw2 : P.w2) + (e * P.H + lo + g) * a.row + c * 32;
+    a.w = reinterpret_cast<const uint8_t*>(shared ? P.sw2 : P.w2) + (e * P.H + lo + cr) * a.row + cq * 16;
     a.ws = FP8 ? (shared ? P.sw2s : P.w2s) + (e * blocks + block) * (int64_t)(width / 128) : nullptr;
-    a.h = reinterpret_cast<const T*>(P.h) + (int64_t)S.slots * kTokens * (shared ? P.I : 0) + (int64_t)(shared ? 0 : s) * kTokens * width +
-          (int64_t)g * width + c * (32 / ES);
+    a.h = reinterpret_cast<const T*>(P.h) + (int64_t)s * kTokens * P.I;  // the shared expert's lies behind the others'
     return a;
   };
   auto locate = [&](int i) { return i < routed ? enter(i / KB, i % KB) : enter(S.slots, i - routed); };
   auto advance = [&](At& a) {
     if (++a.kb == a.KB && a.s < S.slots && (a.s + 1 < S.slots || SB > 0)) a = enter(a.s + 1, 0);
   };
-  B32 w[D][RT][2], hv[D][HV];
-  float s0[D], s1[D];
-  auto load = [&](int d, const At& a) {
+  auto copy = [&](const At& a, int t, uint32_t slot) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (lo + 16 * t + 8 * j + g < hi) load_weights(w[d][t][j], a.w + (16 * t + 8 * j) * a.row + a.kb * 128);
-        else zero(w[d][t][j]);
-      }
-    if constexpr (FP8) {
-      const int width = (int)(a.row / 128);
-      s0[d] = __ldg(a.ws + a.kb);
-      s1[d] = block + 1 < blocks ? __ldg(a.ws + width + a.kb) : 0.0f;
-    }
+    for (int j = 0; j < 4; ++j)
+      if (lo + 16 * t + 4 * j + cr < hi) copy16(slot + place(4 * j + cr, cq), a.w + (16 * t + 4 * j) * a.row + a.kb * 128);
   };
-  auto load_h = [&](int d, const At& a) {  // written by other blocks of this kernel: not through the read-only path
-    if ((S.mask[a.s] >> g) & 1) {
+  auto copy_h = [&](const At& a, uint32_t slot) {
+    const uint32_t mask = S.mask[a.s];
+    const int64_t width = a.row / ES;
+    if constexpr (FP8) {  // 256 bytes of a token for 128 of its 8-bit ones; pieces of odd rows change places with their neighbours
 #pragma unroll
-      for (int i = 0; i < HV; ++i) load_row(hv[d][i], a.h + a.kb * (128 / ES) + 16 * i);
+      for (int j = 0; j < 4; ++j) {
+        const int m = 2 * j + (lane >> 4), q = lane & 15;
+        if ((mask >> m) & 1) copy16(slot + m * 256 + (q ^ (m & 1)) * 16, a.h + m * width + a.kb * 128 + q * 8);
+      }
+      if (lane < 2 && block + lane < blocks) copy4(slot + 2048 + lane * 4, a.ws + lane * (width / 128) + a.kb);
     } else {
 #pragma unroll
-      for (int i = 0; i < HV; ++i) zero(hv[d][i]);
+      for (int j = 0; j < 2; ++j)
+        if ((mask >> (4 * j + cr)) & 1) copy16(slot + place(4 * j + cr, cq), a.h + (4 * j + cr) * width + a.kb * 64 + cq * 8);
     }
   };
+  const int units = (end - begin) * RT;
   At ld = locate(begin < total ? begin : total - 1), at = ld;
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (begin + d < end) {
-      load(d, ld);
+  int lu = 0, lt = 0, to = 0, hto = 0;  // where copying stands: unit, tile of the step, slots
+#pragma unroll 1
+  for (; lu < R::UNITS - 1 && lu < units; ++lu) {  // weights do not wait for h
+    copy(ld, lt, ring + to * 2048);
+    if (++to == R::UNITS) to = 0;
+    if (++lt == RT) {
+      lt = 0;
       advance(ld);
-    }
-  wait();
-  ld = at;
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (begin + d < end) {
-      load_h(d, ld);
-      advance(ld);
-    }
-  float acc[RT][4] = {};
-  for (int i = begin; i < end; i += D) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (i + d < end) {
-        const uint32_t mask = S.mask[at.s];
-        const bool r0 = (mask >> (2 * c)) & 1, r1 = (mask >> (2 * c + 1)) & 1;
-        float f0 = r0 ? S.weight[at.s][2 * c] : 0.0f, f1 = r1 ? S.weight[at.s][2 * c + 1] : 0.0f;
-        B32 x;
-        if constexpr (FP8) {
-          const float s = quantise<T>(hv[d], x);
-          f0 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c);
-          f1 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c + 4);
-        } else {
-          x = hv[d][0];
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          float p[4] = {};
-          multiply<KIND>(p, w[d][t][0], w[d][t][1], x);
-          float a0 = f0, a1 = f1, b0 = f0, b1 = f1;
-          if constexpr (FP8) {
-            const float wa = (lo + 16 * t + g) >> 7 == block ? s0[d] : s1[d], wb = (lo + 16 * t + 8 + g) >> 7 == block ? s0[d] : s1[d];
-            a0 *= wa; a1 *= wa; b0 *= wb; b1 *= wb;
-          }
-          // a token that is not the expert's takes nothing, whatever the weights hold
-          if (r0) { acc[t][0] = fmaf(p[0], a0, acc[t][0]); acc[t][2] = fmaf(p[2], b0, acc[t][2]); }
-          if (r1) { acc[t][1] = fmaf(p[1], a1, acc[t][1]); acc[t][3] = fmaf(p[3], b1, acc[t][3]); }
-        }
-        advance(at);
-        if (i + d + D < end) {
-          load(d, ld);
-          load_h(d, ld);
-          advance(ld);
-        }
-      }
     }
   }
-  __syncthreads();  // `part` may still be read by the first product's last part
+  wait();
+  {
+    At a = at;
+    int t = 0;
+#pragma unroll 1
+    for (int u = 0; u < R::UNITS - 1; ++u) {
+      if (u < units) {
+        if (t == 0) {
+          copy_h(a, hring + hto * R::H_SLOT);
+          if (++hto == R::STEPS) hto = 0;
+        }
+        if (++t == RT) {
+          t = 0;
+          advance(a);
+        }
+      }
+      commit_copies();
+    }
+  }
+  auto next = [&] {  // one more unit on its way
+    if (lu < units) {
+      copy(ld, lt, ring + to * 2048);
+      if (lt == 0) {
+        copy_h(ld, hring + hto * R::H_SLOT);
+        if (++hto == R::STEPS) hto = 0;
+      }
+      if (++to == R::UNITS) to = 0;
+      ++lu;
+      if (++lt == RT) {
+        lt = 0;
+        advance(ld);
+      }
+    }
+    commit_copies();
+  };
+  float acc[RT][4] = {};
+  int from = 0, hfrom = 0;
+#pragma unroll 1
+  for (int i = begin; i < end; ++i) {
+    const uint32_t mask = S.mask[at.s];
+    const bool r0 = (mask >> (2 * c)) & 1, r1 = (mask >> (2 * c + 1)) & 1;
+    float f0 = r0 ? S.weight[at.s][2 * c] : 0.0f, f1 = r1 ? S.weight[at.s][2 * c + 1] : 0.0f;
+    wait_copies<R::UNITS - 2>();
+    next();
+    const uint32_t hs = hring + hfrom * R::H_SLOT;
+    if (++hfrom == R::STEPS) hfrom = 0;
+    B32 x, hv[HV];
+    float s0 = 0.0f, s1 = 0.0f;
+    zero(hv[0]);
+    zero(hv[HV - 1]);
+    if ((mask >> g) & 1) {
+      if constexpr (FP8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) take16(hv[j >> 1].r + 4 * (j & 1), hs + g * 256 + ((8 * (j >> 1) + 2 * c + (j & 1)) ^ (g & 1)) * 16);
+      } else {
+        take(hv[0], hs, g, c);
+      }
+    }
+    if constexpr (FP8) {
+      const float s = quantise<T>(hv, x);
+      f0 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c);
+      f1 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c + 4);
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s0) : "r"(hs + 2048) : "memory");
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s1) : "r"(hs + 2052) : "memory");
+    } else {
+      x = hv[0];
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (t > 0) {
+        wait_copies<R::UNITS - 2>();
+        next();
+      }
+      B32 wa, wb;
+      take(wa, ring + from * 2048, g, c);
+      take(wb, ring + from * 2048, 8 + g, c);
+      if (++from == R::UNITS) from = 0;
+      float p[4] = {};
+      multiply<KIND>(p, wa, wb, x);
+      float a0 = f0, a1 = f1, b0 = f0, b1 = f1;
+      if constexpr (FP8) {
+        const float sa = (lo + 16 * t + g) >> 7 == block ? s0 : s1, sb = (lo + 16 * t + 8 + g) >> 7 == block ? s0 : s1;
+        a0 *= sa; a1 *= sa; b0 *= sb; b1 *= sb;
+      }
+      // a token that is not the expert's takes nothing, whatever the weights hold
+      if (r0) { acc[t][0] = fmaf(p[0], a0, acc[t][0]); acc[t][2] = fmaf(p[2], b0, acc[t][2]); }
+      if (r1) { acc[t][1] = fmaf(p[1], a1, acc[t][1]); acc[t][3] = fmaf(p[3], b1, acc[t][3]); }
+    }
+    advance(at);
+  }
+  __syncthreads();
 #pragma unroll
   for (int t = 0; t < RT; ++t) reinterpret_cast<float4*>(part)[(warp * RT + t) * 32 + lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
   __syncthreads();
@@ -511,7 +620,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& S = *reinterpret_cast<Shared*>(smem);
   float* part = reinterpret_cast<float*>(smem + (sizeof(Shared) + 127) / 128 * 128);
-  uint8_t* xs = reinterpret_cast<uint8_t*>(part) + kPartBytes;
+  uint8_t* rest = reinterpret_cast<uint8_t*>(part) + kPartBytes;  // scores while routing, then W1's ring and the tokens, then W2's ring
+  uint8_t* xs = rest + kWarps * Ring1<FP8>::BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the tokens, older than the kernel in front: into shared memory, in 8 bits where the weights are
   const uint8_t* xrows = xs;
@@ -528,8 +638,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
       zero(v[1]);
       if (i < groups) {
         const T* p = reinterpret_cast<const T*>(P.x) + m * P.x_ld + b * 128 + (lane & 3) * 32;
-        load_row(v[0], p);
-        load_row(v[1], p + 16);
+        load_row<16>(v[0], p);
+        load_row<16>(v[1], p + 16);
       }
       const float s = quantise<T>(v, q);
       if (i < groups) {
@@ -555,19 +665,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
     mine1 = claim(P.counters);
     mine2 = claim(P.counters + 1);
   }
-  if (P.E <= 256) route<8>(P, S, part);
-  else route<32>(P, S, part);
+  if (P.E <= 256) route<8>(P, S, reinterpret_cast<float*>(rest));
+  else route<32>(P, S, reinterpret_cast<float*>(rest));
 
   const int64_t outputs = (int64_t)S.slots * P.I + P.Is;
   const int G = gridDim.x;
-  const int64_t runs1 = (outputs + (int64_t)G * kTiles * 8 - 1) / ((int64_t)G * kTiles * 8) * G;
+  const int64_t runs1 = (outputs + (int64_t)G * kRunTiles * 8 - 1) / ((int64_t)G * kRunTiles * 8) * G;
   for (;;) {
     if (threadIdx.x == 0) S.next1 = mine1;
     __syncthreads();
     const int run = S.next1;
     if (run >= runs1) break;
     if (threadIdx.x == 0) mine1 = claim(P.counters);
-    first_product<T, FP8>(P, S, xrows, xscale, part, outputs * run / runs1, outputs * (run + 1) / runs1);
+    first_product<T, FP8>(P, S, xrows, xscale, part, smem_u32(rest), outputs * run / runs1, outputs * (run + 1) / runs1);
     __syncthreads();  // all of the run's h is written
     if (threadIdx.x == 0) {
       __threadfence();
@@ -596,12 +706,20 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
     const int run = S.next2;
     if (run >= runs2) break;
     if (threadIdx.x == 0) mine2 = claim(P.counters + 1);
-    second_product<T, FP8, RT>(P, S, part, (int)((int64_t)P.H * run / runs2), (int)((int64_t)P.H * (run + 1) / runs2), wait);
+    second_product<T, FP8, RT>(P, S, part, smem_u32(rest), (int)((int64_t)P.H * run / runs2), (int)((int64_t)P.H * (run + 1) / runs2), wait);
   }
 }
 
-static_assert((sizeof(Shared) + 127) / 128 * 128 + kPartBytes + kTokens * (kMaxHidden + 16) + kTokens * (kMaxHidden / 128) * 4 <= 232448,
-              "8-bit tokens fit shared memory");
+constexpr int64_t kHead = (sizeof(Shared) + 127) / 128 * 128 + kPartBytes;
+constexpr int64_t kSmem = 232448;
+constexpr int kScores = 2 * kTokens * kMaxExperts * 4;  // and zeros for a bias
+static_assert(kScores <= kWarps * Ring1<false>::BYTES && kScores <= kWarps * Ring1<true>::BYTES, "the scores lie in front of the tokens");
+static_assert(kHead + kWarps * Ring2<true, 1>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 1>::BYTES <= kSmem, "ring of W2");
+static_assert(kHead + kWarps * Ring2<true, 2>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 2>::BYTES <= kSmem, "ring of W2");
+static_assert(kHead + kWarps * Ring2<true, 4>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 4>::BYTES <= kSmem, "ring of W2");
+// 8-bit tokens: their rows, and scales for all eight
+constexpr int64_t tokens_bytes(int64_t M, int64_t H, bool fp8) { return M * (H * (fp8 ? 1 : 2) + 64) + (fp8 ? kTokens * (H / 128) * 4 : 0); }
+static_assert(kHead + kWarps * Ring1<true>::BYTES + tokens_bytes(kTokens, kMaxHidden8, true) <= kSmem, "8-bit tokens fit shared memory");
 
 // ------------------------------------------------------------------ host side
 struct Layout {
@@ -631,22 +749,22 @@ int run_router(const Few& P, const void* w, cudaStream_t st) {
 
 template <typename T, bool FP8>
 int run_experts(Few P, cudaStream_t st) {
-  constexpr int64_t head = (sizeof(Shared) + 127) / 128 * 128 + kPartBytes;
-  P.x_pitch = P.H * (FP8 ? 1 : 2) + 16;  // neighbouring tokens' pieces lie in other banks
-  int64_t smem = head + (int64_t)P.M * P.x_pitch + (FP8 ? kTokens * (P.H / 128) * 4 : 0);
-  P.staged = smem <= 232448;
-  if (!P.staged) {
-    if (FP8) return fail(MOE_E_TOOBIG, "fused_moe_few_tokens: %d tokens of %d elements do not fit shared memory", P.M, P.H);  // kMaxHidden lets none
-    smem = head;  // the rows then come out of L1
+  P.x_pitch = P.H * (FP8 ? 1 : 2) + 64;  // neighbouring tokens' pieces lie in other banks
+  const int64_t first = kHead + kWarps * Ring1<FP8>::BYTES;
+  int64_t smem = first + tokens_bytes(P.M, P.H, FP8);
+  P.staged = FP8 || smem <= kSmem;
+  if (!P.staged) {  // the rows then come out of L1
+    smem = first;
     P.x_pitch = (int)(P.x_ld * 2);
   }
   const int G = sm_count();
   const int rows = (P.H + G - 1) / G;
   auto go = [&](auto rt) {
     auto kern = few_experts_kernel<T, FP8, decltype(rt)::value>;
-    const int rc = allow_smem((const void*)kern, 232448);
+    const int rc = allow_smem((const void*)kern, (int)kSmem);
     if (rc) return rc;
-    return launch_pdl(kern, dim3((unsigned)G), kThreads, (size_t)smem, 1, st, "fused_moe_few_tokens", P);
+    const int64_t second = kHead + kWarps * Ring2<FP8, decltype(rt)::value>::BYTES;
+    return launch_pdl(kern, dim3((unsigned)G), kThreads, (size_t)(smem > second ? smem : second), 1, st, "fused_moe_few_tokens", P);
   };
   if (rows <= 16) return go(std::integral_constant<int, 1>());
   if (rows <= 32) return go(std::integral_constant<int, 2>());
@@ -678,8 +796,8 @@ extern "C" int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void
   if (M == 0) return 0;
   const bool fp8 = w1_scale != nullptr;
   const int unit = fp8 ? 128 : 64;
-  if (E <= 0 || E > kMaxExperts || H <= 0 || H > kMaxHidden || I <= 0 || shared_I < 0 || H % unit || I % unit || shared_I % unit)
-    return fail(MOE_E_SHAPE, "%s: at most %d experts, hidden sizes up to %d; sizes in multiples of %d", who, kMaxExperts, kMaxHidden, unit);
+  if (E <= 0 || E > kMaxExperts || H <= 0 || H > (fp8 ? kMaxHidden8 : kMaxHidden) || I <= 0 || I > kMaxWidth || shared_I > kMaxWidth || shared_I < 0 || H % unit || I % unit || shared_I % unit)
+    return fail(MOE_E_SHAPE, "%s: at most %d experts, hidden sizes up to %d; sizes in multiples of %d", who, kMaxExperts, fp8 ? kMaxHidden8 : kMaxHidden, unit);
   if (topk <= 0 || topk > 32 || topk > E || n_group <= 0 || n_group > 32 || E % n_group || topk_group <= 0 || topk_group > n_group ||
       (int64_t)topk > (int64_t)E / n_group * topk_group)
     return fail(MOE_E_SHAPE, "%s: groups and topk do not fit the experts", who);

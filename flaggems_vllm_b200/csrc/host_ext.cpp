@@ -918,7 +918,7 @@ PyObject* few_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto type = fp8 ? at::kFloat8_e4m3fn : x.scalar_type();
   const int64_t unit = fp8 ? 128 : 64;
   if (!status || (code != MOE_BF16 && code != MOE_F16) || (router_code != code && router_code != MOE_F32) || M > 8 || M <= 0 || H <= 0 || E <= 0 ||
-      E > 1024 || I <= 0 || Is < 0 || H % unit || I % unit || Is % unit || H > 16384 || I > (1 << 24) || Is > (1 << 24) || topk <= 0 ||
+      E > 1024 || I <= 0 || Is < 0 || H % unit || I % unit || Is % unit || H > (fp8 ? 8192 : 16384) || I > (1 << 22) || Is > (1 << 22) || topk <= 0 ||
       topk > 32 || topk > E || n_group <= 0 || n_group > 32 || E % n_group || topk_group <= 0 || topk_group > n_group ||
       topk > E / n_group * topk_group || !(scaling > -3e38 && scaling < 3e38) || (w1x != nullptr) != (w2x != nullptr) || (s2 != nullptr) != fp8 ||
       (s1x != nullptr) != (fp8 && w1x) || (s2x != nullptr) != (fp8 && w1x))

@@ -13,7 +13,8 @@ from . import _lib
 logger = logging.getLogger(__name__)
 
 MAX_FEW_TOKENS = 8
-_MAX_EXPERTS, _MAX_TOPK, _MAX_GROUPS, _MAX_HIDDEN = 1024, 32, 32, 16384
+_MAX_EXPERTS, _MAX_TOPK, _MAX_GROUPS, _MAX_WIDTH = 1024, 32, 32, 1 << 22
+_MAX_HIDDEN, _MAX_HIDDEN_FP8 = 16384, 8192
 
 
 def fused_moe_few_tokens(
@@ -48,8 +49,8 @@ def fused_moe_few_tokens(
     ``w1`` [E, 2 I, H] (gate rows first), ``w2`` [E, H, I] as ``fused_experts_impl`` has them, in the type of the activations, or
     float8_e4m3fn with ``w1_scale`` [E, 2 I / 128, H / 128] and ``w2_scale`` [E, H / 128, I / 128]: the activations are then taken in
     e4m3 too, in groups of 128, as with ``use_fp8_w8a8`` and ``block_shape=[128, 128]``.  The shared expert, [2 Is, H] and [H, Is],
-    has the format of the others.  H (at most 16384), I and Is are multiples of 64, in 8 bits of
-    128; at most 1024 experts, 32 per token.
+    has the format of the others.  H (at most 16384, in 8 bits 8192), I and Is are multiples of
+    64, in 8 bits of 128; at most 1024 experts, 32 per token.
 
     More tokens: ``router_gemm_grouped_topk``, ``fused_experts_impl`` and ``fused_linear``.  Not differentiable: refused where a
     gradient is wanted.  The same bits in every run."""
@@ -85,8 +86,10 @@ def _slow(x, router, w1, w2, topk, renormalize, sigmoid, groups, kept, factor, b
                          f"w2 {list(w2.shape)} do not belong together")
     if router.dtype not in (x.dtype, torch.float32):
         raise ValueError(f"{what}: router_weight must be of the type of hidden_states or float32, got {router.dtype}")
-    if not 1 <= E <= _MAX_EXPERTS or I == 0 or not 1 <= H <= _MAX_HIDDEN:
-        raise ValueError(f"{what}: 1 to {_MAX_EXPERTS} experts, none of them empty, and hidden sizes up to {_MAX_HIDDEN}")
+    fp8 = w1.dtype == torch.float8_e4m3fn
+    most = _MAX_HIDDEN_FP8 if fp8 else _MAX_HIDDEN
+    if not 1 <= E <= _MAX_EXPERTS or not 1 <= I <= _MAX_WIDTH or not 1 <= H <= most:
+        raise ValueError(f"{what}: 1 to {_MAX_EXPERTS} experts of 1 to {_MAX_WIDTH} columns, and hidden sizes up to {most}")
     topk, groups, kept = int(topk), int(groups), int(kept)
     if not 1 <= groups <= _MAX_GROUPS or E % groups != 0 or not 1 <= kept <= groups:
         raise ValueError(f"{what}: {groups} groups, {kept} of them kept, do not divide {E} experts")
@@ -101,7 +104,8 @@ def _slow(x, router, w1, w2, topk, renormalize, sigmoid, groups, kept, factor, b
         if sw2.ndim != 2 or sw1.shape != (2 * sw2.shape[1], H) or sw2.shape[0] != H or sw2.shape[1] == 0:
             raise ValueError(f"{what}: shared_w1 must be [2 Is, {H}] and shared_w2 [{H}, Is]")
         Is = sw2.shape[1]
-    fp8 = w1.dtype == torch.float8_e4m3fn
+        if Is > _MAX_WIDTH:
+            raise ValueError(f"{what}: a shared expert of at most {_MAX_WIDTH} columns")
     held = torch.float8_e4m3fn if fp8 else x.dtype
     for t, n in ((w1, "w1"), (w2, "w2"), (sw1, "shared_w1"), (sw2, "shared_w2")):
         if t is not None and t.dtype != held:

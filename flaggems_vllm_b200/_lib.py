@@ -108,7 +108,7 @@ SYMBOLS = {
                                                 c_void_p]),
     "moe_fused_linear_grad": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64,
                                       c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
-    "moe_few_tokens_workspace": (c_int, [c_int64, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "moe_few_tokens_workspace": (c_int, [c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p]),
     "moe_few_tokens": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int] + [c_void_p] * 10 + [c_int64, c_int64] + [c_int] * 8 +
                        [c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "moe_sum_ld": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int64, c_void_p, c_int, c_int, c_void_p,

@@ -17,7 +17,7 @@
 // warps divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in registers.
 //
 // FP8 (128 x 128 block scales): activations in groups of 128 as per_token_group_quant_fp8 has them, h after its rounding to the
-// activations' type, as in the layer of many tokens; every 128 k are folded with both scales in fp32.
+// activations' type, as in the layer of many tokens (quantise_groups); every 128 k are folded with both scales in fp32.
 //
 // A block waits for others once, between W1 and W2.  Work is claimed from counters, and a block waits only for work that some running
 // block has claimed: it needs no co-residency, and two calls on two streams cannot wait for each other.  The wait has the
@@ -41,11 +41,14 @@ struct Few {
   void* out;
   const void *w1, *w2, *sw1, *sw2;              // sw: shared expert
   const float *w1s, *w2s, *sw1s, *sw2s;         // block scales
-  const float *logits, *bias;
+  const float *scores, *bias;                   // [M, E] sigmoids, or logits of a softmax
   float* topk_w;
   int32_t* topk_ids;
   void* h;                                      // [slots][8][I], then the shared expert's [8][Is]
-  int32_t* counters;                            // claims of W1 and W2, finished runs of W1
+  uint8_t* h8;                                  // the same in 8 bits, and the scales of its groups
+  float* h8_scale;
+  int32_t* counters;                            // claims of W1 and W2, finished runs of W1, one unused, outputs of each group of 128
+  int64_t cleared;                              // counters to clear
   int64_t x_ld, residual_ld;
   int M, E, H, I, Is, topk, n_group, topk_group, renormalize, sigmoid;
   float scaling;
@@ -140,13 +143,14 @@ __device__ __forceinline__ float quantise(const B32 (&v)[2], B32& q) {
 }
 
 // ------------------------------------------------------------------ logits
-// A block per expert; the sums are formed in the order of router_gemm's row-streaming kernel, whose bits they are.
+// A block per expert; the sums are formed in the order of router_gemm's row-streaming kernel, whose bits they are.  Clears the
+// counters of the kernel behind it.
 template <typename XT, typename WT, int ROWS>
 __global__ void __launch_bounds__(128) few_router_kernel(const XT* __restrict__ x, int64_t x_ld, const WT* __restrict__ w, int M, int E, int K,
-                                                         float* __restrict__ out, int32_t* counters) {
+                                                         int sigmoid, float* __restrict__ out, int32_t* counters, int64_t cleared) {
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x == 0 && threadIdx.x < 4) counters[threadIdx.x] = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x; i < cleared; i += (int64_t)gridDim.x * 128) counters[i] = 0;
   const WT* row = w + (int64_t)blockIdx.x * K;
   float acc[ROWS] = {};
 #pragma unroll(ROWS <= 2 ? 4 : 2)
@@ -177,93 +181,111 @@ __global__ void __launch_bounds__(128) few_router_kernel(const XT* __restrict__ 
     float v = part[0][threadIdx.x];
 #pragma unroll
     for (int i = 1; i < 4; ++i) v += part[i][threadIdx.x];
+    if (sigmoid) v = (float)(1.0 / (1.0 + exp(-(double)v)));  // grouped_topk's
     out[(int64_t)threadIdx.x * E + blockIdx.x] = v;
   }
 }
 
 // ------------------------------------------------------------------ experts
 struct Shared {
-  float weight[kMaxSlots + 1][kTokens];   // of every routed expert for every token; the shared expert's are 1
+  float weight[kMaxSlots + 1][kTokens];   // of every routed expert for the tokens that it has; the shared expert's are 1
   uint32_t mask[kMaxSlots + 1];           // tokens of the expert
   int32_t list[kMaxSlots];                // routed experts, ascending
-  uint16_t slot[kMaxExperts];
+  uint32_t used[kMaxExperts / 32];        // a bit for each
+  float bias[kMaxExperts];
   float w[kTokens][32];
   int32_t id[kTokens][32];
-  int32_t slots, next1, next2;
+  int32_t whole[kMaxSlots];               // groups of h that this block has to quantise
+  int32_t slots, next1, next2, wholes;
 };
 constexpr int kPartBytes = kWarps * 4 * 512;  // partial sums: two tiles of W1 a warp, four of W2
 // W1's ring: a unit is a tile's 128 bytes of k, 2 KB, and in 8 bits its scales
 template <bool FP8> struct Ring1 {
   static constexpr int UNITS = 7, SLOT = 2048 + (FP8 ? 64 : 0), BYTES = UNITS * SLOT;
 };
-// W2's: a unit is 16 rows' 128 bytes of k; a step's h (and scales) come with its first unit.  As many as fit
+// W2's: a unit is 16 rows' 128 bytes of k; a step's h, and in 8 bits its scales and W2's, come with its first unit.  As many as fit
 template <bool FP8, int RT> struct Ring2 {
-  static constexpr int UNITS = RT == 1 ? (FP8 ? 5 : 7) : (RT == 2 && FP8 ? 6 : 8), STEPS = (UNITS + RT - 1) / RT + 1;
-  static constexpr int H_SLOT = FP8 ? 2048 + 16 : 1024, BYTES = UNITS * 2048 + STEPS * H_SLOT;
+  static constexpr int UNITS = RT == 1 ? 7 : 8, STEPS = (UNITS + RT - 1) / RT + 1;
+  static constexpr int H_SLOT = FP8 ? 1024 + 64 : 1024, BYTES = UNITS * 2048 + STEPS * H_SLOT;
 };
 
+// What routing needs and the kernel in front does not make
+__device__ __forceinline__ void prepare_route(const Few& P, Shared& S) {
+  for (int e = threadIdx.x; e < P.E; e += kThreads) S.bias[e] = P.bias ? P.bias[e] : 0.0f;
+  for (int i = threadIdx.x; i < kMaxSlots; i += kThreads) S.mask[i] = 0;
+  if (threadIdx.x < kMaxExperts / 32) S.used[threadIdx.x] = 0;
+  __syncthreads();
+}
 // every token's experts, by a warp each; the list of all of them
 template <int VPT>
 __device__ __forceinline__ void route(const Few& P, Shared& S, float* scratch) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp < P.M) {
-    float* u = scratch + warp * P.E;
-    const float* logits = P.logits + (int64_t)warp * P.E;
-    if (P.sigmoid) {
-      for (int e = lane; e < P.E; e += 32) u[e] = (float)(1.0 / (1.0 + exp(-(double)__ldcg(logits + e))));
-    } else {
-      float m = -INFINITY;
-      for (int e = lane; e < P.E; e += 32) {
-        u[e] = __ldcg(logits + e);
-        m = fmaxf(m, u[e]);
+    const float* u = P.scores + (int64_t)warp * P.E;
+    if (!P.sigmoid) {
+      float l[VPT], m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        l[j] = j * 32 + lane < P.E ? u[j * 32 + lane] : -INFINITY;
+        m = fmaxf(m, l[j]);
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+      float* s = scratch + warp * P.E;
       double sum = 0.0;
-      for (int e = lane; e < P.E; e += 32) sum += exp((double)u[e] - (double)m);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        if (j * 32 + lane < P.E) {
+          const double x = exp((double)l[j] - (double)m);
+          sum += x;
+          l[j] = (float)x;
+        }
+      }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
-      for (int e = lane; e < P.E; e += 32) u[e] = (float)(exp((double)u[e] - (double)m) / sum);
+      const double inv = 1.0 / sum;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+        if (j * 32 + lane < P.E) s[j * 32 + lane] = (float)(l[j] * inv);
+      __syncwarp();
+      u = s;
     }
-    float* none = scratch + kTokens * P.E + warp * P.E;  // no bias: zeros
-    if (P.bias == nullptr)
-      for (int e = lane; e < P.E; e += 32) none[e] = 0.0f;
+    route_row<float, float, VPT>(u, 1, S.bias, P.E, P.n_group, P.topk_group, P.topk, P.renormalize, P.scaling, 0, S.w[warp], S.id[warp], lane);
     __syncwarp();
-    route_row<float, float, VPT>(u, 1, P.bias ? P.bias : none, P.E, P.n_group, P.topk_group, P.topk, P.renormalize, P.scaling, 0, S.w[warp], S.id[warp], lane);
-  }
-  for (int e = threadIdx.x; e < P.E; e += kThreads) S.slot[e] = 0;
-  __syncthreads();
-  const int n = P.M * P.topk;
-  for (int i = threadIdx.x; i < n; i += kThreads) S.slot[S.id[i / P.topk][i % P.topk]] = 1;
-  __syncthreads();
-  if (warp == 0) {
-    int count = 0;
-    for (int e0 = 0; e0 < P.E; e0 += 32) {
-      const int e = e0 + lane;
-      const bool used = e < P.E && S.slot[e] != 0;
-      const uint32_t b = __ballot_sync(0xFFFFFFFFu, used);
-      const int at = count + __popc(b & ((1u << lane) - 1));
-      if (used) {
-        S.list[at] = e;
-        S.slot[e] = (uint16_t)at;
-        S.mask[at] = 0;
+    if (lane < P.topk) {
+      const int id = S.id[warp][lane];
+      atomicOr(&S.used[id >> 5], 1u << (id & 31));
+      if (blockIdx.x == 0) {
+        P.topk_w[warp * P.topk + lane] = S.w[warp][lane];
+        P.topk_ids[warp * P.topk + lane] = id;
       }
-      count += __popc(b);
     }
-    if (lane == 0) {
-      S.slots = count;
-      S.mask[count] = (1u << P.M) - 1;
-    }
-    if (lane < kTokens) S.weight[count][lane] = 1.0f;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int t = i / P.topk, j = i % P.topk, s = S.slot[S.id[t][j]];
-    S.weight[s][t] = S.w[t][j];
-    atomicOr(&S.mask[s], 1u << t);
-    if (blockIdx.x == 0) {
-      P.topk_w[i] = S.w[t][j];
-      P.topk_ids[i] = S.id[t][j];
+  // an expert's place is the number of used ones below it; lane i has those of the first 32 i
+  const uint32_t word = S.used[lane];
+  int below = __popc(word);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, below, off);
+    if (lane >= off) below += v;
+  }
+  const int slots = __shfl_sync(0xFFFFFFFFu, below, 31);
+  below -= __popc(word);
+  if (warp < P.M) {
+    const int id = lane < P.topk ? S.id[warp][lane] : 0;
+    const int s = __shfl_sync(0xFFFFFFFFu, below, id >> 5) + __popc(S.used[id >> 5] & ((1u << (id & 31)) - 1));
+    if (lane < P.topk) {
+      S.list[s] = id;
+      S.weight[s][warp] = S.w[warp][lane];
+      atomicOr(&S.mask[s], 1u << warp);
+    }
+  }
+  if (warp == 0) {
+    if (lane < kTokens) S.weight[slots][lane] = 1.0f;
+    if (lane == 0) {
+      S.slots = slots;
+      S.mask[slots] = (1u << P.M) - 1;  // nobody's slot
     }
   }
   __syncthreads();
@@ -431,11 +453,69 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
   }
 }
 
+// 8 bits: a group's scale needs all of its 128 outputs, which several blocks may have made.  Whoever adds the last ones quantises the
+// group, once for all blocks that read it.  (Done by every reader on its way into W2's products it cost 240 instructions a step:
+// 6 tokens of 256 experts of 2048 x 7168, 367 us; XXX so.)
+template <typename T>
+__device__ __forceinline__ void quantise_groups(const Few& P, Shared& S, int64_t lo, int64_t hi) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t last = hi > lo ? (hi - 1) / 128 : -1;
+  for (int64_t first = lo / 128; first <= last; first += kMaxSlots) {
+    __syncthreads();  // this block's h is written; the list has been read
+    if (threadIdx.x == 0) S.wholes = 0;
+    __syncthreads();
+    const int64_t g = first + threadIdx.x;
+    if (threadIdx.x < kMaxSlots && g <= last) {
+      const int64_t a = g * 128 > lo ? g * 128 : lo, z = (g + 1) * 128 < hi ? (g + 1) * 128 : hi;
+      const int mine = (int)(z - a);
+      __threadfence();
+      const int old = atomicAdd(P.counters + 4 + g, mine);
+      __threadfence();
+      if (old + mine == 128) S.whole[atomicAdd(&S.wholes, 1)] = (int)(g - first);
+    }
+    __syncthreads();
+    const int n = S.wholes;
+    const int64_t routed = (int64_t)S.slots * P.I;
+    for (int i = warp; i < n; i += kWarps) {
+      const int64_t o = (first + S.whole[i]) * 128;
+      int s = S.slots;
+      int64_t width = P.Is, p = o - routed;
+      if (o < routed) {
+        s = (int)((uint32_t)o / (uint32_t)P.I);
+        width = P.I;
+        p = o - (int64_t)s * P.I;
+      }
+      const int m = lane >> 2, c = lane & 3;
+      const int64_t at = (int64_t)s * kTokens * P.I + m * width + p + c * 32;
+      B32 v[2], q;
+      zero(v[0]);
+      zero(v[1]);
+      const bool mine = (S.mask[s] >> m) & 1;
+      if (mine) {
+        const uint4* h = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.h) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 w = __ldcg(h + j);  // other blocks' stores: past L1
+          uint32_t* r = v[j >> 1].r + 4 * (j & 1);
+          r[0] = w.x; r[1] = w.y; r[2] = w.z; r[3] = w.w;
+        }
+      }
+      const float scale = quantise<T>(v, q);
+      if (mine) {
+        uint4* d = reinterpret_cast<uint4*>(P.h8 + at);
+        d[0] = make_uint4(q.r[0], q.r[1], q.r[2], q.r[3]);
+        d[1] = make_uint4(q.r[4], q.r[5], q.r[6], q.r[7]);
+        if (c == 0) P.h8_scale[((int64_t)s * kTokens * P.I + m * width + p) / 128] = scale;
+      }
+    }
+  }
+}
+
 // Rows [lo, hi) of W2, at most 16 RT, of all experts, and the output columns that they are.  `wait`: returns when h is there
 template <typename T, bool FP8, int RT, typename Wait>
 __device__ __forceinline__ void second_product(const Few& P, const Shared& S, float* part, uint32_t ring, int lo, int hi, Wait wait) {
   using R = Ring2<FP8, RT>;
-  constexpr int ES = FP8 ? 1 : 2, HV = FP8 ? 2 : 1;
+  constexpr int ES = FP8 ? 1 : 2;
   using KIND = Kind<T, FP8>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int KB = P.I * ES / 128, SB = P.Is * ES / 128, routed = S.slots * KB, total = routed + SB;
@@ -448,7 +528,8 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     const uint8_t* w;  // this lane's piece of row lo + cr
     int64_t row;       // bytes of a row
     const float* ws;
-    const T* h;        // the expert's
+    const uint8_t* h;  // the expert's, as it is multiplied
+    const float* hs;
   };
   const int cr = lane >> 3, cq = lane & 7;  // what this lane copies: piece cq of rows cr, cr + 4, ..
   auto enter = [&](int s, int kb) {  // expert s, S.slots = the shared one
@@ -462,7 +543,8 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     const int64_t e = shared ? 0 : S.list[s];
     a.w = reinterpret_cast<const uint8_t*>(shared ? P.sw2 : P.w2) + (e * P.H + lo + cr) * a.row + cq * 16;
     a.ws = FP8 ? (shared ? P.sw2s : P.w2s) + (e * blocks + block) * (int64_t)(width / 128) : nullptr;
-    a.h = reinterpret_cast<const T*>(P.h) + (int64_t)s * kTokens * P.I;  // the shared expert's lies behind the others'
+    a.h = (FP8 ? P.h8 : reinterpret_cast<const uint8_t*>(P.h)) + (int64_t)s * kTokens * P.I * ES;  // the shared expert's lies behind the others'
+    a.hs = FP8 ? P.h8_scale + (int64_t)s * kTokens * (P.I / 128) : nullptr;
     return a;
   };
   auto locate = [&](int i) { return i < routed ? enter(i / KB, i % KB) : enter(S.slots, i - routed); };
@@ -476,18 +558,16 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
   };
   auto copy_h = [&](const At& a, uint32_t slot) {
     const uint32_t mask = S.mask[a.s];
-    const int64_t width = a.row / ES;
-    if constexpr (FP8) {  // 256 bytes of a token for 128 of its 8-bit ones; pieces of odd rows change places with their neighbours
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = 2 * j + (lane >> 4), q = lane & 15;
-        if ((mask >> m) & 1) copy16(slot + m * 256 + (q ^ (m & 1)) * 16, a.h + m * width + a.kb * 128 + q * 8);
+    for (int j = 0; j < 2; ++j)
+      if ((mask >> (4 * j + cr)) & 1) copy16(slot + place(4 * j + cr, cq), a.h + (4 * j + cr) * a.row + a.kb * 128 + cq * 16);
+    if constexpr (FP8) {
+      const int64_t groups = a.row / 128;
+      if (lane < kTokens) {
+        if ((mask >> lane) & 1) copy4(slot + 1024 + lane * 4, a.hs + lane * groups + a.kb);
+      } else if (lane < kTokens + 2 && block + lane - kTokens < blocks) {
+        copy4(slot + 1024 + lane * 4, a.ws + (lane - kTokens) * groups + a.kb);
       }
-      if (lane < 2 && block + lane < blocks) copy4(slot + 2048 + lane * 4, a.ws + lane * (width / 128) + a.kb);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if ((mask >> (4 * j + cr)) & 1) copy16(slot + place(4 * j + cr, cq), a.h + (4 * j + cr) * width + a.kb * 64 + cq * 8);
     }
   };
   const int units = (end - begin) * RT;
@@ -548,26 +628,16 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     next();
     const uint32_t hs = hring + hfrom * R::H_SLOT;
     if (++hfrom == R::STEPS) hfrom = 0;
-    B32 x, hv[HV];
+    B32 x;
+    if ((mask >> g) & 1) take(x, hs, g, c);
+    else zero(x);
     float s0 = 0.0f, s1 = 0.0f;
-    zero(hv[0]);
-    zero(hv[HV - 1]);
-    if ((mask >> g) & 1) {
-      if constexpr (FP8) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) take16(hv[j >> 1].r + 4 * (j & 1), hs + g * 256 + ((8 * (j >> 1) + 2 * c + (j & 1)) ^ (g & 1)) * 16);
-      } else {
-        take(hv[0], hs, g, c);
-      }
-    }
     if constexpr (FP8) {
-      const float s = quantise<T>(hv, x);
-      f0 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c);
-      f1 *= __shfl_sync(0xFFFFFFFFu, s, 8 * c + 4);
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s0) : "r"(hs + 2048) : "memory");
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s1) : "r"(hs + 2052) : "memory");
-    } else {
-      x = hv[0];
+      float h0, h1;
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(h0), "=f"(h1) : "r"(hs + 1024 + c * 8) : "memory");
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(s0), "=f"(s1) : "r"(hs + 1024 + kTokens * 4) : "memory");
+      f0 *= h0;
+      f1 *= h1;
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -658,7 +728,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
   } else {
     xrows = reinterpret_cast<const uint8_t*>(P.x);
   }
-  pdl_wait();  // logits and cleared counters
+  prepare_route(P, S);
+  pdl_wait();  // scores and cleared counters
   pdl_trigger();
   int mine1 = 0, mine2 = 0;  // thread 0: claimed, not begun
   if (threadIdx.x == 0) {
@@ -678,6 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
     if (run >= runs1) break;
     if (threadIdx.x == 0) mine1 = claim(P.counters);
     first_product<T, FP8>(P, S, xrows, xscale, part, smem_u32(rest), outputs * run / runs1, outputs * (run + 1) / runs1);
+    if constexpr (FP8) quantise_groups<T>(P, S, outputs * run / runs1, outputs * (run + 1) / runs1);
     __syncthreads();  // all of the run's h is written
     if (threadIdx.x == 0) {
       __threadfence();
@@ -712,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
 
 constexpr int64_t kHead = (sizeof(Shared) + 127) / 128 * 128 + kPartBytes;
 constexpr int64_t kSmem = 232448;
-constexpr int kScores = 2 * kTokens * kMaxExperts * 4;  // and zeros for a bias
+constexpr int kScores = kTokens * kMaxExperts * 4;
 static_assert(kScores <= kWarps * Ring1<false>::BYTES && kScores <= kWarps * Ring1<true>::BYTES, "the scores lie in front of the tokens");
 static_assert(kHead + kWarps * Ring2<true, 1>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 1>::BYTES <= kSmem, "ring of W2");
 static_assert(kHead + kWarps * Ring2<true, 2>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 2>::BYTES <= kSmem, "ring of W2");
@@ -723,15 +795,18 @@ static_assert(kHead + kWarps * Ring1<true>::BYTES + tokens_bytes(kTokens, kMaxHi
 
 // ------------------------------------------------------------------ host side
 struct Layout {
-  int64_t logits, h, bytes;  // counters in front
+  int64_t counters, scores, h, h8, h8_scale, bytes;
 };
-Layout layout(int64_t M, int E, int64_t I, int64_t Is, int topk) {
+Layout layout(int64_t M, int E, int64_t I, int64_t Is, int topk, bool fp8) {
   auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   Layout l;
-  const int64_t slots = M * topk < E ? M * topk : E;
-  l.logits = 256;
-  l.h = l.logits + up(M * E * 4);
-  l.bytes = l.h + up((slots * I + Is) * kTokens * 2);
+  const int64_t slots = M * topk < E ? M * topk : E, outputs = slots * I + Is;
+  l.counters = 4 + (fp8 ? outputs / 128 : 0);
+  l.scores = up(l.counters * 4);
+  l.h = l.scores + up(M * E * 4);
+  l.h8 = l.h + up(outputs * kTokens * 2);
+  l.h8_scale = l.h8 + (fp8 ? up(outputs * kTokens) : 0);
+  l.bytes = l.h8_scale + (fp8 ? up(outputs / 128 * kTokens * 4) : 0);
   return l;
 }
 
@@ -739,7 +814,7 @@ template <typename XT, typename WT>
 int run_router(const Few& P, const void* w, cudaStream_t st) {
 #define MOE_FEW_ROUTER(ROWS)                                                                                                             \
   launch_pdl(few_router_kernel<XT, WT, ROWS>, dim3((unsigned)P.E), 128, 0, 1, st, "fused_moe_few_tokens (router)", (const XT*)P.x, P.x_ld, \
-             (const WT*)w, P.M, P.E, P.H, const_cast<float*>(P.logits), P.counters)
+             (const WT*)w, P.M, P.E, P.H, P.sigmoid, const_cast<float*>(P.scores), P.counters, P.cleared)
   if (P.M == 1) return MOE_FEW_ROUTER(1);
   if (P.M == 2) return MOE_FEW_ROUTER(2);
   if (P.M <= 4) return MOE_FEW_ROUTER(4);
@@ -774,11 +849,11 @@ int run_experts(Few P, cudaStream_t st) {
 }  // namespace
 }  // namespace moe
 
-extern "C" int moe_few_tokens_workspace(int64_t M, int E, int64_t I, int64_t shared_I, int topk, int64_t* bytes) {
+extern "C" int moe_few_tokens_workspace(int64_t M, int E, int64_t I, int64_t shared_I, int topk, int fp8, int64_t* bytes) {
   using namespace moe;
   if (M < 0 || M > kTokens || E <= 0 || E > kMaxExperts || I <= 0 || shared_I < 0 || topk <= 0 || topk > 32 || !bytes)
     return fail(MOE_E_BADARG, "few_tokens_workspace: bad extent");
-  *bytes = layout(M, E, I, shared_I, topk).bytes;
+  *bytes = layout(M, E, I, shared_I, topk, fp8 != 0).bytes;
   return 0;
 }
 
@@ -809,16 +884,16 @@ extern "C" int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void
     if ((uintptr_t)p & 31) return fail(MOE_E_BADARG, "%s: weights must be 32-byte aligned", who);
   for (const void* p : {x, router, (const void*)workspace})
     if ((uintptr_t)p & 15) return fail(MOE_E_BADARG, "%s: operands must be 16-byte aligned", who);
-  const Layout l = layout(M, E, I, shared_I, topk);
+  const Layout l = layout(M, E, I, shared_I, topk, fp8);
   if (workspace_bytes < l.bytes) return fail(MOE_E_BADARG, "%s: workspace too small", who);
   uint8_t* ws = (uint8_t*)workspace;
   Few P = {};
   P.x = x; P.x_ld = x_ld; P.residual = residual; P.residual_ld = residual_ld; P.out = out;
   P.w1 = w1; P.w2 = w2; P.sw1 = shared_w1; P.sw2 = shared_w2;
   P.w1s = w1_scale; P.w2s = w2_scale; P.sw1s = shared_w1_scale; P.sw2s = shared_w2_scale;
-  P.logits = (const float*)(ws + l.logits); P.bias = bias;
+  P.scores = (const float*)(ws + l.scores); P.bias = bias;
   P.topk_w = topk_weights; P.topk_ids = topk_ids;
-  P.h = ws + l.h; P.counters = (int32_t*)ws;
+  P.h = ws + l.h; P.h8 = ws + l.h8; P.h8_scale = (float*)(ws + l.h8_scale); P.counters = (int32_t*)ws; P.cleared = l.counters;
   P.M = (int)M; P.E = E; P.H = H; P.I = I; P.Is = shared_I; P.topk = topk; P.n_group = n_group; P.topk_group = topk_group;
   P.renormalize = renormalize; P.sigmoid = sigmoid; P.scaling = scaling;
   P.status = status; P.wait_ns = wait_limit_ns();

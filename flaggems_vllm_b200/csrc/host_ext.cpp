@@ -950,7 +950,7 @@ PyObject* few_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Unlocked unlocked;
     c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     int64_t bytes = 0;
-    must(moe_few_tokens_workspace(M, (int)E, I, Is, (int)topk, &bytes));
+    must(moe_few_tokens_workspace(M, (int)E, I, Is, (int)topk, fp8, &bytes));
     out = fresh({M, H}, x.scalar_type(), dev);
     tw = fresh({M, topk}, at::kFloat, dev);
     ti = fresh({M, topk}, at::kInt, dev);

@@ -542,7 +542,7 @@ int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld, const voi
  * [E, 2I/128, H/128] and so on), e4m3: x and the intermediate are then taken in e4m3 too, in groups of 128.  shared_I = 0: none.
  * Sizes in multiples of 64, in e4m3 128; at most 1024 experts, topk 32.  Weights 32-byte aligned.  out [M, H], topk_weights fp32 and
  * topk_ids int32 [M, topk] without gaps.  out shares no memory with an operand. */
-int moe_few_tokens_workspace(int64_t M, int E, int64_t I, int64_t shared_I, int topk, int64_t* bytes /* host */);
+int moe_few_tokens_workspace(int64_t M, int E, int64_t I, int64_t shared_I, int topk, int fp8, int64_t* bytes /* host */);
 int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void* router, int router_dtype, const float* bias, const void* w1,
                    const void* w2, const float* w1_scale, const float* w2_scale, const void* shared_w1, const void* shared_w2,
                    const float* shared_w1_scale, const float* shared_w2_scale, const void* residual, int64_t residual_ld, int64_t M,

@@ -20,7 +20,7 @@ HOST_EXT = os.path.join(HERE, "_host_ext.so")
 STAMP = LIB + ".srchash"
 SOURCES = ["common.cu", "grouped_topk.cu", "topk_route.cu", "align.cu", "quant.cu", "gemm_simt.cu", "gemm_tc.cu",
            "gemm_wt.cu", "gemm_w8t.cu", "plan.cu", "route_rows.cu", "layer.cu", "gemm_w8.cu", "gemm_small.cu", "gemm_api.cu", "router_gemm.cu", "ep_pack.cu",
-           "rms_norm.cu", "balance.cu", "linear.cu", "few_tokens.cu"]
+           "rms_norm.cu", "balance.cu", "linear.cu", "few_tokens.cu", "few_tokens_fp8.cu"]
 
 
 def _nvcc() -> str:

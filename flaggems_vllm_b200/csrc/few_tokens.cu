@@ -16,46 +16,19 @@
 // and the warps of a block divide the run of (tile, k step) evenly, joining the tiles that they share in a fixed order.  W2: the
 // warps divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in registers.
 //
-// FP8 (128 x 128 block scales): activations in groups of 128 as per_token_group_quant_fp8 has them, h after its rounding to the
-// activations' type, as in the layer of many tokens (quantise_groups); every 128 k are folded with both scales in fp32.
+// Weights in e4m3 take few_tokens_fp8.cu behind the router.
 //
 // A block waits for others once, between W1 and W2.  Work is claimed from counters, and a block waits only for work that some running
 // block has claimed: it needs no co-residency, and two calls on two streams cannot wait for each other.  The wait has the
 // library's limit.
-#include <type_traits>
-
-#include "route_row.cuh"
-#include "tc_common.cuh"
+#include "few_tokens.cuh"
 
 namespace moe {
 namespace {
 using namespace tc;
 
-constexpr int kTokens = 8, kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kMaxSlots = 256;   // routed experts of a call: 8 tokens x 32
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kRunTiles = 4096;  // tiles of W1 in a block's run, at most
-constexpr int kMaxExperts = 1024, kMaxHidden = 16384, kMaxHidden8 = 8192, kMaxWidth = 1 << 22;
-
-struct Few {
-  const void *x, *residual;
-  void* out;
-  const void *w1, *w2, *sw1, *sw2;              // sw: shared expert
-  const float *w1s, *w2s, *sw1s, *sw2s;         // block scales
-  const float *scores, *bias;                   // [M, E] sigmoids, or logits of a softmax
-  float* topk_w;
-  int32_t* topk_ids;
-  void* h;                                      // [slots][8][I], then the shared expert's [8][Is]
-  uint8_t* h8;                                  // the same in 8 bits, and the scales of its groups
-  float* h8_scale;
-  int32_t* counters;                            // claims of W1 and W2, finished runs of W1, one unused, outputs of each group of 128
-  int64_t cleared;                              // counters to clear
-  int64_t x_ld, residual_ld;
-  int M, E, H, I, Is, topk, n_group, topk_group, renormalize, sigmoid;
-  float scaling;
-  int x_pitch, staged;                          // bytes of a token's row in shared memory; whether the rows are there
-  int32_t* status;
-  unsigned long long wait_ns;
-};
 
 __device__ __forceinline__ void mma8(float (&d)[4], std::integral_constant<int, 0>, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -65,25 +38,8 @@ __device__ __forceinline__ void mma8(float (&d)[4], std::integral_constant<int, 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma8(float (&d)[4], std::integral_constant<int, 2>, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <typename T, bool FP8> using Kind = std::integral_constant<int, FP8 ? 2 : (std::is_same<T, __nv_bfloat16>::value ? 0 : 1)>;
+template <typename T> using Kind = std::integral_constant<int, std::is_same<T, __nv_bfloat16>::value ? 0 : 1>;
 
-struct B32 {  // 32 bytes of a row
-  uint32_t r[8];
-};
-__device__ __forceinline__ void zero(B32& v) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v.r[i] = 0;
-}
-// 16 bytes from p on and 16 from p + APART on, in shared or global memory
-template <int APART>
-__device__ __forceinline__ void load_row(B32& v, const void* p) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + APART);
-  v.r[0] = a.x; v.r[1] = a.y; v.r[2] = a.z; v.r[3] = a.w; v.r[4] = b.x; v.r[5] = b.y; v.r[6] = b.z; v.r[7] = b.w;
-}
 // 16 rows (lo: this lane's row of the first eight, hi: of the others) times 8 tokens over the 128 bytes that four lanes hold
 template <typename KIND>
 __device__ __forceinline__ void multiply(float (&d)[4], const B32& lo, const B32& hi, const B32& x) {
@@ -97,9 +53,6 @@ __device__ __forceinline__ uint32_t place(int row, int piece) { return (uint32_t
 __device__ __forceinline__ void copy16(uint32_t at, const void* p) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(at), "l"(p) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t at, const void* p) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(p) : "memory");
-}
 __device__ __forceinline__ void take16(uint32_t* r, uint32_t at) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -112,34 +65,6 @@ __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_
 template <int PENDING> __device__ __forceinline__ void wait_copies() {  // of all lanes
   asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
   __syncwarp();
-}
-
-__device__ __forceinline__ int claim(int32_t* counter) { return atomicAdd(counter, 1); }
-
-template <typename T> __device__ __forceinline__ float2 widen2(uint32_t v);
-template <> __device__ __forceinline__ float2 widen2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
-template <> __device__ __forceinline__ float2 widen2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-
-// 32 values of a lane, 128 of the four lanes of a group: their e4m3 bytes and the group's scale
-template <typename T>
-__device__ __forceinline__ float quantise(const B32 (&v)[2], B32& q) {
-  float m = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 f = widen2<T>(v[i >> 3].r[i & 7]);
-    m = max_nan(m, max_nan(fabsf(f.x), fabsf(f.y)));
-  }
-  m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-  m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-  const float s = (m > kQuantEps || m != m ? m : kQuantEps) * (1.0f / kFp8Max), inv = 1.0f / s;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 a = widen2<T>(v[i >> 2].r[2 * i & 7]), b = widen2<T>(v[i >> 2].r[(2 * i + 1) & 7]);
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(div_by_scale(a.x, s, inv), div_by_scale(a.y, s, inv)), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(div_by_scale(b.x, s, inv), div_by_scale(b.y, s, inv)), __NV_SATFINITE, __NV_E4M3);
-    q.r[i] = lo | hi << 16;
-  }
-  return s;
 }
 
 // ------------------------------------------------------------------ logits
@@ -187,137 +112,38 @@ __global__ void __launch_bounds__(128) few_router_kernel(const XT* __restrict__ 
 }
 
 // ------------------------------------------------------------------ experts
-struct Shared {
-  float weight[kMaxSlots + 1][kTokens];   // of every routed expert for the tokens that it has; the shared expert's are 1
-  uint32_t mask[kMaxSlots + 1];           // tokens of the expert
-  int32_t list[kMaxSlots];                // routed experts, ascending
-  uint32_t used[kMaxExperts / 32];        // a bit for each
-  float bias[kMaxExperts];
-  float w[kTokens][32];
-  int32_t id[kTokens][32];
-  int32_t whole[kMaxSlots];               // groups of h that this block has to quantise
-  int32_t slots, next1, next2, wholes;
-};
 constexpr int kPartBytes = kWarps * 4 * 512;  // partial sums: two tiles of W1 a warp, four of W2
-// W1's ring: a unit is a tile's 128 bytes of k, 2 KB, and in 8 bits its scales
-template <bool FP8> struct Ring1 {
-  static constexpr int UNITS = 7, SLOT = 2048 + (FP8 ? 64 : 0), BYTES = UNITS * SLOT;
+// W1's ring: a unit is a tile's 128 bytes of k, 2 KB
+struct Ring1 {
+  static constexpr int UNITS = 7, BYTES = UNITS * 2048;
 };
-// W2's: a unit is 16 rows' 128 bytes of k; a step's h, and in 8 bits its scales and W2's, come with its first unit.  As many as fit
-template <bool FP8, int RT> struct Ring2 {
-  static constexpr int UNITS = RT == 1 ? 7 : 8, STEPS = (UNITS + RT - 1) / RT + 1;
-  static constexpr int H_SLOT = FP8 ? 1024 + 64 : 1024, BYTES = UNITS * 2048 + STEPS * H_SLOT;
+// W2's: a unit is 16 rows' 128 bytes of k; a step's h comes with its first unit.  As many as fit
+template <int RT> struct Ring2 {
+  static constexpr int UNITS = RT == 1 ? 7 : 8, STEPS = (UNITS + RT - 1) / RT + 1, BYTES = UNITS * 2048 + STEPS * 1024;
 };
-
-// What routing needs and the kernel in front does not make
-__device__ __forceinline__ void prepare_route(const Few& P, Shared& S) {
-  for (int e = threadIdx.x; e < P.E; e += kThreads) S.bias[e] = P.bias ? P.bias[e] : 0.0f;
-  for (int i = threadIdx.x; i < kMaxSlots; i += kThreads) S.mask[i] = 0;
-  if (threadIdx.x < kMaxExperts / 32) S.used[threadIdx.x] = 0;
-  __syncthreads();
-}
-// every token's experts, by a warp each; the list of all of them
-template <int VPT>
-__device__ __forceinline__ void route(const Few& P, Shared& S, float* scratch) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < P.M) {
-    const float* u = P.scores + (int64_t)warp * P.E;
-    if (!P.sigmoid) {
-      float l[VPT], m = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        l[j] = j * 32 + lane < P.E ? u[j * 32 + lane] : -INFINITY;
-        m = fmaxf(m, l[j]);
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
-      float* s = scratch + warp * P.E;
-      double sum = 0.0;
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        if (j * 32 + lane < P.E) {
-          const double x = exp((double)l[j] - (double)m);
-          sum += x;
-          l[j] = (float)x;
-        }
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
-      const double inv = 1.0 / sum;
-#pragma unroll
-      for (int j = 0; j < VPT; ++j)
-        if (j * 32 + lane < P.E) s[j * 32 + lane] = (float)(l[j] * inv);
-      __syncwarp();
-      u = s;
-    }
-    route_row<float, float, VPT>(u, 1, S.bias, P.E, P.n_group, P.topk_group, P.topk, P.renormalize, P.scaling, 0, S.w[warp], S.id[warp], lane);
-    __syncwarp();
-    if (lane < P.topk) {
-      const int id = S.id[warp][lane];
-      atomicOr(&S.used[id >> 5], 1u << (id & 31));
-      if (blockIdx.x == 0) {
-        P.topk_w[warp * P.topk + lane] = S.w[warp][lane];
-        P.topk_ids[warp * P.topk + lane] = id;
-      }
-    }
-  }
-  __syncthreads();
-  // an expert's place is the number of used ones below it; lane i has those of the first 32 i
-  const uint32_t word = S.used[lane];
-  int below = __popc(word);
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int v = __shfl_up_sync(0xFFFFFFFFu, below, off);
-    if (lane >= off) below += v;
-  }
-  const int slots = __shfl_sync(0xFFFFFFFFu, below, 31);
-  below -= __popc(word);
-  if (warp < P.M) {
-    const int id = lane < P.topk ? S.id[warp][lane] : 0;
-    const int s = __shfl_sync(0xFFFFFFFFu, below, id >> 5) + __popc(S.used[id >> 5] & ((1u << (id & 31)) - 1));
-    if (lane < P.topk) {
-      S.list[s] = id;
-      S.weight[s][warp] = S.w[warp][lane];
-      atomicOr(&S.mask[s], 1u << warp);
-    }
-  }
-  if (warp == 0) {
-    if (lane < kTokens) S.weight[slots][lane] = 1.0f;
-    if (lane == 0) {
-      S.slots = slots;
-      S.mask[slots] = (1u << P.M) - 1;  // nobody's slot
-    }
-  }
-  __syncthreads();
-}
 
 // Rows [lo, hi) of all experts' W1, counted in outputs: routed experts one behind another, then the shared one.
-template <typename T, bool FP8>
-__device__ __forceinline__ void first_product(const Few& P, const Shared& S, const uint8_t* xrows, const float* xscale, float* part, uint32_t ring,
-                                              int64_t lo, int64_t hi) {
-  using R = Ring1<FP8>;
-  constexpr int ES = FP8 ? 1 : 2;
-  using KIND = Kind<T, FP8>;
+template <typename T>
+__device__ __forceinline__ void first_product(const Few& P, const Shared& S, const uint8_t* xrows, float* part, uint32_t ring, int64_t lo, int64_t hi) {
+  using R = Ring1;
+  using KIND = Kind<T>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int KB = P.H * ES / 128, tiles = (int)((hi - lo + 7) / 8), total = tiles * KB;
+  const int KB = P.H / 64, tiles = (int)((hi - lo + 7) / 8), total = tiles * KB;
   auto bound = [&](int w) { return (int)((int64_t)total * w / kWarps); };
   const int begin = bound(warp), end = bound(warp + 1);
-  const int64_t routed = (int64_t)S.slots * P.I, row_bytes = (int64_t)P.H * ES;
-  const int sblocks = P.H / 128;
+  const int64_t routed = (int64_t)S.slots * P.I, row_bytes = (int64_t)P.H * 2;
   ring += (uint32_t)warp * R::BYTES;
   const int cr = lane >> 3, cq = lane & 7;  // what this lane copies: piece cq of rows cr and cr + 4
   // output o of all experts': its gate row, and how far behind it the up row is
   struct Row {
     const uint8_t* gate;
     int64_t up;
-    const float *gs, *us;  // scales of the rows' blocks
   };
   auto row_of = [&](int64_t o) {
-    Row r = {nullptr, 0, nullptr, nullptr};
+    Row r = {nullptr, 0};
     if (o >= hi) return r;
     int64_t p;  // output inside the expert
     const uint8_t* base;
-    const float* scales;
     int width;
     if (o < routed) {
       const int s = (int)((uint32_t)o / (uint32_t)P.I);
@@ -325,35 +151,24 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
       const int64_t e = S.list[s];
       width = P.I;
       base = reinterpret_cast<const uint8_t*>(P.w1) + e * 2 * width * row_bytes;
-      scales = FP8 ? P.w1s + e * (2 * width / 128) * sblocks : nullptr;
     } else {
       p = o - routed;
       width = P.Is;
       base = reinterpret_cast<const uint8_t*>(P.sw1);
-      scales = P.sw1s;
     }
     r.gate = base + p * row_bytes;
     r.up = width * row_bytes;
-    if constexpr (FP8) {
-      r.gs = scales + p / 128 * sblocks;
-      r.us = scales + (p + width) / 128 * sblocks;
-    }
     return r;
   };
   int lt = begin / KB, lk = begin - lt * KB;  // where copying stands
   const uint8_t* src[2];
   int64_t up[2];
-  const float* scale = nullptr;
   auto enter = [&] {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const Row r = row_of(lo + 8 * (int64_t)lt + cr + 4 * j);
       src[j] = r.gate;
       up[j] = r.up;
-    }
-    if constexpr (FP8) {  // lanes 0 to 15: of the eight gate and the eight up rows
-      const Row r = row_of(lo + 8 * (int64_t)lt + cq);
-      scale = lane < 8 ? r.gs : (lane < 16 ? r.us : nullptr);
     }
   };
   enter();
@@ -366,7 +181,6 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
         copy16(slot + 1024 + place(cr + 4 * j, cq), p + up[j]);
       }
     }
-    if (FP8 && scale != nullptr) copy4(slot + 2048 + lane * 4, scale + lk);
     if (++lk == KB) {
       lk = 0;
       ++lt;
@@ -375,7 +189,7 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
   };
 #pragma unroll 1
   for (int d = 0; d < R::UNITS - 1; ++d) {
-    if (begin + d < end) copy(ring + d * R::SLOT);
+    if (begin + d < end) copy(ring + d * 2048);
     commit_copies();
   }
   auto finish = [&](int tile, const float4& v) {
@@ -402,10 +216,10 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
 #pragma unroll 1
   for (int i = begin; i < end; ++i) {
     wait_copies<R::UNITS - 2>();
-    if (i + R::UNITS - 1 < end) copy(ring + to * R::SLOT);  // the slot that the last step has read
+    if (i + R::UNITS - 1 < end) copy(ring + to * 2048);  // the slot that the last step has read
     commit_copies();
     if (++to == R::UNITS) to = 0;
-    const uint32_t slot = ring + at * R::SLOT;
+    const uint32_t slot = ring + at * 2048;
     if (++at == R::UNITS) at = 0;
     B32 x, wg, wu;
     take(wg, slot, g, c);
@@ -414,19 +228,8 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
     else zero(x);
     float p[4] = {};
     multiply<KIND>(p, wg, wu, x);
-    if constexpr (FP8) {
-      const float s0 = xscale[(2 * c) * sblocks + kb], s1 = xscale[(2 * c + 1) * sblocks + kb];
-      float sg, su;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sg) : "r"(slot + 2048 + g * 4) : "memory");
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(su) : "r"(slot + 2080 + g * 4) : "memory");
-      acc[0] = fmaf(p[0], s0 * sg, acc[0]);
-      acc[1] = fmaf(p[1], s1 * sg, acc[1]);
-      acc[2] = fmaf(p[2], s0 * su, acc[2]);
-      acc[3] = fmaf(p[3], s1 * su, acc[3]);
-    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] += p[j];
-    }
+    for (int j = 0; j < 4; ++j) acc[j] += p[j];
     if (++kb == KB || i + 1 == end) {
       const float4 v = make_float4(acc[0], acc[1], acc[2], acc[3]);
       const bool from_start = tile * KB >= begin;
@@ -453,83 +256,21 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
   }
 }
 
-// 8 bits: a group's scale needs all of its 128 outputs, which several blocks may have made.  Whoever adds the last ones quantises the
-// group, once for all blocks that read it.  (Done by every reader on its way into W2's products it cost 240 instructions a step:
-// 6 tokens of 256 experts of 2048 x 7168, 367 us; XXX so.)
-template <typename T>
-__device__ __forceinline__ void quantise_groups(const Few& P, Shared& S, int64_t lo, int64_t hi) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t last = hi > lo ? (hi - 1) / 128 : -1;
-  for (int64_t first = lo / 128; first <= last; first += kMaxSlots) {
-    __syncthreads();  // this block's h is written; the list has been read
-    if (threadIdx.x == 0) S.wholes = 0;
-    __syncthreads();
-    const int64_t g = first + threadIdx.x;
-    if (threadIdx.x < kMaxSlots && g <= last) {
-      const int64_t a = g * 128 > lo ? g * 128 : lo, z = (g + 1) * 128 < hi ? (g + 1) * 128 : hi;
-      const int mine = (int)(z - a);
-      __threadfence();
-      const int old = atomicAdd(P.counters + 4 + g, mine);
-      __threadfence();
-      if (old + mine == 128) S.whole[atomicAdd(&S.wholes, 1)] = (int)(g - first);
-    }
-    __syncthreads();
-    const int n = S.wholes;
-    const int64_t routed = (int64_t)S.slots * P.I;
-    for (int i = warp; i < n; i += kWarps) {
-      const int64_t o = (first + S.whole[i]) * 128;
-      int s = S.slots;
-      int64_t width = P.Is, p = o - routed;
-      if (o < routed) {
-        s = (int)((uint32_t)o / (uint32_t)P.I);
-        width = P.I;
-        p = o - (int64_t)s * P.I;
-      }
-      const int m = lane >> 2, c = lane & 3;
-      const int64_t at = (int64_t)s * kTokens * P.I + m * width + p + c * 32;
-      B32 v[2], q;
-      zero(v[0]);
-      zero(v[1]);
-      const bool mine = (S.mask[s] >> m) & 1;
-      if (mine) {
-        const uint4* h = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.h) + at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 w = __ldcg(h + j);  // other blocks' stores: past L1
-          uint32_t* r = v[j >> 1].r + 4 * (j & 1);
-          r[0] = w.x; r[1] = w.y; r[2] = w.z; r[3] = w.w;
-        }
-      }
-      const float scale = quantise<T>(v, q);
-      if (mine) {
-        uint4* d = reinterpret_cast<uint4*>(P.h8 + at);
-        d[0] = make_uint4(q.r[0], q.r[1], q.r[2], q.r[3]);
-        d[1] = make_uint4(q.r[4], q.r[5], q.r[6], q.r[7]);
-        if (c == 0) P.h8_scale[((int64_t)s * kTokens * P.I + m * width + p) / 128] = scale;
-      }
-    }
-  }
-}
-
 // Rows [lo, hi) of W2, at most 16 RT, of all experts, and the output columns that they are.  `wait`: returns when h is there
-template <typename T, bool FP8, int RT, typename Wait>
+template <typename T, int RT, typename Wait>
 __device__ __forceinline__ void second_product(const Few& P, const Shared& S, float* part, uint32_t ring, int lo, int hi, Wait wait) {
-  using R = Ring2<FP8, RT>;
-  constexpr int ES = FP8 ? 1 : 2;
-  using KIND = Kind<T, FP8>;
+  using R = Ring2<RT>;
+  using KIND = Kind<T>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int KB = P.I * ES / 128, SB = P.Is * ES / 128, routed = S.slots * KB, total = routed + SB;
+  const int KB = P.I / 64, SB = P.Is / 64, routed = S.slots * KB, total = routed + SB;
   const int begin = (int)((int64_t)total * warp / kWarps), end = (int)((int64_t)total * (warp + 1) / kWarps);
-  const int block = lo >> 7, blocks = P.H >> 7;
   ring += (uint32_t)warp * R::BYTES;
   const uint32_t hring = ring + R::UNITS * 2048;
   struct At {
     int s, kb, KB;
     const uint8_t* w;  // this lane's piece of row lo + cr
     int64_t row;       // bytes of a row
-    const float* ws;
-    const uint8_t* h;  // the expert's, as it is multiplied
-    const float* hs;
+    const uint8_t* h;  // the expert's
   };
   const int cr = lane >> 3, cq = lane & 7;  // what this lane copies: piece cq of rows cr, cr + 4, ..
   auto enter = [&](int s, int kb) {  // expert s, S.slots = the shared one
@@ -539,12 +280,10 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     const bool shared = s == S.slots;
     const int width = shared ? P.Is : P.I;
     a.KB = shared ? SB : KB;
-    a.row = (int64_t)width * ES;
+    a.row = (int64_t)width * 2;
     const int64_t e = shared ? 0 : S.list[s];
     a.w = reinterpret_cast<const uint8_t*>(shared ? P.sw2 : P.w2) + (e * P.H + lo + cr) * a.row + cq * 16;
-    a.ws = FP8 ? (shared ? P.sw2s : P.w2s) + (e * blocks + block) * (int64_t)(width / 128) : nullptr;
-    a.h = (FP8 ? P.h8 : reinterpret_cast<const uint8_t*>(P.h)) + (int64_t)s * kTokens * P.I * ES;  // the shared expert's lies behind the others'
-    a.hs = FP8 ? P.h8_scale + (int64_t)s * kTokens * (P.I / 128) : nullptr;
+    a.h = reinterpret_cast<const uint8_t*>(P.h) + (int64_t)s * kTokens * P.I * 2;  // the shared expert's lies behind the others'
     return a;
   };
   auto locate = [&](int i) { return i < routed ? enter(i / KB, i % KB) : enter(S.slots, i - routed); };
@@ -561,14 +300,6 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       if ((mask >> (4 * j + cr)) & 1) copy16(slot + place(4 * j + cr, cq), a.h + (4 * j + cr) * a.row + a.kb * 128 + cq * 16);
-    if constexpr (FP8) {
-      const int64_t groups = a.row / 128;
-      if (lane < kTokens) {
-        if ((mask >> lane) & 1) copy4(slot + 1024 + lane * 4, a.hs + lane * groups + a.kb);
-      } else if (lane < kTokens + 2 && block + lane - kTokens < blocks) {
-        copy4(slot + 1024 + lane * 4, a.ws + (lane - kTokens) * groups + a.kb);
-      }
-    }
   };
   const int units = (end - begin) * RT;
   At ld = locate(begin < total ? begin : total - 1), at = ld;
@@ -590,7 +321,7 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     for (int u = 0; u < R::UNITS - 1; ++u) {
       if (u < units) {
         if (t == 0) {
-          copy_h(a, hring + hto * R::H_SLOT);
+          copy_h(a, hring + hto * 1024);
           if (++hto == R::STEPS) hto = 0;
         }
         if (++t == RT) {
@@ -605,7 +336,7 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     if (lu < units) {
       copy(ld, lt, ring + to * 2048);
       if (lt == 0) {
-        copy_h(ld, hring + hto * R::H_SLOT);
+        copy_h(ld, hring + hto * 1024);
         if (++hto == R::STEPS) hto = 0;
       }
       if (++to == R::UNITS) to = 0;
@@ -626,19 +357,11 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
     float f0 = r0 ? S.weight[at.s][2 * c] : 0.0f, f1 = r1 ? S.weight[at.s][2 * c + 1] : 0.0f;
     wait_copies<R::UNITS - 2>();
     next();
-    const uint32_t hs = hring + hfrom * R::H_SLOT;
+    const uint32_t hs = hring + hfrom * 1024;
     if (++hfrom == R::STEPS) hfrom = 0;
     B32 x;
     if ((mask >> g) & 1) take(x, hs, g, c);
     else zero(x);
-    float s0 = 0.0f, s1 = 0.0f;
-    if constexpr (FP8) {
-      float h0, h1;
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(h0), "=f"(h1) : "r"(hs + 1024 + c * 8) : "memory");
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(s0), "=f"(s1) : "r"(hs + 1024 + kTokens * 4) : "memory");
-      f0 *= h0;
-      f1 *= h1;
-    }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if (t > 0) {
@@ -652,10 +375,6 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
       float p[4] = {};
       multiply<KIND>(p, wa, wb, x);
       float a0 = f0, a1 = f1, b0 = f0, b1 = f1;
-      if constexpr (FP8) {
-        const float sa = (lo + 16 * t + g) >> 7 == block ? s0 : s1, sb = (lo + 16 * t + 8 + g) >> 7 == block ? s0 : s1;
-        a0 *= sa; a1 *= sa; b0 *= sb; b1 *= sb;
-      }
       // a token that is not the expert's takes nothing, whatever the weights hold
       if (r0) { acc[t][0] = fmaf(p[0], a0, acc[t][0]); acc[t][2] = fmaf(p[2], b0, acc[t][2]); }
       if (r1) { acc[t][1] = fmaf(p[1], a1, acc[t][1]); acc[t][3] = fmaf(p[3], b1, acc[t][3]); }
@@ -685,41 +404,16 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
   }
 }
 
-template <typename T, bool FP8, int RT>
+template <typename T, int RT>
 __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& S = *reinterpret_cast<Shared*>(smem);
   float* part = reinterpret_cast<float*>(smem + (sizeof(Shared) + 127) / 128 * 128);
   uint8_t* rest = reinterpret_cast<uint8_t*>(part) + kPartBytes;  // scores while routing, then W1's ring and the tokens, then W2's ring
-  uint8_t* xs = rest + kWarps * Ring1<FP8>::BYTES;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the tokens, older than the kernel in front: into shared memory, in 8 bits where the weights are
+  uint8_t* xs = rest + kWarps * Ring1::BYTES;
+  // the tokens, older than the kernel in front: into shared memory
   const uint8_t* xrows = xs;
-  float* xscale = nullptr;
-  if constexpr (FP8) {
-    const int blocks = P.H / 128;
-    xscale = reinterpret_cast<float*>(xs + P.M * P.x_pitch);
-    for (int i = threadIdx.x; i < (kTokens - P.M) * blocks; i += kThreads) xscale[P.M * blocks + i] = 0.0f;
-    const int groups = P.M * blocks;  // eight of them to a warp, four lanes each
-    for (int i0 = warp * 8; i0 < groups; i0 += 8 * kWarps) {
-      const int i = i0 + (lane >> 2), m = i / blocks, b = i - m * blocks;
-      B32 v[2], q;
-      zero(v[0]);
-      zero(v[1]);
-      if (i < groups) {
-        const T* p = reinterpret_cast<const T*>(P.x) + m * P.x_ld + b * 128 + (lane & 3) * 32;
-        load_row<16>(v[0], p);
-        load_row<16>(v[1], p + 16);
-      }
-      const float s = quantise<T>(v, q);
-      if (i < groups) {
-        uint4* d = reinterpret_cast<uint4*>(xs + m * P.x_pitch + b * 128 + (lane & 3) * 32);
-        d[0] = make_uint4(q.r[0], q.r[1], q.r[2], q.r[3]);
-        d[1] = make_uint4(q.r[4], q.r[5], q.r[6], q.r[7]);
-        if ((lane & 3) == 0) xscale[i] = s;
-      }
-    }
-  } else if (P.staged) {
+  if (P.staged) {
     const int pieces = P.H / 8;
     for (int i = threadIdx.x; i < P.M * pieces; i += kThreads) {
       const int m = i / pieces, k = i - m * pieces;
@@ -748,8 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
     const int run = S.next1;
     if (run >= runs1) break;
     if (threadIdx.x == 0) mine1 = claim(P.counters);
-    first_product<T, FP8>(P, S, xrows, xscale, part, smem_u32(rest), outputs * run / runs1, outputs * (run + 1) / runs1);
-    if constexpr (FP8) quantise_groups<T>(P, S, outputs * run / runs1, outputs * (run + 1) / runs1);
+    first_product<T>(P, S, xrows, part, smem_u32(rest), outputs * run / runs1, outputs * (run + 1) / runs1);
     __syncthreads();  // all of the run's h is written
     if (threadIdx.x == 0) {
       __threadfence();
@@ -760,15 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
   auto wait = [&] {
     if (waited) return;
     waited = true;
-    if (threadIdx.x == 0) {
-      unsigned long long t0 = 0;
-      for (uint32_t spins = 1;; ++spins) {
-        int done;
-        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(P.counters + 2) : "memory");
-        if (done >= runs1) break;
-        if ((spins & 0x3F) == 0 && wait_expired(t0, P.status, P.wait_ns)) break;  // goes on, on whatever is there
-      }
-    }
+    if (threadIdx.x == 0) wait_for_runs(P.counters + 2, runs1, P.status, P.wait_ns);
     __syncthreads();
   };
   const int runs2 = (P.H + 16 * RT - 1) / (16 * RT) > G ? (P.H + 16 * RT - 1) / (16 * RT) : G;
@@ -778,24 +463,18 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
     const int run = S.next2;
     if (run >= runs2) break;
     if (threadIdx.x == 0) mine2 = claim(P.counters + 1);
-    second_product<T, FP8, RT>(P, S, part, smem_u32(rest), (int)((int64_t)P.H * run / runs2), (int)((int64_t)P.H * (run + 1) / runs2), wait);
+    second_product<T, RT>(P, S, part, smem_u32(rest), (int)((int64_t)P.H * run / runs2), (int)((int64_t)P.H * (run + 1) / runs2), wait);
   }
 }
 
 constexpr int64_t kHead = (sizeof(Shared) + 127) / 128 * 128 + kPartBytes;
-constexpr int64_t kSmem = 232448;
-constexpr int kScores = kTokens * kMaxExperts * 4;
-static_assert(kScores <= kWarps * Ring1<false>::BYTES && kScores <= kWarps * Ring1<true>::BYTES, "the scores lie in front of the tokens");
-static_assert(kHead + kWarps * Ring2<true, 1>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 1>::BYTES <= kSmem, "ring of W2");
-static_assert(kHead + kWarps * Ring2<true, 2>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 2>::BYTES <= kSmem, "ring of W2");
-static_assert(kHead + kWarps * Ring2<true, 4>::BYTES <= kSmem && kHead + kWarps * Ring2<false, 4>::BYTES <= kSmem, "ring of W2");
-// 8-bit tokens: their rows, and scales for all eight
-constexpr int64_t tokens_bytes(int64_t M, int64_t H, bool fp8) { return M * (H * (fp8 ? 1 : 2) + 64) + (fp8 ? kTokens * (H / 128) * 4 : 0); }
-static_assert(kHead + kWarps * Ring1<true>::BYTES + tokens_bytes(kTokens, kMaxHidden8, true) <= kSmem, "8-bit tokens fit shared memory");
+static_assert(kTokens * kMaxExperts * 4 <= kWarps * Ring1::BYTES, "the scores of a softmax lie in front of the tokens");
+static_assert(kHead + kWarps * Ring2<1>::BYTES <= kFewSmem && kHead + kWarps * Ring2<2>::BYTES <= kFewSmem &&
+                  kHead + kWarps * Ring2<4>::BYTES <= kFewSmem, "ring of W2");
 
 // ------------------------------------------------------------------ host side
 struct Layout {
-  int64_t counters, scores, h, h8, h8_scale, bytes;
+  int64_t counters, scores, h, h8, h8_shared, h8_scale, h8_scale_shared, bytes;
 };
 Layout layout(int64_t M, int E, int64_t I, int64_t Is, int topk, bool fp8) {
   auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
@@ -805,8 +484,10 @@ Layout layout(int64_t M, int E, int64_t I, int64_t Is, int topk, bool fp8) {
   l.scores = up(l.counters * 4);
   l.h = l.scores + up(M * E * 4);
   l.h8 = l.h + up(outputs * kTokens * 2);
-  l.h8_scale = l.h8 + (fp8 ? up(outputs * kTokens) : 0);
-  l.bytes = l.h8_scale + (fp8 ? up(outputs / 128 * kTokens * 4) : 0);
+  l.h8_shared = l.h8 + (fp8 ? up(slots * I * kTokens) : 0);
+  l.h8_scale = l.h8_shared + (fp8 ? up(Is * kTokens) : 0);
+  l.h8_scale_shared = l.h8_scale + (fp8 ? up(slots * I / 128 * kTokens * 4) : 0);
+  l.bytes = l.h8_scale_shared + (fp8 ? up(Is / 128 * kTokens * 4) : 0);
   return l;
 }
 
@@ -822,12 +503,12 @@ int run_router(const Few& P, const void* w, cudaStream_t st) {
 #undef MOE_FEW_ROUTER
 }
 
-template <typename T, bool FP8>
+template <typename T>
 int run_experts(Few P, cudaStream_t st) {
-  P.x_pitch = P.H * (FP8 ? 1 : 2) + 64;  // neighbouring tokens' pieces lie in other banks
-  const int64_t first = kHead + kWarps * Ring1<FP8>::BYTES;
-  int64_t smem = first + tokens_bytes(P.M, P.H, FP8);
-  P.staged = FP8 || smem <= kSmem;
+  P.x_pitch = P.H * 2 + 64;  // neighbouring tokens' pieces lie in other banks
+  const int64_t first = kHead + kWarps * Ring1::BYTES;
+  int64_t smem = first + (int64_t)P.M * P.x_pitch;
+  P.staged = smem <= kFewSmem;
   if (!P.staged) {  // the rows then come out of L1
     smem = first;
     P.x_pitch = (int)(P.x_ld * 2);
@@ -835,10 +516,10 @@ int run_experts(Few P, cudaStream_t st) {
   const int G = sm_count();
   const int rows = (P.H + G - 1) / G;
   auto go = [&](auto rt) {
-    auto kern = few_experts_kernel<T, FP8, decltype(rt)::value>;
-    const int rc = allow_smem((const void*)kern, (int)kSmem);
+    auto kern = few_experts_kernel<T, decltype(rt)::value>;
+    const int rc = allow_smem((const void*)kern, (int)kFewSmem);
     if (rc) return rc;
-    const int64_t second = kHead + kWarps * Ring2<FP8, decltype(rt)::value>::BYTES;
+    const int64_t second = kHead + kWarps * Ring2<decltype(rt)::value>::BYTES;
     return launch_pdl(kern, dim3((unsigned)G), kThreads, (size_t)(smem > second ? smem : second), 1, st, "fused_moe_few_tokens", P);
   };
   if (rows <= 16) return go(std::integral_constant<int, 1>());
@@ -893,7 +574,8 @@ extern "C" int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void
   P.w1s = w1_scale; P.w2s = w2_scale; P.sw1s = shared_w1_scale; P.sw2s = shared_w2_scale;
   P.scores = (const float*)(ws + l.scores); P.bias = bias;
   P.topk_w = topk_weights; P.topk_ids = topk_ids;
-  P.h = ws + l.h; P.h8 = ws + l.h8; P.h8_scale = (float*)(ws + l.h8_scale); P.counters = (int32_t*)ws; P.cleared = l.counters;
+  P.h = ws + l.h; P.h8 = ws + l.h8; P.h8_shared = ws + l.h8_shared; P.h8_scale = (float*)(ws + l.h8_scale);
+  P.h8_scale_shared = (float*)(ws + l.h8_scale_shared); P.counters = (int32_t*)ws; P.cleared = l.counters;
   P.M = (int)M; P.E = E; P.H = H; P.I = I; P.Is = shared_I; P.topk = topk; P.n_group = n_group; P.topk_group = topk_group;
   P.renormalize = renormalize; P.sigmoid = sigmoid; P.scaling = scaling;
   P.status = status; P.wait_ns = wait_limit_ns();
@@ -902,6 +584,6 @@ extern "C" int moe_few_tokens(const void* x, int64_t x_ld, int dtype, const void
   int rc = dtype == MOE_BF16 ? (f32 ? run_router<__nv_bfloat16, float>(P, router, st) : run_router<__nv_bfloat16, __nv_bfloat16>(P, router, st))
                              : (f32 ? run_router<__half, float>(P, router, st) : run_router<__half, __half>(P, router, st));
   if (rc) return rc;
-  if (dtype == MOE_BF16) return fp8 ? run_experts<__nv_bfloat16, true>(P, st) : run_experts<__nv_bfloat16, false>(P, st);
-  return fp8 ? run_experts<__half, true>(P, st) : run_experts<__half, false>(P, st);
+  if (fp8) return few_experts_fp8(P, dtype, st);
+  return dtype == MOE_BF16 ? run_experts<__nv_bfloat16>(P, st) : run_experts<__half>(P, st);
 }

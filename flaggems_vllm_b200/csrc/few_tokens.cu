@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& S = *reinterpret_cast<Shared*>(smem);
   float* part = reinterpret_cast<float*>(smem + (sizeof(Shared) + 127) / 128 * 128);
-  uint8_t* rest = reinterpret_cast<uint8_t*>(part) + kPartBytes;  // scores while routing, then W1's ring and the tokens, then W2's ring
+  uint8_t* rest = reinterpret_cast<uint8_t*>(part) + kPartBytes;  // routing, then W1's ring and the tokens, then W2's ring
   uint8_t* xs = rest + kWarps * Ring1::BYTES;
   // the tokens, older than the kernel in front: into shared memory
   const uint8_t* xrows = xs;
@@ -430,8 +430,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
     mine1 = claim(P.counters);
     mine2 = claim(P.counters + 1);
   }
-  if (P.E <= 256) route<8>(P, S, reinterpret_cast<float*>(rest));
-  else route<32>(P, S, reinterpret_cast<float*>(rest));
+  if (P.E <= 256) route<8>(P, S, reinterpret_cast<uint32_t*>(rest));
+  else route<32>(P, S, reinterpret_cast<uint32_t*>(rest));
 
   const int64_t outputs = (int64_t)S.slots * P.I + P.Is;
   const int G = gridDim.x;
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_experts_kernel(const Few P) {
 }
 
 constexpr int64_t kHead = (sizeof(Shared) + 127) / 128 * 128 + kPartBytes;
-static_assert(kTokens * kMaxExperts * 4 <= kWarps * Ring1::BYTES, "the scores of a softmax lie in front of the tokens");
+static_assert(kTokens * kMaxExperts * 4 <= kWarps * Ring1::BYTES, "what routing needs lies in front of the tokens");
 static_assert(kHead + kWarps * Ring2<1>::BYTES <= kFewSmem && kHead + kWarps * Ring2<2>::BYTES <= kFewSmem &&
                   kHead + kWarps * Ring2<4>::BYTES <= kFewSmem, "ring of W2");
 

@@ -111,41 +111,114 @@ __device__ __forceinline__ void prepare_route(const Few& P, Shared& S) {
   if (threadIdx.x < kMaxExperts / 32) S.used[threadIdx.x] = 0;
   __syncthreads();
 }
-// every token's experts, by a warp each; the list of all of them
+// The choice of one token by one warp: route_row's rule and order (route_row.cuh), in fewer steps of a lone warp, which takes four or
+// five clocks for each.  u: scores of expert 32 j + lane.  ranks: E words of the warp's own.
 template <int VPT>
-__device__ __forceinline__ void route(const Few& P, Shared& S, float* scratch) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < P.M) {
-    const float* u = P.scores + (int64_t)warp * P.E;
-    if (!P.sigmoid) {
-      float l[VPT], m = -INFINITY;
+__device__ __forceinline__ void choose(const Few& P, const Shared& S, const float (&u)[VPT], uint32_t* ranks, float* w_row, int32_t* id_row, int lane) {
+  uint64_t key[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int e = j * 32 + lane;
+    key[j] = e < P.E ? make_key(u[j] + S.bias[e], (uint32_t)e) : 0;
+  }
+  if (P.n_group > 1) {
+    const int per_group = P.E / P.n_group;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+      if (j * 32 + lane < P.E) ranks[j * 32 + lane] = (uint32_t)(key[j] >> 32);
+    __syncwarp();
+    // neighbouring lanes share a group; its two largest out of their own
+    const int share = P.n_group <= 4 ? 8 : (P.n_group <= 8 ? 4 : (P.n_group <= 16 ? 2 : 1));
+    const int group = lane / share;
+    uint32_t b1 = 0, b2 = 0;
+    if (group < P.n_group) {
+      for (int i = lane % share; i < per_group; i += share) {
+        const uint32_t v = ranks[group * per_group + i];
+        b2 = max(b2, min(b1, v));
+        b1 = max(b1, v);
+      }
+    }
+    for (int off = 1; off < share; off <<= 1) {
+      const uint32_t o1 = __shfl_xor_sync(0xFFFFFFFFu, b1, off), o2 = __shfl_xor_sync(0xFFFFFFFFu, b2, off);
+      b2 = max(max(b2, o2), min(b1, o1));
+      b1 = max(b1, o1);
+    }
+    const float score = per_group >= 2 ? from_ordered_bits(b1) + from_ordered_bits(b2) : from_ordered_bits(b1);
+    const uint32_t mine = ordered_bits(score);
+    int rank = 0;
+    for (int q = 0; q < P.n_group; ++q) {
+      const uint32_t other = __shfl_sync(0xFFFFFFFFu, mine, q * share);
+      rank += other > mine || (other == mine && q < group);
+    }
+    const uint32_t kept = __ballot_sync(0xFFFFFFFFu, group < P.n_group && rank < P.topk_group);  // bit q share: group q
+    const float inv = 1.0f / (float)per_group;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int e = j * 32 + lane, q = (int)(((float)e + 0.5f) * inv);  // e / per_group: both below 2^10
+      // experts of dropped groups rank as -inf (still ordered by index)
+      if (e < P.E && !((kept >> (q * share)) & 1u)) key[j] = make_key(__int_as_float(0xff800000), (uint32_t)e);
+    }
+  }
+  float my_w = 0.0f;
+  int32_t my_id = 0;
+  uint64_t local = 0;
+  float local_u = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j)
+    if (key[j] > local) { local = key[j]; local_u = u[j]; }
+  for (int t = 0; t < P.topk; ++t) {
+    const uint64_t best = warp_max_u64(local);
+    const uint32_t id = 0xFFFFFFFFu - (uint32_t)(best & 0xFFFFFFFFu);
+    const float w = __shfl_sync(0xFFFFFFFFu, local_u, id & 31);  // the lane that holds it
+    if (lane == t) { my_w = w; my_id = (int32_t)id; }
+    if (local == best) {  // consumed: the lane's next largest
+      local = 0;
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
-        l[j] = j * 32 + lane < P.E ? u[j * 32 + lane] : -INFINITY;
-        m = fmaxf(m, l[j]);
+        if (key[j] < best && key[j] > local) { local = key[j]; local_u = u[j]; }
       }
+    }
+  }
+  float sum = lane < P.topk ? my_w : 0.0f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+  if (lane < P.topk) {
+    w_row[lane] = (P.renormalize ? my_w / (sum + 1e-20f) : my_w) * P.scaling;
+    id_row[lane] = my_id;
+  }
+}
+
+// every token's experts, by a warp each; the list of all of them.  scratch: E words for each of eight warps
+template <int VPT>
+__device__ __forceinline__ void route(const Few& P, Shared& S, uint32_t* scratch) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < P.M) {
+    const float* row = P.scores + (int64_t)warp * P.E;
+    float u[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) u[j] = j * 32 + lane < P.E ? row[j * 32 + lane] : -INFINITY;
+    if (!P.sigmoid) {
+      float m = u[0];
+#pragma unroll
+      for (int j = 1; j < VPT; ++j) m = fmaxf(m, u[j]);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
-      float* s = scratch + warp * P.E;
       double sum = 0.0;
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
         if (j * 32 + lane < P.E) {
-          const double x = exp((double)l[j] - (double)m);
+          const double x = exp((double)u[j] - (double)m);
           sum += x;
-          l[j] = (float)x;
+          u[j] = (float)x;
         }
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
       const double inv = 1.0 / sum;
 #pragma unroll
-      for (int j = 0; j < VPT; ++j)
-        if (j * 32 + lane < P.E) s[j * 32 + lane] = (float)(l[j] * inv);
-      __syncwarp();
-      u = s;
+      for (int j = 0; j < VPT; ++j) u[j] = (float)(u[j] * inv);
     }
-    route_row<float, float, VPT>(u, 1, S.bias, P.E, P.n_group, P.topk_group, P.topk, P.renormalize, P.scaling, 0, S.w[warp], S.id[warp], lane);
+    choose<VPT>(P, S, u, scratch + warp * P.E, S.w[warp], S.id[warp], lane);
     __syncwarp();
     if (lane < P.topk) {
       const int id = S.id[warp][lane];

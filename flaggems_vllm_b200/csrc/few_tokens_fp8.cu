@@ -9,13 +9,13 @@
 // The tensor core cannot apply 128 x 128 block scales, so each 128 k go to an accumulator of their own, and two groups of four warps, in turn, add  accumulator * (token's scale * weight's scale)  to eight fp32 registers a lane,
 // a lane being a weight row.  8 columns make that cheap; for the layer of many tokens it would not be.
 //
-//   W1  a tile is up to 64 outputs of one expert: their gate rows and their up rows, in units of 8, so that a block's run of
-//       outputs, a multiple of 8, reads no row twice.  What the two groups hold is joined in shared memory at the tile's end.
+//   W1  a tile is up to 64 outputs: their gate rows and their up rows, in units of 8, so that a block's run of outputs, a multiple
+//       of 8, reads no row twice.  What the two groups hold is joined in shared memory at the tile's end.
 //   h   is rounded to the activations' type, as in the layer of many tokens, then quantised in groups of 128 by whichever block
 //       adds a group's last output: once for all blocks that read it.
 //   W2  a K block of all rows of the block's run (48 or 49 of 7168) is one box, with the same k of h.
 //
-// Warps: 0 TMA, 1 MMA, 2 TMEM, 4 to 11 the two groups.  W2's first weights are on their way while W1's results are still being
+// Warps: 0 and 3 TMA, in turn, 1 MMA, 2 TMEM, 4 to 11 the two groups.  W2's first weights are on their way while W1's results are still being
 // quantised and other blocks are waited for.
 #include "few_tokens.cuh"
 
@@ -25,17 +25,17 @@ using namespace tc;
 
 constexpr int kConsumers = 256, kThreads = 128 + kConsumers;
 // A stage is what one wait, one commit and one turn of a group of consumers are for: each of these costs its thread 100 to 200 clocks
-// whatever it is for, and an instruction of TMA another 90 (one K block of 128 a stage and boxes of 8 rows: 2.9 TB/s, bound by the
+// whatever it is for, and an instruction of TMA another 90 (one K block a stage and boxes of 8 rows: 2.9 TB/s, bound by the
 // thread that issues them).
 constexpr int kBlocks1 = 2, kBlocks2 = 4;  // K blocks of 128 in a stage of W1, of W2
 constexpr int kStage1 = kBlocks1 * 128 * 128;
-constexpr int kMaxStages = 8;
-constexpr int kAccs = 8, kAccCols = 16;    // accumulators of a stage's blocks, 16 columns each
+constexpr int kMaxStages = 12;
+constexpr int kAccs = 8, kAccCols = 16, kAccBlocks = kBlocks1 > kBlocks2 ? kBlocks1 : kBlocks2;    // accumulators of a stage's blocks, 16 columns each
 constexpr int kJoinBytes = 2 * 128 * kTokens * 4;
 
 struct Aux {
   uint64_t full1[kMaxStages], empty1[kMaxStages], full2[kMaxStages], empty2[kMaxStages], acc_full[kAccs], acc_empty[kAccs];
-  int32_t run1[2], run2[2];
+  int32_t run1[2], run2[2], more1;
   uint32_t tmem_base;
 };
 struct Few8 {
@@ -83,27 +83,22 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
       : "memory");
 }
 
-// outputs [o, o + n) of a run: up to 64 of one expert
-struct Tile {
-  int s, n;
-  int64_t p;  // the first one inside the expert
+// An output of all experts' W1: its expert, its place there
+struct Output {
+  int s, p, width;
 };
-__device__ __forceinline__ Tile tile_at(const Few& P, int slots, int64_t o, int64_t hi) {
+__device__ __forceinline__ Output output_at(const Few& P, int slots, int64_t o) {
   const int64_t routed = (int64_t)slots * P.I;
-  Tile t;
-  int64_t left;
-  if (o < routed) {
-    t.s = (int)((uint32_t)o / (uint32_t)P.I);
-    t.p = o - (int64_t)t.s * P.I;
-    left = P.I - t.p;
-  } else {
-    t.s = slots;
-    t.p = o - routed;
-    left = P.Is - t.p;
-  }
-  if (left > hi - o) left = hi - o;
-  t.n = left < 64 ? (int)left : 64;
-  return t;
+  if (o >= routed) return {slots, (int)(o - routed), P.Is};
+  const int s = (int)((uint32_t)o / (uint32_t)P.I);
+  return {s, (int)(o - (int64_t)s * P.I), P.I};
+}
+// Outputs of a tile that begins at o: a run is cut into equal tiles of at most 64, whatever experts they are of (every expert takes
+// the same tokens).  With tiles of one expert each, a run over a border had one tile more, whose small stages bring few bytes:
+// 47 us for W1 where the other blocks took 39.
+__device__ __forceinline__ int tile_size(int64_t o, int64_t hi) {
+  const int units = (int)((hi - o) / 8 < 1 << 20 ? (hi - o) / 8 : 1 << 20), tiles = (units + 7) / 8;
+  return (units + tiles - 1) / tiles * 8;
 }
 
 // 8 bits: a group's scale needs all of its 128 outputs, which several blocks may have made.  Whoever adds the last ones quantises the
@@ -189,7 +184,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&aux->tmem_base)), "r"(kAccs * kBlocks2 * kAccCols));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&aux->tmem_base)), "r"(kAccs * kAccBlocks * kAccCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   // the tokens, older than the kernel in front, in 8 bits: rows of 128 bytes in the tensor core's swizzle
@@ -239,15 +234,25 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
   const int BI = (KI + kBlocks2 - 1) / kBlocks2, BS = (KS + kBlocks2 - 1) / kBlocks2, steps = slots * BI + BS;  // stages of a run of W2
   constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kAccCols >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   const bool leader = elect_lane();  // one lane of each warp
-  uint32_t s1 = 0, p1 = warp == 0 ? 1 : 0;  // W1's ring: the producer's or the MMA warp's stage and parity
-  uint32_t s2 = 0, p2 = warp == 0 ? 1 : 0;
+  const bool producer = warp == 0 || warp == 3;
+  const uint32_t mine = warp == 3;          // the two producers take every other stage
+  uint32_t s1 = 0, p1 = producer ? 1 : 0;    // W1's ring: a producer's or the MMA warp's stage and parity
+  uint32_t s2 = 0, p2 = producer ? 1 : 0;
+  uint32_t filled = 0;                       // stages so far: the producers'
   uint32_t batch = 0;                        // stages so far: the MMA warp's and the consumers'
   int early = 0;                             // stages of W2 whose weights are on their way
   bool alive = true;
   const int group = (warp - 4) >> 2, wq = warp & 3, tid = (int)threadIdx.x - 128;
   const uint32_t t_lane = tmem + ((uint32_t)(wq << 5) << 16);
-  auto acc_at = [](uint32_t n) { return n % kAccs * (kBlocks2 * kAccCols); };
+  auto acc_at = [](uint32_t n) { return n % kAccs * (kAccBlocks * kAccCols); };
 
+  // The accumulators of four stages at a time: each group empties its own in order, so the last one of either stands for those before.
+  auto room_for = [&](uint32_t n) {
+    if (n % 4 != 0) return true;
+    for (uint32_t i = n + 2; i < n + 4; ++i)
+      if (!mbar_wait(&aux->acc_empty[i % kAccs], ((i / kAccs) & 1) ^ 1, P.status, P.wait_ns)) return false;
+    return true;
+  };
   // stage i of a run of W2: expert and K blocks
   struct Step {
     int s, kb, n;
@@ -279,47 +284,56 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
     const int run = aux->run1[turn & 1];
     if (run >= runs1) break;
     const int64_t lo = units * run / runs1 * 8, hi = units * (run + 1) / runs1 * 8;
-    if (warp == 0) {
+    if (producer) {
       int next = 0;
-      if (leader) {
+      if (warp == 0 && leader) {
         next = claim(P.counters);
         aux->run1[(turn + 1) & 1] = next;
       }
       for (int64_t o = lo; o < hi && alive;) {
-        const Tile t = tile_at(P, slots, o, hi);
-        const bool shared = t.s == slots;
-        const CUtensorMap* map = shared ? maps.sw1 : maps.w1;
-        const int unit = (int)(((shared ? 0 : (int64_t)S.list[t.s] * 2 * P.I) + t.p) / 8), n = t.n / 8;
-        for (int kb = 0; kb < KB; kb += kBlocks1) {
-          if (!mbar_wait(&aux->empty1[s1], p1, P.status, P.wait_ns)) { alive = false; break; }
-          if (leader) {
-            uint8_t* dst = ring + (size_t)s1 * kStage1;
-            uint64_t* bar = &aux->full1[s1];
-            mbar_expect_tx(bar, n * (2 * kBlocks1 * 1024));
-            int u = 0;
+        const int n = tile_size(o, hi);
+        // boxes of 8, 4, 2 or 1 units of the first expert, then of the next (an expert has 16 units at least)
+        const Output f = output_at(P, slots, o);
+        const int all = n / 8, n0 = (f.width - f.p) / 8 < all ? (f.width - f.p) / 8 : all;
+        auto boxes = [&](uint8_t* dst, uint64_t* bar, int kb, int s, int p, int count) {
+          const CUtensorMap* map = s == slots ? maps.sw1 : maps.w1;
+          int unit = (int)(((s == slots ? 0 : (int64_t)S.list[s] * 2 * P.I) + p) / 8);
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {  // boxes of 8, 4, 2 and 1 units
-              if (n & (8 >> z)) {
-                tma_load_5d(map + z, bar, dst + u * (2 * kBlocks1 * 1024), 0, 0, kb, 0, unit + u);
-                u += 8 >> z;
-              }
+          for (int z = 0; z < 4; ++z) {
+            if (count & (8 >> z)) {
+              tma_load_5d(map + z, bar, dst, 0, 0, kb, 0, unit);
+              dst += (8 >> z) * (2 * kBlocks1 * 1024);
+              unit += 8 >> z;
             }
+          }
+        };
+        for (int kb = 0; kb < KB; kb += kBlocks1) {
+          const bool turns = (filled++ & 1) == mine;
+          if (turns && !mbar_wait(&aux->empty1[s1], p1, P.status, P.wait_ns)) { alive = false; break; }
+          if (turns && leader) {
+            uint8_t* dst = ring + (size_t)s1 * kStage1;
+            mbar_expect_tx(&aux->full1[s1], all * (2 * kBlocks1 * 1024));
+            boxes(dst, &aux->full1[s1], kb, f.s, f.p, n0);
+            if (n0 < all) boxes(dst + n0 * (2 * kBlocks1 * 1024), &aux->full1[s1], kb, f.s + 1, 0, all - n0);
           }
           if (++s1 == (uint32_t)Q.stages1) { s1 = 0; p1 ^= 1; }
         }
-        o += t.n;
+        o += n;
       }
-      next = __reduce_max_sync(0xFFFFFFFFu, next);
+      // W2's weights take the ring as soon as W1's products have left it.  Which run of W2 it will be is known from the start; whether
+      // another one of W1 comes first, both producers hear from the one that claimed it.
+      if (warp == 0 && leader) aux->more1 = next < runs1;
+      asm volatile("bar.sync 2, 64;" ::: "memory");
       const int run2 = aux->run2[0];
-      if (next >= runs1 && run2 < runs2) {
-        // W2's weights take the ring as soon as W1's products have left it
+      if (!aux->more1 && run2 < runs2) {
         for (int d = 0; d < Q.stages1 && alive; ++d) {
           if (!mbar_wait(&aux->empty1[s1], p1, P.status, P.wait_ns)) alive = false;
           if (++s1 == (uint32_t)Q.stages1) { s1 = 0; p1 ^= 1; }
         }
         if (alive) {
+          filled = 0;
           for (; early < Q.stages2 && early < steps; ++early) {
-            if (leader) load_step((int)((int64_t)P.H * run2 / runs2), early, true, false);
+            if ((early & 1) == mine && leader) load_step((int)((int64_t)P.H * run2 / runs2), early, true, false);
             if (++s2 == (uint32_t)Q.stages2) s2 = 0;
           }
           s2 = 0;
@@ -330,11 +344,9 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
       const uint64_t a0 = (make_smem_desc(smem_u32(ring)) & ~((uint64_t)0x3FFF << 32)) | (uint64_t)(kBlocks1 * 1024 >> 4) << 32;
       const uint64_t b0 = make_smem_desc(smem_u32(xt));
       for (int64_t o = lo; o < hi && alive;) {
-        const Tile t = tile_at(P, slots, o, hi);
         for (int kb = 0; kb < KB; kb += kBlocks1, ++batch) {
           const uint32_t a = batch % kAccs;
-          if (!mbar_wait(&aux->acc_empty[a], ((batch / kAccs) & 1) ^ 1, P.status, P.wait_ns) ||
-              !mbar_wait(&aux->full1[s1], p1, P.status, P.wait_ns)) { alive = false; break; }
+          if (!room_for(batch) || !mbar_wait(&aux->full1[s1], p1, P.status, P.wait_ns)) { alive = false; break; }
           tc_fence_after();
 #pragma unroll
           for (int j = 0; j < kBlocks1; ++j)
@@ -346,17 +358,15 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
           }
           if (++s1 == (uint32_t)Q.stages1) { s1 = 0; p1 ^= 1; }
         }
-        o += t.n;
+        o += tile_size(o, hi);
       }
     } else if (warp >= 4) {
       const int row = wq * 32 + lane, out = (row >> 4) * 8 + (row & 7);  // eight gate rows, the up rows of the same outputs, and so on
       for (int64_t o = lo; o < hi;) {
-        const Tile t = tile_at(P, slots, o, hi);
-        const bool shared = t.s == slots;
-        const int width = shared ? P.Is : P.I, batches = (KB + kBlocks1 - 1) / kBlocks1;
+        const int tn = tile_size(o, hi), batches = (KB + kBlocks1 - 1) / kBlocks1;
         // this lane's row of the tile (one that is not there takes the last one's scale)
-        const int64_t p = t.p + (out < t.n ? out : t.n - 1) + (row & 8 ? width : 0);
-        const float* ws = (shared ? P.sw1s : P.w1s + (int64_t)S.list[t.s] * (2 * width / 128) * KB) + p / 128 * KB;
+        const Output q = output_at(P, slots, o + (out < tn ? out : tn - 1));
+        const float* ws = (q.s == slots ? P.sw1s : P.w1s + (int64_t)S.list[q.s] * (2 * P.I / 128) * KB) + (int64_t)((q.p + (row & 8 ? q.width : 0)) / 128) * KB;
         float acc[kTokens] = {};
         const int first = ((int)(batch & 1) == group) ? 0 : 1;  // this group's stages are every other one
         float w[kBlocks1];                                      // their scales, one stage ahead
@@ -393,17 +403,19 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
         j[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         j[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
         consumers_sync();
-        const uint32_t mask = S.mask[t.s];
 #pragma unroll
         for (int i = 0; i < 64 * kTokens / kConsumers; ++i) {
           const int at = tid + i * kConsumers, n = at & 63, m = at >> 6;
-          if (n < t.n && ((mask >> m) & 1)) {
-            const float* q = join + ((n >> 3) * 16 + (n & 7)) * kTokens + m;
-            const float gate = q[0] + q[128 * kTokens], up = q[8 * kTokens] + q[136 * kTokens];
-            reinterpret_cast<T*>(P.h)[(int64_t)t.s * kTokens * P.I + (int64_t)m * width + t.p + n] = from_f32<T>(silu_mul(gate, up));
+          if (n < tn) {
+            const Output y = output_at(P, slots, o + n);
+            if ((S.mask[y.s] >> m) & 1) {
+              const float* s = join + ((n >> 3) * 16 + (n & 7)) * kTokens + m;
+              const float gate = s[0] + s[128 * kTokens], up = s[8 * kTokens] + s[136 * kTokens];
+              reinterpret_cast<T*>(P.h)[(int64_t)y.s * kTokens * P.I + (int64_t)m * y.width + y.p] = from_f32<T>(silu_mul(gate, up));
+            }
           }
         }
-        o += t.n;
+        o += tn;
       }
       quantise_groups<T>(P, S, lo, hi);
       proxy_fence();  // h in 8 bits is read by TMA
@@ -422,21 +434,21 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
     const int run = aux->run2[turn & 1];
     if (run >= runs2) break;
     const int lo = (int)((int64_t)P.H * run / runs2), hi = (int)((int64_t)P.H * (run + 1) / runs2);
-    if (warp == 0) {
+    if (producer) {
       if (leader) {
-        aux->run2[(turn + 1) & 1] = claim(P.counters + 1);
+        if (warp == 0) aux->run2[(turn + 1) & 1] = claim(P.counters + 1);
         if (!waited) wait_for_runs(P.counters + 2, runs1, P.status, P.wait_ns);
         proxy_fence();
       }
       waited = true;
       __syncwarp();
+      if (early == 0) filled = 0;
       for (int i = 0; i < steps && alive; ++i) {
-        if (early > 0) {
-          --early;
-          if (leader) load_step(lo, i, false, true);
-        } else {
-          if (!mbar_wait(&aux->empty2[s2], p2, P.status, P.wait_ns)) { alive = false; break; }
-          if (leader) load_step(lo, i, true, true);
+        const bool turns = (filled++ & 1) == mine, sent = early > 0;
+        if (sent) --early;
+        if (turns) {
+          if (!sent && !mbar_wait(&aux->empty2[s2], p2, P.status, P.wait_ns)) { alive = false; break; }
+          if (leader) load_step(lo, i, !sent, true);
         }
         if (++s2 == (uint32_t)Q.stages2) { s2 = 0; p2 ^= 1; }
       }
@@ -445,8 +457,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
       for (int i = 0; i < steps && alive; ++i, ++batch) {
         const uint32_t a = batch % kAccs;
         const int n = step_at(i).n;
-        if (!mbar_wait(&aux->acc_empty[a], ((batch / kAccs) & 1) ^ 1, P.status, P.wait_ns) ||
-            !mbar_wait(&aux->full2[s2], p2, P.status, P.wait_ns)) { alive = false; break; }
+        if (!room_for(batch) || !mbar_wait(&aux->full2[s2], p2, P.status, P.wait_ns)) { alive = false; break; }
         tc_fence_after();
         const uint64_t at = (uint64_t)(s2 * (uint32_t)(Q.slot2 >> 4));
 #pragma unroll
@@ -534,7 +545,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
   __syncthreads();
   if (warp == 2) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kAccs * kBlocks2 * kAccCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kAccs * kAccBlocks * kAccCols));
   }
 }
 
@@ -543,7 +554,7 @@ constexpr int64_t fixed_bytes(int64_t H) {
 }
 static_assert(fixed_bytes(kMaxHidden8) + 4 * kStage1 <= kFewSmem, "four stages at the largest hidden size");
 static_assert(4 * kStage1 >= kTokens * kMaxExperts * 4, "what routing needs takes the ring's place");
-static_assert(4 * kStage1 >= 2 * kBlocks2 * (64 * 128 + 1024), "two stages of W2");
+static_assert(4 * kStage1 >= 3 * kBlocks2 * (64 * 128 + 1024), "three stages of W2");
 // the tensor core reads 128 rows from a block of W2 that holds fewer: what lies behind the ring is as long
 static_assert(kJoinBytes + (int64_t)sizeof(Shared) >= 128 * 128, "reads behind the last block stay in shared memory");
 
@@ -593,7 +604,7 @@ int few_experts_fp8(const Few& P, int dtype, cudaStream_t st) {
   auto stages = [](int64_t n) { return (int)(n < kMaxStages ? n : kMaxStages); };
   Q.stages1 = stages((kFewSmem - fixed_bytes(P.H)) / kStage1);
   Q.ring = Q.stages1 * kStage1;
-  Q.stages2 = stages(Q.ring / Q.slot2);
+  Q.stages2 = stages((Q.ring + (P.H / 128 + 1) * 1024) / Q.slot2);  // W2's ring also takes the tokens' place
   Maps m;
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = encode_w1(m.w1, P.w1, (uint64_t)P.E, (uint64_t)P.I, (uint64_t)P.H);

@@ -233,6 +233,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
   const int KI = P.I / 128, KS = P.Is / 128;
   const int BI = (KI + kBlocks2 - 1) / kBlocks2, BS = (KS + kBlocks2 - 1) / kBlocks2, steps = slots * BI + BS;  // stages of a run of W2
   constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kAccCols >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  constexpr uint32_t idesc2 = (1u << 4) | ((uint32_t)(kAccCols >> 3) << 17) | ((uint32_t)(64 >> 4) << 24);
   const bool leader = elect_lane();  // one lane of each warp
   const bool producer = warp == 0 || warp == 3;
   const uint32_t mine = warp == 3;          // the two producers take every other stage
@@ -462,7 +463,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
         const uint64_t at = (uint64_t)(s2 * (uint32_t)(Q.slot2 >> 4));
 #pragma unroll
         for (int j = 0; j < kBlocks2; ++j)
-          if (j < n) mma_block(leader, tmem + acc_at(batch) + j * kAccCols, a0 + at + (uint64_t)(j * (Q.block2 >> 4)), b0 + at + (uint64_t)(j * 64), idesc);
+          if (j < n) mma_block(leader, tmem + acc_at(batch) + j * kAccCols, a0 + at + (uint64_t)(j * (Q.block2 >> 4)), b0 + at + (uint64_t)(j * 64), idesc2);
         if (leader) {
           tc_commit(&aux->acc_full[a]);
           tc_commit(&aux->empty2[s2]);
@@ -475,8 +476,9 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
         if (tid == 0) wait_for_runs(P.counters + 2, runs1, P.status, P.wait_ns);
         consumers_sync();
       }
-      const int row = wq * 32 + lane, r0 = lo + row < hi ? lo + row : hi - 1;  // a row that is not there takes the last one's scale
-      const bool rows_here = lo + wq * 32 < hi;
+      // 64 rows lie in the lower 16 lanes of each quarter.  A row that is not there takes the last one's scale
+      const int row = wq * 16 + (lane & 15), r0 = lo + row < hi ? lo + row : hi - 1;
+      const bool rows_here = lo + wq * 16 < hi;
       float acc[kTokens] = {};
       const int first = ((int)(batch & 1) == group) ? 0 : 1;
       // of this group's next stage: scales of the row's blocks; lane 8 j + m has token m's scale and routing weight for block j
@@ -524,7 +526,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
       }
       batch += steps;
       consumers_sync();
-      if (row < 64) {
+      if (lane < 16) {
         float4* j = reinterpret_cast<float4*>(join + (group * 64 + row) * kTokens);
         j[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         j[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
@@ -555,8 +557,8 @@ constexpr int64_t fixed_bytes(int64_t H) {
 static_assert(fixed_bytes(kMaxHidden8) + 4 * kStage1 <= kFewSmem, "four stages at the largest hidden size");
 static_assert(4 * kStage1 >= kTokens * kMaxExperts * 4, "what routing needs takes the ring's place");
 static_assert(4 * kStage1 >= 3 * kBlocks2 * (64 * 128 + 1024), "three stages of W2");
-// the tensor core reads 128 rows from a block of W2 that holds fewer: what lies behind the ring is as long
-static_assert(kJoinBytes + (int64_t)sizeof(Shared) >= 128 * 128, "reads behind the last block stay in shared memory");
+// the tensor core reads 64 rows from a block of W2 that holds fewer: what lies behind the ring is as long
+static_assert(kJoinBytes + (int64_t)sizeof(Shared) >= 64 * 128, "reads behind the last block stay in shared memory");
 
 template <typename T>
 int launch(const Maps& maps, const Few& P, const Few8& Q, int G, cudaStream_t st) {

@@ -6,6 +6,7 @@
 // N' = N, or 2 N for the gated activation silu(z[:, :N]) * z[:, N:].  Sums, bias, activation and residual are fp32, y is rounded
 // once.  z is kept for the backward pass in the operands' type: its rounding reaches the gradients through act' only, and dz has
 // to be rounded to that type anyway, because it is an operand of two products; the bias' gradient sums dz before its rounding.
+// The gated activation keeps z in fp32: there dz is a product of both halves of z and takes their roundings in full.
 //
 // All products are one form, D[r, c] = sum_k A[r, k] B[c, k], in which each operand may lie either way in memory: rows of k
 // ("K-major": x and W forward, dz for dx) or rows of r or c ("MN-major": W for dx, dz and x for dW).  The tensor core takes both
@@ -148,7 +149,7 @@ struct Product {
   int a_mn, b_mn;
   int gate;            // distance of the up rows from the gate rows in the weights (N of a gated call), else 0
   int swapped;         // rows of D are columns of y
-  int split, BN;       // tile_kernel
+  int split, BN, ring; // tile_kernel
   int group;           // pair_kernel: row tiles that walk the column tiles together
   int32_t* status;
   unsigned long long wait_ns;
@@ -160,11 +161,15 @@ struct TAux {
   uint64_t full[12], empty[12], done;
   uint32_t tmem_base;
 };
-constexpr int kTileRing = 196608;
+// Two waves of blocks and more: tiles of up to 128 columns leave room for a second block on the multiprocessor, which streams while the
+// first one adds up and stores (64 x 4096 -> 2 x 14336 gated 50.5 -> 44.1 us).  One wave: all of the memory is one block's ring (33 x
+// 14336 -> 4096 24.8 -> 23.9).
+constexpr int kRingWhole = 196608, kRingHalf = 98304;
 __host__ __device__ constexpr int tile_stage(int bn) { return (128 + bn) * 128; }
-__host__ __device__ constexpr int tile_stages(int bn) { return kTileRing / tile_stage(bn) < 12 ? kTileRing / tile_stage(bn) : 12; }
-constexpr size_t kTileSmem = (size_t)kTileRing + 1024 + sizeof(TAux);
-static_assert(128 * 260 * 4 <= kTileRing, "the partial tile takes the ring's place");
+__host__ __device__ constexpr int tile_stages(int bn, int ring) { return ring / tile_stage(bn) < 12 ? ring / tile_stage(bn) : 12; }
+constexpr size_t tile_smem(int ring) { return (size_t)ring + 1024 + sizeof(TAux); }
+static_assert(128 * 260 * 4 <= kRingWhole && 128 * 132 * 4 <= kRingHalf, "the partial tile takes the ring's place");
+static_assert(2 * (tile_smem(kRingHalf) + 1024) <= 233472, "two blocks on a multiprocessor");
 
 __device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* a) {
   asm volatile(
@@ -227,15 +232,15 @@ __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t
 // One 128 x BN tile of D by the `split` CTAs of a cluster, each over its share of K.  A gated call's tile is half gate rows and
 // half up rows of the weights, whichever side they are on.
 template <typename T>
-__global__ void __launch_bounds__(TTHREADS, 1)
+__global__ void __launch_bounds__(TTHREADS, 2)
 tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product P, const Epilogue E) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_1024(smem_raw);
-  TAux* aux = reinterpret_cast<TAux*>(smem + kTileRing);
+  TAux* aux = reinterpret_cast<TAux*>(smem + P.ring);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank();
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int BN = P.BN, stage = tile_stage(BN), stages = tile_stages(BN);
+  const int BN = P.BN, stage = tile_stage(BN), stages = tile_stages(BN, P.ring);
   const bool gate_a = P.gate != 0 && P.swapped, gate_b = P.gate != 0 && !P.swapped;
   const int out_rows = gate_a ? 64 : 128, out_cols = gate_b ? BN / 2 : BN;  // of D that the tile finishes
   const int64_t r0 = (int64_t)blockIdx.y * out_rows;
@@ -358,8 +363,8 @@ __device__ __forceinline__ void tile_at(int item, int RT, int CT, int group, int
 }
 
 // 32 columns of 32 rows between a warp's registers (lane = row) and memory.  `wide`: the rows are whole 16-byte pieces, and each
-// lane moves its own; else they go through shared memory, so that the warp reads and writes along the rows (4096 x 4097 outputs:
-// XXX us, XXX with each lane at its own row).
+// lane moves its own; else they go through shared memory, so that the warp reads and writes along the rows (4096 x 2048 -> 4097:
+// 57 us, 232 with each lane at its own row).
 struct Rows {
   int64_t m0, end;  // the warp's first row, the first row that is not there
   int n0, n;        // first column, columns that are there (n > 0)
@@ -620,15 +625,17 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // ------------------------------------------------------------------ fp32 operands
-// 8 RM x 64 tiles of D by 64 threads, RM x 8 outputs each, 16 k at a time out of a ring in shared memory that asynchronous copies
-// fill (each element to its place, which transposes operands with rows of k; whole 16-byte pieces where rows of r or c allow it);
-// K divided over a cluster as in tile_kernel.  A gated call's tile has 32 gate columns and the 32 up columns that go with them.
+// Tiles of D of TM rows and TN columns, RM x 8 outputs to a thread, 16 k at a time out of a ring in shared memory that asynchronous
+// copies fill (each element to its place, which transposes operands with rows of k; whole 16-byte pieces where rows of r or c allow
+// it); K divided over a cluster as in tile_kernel.  Half of a gated call's columns are gates, the other half the ups that go with
+// them.  A copy is an address and an instruction for every element, and a tile of 128 x 128 has half as many for a product as one
+// of 64 x 64.
 struct F32Operand {
   const float* p;
   int64_t rs, ks;  // strides of the row (r or c) and of k, one of them 1
   int wide;        // rows of r or c in whole 16-byte pieces
 };
-constexpr int FTHREADS = 64, FPITCH = 68, FSTAGES = 4;
+constexpr int FSTAGES = 3;
 __device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void* src, bool yes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(yes ? 4 : 0) : "memory");
 }
@@ -636,8 +643,9 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // ROWS x 16 elements from (base, k0) on; zeros beyond `end` and `kend`.  gate: rows from ROWS / 2 on lie that far behind the first
-template <int ROWS>
+template <int ROWS, int FTHREADS>
 __device__ __forceinline__ void f32_fill(const F32Operand& X, int64_t base, int64_t end, int64_t gate, int64_t k0, int64_t kend, uint32_t dst) {
+  constexpr int FPITCH = (ROWS < 64 ? 64 : ROWS) + 4, ROUND = FTHREADS / 16;  // rows of a round of copies
   const int t = threadIdx.x;
   if (X.ks == 1) {
     const int k = t & 15;
@@ -645,16 +653,26 @@ __device__ __forceinline__ void f32_fill(const F32Operand& X, int64_t base, int6
     dst += (uint32_t)(k * FPITCH + (t >> 4)) * 4;
     const float* p = X.p + (base + (t >> 4)) * X.rs + k0 + k;
     int64_t left = end - base - (t >> 4);  // rows that are there from this thread's first on
+    const int64_t step = ROUND * X.rs;
+    if (end - base >= (gate != 0 ? ROWS / 2 : ROWS) && k0 + 16 <= kend) {  // all there: an address and a copy each
 #pragma unroll
-    for (int i = 0; i < ROWS / 4; ++i) {
-      if (gate != 0 && i == ROWS / 8) {
+      for (int i = 0; i < ROWS / ROUND; ++i) {
+        if (gate != 0 && i == ROWS / ROUND / 2) p += (gate - ROWS / 2) * X.rs;
+        cp_async4(dst + 4 * ROUND * i, p);
+        p += step;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS / ROUND; ++i) {
+      if (gate != 0 && i == ROWS / ROUND / 2) {
         p += (gate - ROWS / 2) * X.rs;
         left += ROWS / 2;
       }
       const bool yes = in && left > 0;
-      cp_async4_or_zero(dst + 16 * i, yes ? p : X.p, yes);
-      p += 4 * X.rs;
-      left -= 4;
+      cp_async4_or_zero(dst + 4 * ROUND * i, yes ? p : X.p, yes);
+      p += step;
+      left -= ROUND;
     }
   } else if (X.wide) {
     constexpr int LANES = ROWS / 4, PER = FTHREADS / LANES;  // pieces of a k, k of a round
@@ -678,48 +696,51 @@ __device__ __forceinline__ void f32_fill(const F32Operand& X, int64_t base, int6
     }
   }
 }
-template <int RM>
-__global__ void __launch_bounds__(FTHREADS, RM == 8 ? 7 : 10) f32_kernel(const F32Operand A, const F32Operand B, int64_t K, const Product P, const Epilogue E) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];  // FSTAGES x {A, B}[16][FPITCH], then the partial tile
+template <int RM, int T, int FTHREADS>
+__global__ void __launch_bounds__(FTHREADS, FTHREADS == 64 ? 7 : 2) f32_kernel(const F32Operand A, const F32Operand B, int64_t K, const Product P, const Epilogue E) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];  // FSTAGES x {A, B}[16][pitch], then the partial tile
   float* s_mem = reinterpret_cast<float*>(smem_raw);
-  static_assert(64 * FPITCH <= FSTAGES * 2 * 16 * FPITCH, "the partial tile takes the operands' place");
-  constexpr int TM = 8 * RM, HALF = 16 * FPITCH;  // floats of an operand's tile
+  constexpr int TM = RM == 8 ? T : 8, PITCH = T + 4, TILE = 16 * PITCH;  // floats of an operand's tile
+  static_assert(FTHREADS == T * T / 64 && (RM == 8 || T == 64), "threads");
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank();
-  const int t = threadIdx.x, tx = t & 7, ty = t >> 3;
-  const int out_cols = P.gate ? 32 : 64;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  // a warp is 4 x 8 threads: its 16-byte pieces of a k are 64 and 128 bytes
+  const int tx = T == 64 ? (t & 7) : (warp & 1) * 8 + (lane & 7), ty = T == 64 ? (t >> 3) : (warp >> 1) * 4 + (lane >> 3);
+  const int out_cols = P.gate ? T / 2 : T;
   const int64_t r0 = (int64_t)blockIdx.y * TM, c0 = (int64_t)(blockIdx.x / P.split) * out_cols;
   const int64_t steps = (K + 15) / 16, first = steps * rank / P.split, last = steps * (rank + 1) / P.split;
   const uint32_t s0 = smem_u32(s_mem);
-  pdl_wait();
-  pdl_trigger();
   float acc[RM][8] = {};
-  auto fill = [&](int64_t step) {
+  auto fill = [&](int64_t step, int stage) {
     if (step < last) {
-      const uint32_t dst = s0 + (uint32_t)((step - first) % FSTAGES) * (2 * HALF * 4);
-      f32_fill<TM>(A, r0, P.rows, 0, step * 16, K, dst);
-      f32_fill<64>(B, c0, P.cols, P.gate, step * 16, K, dst + HALF * 4);
+      const uint32_t dst = s0 + (uint32_t)stage * (2 * TILE * 4);
+      f32_fill<TM, FTHREADS>(A, r0, P.rows, 0, step * 16, K, dst);
+      f32_fill<T, FTHREADS>(B, c0, P.cols, P.gate, step * 16, K, dst + TILE * 4);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll 1
-  for (int s = 0; s < FSTAGES - 1; ++s) fill(first + s);
+  for (int s = 0; s < FSTAGES - 1; ++s) fill(first + s, s);
+  int to = FSTAGES - 1, from = 0;
 #pragma unroll 1
   for (int64_t step = first; step < last; ++step) {
     asm volatile("cp.async.wait_group %0;" ::"n"(FSTAGES - 2) : "memory");
     __syncthreads();  // this step's tiles are there, the last one's have been read
-    fill(step + FSTAGES - 1);
-    const float* sa = s_mem + ((step - first) % FSTAGES) * (2 * HALF);
-    const float* sb = sa + HALF;
+    fill(step + FSTAGES - 1, to);
+    if (++to == FSTAGES) to = 0;
+    const float* sa = s_mem + from * (2 * TILE);
+    const float* sb = sa + TILE;
+    if (++from == FSTAGES) from = 0;
 #pragma unroll 4
     for (int k = 0; k < 16; ++k) {
-      const float4 b0 = *reinterpret_cast<const float4*>(sb + k * FPITCH + 4 * tx), b1 = *reinterpret_cast<const float4*>(sb + k * FPITCH + 32 + 4 * tx);
+      const float4 b0 = *reinterpret_cast<const float4*>(sb + k * PITCH + 4 * tx), b1 = *reinterpret_cast<const float4*>(sb + k * PITCH + T / 2 + 4 * tx);
       float a[RM];
       if constexpr (RM == 8) {
-        const float4 p = *reinterpret_cast<const float4*>(sa + k * FPITCH + 4 * ty), q = *reinterpret_cast<const float4*>(sa + k * FPITCH + 32 + 4 * ty);
+        const float4 p = *reinterpret_cast<const float4*>(sa + k * PITCH + 4 * ty), q = *reinterpret_cast<const float4*>(sa + k * PITCH + T / 2 + 4 * ty);
         a[0] = p.x; a[1] = p.y; a[2] = p.z; a[3] = p.w; a[4] = q.x; a[5] = q.y; a[6] = q.z; a[7] = q.w;
       } else {
-        a[0] = sa[k * FPITCH + ty];
+        a[0] = sa[k * PITCH + ty];
       }
 #pragma unroll
       for (int i = 0; i < RM; ++i) {
@@ -734,9 +755,9 @@ __global__ void __launch_bounds__(FTHREADS, RM == 8 ? 7 : 10) f32_kernel(const F
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
-    float* part = s_mem + (RM == 8 ? (i < 4 ? 4 * ty + i : 28 + 4 * ty + i) : ty) * FPITCH + 4 * tx;
+    float* part = s_mem + (RM == 8 ? (i < 4 ? 4 * ty + i : T / 2 - 4 + 4 * ty + i) : ty) * PITCH + 4 * tx;
     *reinterpret_cast<float4*>(part) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-    *reinterpret_cast<float4*>(part + 32) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+    *reinterpret_cast<float4*>(part + T / 2) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
   }
   if (P.split > 1) cluster.sync();
   else __syncthreads();
@@ -989,12 +1010,13 @@ int run_product(Matrix a, Matrix b, bool a_mn, bool b_mn, int64_t rows, int64_t 
     return launch_pdl(kern, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), PTHREADS, kPairSmem, 2, st, "fused_linear (pair)", ma, mb, P, E);
   }
   auto kern = tile_kernel<T>;
-  rc = allow_smem((const void*)kern, (int)kTileSmem);
+  rc = allow_smem((const void*)kern, (int)tile_smem(kRingWhole));
   if (rc) return rc;
-  while (P.split > 1 && max_clusters((const void*)kern, P.split, TTHREADS, kTileSmem) == 0) P.split /= 2;
+  while (P.split > 1 && max_clusters((const void*)kern, P.split, TTHREADS, tile_smem(kRingWhole)) == 0) P.split /= 2;
   const int rt = gated && p.swapped ? 64 : 128, ct = gated && !p.swapped ? p.BN / 2 : p.BN;
   const dim3 grid((unsigned)((P.cols + ct - 1) / ct * P.split), (unsigned)((P.rows + rt - 1) / rt));
-  return launch_pdl(kern, grid, TTHREADS, kTileSmem, P.split, st, "fused_linear (tile)", ma, mb, P, E);
+  P.ring = p.BN <= 128 && (int64_t)grid.x * grid.y > sm_count() ? kRingHalf : kRingWhole;
+  return launch_pdl(kern, grid, TTHREADS, tile_smem(P.ring), P.split, st, "fused_linear (tile)", ma, mb, P, E);
 }
 
 int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, bool gated, const Epilogue& E, cudaStream_t st) {
@@ -1003,17 +1025,52 @@ int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, b
   P.rows = rows;
   P.cols = cols;
   P.gate = gated ? (int)cols : 0;
-  P.BN = 64;
-  const int TM = rows <= 8 ? 8 : 64;
-  const int64_t ct = (cols + (gated ? 31 : 63)) / (gated ? 32 : 64), rt = (rows + TM - 1) / TM;
-  if (rt > 65535) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d rows", 65535 * 64);
-  // four blocks an SM hide each other's latency; a share of K stays at 64 or more
+  // Tile and split of K by what a multiprocessor has to do: `fit` blocks at once, as fast together as four of 64 x 64 or one and a half
+  // of 128 x 128; a block's share of K and a fixed part.  A share of K stays at 64 or more.
+  const int64_t sms = sm_count();
+  double best = 0.0;
+  int T = 64;
   P.split = 1;
-  while (P.split < 8 && ct * rt * P.split < 4 * (int64_t)sm_count() && K / (2 * P.split) >= 64) P.split *= 2;
-  const dim3 grid((unsigned)(ct * P.split), (unsigned)rt);
-  constexpr size_t smem = FSTAGES * 2 * 16 * FPITCH * 4;  // below the 48 KB that need no leave
-  if (TM == 8) return launch_pdl(f32_kernel<1>, grid, FTHREADS, smem, P.split, st, "fused_linear (fp32)", a, b, K, P, E);
-  return launch_pdl(f32_kernel<8>, grid, FTHREADS, smem, P.split, st, "fused_linear (fp32)", a, b, K, P, E);
+  for (int t = 64; t <= 128; t *= 2) {
+    if (t == 128 && rows <= 64) break;
+    const int TM = rows <= 8 ? 8 : t;
+    const int64_t tiles = ((gated ? 2 * cols : cols) + t - 1) / t * ((rows + TM - 1) / TM);
+    const double one = t == 64 ? 1.0 : 3.1, full = t == 64 ? 4.0 : 1.5;  // a block's products; blocks that fill a multiprocessor
+    const int64_t fit = t == 64 ? 7 : 2;
+    for (int s = 1; s <= 8 && (s == 1 || K / s >= 64); s *= 2) {
+      const int64_t per = (tiles * s + sms - 1) / sms, rounds = (per + fit - 1) / fit, last = per - (rounds - 1) * fit;
+      const double cost = one * (((double)(rounds - 1) * fit + ((double)last < full ? full : (double)last)) * ((double)K / s + 100.0));
+      if (best == 0.0 || cost < best) { best = cost; P.split = s; T = t; }
+    }
+  }
+  P.BN = T;
+  const int TM = rows <= 8 ? 8 : T;
+  const int64_t ct = ((gated ? 2 * cols : cols) + T - 1) / T, rt = (rows + TM - 1) / TM;
+  if (rt > 65535) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d rows", 65535 * 64);
+  auto go = [&](auto kern, int t, int threads) {
+    const int64_t ring = (int64_t)FSTAGES * 2 * 16 * (t + 4) * 4, part = (int64_t)TM * (t + 4) * 4, smem = ring > part ? ring : part;
+    const int rc = allow_smem((const void*)kern, (int)smem);
+    if (rc) return rc;
+    while (P.split > 1 && max_clusters((const void*)kern, P.split, threads, (size_t)smem) == 0) P.split /= 2;
+    // Launched behind its predecessor's end: blocks that come while it drains crowd on the multiprocessors that are free first
+    // (8192 x 512 -> 512, dW: 264 us so, 159 with each multiprocessor at its share).
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ct * P.split), (unsigned)rt);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)P.split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t ce = cudaLaunchKernelEx(&cfg, kern, a, b, K, P, E);
+    if (ce != cudaSuccess) return fail((int)ce, "fused_linear (fp32): %s", cudaGetErrorString(ce));
+    return check_launch("fused_linear (fp32)");
+  };
+  if (TM == 8) return go(f32_kernel<1, 64, 64>, 64, 64);
+  return T == 64 ? go(f32_kernel<8, 64, 64>, 64, 64) : go(f32_kernel<8, 128, 256>, 128, 256);
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K, int dtype, int act) {

@@ -10,11 +10,12 @@
 //
 // Rows are shared out singly, so the blocks' parts are equal to one row: 8 experts of 2048 rows are 110.7 rows a block, where
 // tiles of 128 rows would be 128 tiles for 148 multiprocessors.  Every warp copies its rows asynchronously
-// into a ring of its own in shared memory, in whole lines, 12 KB a warp and 96 KB a multiprocessor in flight, and feeds warp-level mma.sync with 16 weight rows as M and the tokens as N = 8.
-// The order of k inside an instruction is free, so a lane's operand is whole 16-byte pieces of a row.
-// (No tcgen05: with 8 columns the tensor core idles either way.)  W1: a tile is 8 gate rows and the up rows of the same outputs,
-// and the warps of a block divide the run of (tile, k step) evenly, joining the tiles that they share in a fixed order.  W2: the
-// warps divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in registers.
+// into a ring of its own in shared memory, in whole lines, 12 KB a warp and 96 KB a multiprocessor in flight, and feeds warp-level
+// mma.sync with 16 weight rows as M and the tokens as N = 8.  The order of k inside an instruction is free, so a lane's operand is
+// whole 16-byte pieces of a row.  (No tcgen05: with 8 columns the tensor core idles either way.)  W1: a tile is 8 gate rows and the up
+// rows of the same outputs, and the warps of a block divide the run of (tile, k step) evenly, joining the tiles that they share in a
+// fixed order.  W2: the warps divide the run of (expert, k step), a warp keeps all rows of its block, scaled by the routing weights, in
+// registers.
 //
 // Weights in e4m3 take few_tokens_fp8.cu behind the router.
 //
@@ -71,8 +72,8 @@ template <int PENDING> __device__ __forceinline__ void wait_copies() {  // of al
 // A block per expert; the sums are formed in the order of router_gemm's row-streaming kernel, whose bits they are.  Clears the
 // counters of the kernel behind it.
 template <typename XT, typename WT, int ROWS>
-__global__ void __launch_bounds__(128) few_router_kernel(const XT* __restrict__ x, int64_t x_ld, const WT* __restrict__ w, int M, int E, int K,
-                                                         int sigmoid, float* __restrict__ out, int32_t* counters, int64_t cleared) {
+__global__ void __launch_bounds__(128) few_router_kernel(const XT* x, int64_t x_ld, const WT* w, int M, int E, int K,
+                                                         int sigmoid, float* out, int32_t* counters, int64_t cleared) {
   pdl_wait();
   pdl_trigger();
   for (int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x; i < cleared; i += (int64_t)gridDim.x * 128) counters[i] = 0;

@@ -373,7 +373,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
         float w[kBlocks1];                                      // their scales, one stage ahead
         auto fetch = [&](int i) {
 #pragma unroll
-          for (int j = 0; j < kBlocks1; ++j) w[j] = i * kBlocks1 + j < KB ? __ldg(ws + i * kBlocks1 + j) : 0.0f;
+          for (int j = 0; j < kBlocks1; ++j) w[j] = i * kBlocks1 + j < KB ? ws[i * kBlocks1 + j] : 0.0f;
         };
         fetch(first);
         for (int i = first; i < batches; i += 2) {
@@ -492,7 +492,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
           mask = S.mask[e.s];
           const float* ws = (e.shared ? P.sw2s : P.w2s + (int64_t)S.list[e.s] * KB * K) + (int64_t)(r0 / 128) * K + e.kb;
 #pragma unroll
-          for (int q = 0; q < kBlocks2; ++q) w[q] = q < e.n ? __ldg(ws + q) : 0.0f;
+          for (int q = 0; q < kBlocks2; ++q) w[q] = q < e.n ? ws[q] : 0.0f;
           f = j < e.n && ((mask >> m) & 1) ? __ldcg((e.shared ? P.h8_scale_shared : P.h8_scale + (int64_t)e.s * kTokens * K) + m * K + e.kb + j) : 0.0f;
         }
       };

@@ -908,7 +908,7 @@ PyObject* few_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &x = tensor(a[0]), &router = tensor(a[1]), &w1 = tensor(a[2]), &w2 = tensor(a[3]);
   auto opt = [&](int i) { return a[i] == Py_None ? nullptr : &tensor(a[i]); };
   const at::Tensor *bias = opt(10), *s1 = opt(11), *s2 = opt(12), *w1x = opt(13), *w2x = opt(14), *s1x = opt(15), *s2x = opt(16), *res = opt(17);
-  no_tangent({&x, &router, &w1, &w2, bias, w1x, w2x, res}, "fused_moe_few_tokens");
+  no_tangent({&x, &router, &w1, &w2, bias, s1, s2, w1x, w2x, s1x, s2x, res}, "fused_moe_few_tokens");
   if (wants_grad({&x, &router, &w1, &w2, bias, s1, s2, w1x, w2x, s1x, s2x, res})) MOE_NONE;  // refused by the Python operator
   if (!x.is_cuda() || x.dim() != 2 || router.dim() != 2 || w1.dim() != 3 || w2.dim() != 3) MOE_NONE;
   const int dev = x.get_device(), code = float_code(x), router_code = float_code(router);

@@ -708,7 +708,8 @@ __global__ void __launch_bounds__(FTHREADS, FTHREADS == 64 ? 7 : 2) f32_kernel(c
   // a warp is 4 x 8 threads: its 16-byte pieces of a k are 64 and 128 bytes
   const int tx = T == 64 ? (t & 7) : (warp & 1) * 8 + (lane & 7), ty = T == 64 ? (t >> 3) : (warp >> 1) * 4 + (lane >> 3);
   const int out_cols = P.gate ? T / 2 : T;
-  const int64_t r0 = (int64_t)blockIdx.y * TM, c0 = (int64_t)(blockIdx.x / P.split) * out_cols;
+  const uint32_t across = (uint32_t)((P.cols + out_cols - 1) / out_cols), at = blockIdx.x / P.split;
+  const int64_t r0 = (int64_t)(at / across) * TM, c0 = (int64_t)(at % across) * out_cols;
   const int64_t steps = (K + 15) / 16, first = steps * rank / P.split, last = steps * (rank + 1) / P.split;
   const uint32_t s0 = smem_u32(s_mem);
   float acc[RM][8] = {};
@@ -892,7 +893,7 @@ __global__ void __launch_bounds__(256) pitch_kernel(const uint16_t* src, int64_t
     const int words = (left + ((at & 2) ? 1 : 0) + 1) / 2;  // words that hold them
     uint32_t v[5];
 #pragma unroll
-    for (int k = 0; k < 5; ++k) v[k] = k < words ? __ldg(w + k) : 0u;
+    for (int k = 0; k < 5; ++k) v[k] = k < words ? w[k] : 0u;
     if (at & 2) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = __funnelshift_r(v[k], v[k + 1], 16);
@@ -1046,7 +1047,7 @@ int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, b
   P.BN = T;
   const int TM = rows <= 8 ? 8 : T;
   const int64_t ct = ((gated ? 2 * cols : cols) + T - 1) / T, rt = (rows + TM - 1) / TM;
-  if (rt > 65535) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d rows", 65535 * 64);
+  if (ct * rt * P.split >= (1ll << 31)) return fail(MOE_E_TOOBIG, "fused_linear: too many tiles");
   auto go = [&](auto kern, int t, int threads) {
     const int64_t ring = (int64_t)FSTAGES * 2 * 16 * (t + 4) * 4, part = (int64_t)TM * (t + 4) * 4, smem = ring > part ? ring : part;
     const int rc = allow_smem((const void*)kern, (int)smem);
@@ -1055,7 +1056,7 @@ int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, b
     // Launched behind its predecessor's end: blocks that come while it drains crowd on the multiprocessors that are free first
     // (8192 x 512 -> 512, dW: 264 us so, 159 with each multiprocessor at its share).
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ct * P.split), (unsigned)rt);
+    cfg.gridDim = dim3((unsigned)(ct * rt * P.split));
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
@@ -1131,6 +1132,7 @@ extern "C" int moe_fused_linear(const void* x, int64_t x_ld, const void* w, int6
   Epilogue E = {bias, residual, y, z, residual_ld, y_ld, z_ld, M, (int)N, act, bias_dtype == MOE_F32};
   const bool gated = act == MOE_LIN_SILU_MUL;
   if (dtype == MOE_F32) return run_f32({(const float*)x, x_ld, 1, 0}, {(const float*)w, w_ld, 1, 0}, M, N, K, gated, E, st);
+  if ((uintptr_t)workspace & 15) return fail(MOE_E_BADARG, "fused_linear: the workspace must be 16-byte aligned");
   Space ws = {(uint8_t*)workspace, workspace ? workspace_bytes : 0};
   Matrix a = {x, M, K, x_ld}, b = {w, W, K, w_ld};
   if (int rc = readable(a, ws, st)) return rc;
@@ -1189,6 +1191,7 @@ extern "C" int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld
   if (db && db_dtype != dtype && db_dtype != MOE_F32) return fail(MOE_E_DTYPE, "fused_linear_grad: the bias has the operands' type or fp32");
   if ((x && x_ld < K) || (w && w_ld < K) || (z && z_ld < W)) return fail(MOE_E_SHAPE, "fused_linear_grad: rows overlap");
   cudaStream_t st = (cudaStream_t)stream;
+  if ((uintptr_t)workspace & 15) return fail(MOE_E_BADARG, "fused_linear_grad: the workspace must be 16-byte aligned");
   Space ws = {(uint8_t*)workspace, workspace ? workspace_bytes : 0};
   const int eb = dtype == MOE_F32 ? 4 : 2;
   const bool products = dx || dw;

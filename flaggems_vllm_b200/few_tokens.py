@@ -4,6 +4,7 @@ speculative draft, in two launches."""
 from __future__ import annotations
 
 import logging
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -43,8 +44,8 @@ def fused_moe_few_tokens(
 
     ``hidden_states`` [M, H] bfloat16 or float16; ``router_weight`` [E, H] of the same type or float32.  Logits, scores
     (``scoring``: "softmax" or "sigmoid") and the choice among ``score + e_score_correction_bias`` within the ``topk_group``
-    best of ``num_expert_group`` groups are those of ``router_gemm`` and ``grouped_topk``, in fp32; weights are the scores,
-    divided by their sum where ``renormalize``, times ``routed_scaling_factor``.
+    best of ``num_expert_group`` groups are those of ``router_gemm`` and ``grouped_topk``, in fp32 (up to four tokens bit for bit);
+    weights are the scores, divided by their sum where ``renormalize``, times ``routed_scaling_factor``.
 
     ``w1`` [E, 2 I, H] (gate rows first), ``w2`` [E, H, I] as ``fused_experts_impl`` has them, in the type of the activations, or
     float8_e4m3fn with ``w1_scale`` [E, 2 I / 128, H / 128] and ``w2_scale`` [E, H / 128, I / 128]: the activations are then taken in
@@ -53,7 +54,8 @@ def fused_moe_few_tokens(
     64, in 8 bits of 128; at most 1024 experts, 32 per token.
 
     More tokens: ``router_gemm_grouped_topk``, ``fused_experts_impl`` and ``fused_linear``.  Not differentiable: refused where a
-    gradient is wanted.  The same bits in every run."""
+    gradient is wanted.  The same bits in every run of the same call; what the other tokens of a call choose may change the order of a
+    token's sums."""
     logger.debug("GEMS FUSED MOE FEW TOKENS")
     what = "fused_moe_few_tokens"
     sigmoid = scoring == "sigmoid"
@@ -90,7 +92,7 @@ def _slow(x, router, w1, w2, topk, renormalize, sigmoid, groups, kept, factor, b
     most = _MAX_HIDDEN_FP8 if fp8 else _MAX_HIDDEN
     if not 1 <= E <= _MAX_EXPERTS or not 1 <= I <= _MAX_WIDTH or not 1 <= H <= most:
         raise ValueError(f"{what}: 1 to {_MAX_EXPERTS} experts of 1 to {_MAX_WIDTH} columns, and hidden sizes up to {most}")
-    topk, groups, kept = int(topk), int(groups), int(kept)
+    topk, groups, kept = operator.index(topk), operator.index(groups), operator.index(kept)
     if not 1 <= groups <= _MAX_GROUPS or E % groups != 0 or not 1 <= kept <= groups:
         raise ValueError(f"{what}: {groups} groups, {kept} of them kept, do not divide {E} experts")
     if not 1 <= topk <= min(_MAX_TOPK, E // groups * kept):

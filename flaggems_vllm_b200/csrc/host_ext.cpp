@@ -754,6 +754,7 @@ bool linear_args(const at::Tensor& x, const at::Tensor& w, const at::Tensor* bia
   if (p->code < 0 || !p->status || p->K <= 0 || p->N <= 0 || (act == MOE_LIN_SILU_MUL && p->W % 2 != 0) || w.size(1) != p->K ||
       !w.is_cuda() || w.get_device() != p->dev || w.scalar_type() != x.scalar_type() || p->K > 0x3FFFFFFF || p->N > 0x1FFFFFFF)
     return false;
+  if (p->code == MOE_F32 && std::max(p->K, p->W) > 65535 * 64) return false;
   int64_t rows;
   if (!rows_of(x, &p->M, &p->x_ld) || !rows_of(w, &rows, &p->w_ld) || p->M > 0x3FFFFFFF) return false;
   if (p->M == 1) p->x_ld = p->K;  // a single row has any distance

@@ -625,7 +625,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // ------------------------------------------------------------------ fp32 operands
-// Tiles of D of TM rows and TN columns, RM x 8 outputs to a thread, 16 k at a time out of a ring in shared memory that asynchronous
+// Tiles of D of TM rows and T columns, RM x 8 outputs to a thread (tiles of 32: 4 x 4), 16 k at a time out of a ring in shared memory that asynchronous
 // copies fill (each element to its place, which transposes operands with rows of k; whole 16-byte pieces where rows of r or c allow
 // it); K divided over a cluster as in tile_kernel.  Half of a gated call's columns are gates, the other half the ups that go with
 // them.  A copy is an address and an instruction for every element, and a tile of 128 x 128 has half as many for a product as one
@@ -643,9 +643,9 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // ROWS x 16 elements from (base, k0) on; zeros beyond `end` and `kend`.  gate: rows from ROWS / 2 on lie that far behind the first
-template <int ROWS, int FTHREADS>
+template <int ROWS, int FTHREADS, int FPITCH>
 __device__ __forceinline__ void f32_fill(const F32Operand& X, int64_t base, int64_t end, int64_t gate, int64_t k0, int64_t kend, uint32_t dst) {
-  constexpr int FPITCH = (ROWS < 64 ? 64 : ROWS) + 4, ROUND = FTHREADS / 16;  // rows of a round of copies
+  constexpr int ROUND = FTHREADS / 16;  // rows of a round of copies
   const int t = threadIdx.x;
   if (X.ks == 1) {
     const int k = t & 15;
@@ -696,28 +696,36 @@ __device__ __forceinline__ void f32_fill(const F32Operand& X, int64_t base, int6
     }
   }
 }
+// four neighbours of thread i's, and of eight the other four `half` behind them
+template <int N>
+__device__ __forceinline__ void take(const float* row, int i, int half, float (&v)[N]) {
+#pragma unroll
+  for (int q = 0; q < N; q += 4) {
+    const float4 p = *reinterpret_cast<const float4*>(row + q / 4 * half + 4 * i);
+    v[q] = p.x; v[q + 1] = p.y; v[q + 2] = p.z; v[q + 3] = p.w;
+  }
+}
 template <int RM, int T, int FTHREADS>
-__global__ void __launch_bounds__(FTHREADS, FTHREADS == 64 ? 7 : 2) f32_kernel(const F32Operand A, const F32Operand B, int64_t K, const Product P, const Epilogue E) {
+__global__ void __launch_bounds__(FTHREADS, T == 32 ? 12 : (T == 64 ? 7 : 2)) f32_kernel(const F32Operand A, const F32Operand B, int64_t K, const Product P, const Epilogue E) {
   extern __shared__ __align__(16) uint8_t smem_raw[];  // FSTAGES x {A, B}[16][pitch], then the partial tile
   float* s_mem = reinterpret_cast<float*>(smem_raw);
-  constexpr int TM = RM == 8 ? T : 8, PITCH = T + 4, TILE = 16 * PITCH;  // floats of an operand's tile
-  static_assert(FTHREADS == T * T / 64 && (RM == 8 || T == 64), "threads");
+  constexpr int TM = RM == 1 ? 8 : T, CN = T == 32 ? 4 : 8, PITCH = T + 4, TILE = 16 * PITCH;  // floats of an operand's tile
+  static_assert(RM == 1 ? T == 64 && FTHREADS == 64 : FTHREADS * RM * CN == T * T, "threads");
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   // a warp is 4 x 8 threads: its 16-byte pieces of a k are 64 and 128 bytes
-  const int tx = T == 64 ? (t & 7) : (warp & 1) * 8 + (lane & 7), ty = T == 64 ? (t >> 3) : (warp >> 1) * 4 + (lane >> 3);
+  const int tx = T <= 64 ? (t & 7) : (warp & 1) * 8 + (lane & 7), ty = T <= 64 ? (t >> 3) : (warp >> 1) * 4 + (lane >> 3);
   const int out_cols = P.gate ? T / 2 : T;
-  const uint32_t across = (uint32_t)((P.cols + out_cols - 1) / out_cols), at = blockIdx.x / P.split;
-  const int64_t r0 = (int64_t)(at / across) * TM, c0 = (int64_t)(at % across) * out_cols;
+  const int64_t r0 = (int64_t)(blockIdx.x / P.split) * TM, c0 = (int64_t)blockIdx.y * out_cols;
   const int64_t steps = (K + 15) / 16, first = steps * rank / P.split, last = steps * (rank + 1) / P.split;
   const uint32_t s0 = smem_u32(s_mem);
-  float acc[RM][8] = {};
+  float acc[RM][CN] = {};
   auto fill = [&](int64_t step, int stage) {
     if (step < last) {
       const uint32_t dst = s0 + (uint32_t)stage * (2 * TILE * 4);
-      f32_fill<TM, FTHREADS>(A, r0, P.rows, 0, step * 16, K, dst);
-      f32_fill<T, FTHREADS>(B, c0, P.cols, P.gate, step * 16, K, dst + TILE * 4);
+      f32_fill<TM, FTHREADS, PITCH>(A, r0, P.rows, 0, step * 16, K, dst);
+      f32_fill<T, FTHREADS, PITCH>(B, c0, P.cols, P.gate, step * 16, K, dst + TILE * 4);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -735,30 +743,23 @@ __global__ void __launch_bounds__(FTHREADS, FTHREADS == 64 ? 7 : 2) f32_kernel(c
     if (++from == FSTAGES) from = 0;
 #pragma unroll 4
     for (int k = 0; k < 16; ++k) {
-      const float4 b0 = *reinterpret_cast<const float4*>(sb + k * PITCH + 4 * tx), b1 = *reinterpret_cast<const float4*>(sb + k * PITCH + T / 2 + 4 * tx);
-      float a[RM];
-      if constexpr (RM == 8) {
-        const float4 p = *reinterpret_cast<const float4*>(sa + k * PITCH + 4 * ty), q = *reinterpret_cast<const float4*>(sa + k * PITCH + T / 2 + 4 * ty);
-        a[0] = p.x; a[1] = p.y; a[2] = p.z; a[3] = p.w; a[4] = q.x; a[5] = q.y; a[6] = q.z; a[7] = q.w;
-      } else {
-        a[0] = sa[k * PITCH + ty];
-      }
+      float av[RM], bv[CN];
+      take<CN>(sb + k * PITCH, tx, T / 2, bv);
+      if constexpr (RM == 1) av[0] = sa[k * PITCH + ty];
+      else take<RM>(sa + k * PITCH, ty, T / 2, av);
 #pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        acc[i][0] = fmaf(a[i], b0.x, acc[i][0]); acc[i][1] = fmaf(a[i], b0.y, acc[i][1]);
-        acc[i][2] = fmaf(a[i], b0.z, acc[i][2]); acc[i][3] = fmaf(a[i], b0.w, acc[i][3]);
-        acc[i][4] = fmaf(a[i], b1.x, acc[i][4]); acc[i][5] = fmaf(a[i], b1.y, acc[i][5]);
-        acc[i][6] = fmaf(a[i], b1.z, acc[i][6]); acc[i][7] = fmaf(a[i], b1.w, acc[i][7]);
-      }
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < CN; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
-    float* part = s_mem + (RM == 8 ? (i < 4 ? 4 * ty + i : T / 2 - 4 + 4 * ty + i) : ty) * PITCH + 4 * tx;
+    float* part = s_mem + (RM == 1 ? ty : (i < 4 ? 4 * ty + i : T / 2 - 4 + 4 * ty + i)) * PITCH + 4 * tx;
     *reinterpret_cast<float4*>(part) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-    *reinterpret_cast<float4*>(part + T / 2) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+    if constexpr (CN == 8) *reinterpret_cast<float4*>(part + T / 2) = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
   }
   if (P.split > 1) cluster.sync();
   else __syncthreads();
@@ -1026,28 +1027,33 @@ int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, b
   P.rows = rows;
   P.cols = cols;
   P.gate = gated ? (int)cols : 0;
-  // Tile and split of K by what a multiprocessor has to do: `fit` blocks at once, as fast together as four of 64 x 64 or one and a half
-  // of 128 x 128; a block's share of K and a fixed part.  A share of K stays at 64 or more.
+  // Tile and split of K, by us (fitted to 18 products from 30 x 64 x 32 to 2048 x 1024 x 1024, each tile with splits of 1 to 8, to 8 %):
+  // a block alone on a multiprocessor takes `alone` for each k, `full` where others hide its waiting; `last` is its outputs, which
+  // the ranks of a cluster share, `next` and `ramp` what a further block of the multiprocessor adds.  32 x 32 answers soonest (300 x
+  // 501 -> 333: 11.2 us, 15.5 with tiles of 64), 128 x 128 reads least (2048 x 1024 -> 1024: 114 us, 123 of 64, 172 of 32).
+  struct Tile { int t; double alone, full, last, next, ramp; };
+  static const Tile tiles_of[3] = {{32, 0.0353, 0.0121, 0.9, 0.0, 0.27}, {64, 0.0775, 0.0318, 4.3, 0.92, 0.36}, {128, 0.119, 0.1015, 8.9, 0.0, 4.2}};
   const int64_t sms = sm_count();
   double best = 0.0;
   int T = 64;
   P.split = 1;
-  for (int t = 64; t <= 128; t *= 2) {
-    if (t == 128 && rows <= 64) break;
-    const int TM = rows <= 8 ? 8 : t;
-    const int64_t tiles = ((gated ? 2 * cols : cols) + t - 1) / t * ((rows + TM - 1) / TM);
-    const double one = t == 64 ? 1.0 : 3.1, full = t == 64 ? 4.0 : 1.5;  // a block's products; blocks that fill a multiprocessor
-    const int64_t fit = t == 64 ? 7 : 2;
+  for (const Tile& tile : tiles_of) {
+    const int t = tile.t, TM = rows <= 8 ? 8 : t;
+    if ((rows <= 8 && t != 64) || (t == 128 && rows <= 64)) continue;
+    const int64_t across = ((gated ? 2 * cols : cols) + t - 1) / t, tiles = across * ((rows + TM - 1) / TM);
+    if (across > 65535) continue;
     for (int s = 1; s <= 8 && (s == 1 || K / s >= 64); s *= 2) {
-      const int64_t per = (tiles * s + sms - 1) / sms, rounds = (per + fit - 1) / fit, last = per - (rounds - 1) * fit;
-      const double cost = one * (((double)(rounds - 1) * fit + ((double)last < full ? full : (double)last)) * ((double)K / s + 100.0));
+      // clusters of 8 and 4 find places on some 112 and 132 of 148 multiprocessors, further ones next to them
+      const int64_t reach = s == 8 ? sms * 112 / 148 : (s == 4 ? sms * 132 / 148 : sms), blocks = tiles * s;
+      const double k = (double)K / s, n = blocks > reach && blocks <= sms ? 2.0 : (double)((blocks + sms - 1) / sms);
+      const double cost = (s > 1 ? 1.0 : 0.0) + fmax(tile.alone, n * tile.full) * k + tile.last / s + (n - 1.0) * (tile.next / s + tile.ramp);
       if (best == 0.0 || cost < best) { best = cost; P.split = s; T = t; }
     }
   }
   P.BN = T;
   const int TM = rows <= 8 ? 8 : T;
   const int64_t ct = ((gated ? 2 * cols : cols) + T - 1) / T, rt = (rows + TM - 1) / TM;
-  if (ct * rt * P.split >= (1ll << 31)) return fail(MOE_E_TOOBIG, "fused_linear: too many tiles");
+  if (ct > 65535 || rt * P.split >= (1ll << 31)) return fail(MOE_E_TOOBIG, "fused_linear: fp32 products of at most %d columns", 65535 * 64);
   auto go = [&](auto kern, int t, int threads) {
     const int64_t ring = (int64_t)FSTAGES * 2 * 16 * (t + 4) * 4, part = (int64_t)TM * (t + 4) * 4, smem = ring > part ? ring : part;
     const int rc = allow_smem((const void*)kern, (int)smem);
@@ -1056,7 +1062,7 @@ int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, b
     // Launched behind its predecessor's end: blocks that come while it drains crowd on the multiprocessors that are free first
     // (8192 x 512 -> 512, dW: 264 us so, 159 with each multiprocessor at its share).
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ct * rt * P.split));
+    cfg.gridDim = dim3((unsigned)(rt * P.split), (unsigned)ct);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
@@ -1065,13 +1071,13 @@ int run_f32(F32Operand a, F32Operand b, int64_t rows, int64_t cols, int64_t K, b
     attr.val.clusterDim.x = (unsigned)P.split;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = P.split > 1 ? 1 : 0;
     const cudaError_t ce = cudaLaunchKernelEx(&cfg, kern, a, b, K, P, E);
     if (ce != cudaSuccess) return fail((int)ce, "fused_linear (fp32): %s", cudaGetErrorString(ce));
     return check_launch("fused_linear (fp32)");
   };
   if (TM == 8) return go(f32_kernel<1, 64, 64>, 64, 64);
-  return T == 64 ? go(f32_kernel<8, 64, 64>, 64, 64) : go(f32_kernel<8, 128, 256>, 128, 256);
+  return T == 32 ? go(f32_kernel<4, 32, 64>, 32, 64) : T == 64 ? go(f32_kernel<8, 64, 64>, 64, 64) : go(f32_kernel<8, 128, 256>, 128, 256);
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K, int dtype, int act) {

@@ -16,7 +16,7 @@ from . import _lib
 logger = logging.getLogger(__name__)
 
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "silu_and_mul": 5}
-_MAX_ROWS, _MAX_COLS = 0x3FFFFFFF, 0x1FFFFFFF
+_MAX_ROWS, _MAX_COLS, _MAX_COLS_F32 = 0x3FFFFFFF, 0x1FFFFFFF, 65535 * 64
 
 
 def fused_linear(
@@ -56,6 +56,8 @@ def fused_linear(
     N = rows // 2 if act == 5 else rows
     if x.numel() // K > _MAX_ROWS or K > _MAX_ROWS or N > _MAX_COLS:
         raise ValueError(f"{what}: at most 2^30 - 1 rows, 2^29 - 1 columns")
+    if x.dtype == torch.float32 and max(K, rows) > _MAX_COLS_F32:
+        raise ValueError(f"{what}: at most {_MAX_COLS_F32} columns in float32")
     if weight.dtype != x.dtype:
         raise ValueError(f"{what}: weight must be of the type of x, got {weight.dtype}")
     if bias is not None:

@@ -41,6 +41,9 @@ def test_linear_refusals():
         fg.fused_linear(torch.zeros(1, 64).expand(1 << 30, 64), w)
     with pytest.raises(ValueError, match="2\\^30"):
         fg.fused_linear(x[:, :1], torch.ones(1, 1).expand(1 << 29, 1))
+    for w in (torch.ones(1, 1).expand(4194241, 1), torch.ones(1, 1).expand(1, 4194241)):
+        with pytest.raises(ValueError, match="4194240 columns in float32"):
+            fg.fused_linear(torch.zeros(1, 1).expand(2, w.shape[1]), w)
 
 
 def layer(dtype=torch.bfloat16, M=2, E=8, H=128, I=128, shared=0, fp8=False):

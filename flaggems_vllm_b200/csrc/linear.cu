@@ -105,9 +105,9 @@ __device__ __forceinline__ float bias_at(const Epilogue& E, int n) {
   if (E.bias == nullptr) return 0.0f;
   return E.bias_f32 ? reinterpret_cast<const float*>(E.bias)[n] : ToF32<T>::get(reinterpret_cast<const T*>(E.bias)[n]);
 }
-// the sum(s) of output (m, n) -> its value, and z where it is kept; z1: the gate's partner
+// the sum(s) of output (m, n) -> its value, and z where it is kept; z1: the gate's partner; add: its residual, if that is at hand
 template <typename T>
-__device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, float z0, float z1) {
+__device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, float z0, float z1, const T* add = nullptr) {
   z0 += bias_at<T>(E, n);
   float v;
   if (E.act == MOE_LIN_SILU_MUL) {
@@ -122,12 +122,13 @@ __device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, floa
     v = act_value<T>(E.act, z0);
     if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(z0);
   }
-  if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
+  if (add) v += ToF32<T>::get(*add);
+  else if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
   return v;
 }
 template <typename T>
-__device__ __forceinline__ void finish(const Epilogue& E, int64_t m, int n, float z0, float z1) {
-  reinterpret_cast<T*>(E.y)[m * E.y_ld + n] = from_f32<T>(value<T>(E, m, n, z0, z1));
+__device__ __forceinline__ void finish(const Epilogue& E, int64_t m, int n, float z0, float z1, const T* add) {
+  reinterpret_cast<T*>(E.y)[m * E.y_ld + n] = from_f32<T>(value<T>(E, m, n, z0, z1, add));
 }
 
 // ------------------------------------------------------------------ operand tiles
@@ -159,7 +160,7 @@ struct Product {
 constexpr int TTHREADS = 256;
 struct TAux {
   uint64_t full[12], empty[12], done;
-  uint32_t tmem_base;
+  uint32_t tmem_base, unused;  // whole 8 bytes: the stash lies behind
 };
 // Two waves of blocks and more: tiles of up to 128 columns leave room for a second block on the multiprocessor, which streams while the
 // first one adds up and stores (64 x 4096 -> 2 x 14336 gated 50.5 -> 44.1 us).  One wave: all of the memory is one block's ring (33 x
@@ -167,7 +168,8 @@ struct TAux {
 constexpr int kRingWhole = 196608, kRingHalf = 98304;
 __host__ __device__ constexpr int tile_stage(int bn) { return (128 + bn) * 128; }
 __host__ __device__ constexpr int tile_stages(int bn, int ring) { return ring / tile_stage(bn) < 12 ? ring / tile_stage(bn) : 12; }
-constexpr size_t tile_smem(int ring) { return (size_t)ring + 1024 + sizeof(TAux); }
+constexpr int kStash = 8192;  // residuals of a share of up to 1024 quads
+constexpr size_t tile_smem(int ring) { return (size_t)ring + 1024 + sizeof(TAux) + kStash; }
 static_assert(128 * 260 * 4 <= kRingWhole && 128 * 132 * 4 <= kRingHalf, "the partial tile takes the ring's place");
 static_assert(2 * (tile_smem(kRingHalf) + 1024) <= 233472, "two blocks on a multiprocessor");
 
@@ -185,7 +187,7 @@ __device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* a) {
 // in rank order.  Lanes run along the rows of y.
 template <typename T, int SPLIT, int THREADS = TTHREADS>
 __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t* smem, const Product& P, const Epilogue& E, int rank, int64_t r0,
-                                             int64_t c0, int out_rows, int out_cols) {
+                                             int64_t c0, int out_rows, int out_cols, const T* stash = nullptr) {
   const int pitch = P.BN + 4, quads = out_cols / 4, share = out_rows * quads / SPLIT;  // all powers of two
   const int row_bits = __ffs(out_rows) - 1, quad_bits = __ffs(quads) - 1;
   const int up = P.gate == 0 ? 0 : (P.swapped ? 64 * pitch : P.BN / 2);
@@ -198,6 +200,7 @@ __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t
     const int r = P.swapped ? i & (out_rows - 1) : i >> quad_bits, c = 4 * (P.swapped ? i >> row_bits : i & (quads - 1));
     if (r0 + r >= P.rows || c0 + c >= P.cols) continue;
     const int at = r * pitch + c;
+    const T* add = stash ? stash + 4 * (i - rank * share) : nullptr;
     float4 v[SPLIT], u[SPLIT];
 #pragma unroll
     for (int j = 0; j < SPLIT; ++j) v[j] = *reinterpret_cast<const float4*>(base[j] + at);
@@ -217,15 +220,34 @@ __device__ __forceinline__ void finish_share(cg::cluster_group& cluster, uint8_t
       const int n = (int)(c0 + c);
       float o[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = value<T>(E, m, n + q, z0[q], z1[q]);
+      for (int q = 0; q < 4; ++q) o[q] = value<T>(E, m, n + q, z0[q], z1[q], add ? add + q : nullptr);
       T* y = reinterpret_cast<T*>(E.y) + m * E.y_ld + n;
       if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
       else *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (c0 + c + q < P.cols) finish<T>(E, P.swapped ? c0 + c + q : r0 + r, (int)(P.swapped ? r0 + r : c0 + c + q), z0[q], z1[q]);
+        if (c0 + c + q < P.cols) finish<T>(E, P.swapped ? c0 + c + q : r0 + r, (int)(P.swapped ? r0 + r : c0 + c + q), z0[q], z1[q], add ? add + q : nullptr);
     }
+  }
+}
+
+// The residual of this CTA's share, quad by quad as finish_share takes it, into shared memory while the products run: there each of
+// its steps would wait for memory (33 x 14336 -> 4096 with a residual 27.4 -> 24.1 us, 501 x 1024 -> 768 13.2 -> 9.4).
+template <typename T>
+__device__ __forceinline__ void stash_residual(const Product& P, const Epilogue& E, int rank, int64_t r0, int64_t c0, int out_rows, int out_cols,
+                                               T* stash, int t, int threads) {
+  const int quads = out_cols / 4, share = out_rows * quads / P.split, row_bits = __ffs(out_rows) - 1, quad_bits = __ffs(quads) - 1;
+#pragma unroll 4
+  for (int k = t; k < share; k += threads) {
+    const int i = rank * share + k;
+    const int64_t r = r0 + (P.swapped ? i & (out_rows - 1) : i >> quad_bits), c = c0 + 4 * (P.swapped ? i >> row_bits : i & (quads - 1));
+    T v[4] = {};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (r < P.rows && c + q < P.cols) v[q] = reinterpret_cast<const T*>(E.residual)[P.swapped ? (c + q) * E.residual_ld + r : r * E.residual_ld + c + q];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) stash[4 * k + q] = v[q];
   }
 }
 
@@ -262,6 +284,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   const uint32_t tmem = aux->tmem_base;
   pdl_wait();  // operands, weights among them, may be the kernel's in front
   pdl_trigger();
+  T* stash = E.residual != nullptr && out_rows * out_cols / 4 / P.split <= kStash / 8 ? reinterpret_cast<T*>(aux + 1) : nullptr;
   if (warp == 0) {
     const bool leader = elect_lane();
     const int bbox = gate_b ? (BN / 2 < 64 ? BN / 2 : 64) : (BN < 64 ? BN : 64);  // rows of a box of B
@@ -305,7 +328,10 @@ tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       if (++s == stages) { s = 0; ph ^= 1; }
     }
     if (leader) tc_commit(&aux->done);
-  } else if (warp >= 4) {
+  } else if (stash != nullptr) {
+    stash_residual<T>(P, E, rank, r0, c0, out_rows, out_cols, stash, threadIdx.x - 64, TTHREADS - 64);
+  }
+  if (warp >= 4) {
     // every product has finished reading the ring: it now holds the partial tile, rows of BN + 4 floats (a pitch that spreads
     // 16-byte pieces over the banks down a column as well as along the lanes' rows)
     const bool ok = warp_agrees(mbar_wait(&aux->done, 0, P.status, P.wait_ns));
@@ -326,10 +352,10 @@ tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   if (P.split > 1) cluster.sync();
   else __syncthreads();
   switch (P.split) {
-    case 1: finish_share<T, 1>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols); break;
-    case 2: finish_share<T, 2>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols); break;
-    case 4: finish_share<T, 4>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols); break;
-    default: finish_share<T, 8>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols);
+    case 1: finish_share<T, 1>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols, stash); break;
+    case 2: finish_share<T, 2>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols, stash); break;
+    case 4: finish_share<T, 4>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols, stash); break;
+    default: finish_share<T, 8>(cluster, smem, P, E, rank, r0, c0, out_rows, out_cols, stash);
   }
   tc_fence_before();
   if (P.split > 1) cluster.sync();  // no CTA leaves while its partial tile may still be read

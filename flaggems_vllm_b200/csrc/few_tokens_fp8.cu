@@ -6,8 +6,9 @@
 // as TMA puts it there, and no thread touches a weight.  One instruction multiplies 128 weight rows by 16 columns, of which the
 // tokens are 8; the rest is whatever lies behind them in shared memory, in accumulator columns that nobody reads.
 //
-// The tensor core cannot apply 128 x 128 block scales, so each 128 k go to an accumulator of their own, and two groups of four warps, in turn, add  accumulator * (token's scale * weight's scale)  to eight fp32 registers a lane,
-// a lane being a weight row.  8 columns make that cheap; for the layer of many tokens it would not be.
+// The tensor core cannot apply 128 x 128 block scales, so each 128 k go to an accumulator of their own, and two groups of four warps,
+// in turn, add  accumulator * (token's scale * weight's scale)  to eight fp32 registers a lane, a lane being a weight row.  8 columns
+// make that cheap; for the layer of many tokens it would not be.
 //
 //   W1  a tile is up to 64 outputs: their gate rows and their up rows, in units of 8, so that a block's run of outputs, a multiple
 //       of 8, reads no row twice.  What the two groups hold is joined in shared memory at the tile's end.
@@ -15,8 +16,8 @@
 //       adds a group's last output: once for all blocks that read it.
 //   W2  a K block of all rows of the block's run (48 or 49 of 7168) is one box, with the same k of h.
 //
-// Warps: 0 and 3 TMA, in turn, 1 MMA, 2 TMEM, 4 to 11 the two groups.  W2's first weights are on their way while W1's results are still being
-// quantised and other blocks are waited for.
+// Warps: 0 and 3 TMA, in turn, 1 MMA, 2 TMEM, 4 to 11 the two groups.  W2's first weights are on their way while W1's results are
+// still being quantised and other blocks are waited for.
 #include "few_tokens.cuh"
 
 namespace moe {
@@ -30,7 +31,7 @@ constexpr int kConsumers = 256, kThreads = 128 + kConsumers;
 constexpr int kBlocks1 = 2, kBlocks2 = 4;  // K blocks of 128 in a stage of W1, of W2
 constexpr int kStage1 = kBlocks1 * 128 * 128;
 constexpr int kMaxStages = 12;
-constexpr int kAccs = 8, kAccCols = 16, kAccBlocks = kBlocks1 > kBlocks2 ? kBlocks1 : kBlocks2;    // accumulators of a stage's blocks, 16 columns each
+constexpr int kAccs = 8, kAccCols = 16, kAccBlocks = kBlocks1 > kBlocks2 ? kBlocks1 : kBlocks2;  // a stage's blocks, 16 columns each
 constexpr int kJoinBytes = 2 * 128 * kTokens * 4;
 
 struct Aux {
@@ -324,6 +325,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
       // W2's weights take the ring as soon as W1's products have left it.  Which run of W2 it will be is known from the start; whether
       // another one of W1 comes first, both producers hear from the one that claimed it.
       if (warp == 0 && leader) aux->more1 = next < runs1;
+      __syncwarp();  // a wait that gave up may have ended for some lanes first
       asm volatile("bar.sync 2, 64;" ::: "memory");
       const int run2 = aux->run2[0];
       if (!aux->more1 && run2 < runs2) {
@@ -543,6 +545,7 @@ few_experts8_kernel(const __grid_constant__ Maps maps, const Few P, const Few8 Q
       }
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 2) {

@@ -349,6 +349,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     tc_fence_before();
   }
+  __syncwarp();  // a wait that gave up may have ended for some lanes first
   if (P.split > 1) cluster.sync();
   else __syncthreads();
   switch (P.split) {
@@ -641,6 +642,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
   }
   // -------------------------------------------------------------------- teardown
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while its partner may still signal its barriers

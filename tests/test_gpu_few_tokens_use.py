@@ -1,6 +1,8 @@
 """fused_moe_few_tokens in use: graphs, streams, threads, guard bands, bad values, long offsets; together with the operators around it."""
 
 import ctypes
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -340,3 +342,41 @@ def test_training_step_of_a_shared_expert_beside_the_router():
     b = [t.double().requires_grad_() for t in leaves]
     for p, q in zip(torch.autograd.grad(own(*a), a), torch.autograd.grad(plain(*b), b)):
         assert (p.double() - q).abs().max() <= 2.0**-9.5 * q.abs().max()
+
+
+@pytest.mark.parametrize("dtype,fp8", [(BF, False), (BF, True)])
+def test_more_work_than_one_run_for_a_block(dtype, fp8):
+    """8.4 million outputs of W1: more than a block takes at once, more groups of 128 than its list holds."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("not enough free memory")
+    check(make(1, 8, 128 if fp8 else 64, 1 << 20, 0, dtype, fp8), 8)
+
+
+PROGRAM = """
+import torch
+import flaggems_vllm_b200 as fg
+from flaggems_vllm_b200 import _lib
+
+g = torch.Generator(device="cuda").manual_seed(0)
+rand = lambda *s: (0.1 * torch.randn(s, generator=g, device="cuda")).bfloat16()
+x, w, router, w1, w2 = rand(3, 256), rand(64, 256), rand(16, 256), rand(16, 256, 256), rand(16, 256, 128)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph), torch.no_grad():
+    y = fg.fused_linear(x, w, activation="silu")
+    out = fg.fused_moe_few_tokens(x, router, w1, w2, 4)
+    z = fg.fused_linear(out.float(), w.float())
+assert _lib.read_status() == 0
+graph.replay()
+held = [t.clone() for t in (y, out, z)]
+with torch.no_grad():
+    want = [fg.fused_linear(x, w, activation="silu"), fg.fused_moe_few_tokens(x, router, w1, w2, 4)]
+    want.append(fg.fused_linear(want[1].float(), w.float()))
+assert all(torch.equal(a, b) for a, b in zip(held, want)) and _lib.read_status() == 0
+print("done")
+"""
+
+
+def test_a_first_call_that_is_captured():
+    run = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "done" in run.stdout, run.stderr[-2000:]

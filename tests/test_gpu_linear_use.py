@@ -237,6 +237,20 @@ def test_checkpoint_computes_the_same_again(reentrant):
     assert all(torch.equal(t.grad, g) for t, g in zip((x, w, b, r), want))
 
 
+def test_a_graph_that_is_kept_and_values_that_change():
+    """A second backward pass through one forward; y may be changed afterwards, an operand that the gradient needs may not."""
+    leaves = leaves_of(*make(33, 72, 40, BF, "silu", "same", True))
+    dy = torch.randn(33, 40, device=DEV).to(BF)
+    y = fg.fused_linear(leaves[0], leaves[1], leaves[2], "silu", leaves[3])
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    z = y.add_(1.0)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(z, leaves, dy, retain_graph=True)))
+    with torch.no_grad():
+        leaves[1].mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z, leaves, dy)
+
+
 def test_inference_mode_and_no_grad():
     x, w, b, r = make(20, 64, 40, BF, "relu", "same", True)
     want = fg.fused_linear(x, w, b, "relu", r)

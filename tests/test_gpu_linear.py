@@ -6,9 +6,10 @@ Tolerances, element by element, with u = eps / 2 of the type and S = |x| |W|^T (
 * the activations have slopes of at most 1.13 (gelu) and 1.1 (silu), and are evaluated to 2^-20 of |z| + 1; the gate's product is
   off by |up| 1.1 dgate + |silu(gate)| dup + 2^-19 |y|;
 * y is rounded once: u |y|, and half of the smallest subnormal of f16 below 2^-14;
-* z is kept rounded (for the gated activation in fp32), which moves act' by at most u |z| max|act''| (0.8 gelu, 0.5 silu; relu's step only where z is within its own
-  error of zero, and those elements are given the whole of |dy|); dz itself is rounded, u |dz|.  Both reach dx and dW through the
-  products of absolute values."""
+* z is kept rounded (for the gated activation in fp32; below 2^-14 in f16 by half of the smallest subnormal, which takes a z of less
+  than 2^-25 to the zero at relu's step), which moves act' by at most u |z| max|act''| (0.8 gelu, 0.5 silu; relu's step only where z is
+  within its own error of zero, and those elements are given the whole of |dy|); dz itself is rounded, u |dz|.  Both reach dx and dW
+  through the products of absolute values."""
 
 import pytest
 import torch
@@ -67,7 +68,7 @@ def reference(x, w, b, r, act, dy=None):
     if dy is not None:
         out.backward(dy.double())
         D, dZ = dy.double().abs(), z.grad
-        e = (0 if act == "silu_and_mul" else u) * z.abs() + dz_err  # of the z that the backward pass sees
+        e = dz_err if act == "silu_and_mul" else u * z.abs() + TINY[dtype] + dz_err  # of the z that the backward pass sees
         if act == "silu_and_mul":
             eg, eu = e[:, :h], e[:, h:]
             err = torch.cat([D * ((up.abs() + eu) * 0.5 * eg + 1.1 * eu), D * 1.1 * eg], 1)

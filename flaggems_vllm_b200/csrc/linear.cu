@@ -976,7 +976,7 @@ struct Plan {
   bool pair, swapped;
   int BN, split;
 };
-Plan choose(int64_t rows, int64_t cols, int64_t K, bool gated, bool a_mn, bool b_mn, int sms) {
+Plan choose(int64_t rows, int64_t cols, int64_t K, bool gated, bool a_mn, int sms) {
   Plan best = {false, false, 64, 1};
   double cost = 1e300;
   const int64_t kb = (K + 63) / 64;
@@ -1010,7 +1010,7 @@ template <typename T>
 int run_product(Matrix a, Matrix b, bool a_mn, bool b_mn, int64_t rows, int64_t cols, int64_t K, bool gated, const Epilogue& E,
                 int32_t* status, cudaStream_t st) {
   // a, b: the operands of D [rows, cols]; a_mn: a is [K, rows] in memory.  gated: b has 2 cols rows
-  Plan p = choose(rows, cols, K, gated, a_mn, b_mn, sm_count());
+  Plan p = choose(rows, cols, K, gated, a_mn, sm_count());
   const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   Product P = {};
   P.KB = (int)((K + 63) / 64);

@@ -213,7 +213,7 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
   int tile = begin / KB, kb = begin - tile * KB;
   int to = R::UNITS - 1, at = 0;  // slots
   float acc[4] = {};
-  const uint8_t* xr = xrows + (int64_t)g * P.x_pitch + c * 16;
+  const uint8_t* xr = xrows + g * P.x_pitch + c * 16;
 #pragma unroll 1
   for (int i = begin; i < end; ++i) {
     wait_copies<R::UNITS - 2>();
@@ -506,13 +506,13 @@ int run_router(const Few& P, const void* w, cudaStream_t st) {
 
 template <typename T>
 int run_experts(Few P, cudaStream_t st) {
-  P.x_pitch = P.H * 2 + 64;  // neighbouring tokens' pieces lie in other banks
+  P.x_pitch = (int64_t)P.H * 2 + 64;  // neighbouring tokens' pieces lie in other banks
   const int64_t first = kHead + kWarps * Ring1::BYTES;
-  int64_t smem = first + (int64_t)P.M * P.x_pitch;
+  int64_t smem = first + P.M * P.x_pitch;
   P.staged = smem <= kFewSmem;
   if (!P.staged) {  // the rows then come out of L1
     smem = first;
-    P.x_pitch = (int)(P.x_ld * 2);
+    P.x_pitch = P.x_ld * 2;  // rows may lie any distance apart
   }
   const int G = sm_count();
   const int rows = (P.H + G - 1) / G;

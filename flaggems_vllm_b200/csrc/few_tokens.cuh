@@ -30,7 +30,8 @@ struct Few {
   int64_t x_ld, residual_ld;
   int M, E, H, I, Is, topk, n_group, topk_group, renormalize, sigmoid;
   float scaling;
-  int x_pitch, staged;                          // bytes of a token's row in shared memory; whether the rows are there
+  int64_t x_pitch;                              // bytes from a token's row to the next, where the kernel reads them
+  int staged;                                   // whether that is in shared memory
   int32_t* status;
   unsigned long long wait_ns;
 };

@@ -7,7 +7,7 @@
 #include <set>
 #include <utility>
 
-#include "moe_common.cuh"
+#include "tc_common.cuh"
 
 namespace moe {
 
@@ -58,6 +58,7 @@ int sm_count() {
   }
   return n;
 }
+
 static thread_local char g_err[512] = "";
 static unsigned long long g_wait_limit_ns = 2000000000ull;
 unsigned long long wait_limit_ns() { return g_wait_limit_ns; }
@@ -69,6 +70,41 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+
+namespace tc {
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encoder() {
+  static EncodeTiledFn fn = nullptr;
+  static bool tried = false;
+  if (!tried) {
+    tried = true;
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = (EncodeTiledFn)p;
+  }
+  return fn;
+}
+
+int encode_map(CUtensorMap* m, const char* what, CUtensorMapDataType dt, int dims, const void* base, const cuuint64_t* size, const cuuint64_t* stride,
+               const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  const EncodeTiledFn enc = encoder();
+  if (!enc) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  auto call = [&] {
+    return enc(m, dt, (cuuint32_t)dims, const_cast<void*>(base), size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = call();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has not used the device yet: the driver's calls do not bind it, the runtime's do
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = call();
+  }
+  if (r != CUDA_SUCCESS) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled%s failed with CUresult %d", what, (int)r);
+  return 0;
+}
+}  // namespace tc
 
 static std::atomic<unsigned long long> g_launches{0};
 

@@ -572,12 +572,7 @@ int launch(const Maps& maps, const Few& P, const Few8& Q, int G, cudaStream_t st
 }
 
 int encode(CUtensorMap* m, const void* base, int dims, const cuuint64_t* size, const cuuint64_t* stride, const cuuint32_t* box) {
-  EncodeTiledFn enc = get_encode();
-  if (!enc) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, const_cast<void*>(base), size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return encode_map(m, "", CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, base, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 // W1 of `experts`, [2 width, H] each
 int encode_w1(CUtensorMap* m, const void* base, uint64_t experts, uint64_t width, uint64_t H) {

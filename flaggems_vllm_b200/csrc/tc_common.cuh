@@ -456,42 +456,21 @@ __device__ __forceinline__ void widen4<__half>(uint32_t w, uint32_t& lo, uint32_
 }
 
 // ------------------------------------------------------------------ host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static inline EncodeTiledFn get_encode() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiledFn)p;
-  }
-  return fn;
-}
+// A tiled tensor map of `dims` dimensions, elements next to each other, zeros outside; 0 or the library's error (common.cu).
+int encode_map(CUtensorMap* m, const char* what, CUtensorMapDataType dt, int dims, const void* base, const cuuint64_t* size, const cuuint64_t* stride,
+               const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion);
 
 // 2-D row-major [rows, cols] tensor, box = `box_bytes` of a row x box_rows rows.  128-byte
 // boxes use the 128-byte swizzle (tensor-core operand layout); narrower boxes land unswizzled.
 static inline int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t rows,
                            uint64_t cols, uint32_t box_rows, bool weights, int box_bytes = 128, uint64_t ld = 0) {
-  EncodeTiledFn enc = get_encode();
-  if (!enc) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
   if (((uintptr_t)base & 15) != 0) return fail(MOE_E_BADARG, "tensor-core GEMM: operand not 16-byte aligned");
   if (((ld != 0 ? ld : cols) * elem_bytes) % 16 != 0) return fail(MOE_E_SHAPE, "tensor-core GEMM: row pitch must be a multiple of 16 bytes");
   cuuint64_t gdim[2] = {cols, rows};
   cuuint64_t gstr[1] = {(ld != 0 ? ld : cols) * (uint64_t)elem_bytes};  // ld: row pitch in elements
   cuuint32_t box[2] = {(cuuint32_t)(box_bytes / elem_bytes), box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, dt, 2, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                   weights ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  return 0;
+  return encode_map(m, "", dt, 2, base, gdim, gstr, box, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    weights ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 // Gate | up weights [E, 2I, K] as five dimensions, so that one box of 128 rows is eight times {8 gate rows, the
@@ -499,19 +478,13 @@ static inline int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType
 // tmem_ld_frag32_async a thread then holds gate and up of the same output and token.
 static inline int make_gate_up_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t E,
                                    uint64_t I, uint64_t K) {
-  EncodeTiledFn enc = get_encode();
-  if (!enc) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
   if (((uintptr_t)base & 15) != 0) return fail(MOE_E_BADARG, "tensor-core GEMM: weights not 16-byte aligned");
   if ((K * elem_bytes) % 16 != 0 || I % 8 != 0) return fail(MOE_E_SHAPE, "tensor-core GEMM: weight shape");
   const uint64_t row = K * (uint64_t)elem_bytes;
   cuuint64_t gdim[5] = {K, 8, 2, I / 8, E};
   cuuint64_t gstr[4] = {row, I * row, 8 * row, 2 * I * row};
   cuuint32_t box[5] = {(cuuint32_t)(128 / elem_bytes), 8, 2, 8, 1};
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(m, dt, 5, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MOE_E_DRIVER, "cuTensorMapEncodeTiled (gate | up) failed with CUresult %d", (int)r);
-  return 0;
+  return encode_map(m, " (gate | up)", dt, 5, base, gdim, gstr, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 }  // namespace tc

@@ -1,12 +1,14 @@
-"""The first call of a thread."""
+"""The first call of a thread, and the first ones of a process, made by several threads at once."""
 
+import subprocess
+import sys
 import threading
 
 import pytest
 import torch
 
 import flaggems_vllm_b200 as fg
-from flaggems_vllm_b200 import testing
+from flaggems_vllm_b200 import _lib, testing
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +70,21 @@ def test_first_call_of_a_thread():
         (got,) = in_threads(run, 1)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), name
     assert fg.read_status() == 0
+
+
+def first_calls(name):
+    run = operators()[name]
+    _lib.host()
+    _lib.status_word("cuda")
+    torch.cuda.synchronize()
+    sys.setswitchinterval(1e-6)
+    got = in_threads(run, 12)
+    want = run()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want)) and fg.read_status() == 0
+
+
+@pytest.mark.parametrize("name", ["fused_linear", "few tokens e4m3"])
+def test_first_calls_of_a_process(name):
+    program = f"import sys; sys.path[:0] = ['tests', '.']; import test_gpu_first_calls as t; t.first_calls({name!r})"
+    r = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

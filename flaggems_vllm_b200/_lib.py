@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from ctypes import c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 
 import torch
@@ -117,6 +118,7 @@ SYMBOLS = {
 
 _lib = None
 _status = {}
+_status_lock = threading.Lock()
 
 
 class MoeKernelError(RuntimeError):
@@ -190,14 +192,16 @@ def status_word(device) -> torch.Tensor:
     if key is None:
         key = torch.cuda.current_device()
     if key not in _status:
-        # as part of a graph the word would hold anything before the first replay, and every replay would clear what other
-        # calls reported
-        if torch.cuda.is_current_stream_capturing():
-            word = host().word_beside_capture(key)
-        else:
-            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
-        host().set_status(key, word.data_ptr())
-        _status[key] = word
+        with _status_lock:  # of two words the kernels would write one and read_status read the other
+            if key not in _status:
+                # as part of a graph the word would hold anything before the first replay, and every replay would clear what
+                # other calls reported
+                if torch.cuda.is_current_stream_capturing():
+                    word = host().word_beside_capture(key)
+                else:
+                    word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+                host().set_status(key, word.data_ptr())
+                _status[key] = word
     return _status[key]
 
 

@@ -100,6 +100,17 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     default: return 1.0f;
   }
 }
+// A sum as the backward pass gets it: a finite one that the type cannot hold becomes its largest value, not infinity, where the slopes
+// are 0 times infinity (far out they are 0 and 1 long before).  What is no finite number stays as it is.
+template <typename T>
+__device__ __forceinline__ float kept(float z) {
+  if constexpr (sizeof(T) == 2) {
+    constexpr float most = std::is_same<T, __half>::value ? 65504.0f : 0x1.FEp127f;
+    const float a = fabsf(z);
+    z = a > most && a < INFINITY ? copysignf(most, z) : z;
+  }
+  return z;
+}
 template <typename T>
 __device__ __forceinline__ float bias_at(const Epilogue& E, int n) {
   if (E.bias == nullptr) return 0.0f;
@@ -120,7 +131,7 @@ __device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, floa
     }
   } else {
     v = act_value<T>(E.act, z0);
-    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(z0);
+    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(kept<T>(z0));
   }
   if (add) v += ToF32<T>::get(*add);
   else if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
@@ -608,7 +619,12 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = v[i] * sigmoid<T>(v[i]) * u[i];
         } else {
-          if (z) store_rows<T>(z, E.z_ld, z16, z32, R, v);
+          if (z) {
+            float k[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) k[i] = kept<T>(v[i]);
+            store_rows<T>(z, E.z_ld, z16, z32, R, k);
+          }
           switch (E.act) {  // one loop each: the choice is the call's
             case MOE_LIN_NONE: break;
             case MOE_LIN_RELU:

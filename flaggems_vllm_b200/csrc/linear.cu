@@ -101,13 +101,16 @@ __device__ __forceinline__ float act_slope(int act, float z) {
   }
 }
 // A sum as the backward pass gets it: a finite one that the type cannot hold becomes its largest value, not infinity, where the slopes
-// are 0 times infinity (far out they are 0 and 1 long before).  What is no finite number stays as it is.
+// are 0 times infinity (far out they are 0 and 1 long before).  What is no finite number stays as it is.  relu's slope asks for the sign:
+// a positive sum that the type would round to zero becomes its smallest value.
 template <typename T>
-__device__ __forceinline__ float kept(float z) {
+__device__ __forceinline__ float kept(float z, bool relu) {
   if constexpr (sizeof(T) == 2) {
-    constexpr float most = std::is_same<T, __half>::value ? 65504.0f : 0x1.FEp127f;
+    constexpr bool half = std::is_same<T, __half>::value;
+    constexpr float most = half ? 65504.0f : 0x1.FEp127f, least = half ? 0x1p-24f : 0x1p-133f;
     const float a = fabsf(z);
     z = a > most && a < INFINITY ? copysignf(most, z) : z;
+    if (relu && z > 0.0f) z = fmaxf(z, least);
   }
   return z;
 }
@@ -131,7 +134,7 @@ __device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, floa
     }
   } else {
     v = act_value<T>(E.act, z0);
-    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(kept<T>(z0));
+    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(kept<T>(z0, E.act == MOE_LIN_RELU));
   }
   if (add) v += ToF32<T>::get(*add);
   else if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
@@ -622,7 +625,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           if (z) {
             float k[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) k[i] = kept<T>(v[i]);
+            for (int i = 0; i < 32; ++i) k[i] = kept<T>(v[i], E.act == MOE_LIN_RELU);
             store_rows<T>(z, E.z_ld, z16, z32, R, k);
           }
           switch (E.act) {  // one loop each: the choice is the call's

@@ -47,6 +47,16 @@ def test_sums_beyond_the_largest_value(dtype, M, K, N, act):
     assert (y[:, bias < -7e4] == 0).all()
 
 
+@pytest.mark.parametrize("M,K,N", SIZES)
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_relu_of_sums_below_the_smallest_value(dtype, M, K, N):
+    """A positive sum that rounds to zero in the operands' type has relu's slope of positive sums, a negative one or zero has none."""
+    tiny = torch.tensor([2.0**-25, 1e-8, 2.0**-40, -1e-8, 0.0, -0.0, 1e-30, -(2.0**-25), 1.0, 3e-8] if dtype == HF else
+                        [2.0**-134, 1e-41, -1e-41, 0.0, -0.0, 2.0**-149, -(2.0**-149), 1.0, 1e-38], device=DEV)
+    bias = tiny.repeat(N // tiny.numel() + 1)[:N]
+    step(dtype, M, K, N, "relu", bias, bias > 0, 0.0)
+
+
 @pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dtype", [HF, BF])
 def test_sums_that_are_no_numbers_stay_so(dtype, act):

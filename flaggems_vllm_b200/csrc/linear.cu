@@ -43,18 +43,22 @@ struct Epilogue {
   int N, act, bias_f32;
 };
 
-// Distribution function of the normal distribution, Phi.  fp32 results take CUDA's; 16-bit ones formula 7.1.26 of Abramowitz and
-// Stegun, Handbook of Mathematical Functions, for the complementary error function, whose relative error stays near 1e-6 down
-// the tail because the exponential stands outside: a sixth of the instructions (its own error is below 2^-20, theirs 2^-9 and 2^-12).
+// Distribution function of the normal distribution, Phi.  fp32 results take CUDA's; 16-bit ones, on the negative side,
+// e^(-z^2 / 2) erfcx(|z| / sqrt 2) / 2 with erfcx(x) = t P(t), t = 1 / (1 + 0.51 x): the form of formula 7.1.26 in Abramowitz and
+// Stegun, Handbook of Mathematical Functions, whose own coefficients keep the absolute error small.  The seven here keep the relative one
+// below 2^-20 for x up to 10 (least squares reweighted towards the largest error, against erfcx in 64 bits), where Phi is below
+// bf16's smallest number.  What is left is the fast exponential's error, 2^-16 of Phi at z = -13 and 2^-18 at -6; half a step is
+// 2^-8 and 2^-11 of the value.  (4096 x 2048 -> 4096
+// bf16 with gelu: 51.9 us, 51.3 with the published five.)
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z) {
   if constexpr (std::is_same<T, float>::value) {
     return normcdff(z);
   } else {
-    const float x = fabsf(z) * 0.7071067811865476f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * p * __expf(-x * x);
+    const float t = __fdividef(1.0f, fmaf(0.36062446f, fabsf(z), 1.0f));  // 0.51 / sqrt 2
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.0944997968f, -0.359134275f), 0.35844488f), 0.0550533605f), 0.279065958f),
+                                     0.284152342f), 0.287917501f);
+    const float tail = 0.5f * p * __expf(-0.5f * z * z);
     return z < 0.0f ? tail : 1.0f - tail;
   }
 }

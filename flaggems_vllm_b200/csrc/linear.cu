@@ -104,19 +104,37 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     default: return 1.0f;
   }
 }
-// A sum as the backward pass gets it: a finite one that the type cannot hold becomes its largest value, not infinity, where the slopes
-// are 0 times infinity (far out they are 0 and 1 long before).  What is no finite number stays as it is.  relu's slope asks for the sign:
-// a positive sum that the type would round to zero becomes its smallest value.
-template <typename T>
-__device__ __forceinline__ float kept(float z, bool relu) {
-  if constexpr (sizeof(T) == 2) {
-    constexpr bool half = std::is_same<T, __half>::value;
-    constexpr float most = half ? 65504.0f : 0x1.FEp127f, least = half ? 0x1p-24f : 0x1p-133f;
-    const float a = fabsf(z);
-    z = a > most && a < INFINITY ? copysignf(most, z) : z;
-    if (relu && z > 0.0f) z = fmaxf(z, least);
+// How sums are rounded, two at a time: as results, or as the backward pass gets them.  There, those that the type cannot hold become its
+// largest value, not infinity, where the slopes are 0 times infinity (far out they are 0 and 1 long before); what is no number stays
+// so.  relu's slope asks for the sign: a positive sum that the type would round to zero becomes its smallest value.
+struct AsResult {
+  template <typename T>
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack2<T>(lo, hi); }
+};
+struct AsKept {
+  template <typename T>
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
   }
-  return z;
+};
+struct AsKeptSign {
+  template <typename T>
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    constexpr float least = std::is_same<T, __half>::value ? 0x1p-24f : 0x1p-133f;
+    return AsKept::pack<T>(lo > 0.0f ? fmaxf(lo, least) : lo, hi > 0.0f ? fmaxf(hi, least) : hi);
+  }
+};
+template <typename T, typename As>
+__device__ __forceinline__ T rounded(float v) {
+  if constexpr (sizeof(T) == 4) {
+    return v;
+  } else {
+    const uint16_t h = (uint16_t)As::template pack<T>(v, 0.0f);
+    return *reinterpret_cast<const T*>(&h);
+  }
 }
 template <typename T>
 __device__ __forceinline__ float bias_at(const Epilogue& E, int n) {
@@ -138,7 +156,7 @@ __device__ __forceinline__ float value(const Epilogue& E, int64_t m, int n, floa
     }
   } else {
     v = act_value<T>(E.act, z0);
-    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = from_f32<T>(kept<T>(z0, E.act == MOE_LIN_RELU));
+    if (E.z) reinterpret_cast<T*>(E.z)[m * E.z_ld + n] = E.act == MOE_LIN_RELU ? rounded<T, AsKeptSign>(z0) : rounded<T, AsKept>(z0);
   }
   if (add) v += ToF32<T>::get(*add);
   else if (E.residual) v += ToF32<T>::get(reinterpret_cast<const T*>(E.residual)[m * E.residual_ld + n]);
@@ -438,7 +456,7 @@ __device__ __forceinline__ void load_rows(const S* base, int64_t ld, bool wide, 
     for (int i = 0; i < 32; ++i) v[i] = R.stage[R.lane * kStagePitch + i];
   }
 }
-template <typename S>
+template <typename S, typename As = AsResult>
 __device__ __forceinline__ void store_rows(S* base, int64_t ld, bool wide, bool wide32, const Rows& R, const float (&v)[32]) {
   if (wide && R.n == 32) {
     if (R.m0 + R.lane < R.end) {
@@ -453,8 +471,8 @@ __device__ __forceinline__ void store_rows(S* base, int64_t ld, bool wide, bool 
         uint4 q[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          q[i] = make_uint4(pack2<S>(v[8 * i], v[8 * i + 1]), pack2<S>(v[8 * i + 2], v[8 * i + 3]), pack2<S>(v[8 * i + 4], v[8 * i + 5]),
-                            pack2<S>(v[8 * i + 6], v[8 * i + 7]));
+          q[i] = make_uint4(As::template pack<S>(v[8 * i], v[8 * i + 1]), As::template pack<S>(v[8 * i + 2], v[8 * i + 3]),
+                            As::template pack<S>(v[8 * i + 4], v[8 * i + 5]), As::template pack<S>(v[8 * i + 6], v[8 * i + 7]));
         store_row_pieces<4>(p, q, wide32);
       }
     }
@@ -465,7 +483,7 @@ __device__ __forceinline__ void store_rows(S* base, int64_t ld, bool wide, bool 
     __syncwarp();
 #pragma unroll 8
     for (int r = 0; r < 32; ++r)
-      if (R.m0 + r < R.end && R.lane < R.n) base[(R.m0 + r) * ld + R.n0 + R.lane] = from_f32<S>(R.stage[r * kStagePitch + R.lane]);
+      if (R.m0 + r < R.end && R.lane < R.n) base[(R.m0 + r) * ld + R.n0 + R.lane] = rounded<S, As>(R.stage[r * kStagePitch + R.lane]);
   }
 }
 // whole 16 (32) byte pieces, for columns that begin at multiples of 32
@@ -627,10 +645,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           for (int i = 0; i < 32; ++i) v[i] = v[i] * sigmoid<T>(v[i]) * u[i];
         } else {
           if (z) {
-            float k[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) k[i] = kept<T>(v[i], E.act == MOE_LIN_RELU);
-            store_rows<T>(z, E.z_ld, z16, z32, R, k);
+            if (E.act == MOE_LIN_RELU) store_rows<T, AsKeptSign>(z, E.z_ld, z16, z32, R, v);
+            else store_rows<T, AsKept>(z, E.z_ld, z16, z32, R, v);
           }
           switch (E.act) {  // one loop each: the choice is the call's
             case MOE_LIN_NONE: break;

@@ -66,3 +66,11 @@ def test_sums_that_are_no_numbers_stay_so(dtype, act):
     y = fg.fused_linear(*leaves, act)
     dx, dw, db = torch.autograd.grad(y, leaves, torch.ones_like(y))
     assert y.isnan().all() and dx.isnan().all() and dw.isnan().all() and db.isnan().all()
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_infinite_sums_have_the_slope_of_the_limit(dtype, M, K, N, act):
+    bias = torch.tensor([float("inf"), -float("inf"), 1e4, -1e4], device=DEV).repeat(N // 4 + 1)[:N]
+    step(dtype, M, K, N, act, bias, bias > 0, 0.02)

@@ -62,12 +62,19 @@ __device__ __forceinline__ float normal_cdf(float z) {
     return z < 0.0f ? tail : 1.0f - tail;
   }
 }
-// 1 / (1 + e^-z): fast forms where the result is rounded to 16 bits (a couple of ulp of fp32).  The fast division returns zero for
-// divisors beyond 2^126, which is right here.
+// 1 / (1 + e^-z), by e^-|z|, which cannot overflow: below z = -88 too, where the result, or z times it, is still a normal number of
+// fp32 and bf16.  Fast forms where the result is rounded to 16 bits.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (std::is_same<T, float>::value) return 1.0f / (1.0f + expf(-z));
-  else return __fdividef(1.0f, 1.0f + __expf(-z));
+  float e, q;
+  if constexpr (std::is_same<T, float>::value) {
+    e = expf(-fabsf(z));
+    q = 1.0f / (1.0f + e);
+  } else {
+    e = __expf(-fabsf(z));
+    q = __fdividef(1.0f, 1.0f + e);
+  }
+  return z < 0.0f ? e * q : q;
 }
 // (1 + tanh(c (z + a z^3))) / 2 is the sigmoid of twice the argument
 template <typename T>

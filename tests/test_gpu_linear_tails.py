@@ -60,3 +60,17 @@ def test_slope_of_gelu(dtype):
     cdf, slope = 0.5 * torch.special.erfc(-t * 0.5**0.5), t * torch.exp(-t * t / 2) / (2 * torch.pi) ** 0.5
     off = (db.double() - (cdf + slope)).abs()
     assert (off <= relative(t * t / 2) * (cdf + slope.abs()) + 2.0**-140).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "silu_and_mul", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("M,N", SIZES)
+def test_sigmoids(dtype, M, N, act):
+    """z sigmoid(s): s = z, or for gelu_tanh s = 2 sqrt(2/pi) (z + 0.044715 z^3).  Down to exponentials of e^-100."""
+    z = torch.linspace(-9.9 if act == "gelu_tanh" else -100.0, 20.0, N, device=DEV)
+    t = z.double()
+    s = t if act != "gelu_tanh" else 2 * (2 / torch.pi) ** 0.5 * (t + 0.044715 * t**3)
+    want = t * torch.exp(s.clamp(max=0)) / (1 + torch.exp(-s.abs()))
+    up = 0.75 if act == "silu_and_mul" else None
+    roundings = 4.0 if act == "gelu_tanh" else 1.0  # its s is a polynomial in fp32
+    close(values(act, z, dtype, M, up), want * (up or 1.0), relative(roundings * s.abs().clamp(max=110)), dtype)

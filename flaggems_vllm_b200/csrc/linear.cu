@@ -897,8 +897,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad P) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float s = sigmoid<T>(z[i]), d = dy[i];
-          du[i] = d * (z[i] * s);
-          dy[i] = d * u[i] * (s * (1.0f + z[i] * (1.0f - s)));
+          du[i] = __fmul_rn(d, z[i] * s);  // never part of a fused sum, whoever takes dz
+          dy[i] = __fmul_rn(d * u[i], s * (1.0f + z[i] * (1.0f - s)));
           s0[i] += dy[i];
           s1[i] += du[i];
         }
@@ -910,7 +910,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGrad P) {
         if (P.act != MOE_LIN_NONE) {
           load(T(), P.z, m * P.z_ld + n, z);
 #pragma unroll
-          for (int i = 0; i < V; ++i) dy[i] *= act_slope<T>(P.act, z[i]);
+          for (int i = 0; i < V; ++i) dy[i] = __fmul_rn(dy[i], act_slope<T>(P.act, z[i]));
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) s0[i] += dy[i];

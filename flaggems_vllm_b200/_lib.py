@@ -107,6 +107,8 @@ SYMBOLS = {
                                  c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "moe_fused_linear_grad_workspace": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_int,
                                                 c_void_p]),
+    "moe_fused_linear_grad_workspace_of": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_int,
+                                                   c_int, c_int, c_int, c_void_p]),
     "moe_fused_linear_grad": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64,
                                       c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "moe_few_tokens_workspace": (c_int, [c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p]),

@@ -858,13 +858,13 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
       if (want_w) out[1] = fresh({W, K}, dy.scalar_type(), dev);
       if (want_b) out[2] = fresh({W}, bias_type, dev);
       int64_t bytes = 0;
-      must(moe_fused_linear_grad_workspace(want_w ? x.const_data_ptr() : nullptr, x_ld, want_x ? w.const_data_ptr() : nullptr, w_ld, code, M, N, K,
-                                           (int)act, &bytes));
-      ws = fresh({bytes}, at::kByte, dev);
+      must(moe_fused_linear_grad_workspace_of(dy.const_data_ptr(), want_w ? x.const_data_ptr() : nullptr, x_ld,
+                                              want_x ? w.const_data_ptr() : nullptr, w_ld, code, M, N, K, (int)act, want_x, want_w, want_b, &bytes));
+      if (bytes) ws = fresh({bytes}, at::kByte, dev);
       must(moe_fused_linear_grad(dy.const_data_ptr(), z.defined() ? z.const_data_ptr() : nullptr, z_ld, want_w ? x.const_data_ptr() : nullptr, x_ld,
                                  want_x ? w.const_data_ptr() : nullptr, w_ld, code, M, N, K, (int)act, want_x ? out[0].mutable_data_ptr() : nullptr,
                                  want_w ? out[1].mutable_data_ptr() : nullptr, want_b ? out[2].mutable_data_ptr() : nullptr,
-                                 want_b ? (int)bias_code : code, ws.mutable_data_ptr(), bytes, status_of(dev), stream_on(dev)));
+                                 want_b ? (int)bias_code : code, bytes ? ws.mutable_data_ptr() : nullptr, bytes, status_of(dev), stream_on(dev)));
     }
     return once(out, "fused_linear");
   }

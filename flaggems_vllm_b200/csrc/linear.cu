@@ -1227,16 +1227,14 @@ extern "C" int moe_fused_linear(const void* x, int64_t x_ld, const void* w, int6
 
 namespace moe {
 namespace {
-// the parts of the backward pass' workspace: dz (or dy where TMA cannot read it), x and w likewise, the bias' partial sums
+// Elements to a thread of act_grad_kernel, and its blocks of rows
 struct GradPlan {
-  bool need_dz;
   int V;
   int64_t rows_per_block, blocks;
 };
-GradPlan grad_plan(const void* dy, const void* z, int64_t z_ld, const void* dz, int dtype, int64_t M, int64_t N, int act, bool products) {
+GradPlan grad_plan(const void* dy, const void* z, int64_t z_ld, const void* dz, int dtype, int64_t M, int64_t N, int act) {
   GradPlan p;
   const int64_t W = width(N, act);
-  p.need_dz = products && act != MOE_LIN_NONE;
   const int eb = dtype == MOE_F32 ? 4 : 2;
   auto wide = [&](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && ld * eb % 16 == 0; };
   const bool z_wide = act == MOE_LIN_SILU_MUL ? ((uintptr_t)z & 15) == 0 && z_ld % 4 == 0 : act == MOE_LIN_NONE || wide(z, z_ld);
@@ -1244,6 +1242,23 @@ GradPlan grad_plan(const void* dy, const void* z, int64_t z_ld, const void* dz, 
   p.rows_per_block = grad_rows(M, N, p.V, sm_count());
   p.blocks = (M + p.rows_per_block - 1) / p.rows_per_block;
   return p;
+}
+// The parts of the backward pass' workspace, in bytes: dz, or dy where TMA cannot read it; the bias' partial sums; x and w where TMA cannot
+// read them.  dy null: wherever it lies.
+struct GradSpace {
+  int64_t dz, part, x, w;
+  int64_t all() const { return dz + part + x + w; }
+};
+GradSpace grad_space(const void* dy, const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M, int64_t N, int64_t K, int act,
+                     bool dx, bool dw, bool db) {
+  GradSpace s = {};
+  const int64_t W = width(N, act);
+  const bool half = dtype != MOE_F32;
+  if ((dx || dw) && (act != MOE_LIN_NONE || (half && (dy == nullptr || !tma_reads({dy, M, N, N}))))) s.dz = up256(M * padded(W) * (half ? 2 : 4));
+  if (db) s.part = up256(((M + 31) / 32 < 512 ? (M + 31) / 32 : 512) * W * 4);
+  if (half && dw && !tma_reads({x, M, K, x_ld})) s.x = up256(M * padded(K) * 2);
+  if (half && dx && !tma_reads({w, W, K, w_ld})) s.w = up256(W * padded(K) * 2);
+  return s;
 }
 }  // namespace
 }  // namespace moe
@@ -1253,14 +1268,16 @@ extern "C" int moe_fused_linear_grad_workspace(const void* x, int64_t x_ld, cons
   using namespace moe;
   if (const int rc = check_sizes(M, N, K, dtype, act)) return rc;
   if (!bytes) return fail(MOE_E_BADARG, "fused_linear_grad_workspace: null pointer");
-  const int64_t W = width(N, act);
-  const int eb = dtype == MOE_F32 ? 4 : 2;
-  *bytes = up256(M * padded(W) * eb);  // dz, or dy with another pitch
-  *bytes += up256(((M + 31) / 32 < 512 ? (M + 31) / 32 : 512) * W * 4);
-  if (dtype != MOE_F32) {
-    if (!tma_reads({x, M, K, x_ld})) *bytes += up256(M * padded(K) * 2);
-    if (!tma_reads({w, W, K, w_ld})) *bytes += up256(W * padded(K) * 2);
-  }
+  *bytes = grad_space(nullptr, x, x_ld, w, w_ld, dtype, M, N, K, act, true, true, true).all();
+  return 0;
+}
+
+extern "C" int moe_fused_linear_grad_workspace_of(const void* dy, const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M,
+                                                  int64_t N, int64_t K, int act, int dx, int dw, int db, int64_t* bytes) {
+  using namespace moe;
+  if (const int rc = check_sizes(M, N, K, dtype, act)) return rc;
+  if (!bytes) return fail(MOE_E_BADARG, "fused_linear_grad_workspace_of: null pointer");
+  *bytes = grad_space(dy, x, x_ld, w, w_ld, dtype, M, N, K, act, dx != 0, dw != 0, db != 0).all();
   return 0;
 }
 
@@ -1282,7 +1299,7 @@ extern "C" int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld
   const int64_t dz_ld = act == MOE_LIN_NONE ? N : padded(W);
   void* own = products && act != MOE_LIN_NONE ? ws.take(M * dz_ld * eb) : nullptr;
   if (products && act != MOE_LIN_NONE && !own) return fail(MOE_E_BADARG, "fused_linear_grad: workspace too small");
-  GradPlan g = grad_plan(dy, z, z_ld, own, dtype, M, N, act, products);
+  GradPlan g = grad_plan(dy, z, z_ld, own, dtype, M, N, act);
   if (own || db) {
     ActGrad G = {dy, z, own, nullptr, M, N, z_ld, dz_ld, g.rows_per_block, (int)N, act};
     if (db) {

@@ -527,9 +527,13 @@ int moe_fused_linear(const void* x, int64_t x_ld, const void* w, int64_t w_ld, c
                      int64_t z_ld, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 /* Its gradients: dz = dy act'(z), dx = dz w [M, K], dw = dz^T x [N or 2 N, K], db = sums of dz [N or 2 N] in db_dtype (dtype or
  * fp32); each without gaps, null = not wanted.  dy [M, N] without gaps, M > 0; z as moe_fused_linear kept it (act NONE: null).  The
- * workspace may take less than moe_fused_linear_grad_workspace says, never more. */
+ * workspace, 16-byte aligned, is what moe_fused_linear_grad_workspace says for any dy and any results, or what
+ * moe_fused_linear_grad_workspace_of says for this dy and the results that are wanted (0, and then null, where rows are whole
+ * 16-byte pieces and there is no activation and no bias). */
 int moe_fused_linear_grad_workspace(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M, int64_t N,
                                     int64_t K, int act, int64_t* bytes /* host */);
+int moe_fused_linear_grad_workspace_of(const void* dy, const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M,
+                                       int64_t N, int64_t K, int act, int dx, int dw, int db, int64_t* bytes /* host */);
 int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld, const void* x, int64_t x_ld, const void* w, int64_t w_ld,
                           int dtype, int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* db, int db_dtype,
                           void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);

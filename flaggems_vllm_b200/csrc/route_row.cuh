@@ -1,5 +1,6 @@
-// The routing of one token by one warp, shared by the kernels of grouped_topk.cu and few_tokens.cu: the ordering of scores and the
-// group-limited selection of the largest.  The header of grouped_topk.cu has the definition.
+// The ordering of scores as integer keys, which the kernels of grouped_topk.cu and few_tokens.cu share, and grouped_topk.cu's routing of one
+// token by one warp: the group-limited selection of the largest.  The header of grouped_topk.cu has the definition.  few_tokens.cuh has
+// the same choice in fewer steps (choose); the tests hold the two together, ties of experts and of groups included.
 #pragma once
 
 #include "moe_common.cuh"

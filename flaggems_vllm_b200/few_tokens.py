@@ -44,14 +44,15 @@ def fused_moe_few_tokens(
 
     ``hidden_states`` [M, H] bfloat16 or float16; ``router_weight`` [E, H] of the same type or float32.  Logits, scores
     (``scoring``: "softmax" or "sigmoid") and the choice among ``score + e_score_correction_bias`` within the ``topk_group``
-    best of ``num_expert_group`` groups are those of ``router_gemm`` and ``grouped_topk``, in fp32 (up to four tokens bit for bit);
-    weights are the scores, divided by their sum where ``renormalize``, times ``routed_scaling_factor``.
+    best of ``num_expert_group`` groups are those of ``router_gemm`` and ``grouped_topk``, in fp32 (up to four tokens bit for bit): a
+    group ranks by the sum of its two best, in either scoring, and of equal experts or groups the lower index comes first.  Weights are
+    the scores, divided by their sum where ``renormalize``, times ``routed_scaling_factor``.
 
     ``w1`` [E, 2 I, H] (gate rows first), ``w2`` [E, H, I] as ``fused_experts_impl`` has them, in the type of the activations, or
     float8_e4m3fn with ``w1_scale`` [E, 2 I / 128, H / 128] and ``w2_scale`` [E, H / 128, I / 128]: the activations are then taken in
     e4m3 too, in groups of 128, as with ``use_fp8_w8a8`` and ``block_shape=[128, 128]``.  The shared expert, [2 Is, H] and [H, Is],
-    has the format of the others.  H (at most 16384, in 8 bits 8192), I and Is are multiples of
-    64, in 8 bits of 128; at most 1024 experts, 32 per token.
+    has the format of the others.  Each expert's intermediate is rounded to the activations' type, as ``fused_experts_impl`` rounds it.
+    H (at most 16384, in 8 bits 8192), I and Is are multiples of 64, in 8 bits of 128; at most 1024 experts, 32 per token.
 
     More tokens: ``router_gemm_grouped_topk``, ``fused_experts_impl`` and ``fused_linear``.  Not differentiable: refused where a
     gradient is wanted.  The same bits in every run of the same call; what the other tokens of a call choose may change the order of a

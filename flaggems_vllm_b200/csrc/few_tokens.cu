@@ -206,6 +206,7 @@ __device__ __forceinline__ void first_product(const Few& P, const Shared& S, con
         stride = P.Is;
         h = reinterpret_cast<T*>(P.h) + routed * kTokens + (o - routed);
       }
+      // rounded to the activations' type, as in the layer of many tokens: h is an operand of the second product
       if (2 * c < P.M) h[2 * c * stride] = from_f32<T>(silu_mul(v.x, v.z));
       if (2 * c + 1 < P.M) h[(2 * c + 1) * stride] = from_f32<T>(silu_mul(v.y, v.w));
     }
@@ -355,7 +356,7 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
   for (int i = begin; i < end; ++i) {
     const uint32_t mask = S.mask[at.s];
     const bool r0 = (mask >> (2 * c)) & 1, r1 = (mask >> (2 * c + 1)) & 1;
-    float f0 = r0 ? S.weight[at.s][2 * c] : 0.0f, f1 = r1 ? S.weight[at.s][2 * c + 1] : 0.0f;
+    const float f0 = r0 ? S.weight[at.s][2 * c] : 0.0f, f1 = r1 ? S.weight[at.s][2 * c + 1] : 0.0f;
     wait_copies<R::UNITS - 2>();
     next();
     const uint32_t hs = hring + hfrom * 1024;
@@ -375,10 +376,9 @@ __device__ __forceinline__ void second_product(const Few& P, const Shared& S, fl
       if (++from == R::UNITS) from = 0;
       float p[4] = {};
       multiply<KIND>(p, wa, wb, x);
-      float a0 = f0, a1 = f1, b0 = f0, b1 = f1;
       // a token that is not the expert's takes nothing, whatever the weights hold
-      if (r0) { acc[t][0] = fmaf(p[0], a0, acc[t][0]); acc[t][2] = fmaf(p[2], b0, acc[t][2]); }
-      if (r1) { acc[t][1] = fmaf(p[1], a1, acc[t][1]); acc[t][3] = fmaf(p[3], b1, acc[t][3]); }
+      if (r0) { acc[t][0] = fmaf(p[0], f0, acc[t][0]); acc[t][2] = fmaf(p[2], f0, acc[t][2]); }
+      if (r1) { acc[t][1] = fmaf(p[1], f1, acc[t][1]); acc[t][3] = fmaf(p[3], f1, acc[t][3]); }
     }
     advance(at);
   }

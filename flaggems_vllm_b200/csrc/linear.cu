@@ -39,7 +39,6 @@ struct Epilogue {
   void* y;               // [M, N]
   void* z;               // [M, N'], null = not kept
   int64_t residual_ld, y_ld, z_ld;
-  int64_t M;
   int N, act, bias_f32;
 };
 
@@ -1213,7 +1212,7 @@ extern "C" int moe_fused_linear(const void* x, int64_t x_ld, const void* w, int6
   const int64_t W = width(N, act);
   if (x_ld < K || w_ld < K || y_ld < N || (residual && residual_ld < N) || (z && z_ld < W)) return fail(MOE_E_SHAPE, "fused_linear: rows overlap");
   cudaStream_t st = (cudaStream_t)stream;
-  Epilogue E = {bias, residual, y, z, residual_ld, y_ld, z_ld, M, (int)N, act, bias_dtype == MOE_F32};
+  Epilogue E = {bias, residual, y, z, residual_ld, y_ld, z_ld, (int)N, act, bias_dtype == MOE_F32};
   const bool gated = act == MOE_LIN_SILU_MUL;
   if (dtype == MOE_F32) return run_f32({(const float*)x, x_ld, 1, 0}, {(const float*)w, w_ld, 1, 0}, M, N, K, gated, E, st);
   if ((uintptr_t)workspace & 15) return fail(MOE_E_BADARG, "fused_linear: the workspace must be 16-byte aligned");
@@ -1320,11 +1319,11 @@ extern "C" int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld
   E.act = MOE_LIN_NONE;
   if (dtype == MOE_F32) {
     if (dx) {
-      E.y = dx; E.y_ld = K; E.M = M; E.N = (int)K;
+      E.y = dx; E.y_ld = K; E.N = (int)K;
       if (int rc = run_f32({(const float*)dz, dz_ld, 1, 0}, {(const float*)w, 1, w_ld, 0}, M, K, W, false, E, st)) return rc;
     }
     if (dw) {
-      E.y = dw; E.y_ld = K; E.M = W; E.N = (int)K;
+      E.y = dw; E.y_ld = K; E.N = (int)K;
       if (int rc = run_f32({(const float*)dz, 1, dz_ld, 0}, {(const float*)x, 1, x_ld, 0}, W, K, M, false, E, st)) return rc;
     }
     return 0;
@@ -1332,7 +1331,7 @@ extern "C" int moe_fused_linear_grad(const void* dy, const void* z, int64_t z_ld
   Matrix d = {dz, M, W, dz_ld};
   if (int rc = readable(d, ws, st)) return rc;
   auto product = [&](const Matrix& a, const Matrix& b, bool a_mn, int64_t rows, int64_t k) {
-    E.y_ld = K; E.M = rows; E.N = (int)K;
+    E.y_ld = K; E.N = (int)K;
     return dtype == MOE_BF16 ? run_product<__nv_bfloat16>(a, b, a_mn, true, rows, K, k, false, E, status, st)
                              : run_product<__half>(a, b, a_mn, true, rows, K, k, false, E, status, st);
   };

@@ -1084,6 +1084,8 @@ int run_product(Matrix a, Matrix b, bool a_mn, bool b_mn, int64_t rows, int64_t 
     const int ct = gated ? p.BN / 2 : p.BN;
     const int64_t RT = (rows + 255) / 256, CT = (cols + ct - 1) / ct, tiles = RT * CT;
     if (tiles >= (1ll << 31)) return fail(MOE_E_TOOBIG, "fused_linear: too many tiles");
+    // 4096 x 4096 -> 2 x 14336 gated, 8192 x 4096 -> 4096: 854, 179 us with groups of one row tile, 688, 186 of 4, 667, 194 of 8, 657, 182 of
+    // 16, 654, 212 of 64; of the second the runs of one size are as far apart
     P.group = 8;
     const int pairs = sm_count() / 2;
     return launch_pdl(kern, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), PTHREADS, kPairSmem, 2, st, "fused_linear (pair)", ma, mb, P, E);

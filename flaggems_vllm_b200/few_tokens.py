@@ -54,9 +54,9 @@ def fused_moe_few_tokens(
     has the format of the others.  Each expert's intermediate is rounded to the activations' type, as ``fused_experts_impl`` rounds it.
     H (at most 16384, in 8 bits 8192), I and Is are multiples of 64, in 8 bits of 128; at most 1024 experts, 32 per token.
 
-    More tokens: ``router_gemm_grouped_topk``, ``fused_experts_impl`` and ``fused_linear``.  Not differentiable: refused where a
-    gradient is wanted.  The same bits in every run of the same call; what the other tokens of a call choose may change the order of a
-    token's sums."""
+    More tokens: ``router_gemm_grouped_topk``, ``fused_experts_impl`` and, for the shared expert, ``fused_linear`` or in 8 bits a layer
+    of one expert.  Not differentiable: refused where a gradient is wanted.  The same bits in every run of the same call; what the other
+    tokens of a call choose may change the order of a token's sums."""
     logger.debug("GEMS FUSED MOE FEW TOKENS")
     what = "fused_moe_few_tokens"
     sigmoid = scoring == "sigmoid"

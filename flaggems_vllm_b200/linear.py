@@ -35,7 +35,9 @@ def fused_linear(
     bfloat16, float16 or float32, one type for ``x``, ``weight`` and ``residual``; ``bias`` may be float32.  Rows may lie in
     wider buffers.  Rows that are no whole number of 16 bytes, or begin at other addresses, are copied first in the 16-bit types.
     Differentiable once, backwards, in all four; where there is an activation, ``x @ weight.T + bias`` is kept for it in the
-    type of ``x``, for the gated one in float32.  The same bits in every run."""
+    type of ``x`` (beyond its largest value as that value), for the gated one in float32.  The gradient of ``x @ weight.T + bias`` is
+    rounded to the type of ``x`` in front of the products of the others'; the bias' sums are of its fp32 values.  The same bits in
+    every run, whichever gradients are wanted."""
     logger.debug("GEMS FUSED LINEAR")
     act = _ACTIVATIONS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
     if x.is_cuda and act >= 0:

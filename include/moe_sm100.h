@@ -517,8 +517,9 @@ int moe_balance_loss_grad(const void* logits, int64_t ld, int dtype, int64_t tok
 /* Dense product with a fused epilogue (no counterpart in the reference):  z = x w^T + bias,  y = act(z) + residual, in fp32,
  * rounded once; act MOE_LIN_SILU_MUL: z has 2 N columns, act(z) = silu(z[:, :N]) * z[:, N:], and w 2 N rows, bias 2 N elements.
  * x [M, K], w [N or 2 N, K], residual and y [M, N], rows their ld apart; bias contiguous, in dtype or fp32.  z null, or
- * [M, N or 2 N] for the gradient, in dtype, beyond its largest value as that value (SILU_MUL: fp32).  dtype bf16, f16, f32.  bias, residual null = none.  y and z share
- * no memory with each other or the operands.  workspace: bytes of moe_fused_linear_workspace (0 where all rows are whole 16-byte pieces), 16-byte aligned. */
+ * [M, N or 2 N] for the gradient, in dtype, beyond its largest value as that value (SILU_MUL: fp32).  dtype bf16, f16, f32.  bias,
+ * residual null = none.  y and z share no memory with each other or the operands.  workspace: bytes of moe_fused_linear_workspace (0
+ * where all rows are whole 16-byte pieces), 16-byte aligned. */
 enum { MOE_LIN_NONE = 0, MOE_LIN_RELU = 1, MOE_LIN_SILU = 2, MOE_LIN_GELU = 3, MOE_LIN_GELU_TANH = 4, MOE_LIN_SILU_MUL = 5 };
 int moe_fused_linear_workspace(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype, int64_t M, int64_t N, int64_t K,
                                int act, int64_t* bytes /* host */);
